@@ -60,9 +60,9 @@ enum {
  * attention launch, 8,448 bytes more; 15: pa_pack_rows_f16, pa_decode_linear_f16;
  * 16: pa_decode_embed_f16; 17: pa_greedy_f16; 18:
  * pa_decode_rope_prefetch_f16; 19: weight_row_stride of pa_decode_linear_f16, a
- * rotary workspace that never holds queries in the counter region). pa_abi_version
- * returns the library's. */
-#define PA_ABI_VERSION 19
+ * rotary workspace that never holds queries in the counter region; 20:
+ * pa_kv_write_fp8, pa_kv_read_fp8). pa_abi_version returns the library's. */
+#define PA_ABI_VERSION 20
 PA_API int pa_abi_version(void);
 
 /* Message of the last failed call on this thread ("" after a success). */
@@ -475,6 +475,58 @@ PA_API int pa_decode_batched_noalloc_f16(const void* q, const int64_t q_strides[
                                          int num_q_heads, int num_kv_heads, int head_dim,
                                          int block_size, int num_blocks, int max_blocks_per_seq,
                                          float scale, void* stream);
+
+/*
+ * The 8-bit paged pool. No counterpart in the reference, whose pool is fp16
+ * (engine/memory/block_allocator.py:101). Codes are OCP e4m3 bytes in the fp16
+ * pool's layout [num_blocks, block_size, num_kv_heads, head_dim] (strides in
+ * elements, which are bytes here, unit head_dim stride); k_scale and v_scale are
+ * fp32 [num_blocks, num_kv_heads], any strides: a value is code * scale[block, head].
+ * Scales are powers of two from 2^-15 to 2^8, as pa_kv_write_fp8 leaves them.
+ *
+ * Sequences and rows. num_tokens rows belong to num_seqs sequences: sequence b
+ * owns rows query_start_loc[b] .. query_start_loc[b + 1] - 1 (n_b rows; int32
+ * device array of num_seqs + 1 non-decreasing entries), which stand at positions
+ * seq_lens[b] - n_b .. seq_lens[b] - 1: block block_tables[b][p / block_size],
+ * row p % block_size. Rows whose position is negative, or whose block lies
+ * outside the table or the pool, have no slot.
+ *
+ * pa_kv_write_fp8: writes fp16 rows key / value [num_tokens, num_kv_heads,
+ * head_dim] (any strides) into their slots, rows without one nowhere.
+ * query_start_loc may be NULL: one row per sequence, row b, num_tokens =
+ * num_seqs. For each (block, kv head) that gets rows, and for keys and values
+ * apart, the scale becomes 2^e with the smallest e of [-15, 8] for which the new
+ * rows' largest |x| is at most 448 * 2^e; where rows of the block before the new
+ * ones stay, e is at least the present scale's exponent, and if it grew those
+ * rows are coded again from their present values. Codes are round-to-nearest-even
+ * e4m3(x / 2^e); |x| above 61440 (infinities too) is taken as 61440, NaN stays
+ * NaN and does not count for the scale. So a block written from its row 0 on
+ * forgets its old scale, and repeating a call changes nothing. Rows of the block
+ * behind the new ones keep their codes but not their values. No two sequences of
+ * a call may write the same block.
+ *
+ * pa_kv_read_fp8: the same rows' values as fp16 into key / value [num_tokens,
+ * num_kv_heads, head_dim] (unit head_dim stride; exact for the scales above);
+ * zeros for rows without a slot and rows of no sequence.
+ */
+PA_API int pa_kv_write_fp8(const void* key, const int64_t key_strides[3], const void* value,
+                           const int64_t value_strides[3], void* k_cache,
+                           const int64_t k_strides[4], void* v_cache, const int64_t v_strides[4],
+                           float* k_scale, const int64_t k_scale_strides[2], float* v_scale,
+                           const int64_t v_scale_strides[2], const int32_t* block_tables,
+                           const int64_t bt_strides[2], const int32_t* seq_lens,
+                           const int32_t* query_start_loc, int num_seqs, int num_tokens,
+                           int num_kv_heads, int head_dim, int block_size, int num_blocks,
+                           int max_blocks_per_seq, void* stream);
+PA_API int pa_kv_read_fp8(const void* k_cache, const int64_t k_strides[4], const void* v_cache,
+                          const int64_t v_strides[4], const float* k_scale,
+                          const int64_t k_scale_strides[2], const float* v_scale,
+                          const int64_t v_scale_strides[2], const int32_t* block_tables,
+                          const int64_t bt_strides[2], const int32_t* seq_lens,
+                          const int32_t* query_start_loc, void* key, const int64_t key_strides[3],
+                          void* value, const int64_t value_strides[3], int num_seqs,
+                          int num_tokens, int num_kv_heads, int head_dim, int block_size,
+                          int num_blocks, int max_blocks_per_seq, void* stream);
 
 #ifdef __cplusplus
 }

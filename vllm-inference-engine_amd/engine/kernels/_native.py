@@ -18,7 +18,7 @@ import torch  # noqa: F401  (must be loaded before the HIP library, see above)
 
 LIB_NAME = "libpa_gfx950.so"
 LIB_PATH = Path(__file__).with_name(LIB_NAME)
-ABI_VERSION = 19
+ABI_VERSION = 20
 
 PA_OK = 0
 PA_ERR_ARG = 1
@@ -90,6 +90,12 @@ SIGNATURES: dict[str, tuple] = {
     "pa_decode_batched_noalloc_f16": (_i32, [
         _vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _vp, _i64p,
         _i32, _i32, _i32, _i32, _i32, _i32, _i32, _f32, _vp]),
+    "pa_kv_write_fp8": (_i32, [
+        _vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _i64p, _vp,
+        _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _vp]),
+    "pa_kv_read_fp8": (_i32, [
+        _vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _vp, _vp, _i64p, _vp,
+        _i64p, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _vp]),
 }
 
 _lib = None
