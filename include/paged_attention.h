@@ -61,8 +61,8 @@ enum {
  * 16: pa_decode_embed_f16; 17: pa_greedy_f16; 18:
  * pa_decode_rope_prefetch_f16; 19: weight_row_stride of pa_decode_linear_f16, a
  * rotary workspace that never holds queries in the counter region; 20:
- * pa_kv_write_fp8, pa_kv_read_fp8). pa_abi_version returns the library's. */
-#define PA_ABI_VERSION 20
+ * pa_kv_write_fp8, pa_kv_read_fp8; 21: pa_verify_drafts_f32). pa_abi_version returns the library's. */
+#define PA_ABI_VERSION 21
 PA_API int pa_abi_version(void);
 
 /* Message of the last failed call on this thread ("" after a success). */
@@ -527,6 +527,40 @@ PA_API int pa_kv_read_fp8(const void* k_cache, const int64_t k_strides[4], const
                           void* value, const int64_t value_strides[3], int num_seqs,
                           int num_tokens, int num_kv_heads, int head_dim, int block_size,
                           int num_blocks, int max_blocks_per_seq, void* stream);
+
+/*
+ * Verification of drafted tokens (speculative decoding). No counterpart in the
+ * reference, whose decode step selects greedily (engine/kernels/
+ * paged_attention_integration.py:636-651). Sequence b has d = num_drafts[b] drafts
+ * (max_drafts with num_drafts NULL; values outside [0, max_drafts] are clamped).
+ *   target  fp32 [num_seqs, max_drafts + 1, vocab]: the target's probabilities at each
+ *           draft's place and after the last one
+ *   draft   fp32 [num_seqs, max_drafts, vocab], the distributions the drafts were drawn
+ *           from, or NULL: drafts chosen with certainty
+ *   draft_ids int64 and accept_u fp32 [num_seqs, max_drafts], next_u fp32 [num_seqs]:
+ *           the drafts, and random numbers of [0, 1)
+ * Draft i is accepted while accept_u[i] * draft[i][id] < target[i][id] (an id outside
+ * [0, vocab) is not). With n accepted, the next token is the first index whose
+ * cumulative weight exceeds next_u times the sum of weights; the weights are
+ * max(target[n] - draft[n], 0) for n < d (target[n] with draft_ids[n] left out where
+ * draft is NULL), and target[n] for n = d or where those are all 0. Products, sums and
+ * comparisons in 64 bits; negative weights and NaN count as 0; where rounding or
+ * next_u >= 1 leaves no such index, the last index with a weight, and index 0 of a row
+ * without any. accepted[b] = n; tokens [num_seqs, max_drafts + 1] int64 contiguous:
+ * the n drafts, the next token, then -1. At most 16384 sequences and 64 drafts.
+ *
+ * Workspace: its first bytes are arrival counters that must be zero before the first
+ * call that uses the buffer; every call leaves them zero. One buffer per stream, lent
+ * to nothing else.
+ */
+PA_API size_t pa_verify_drafts_workspace_bytes(int num_seqs, int vocab);
+PA_API int pa_verify_drafts_f32(const float* target, const int64_t target_strides[3],
+                                const float* draft, const int64_t draft_strides[3],
+                                const int64_t* draft_ids, const int64_t id_strides[2],
+                                const float* accept_u, const int64_t u_strides[2],
+                                const float* next_u, const int32_t* num_drafts, int64_t* tokens,
+                                int32_t* accepted, int num_seqs, int max_drafts, int vocab,
+                                void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -18,7 +18,7 @@ import torch  # noqa: F401  (must be loaded before the HIP library, see above)
 
 LIB_NAME = "libpa_gfx950.so"
 LIB_PATH = Path(__file__).with_name(LIB_NAME)
-ABI_VERSION = 20
+ABI_VERSION = 21
 
 PA_OK = 0
 PA_ERR_ARG = 1
@@ -96,6 +96,10 @@ SIGNATURES: dict[str, tuple] = {
     "pa_kv_read_fp8": (_i32, [
         _vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _vp, _vp, _i64p, _vp,
         _i64p, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _vp]),
+    "pa_verify_drafts_workspace_bytes": (_sz, [_i32, _i32]),
+    "pa_verify_drafts_f32": (_i32, [
+        _vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _vp,
+        _sz, _vp]),
 }
 
 _lib = None
@@ -226,6 +230,8 @@ WS_SCORES = "scores"
 # "prefill" serves pa_prefill_attention_f16: its counters follow the same
 # zero-between-calls contract as the decode ones, with another layout.
 WS_PREFILL = "prefill"
+# "verify" serves pa_verify_drafts_f32: arrival counters, then sums.
+WS_VERIFY = "verify"
 
 
 # Buffers replaced by larger ones. A HIP graph captured with an older buffer's
@@ -269,6 +275,22 @@ def workspace(nbytes: int, device: torch.device, stream: int, kind: str = WS_DEC
         buf = torch.zeros(size, dtype=torch.uint8, device=device)
         _workspaces[key] = buf
     return buf.data_ptr()
+
+
+def counted_workspace(nbytes: int, counter_bytes: int, device: torch.device, stream: int,
+                      kind: str) -> tuple:
+    """(address, owner) of a workspace whose first counter_bytes must be zero before a call.
+
+    Eagerly the stream's buffer of this kind, as workspace() keeps it. While a graph is
+    being captured, one of the graph's own pool with the counters' clearing recorded
+    before the call: no two graphs, and no graph and eager calls, share it. Hold the
+    owner until the call is made.
+    """
+    if nbytes and torch.cuda.is_current_stream_capturing():
+        own = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        own[:counter_bytes].zero_()
+        return own.data_ptr(), own
+    return workspace(nbytes, device, stream, kind), None
 
 
 def same_device(*tensors: torch.Tensor) -> None:
