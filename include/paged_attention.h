@@ -62,7 +62,7 @@ enum {
  * pa_decode_rope_prefetch_f16; 19: weight_row_stride of pa_decode_linear_f16, a
  * rotary workspace that never holds queries in the counter region; 20:
  * pa_kv_write_fp8, pa_kv_read_fp8; 21: pa_verify_drafts_f32). pa_abi_version returns the library's. */
-#define PA_ABI_VERSION 21
+#define PA_ABI_VERSION 22
 PA_API int pa_abi_version(void);
 
 /* Message of the last failed call on this thread ("" after a success). */
@@ -527,6 +527,30 @@ PA_API int pa_kv_read_fp8(const void* k_cache, const int64_t k_strides[4], const
                           void* value, const int64_t value_strides[3], int num_seqs,
                           int num_tokens, int num_kv_heads, int head_dim, int block_size,
                           int num_blocks, int max_blocks_per_seq, void* stream);
+
+/*
+ * Decode attention over the 8-bit pool: pa_decode_batched_f16 with K and V rows =
+ * code * scale[block, head]. Same arguments and the same treatment of lengths, tables
+ * and block ids out of range; head_dim 32, 64, 128 or 256, query groups up to 16, any
+ * block size; cache strides multiples of 16 bytes, bases of 16-byte alignment.
+ * Probabilities are rounded to fp16 once (the fp16 decode keeps a remainder too).
+ *
+ * Workspace (0 bytes: none needed): its first bytes are arrival counters that must be
+ * zero before the first call that uses the buffer; every call leaves them zero. One
+ * buffer per stream, lent to nothing else.
+ */
+PA_API size_t pa_decode_fp8_workspace_bytes(int num_seqs, int num_q_heads, int num_kv_heads,
+                                            int head_dim, int block_size, int max_blocks_per_seq);
+PA_API int pa_decode_fp8(const void* q, const int64_t q_strides[3], const void* k_cache,
+                         const int64_t k_strides[4], const void* v_cache,
+                         const int64_t v_strides[4], const float* k_scale,
+                         const int64_t k_scale_strides[2], const float* v_scale,
+                         const int64_t v_scale_strides[2], const int32_t* block_tables,
+                         const int64_t bt_strides[2], const int32_t* seq_lens, void* out,
+                         const int64_t out_strides[3], int num_seqs, int num_q_heads,
+                         int num_kv_heads, int head_dim, int block_size, int num_blocks,
+                         int max_blocks_per_seq, float scale, void* workspace,
+                         size_t workspace_bytes, void* stream);
 
 /*
  * Verification of drafted tokens (speculative decoding). No counterpart in the

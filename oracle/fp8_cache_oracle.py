@@ -82,12 +82,21 @@ def read(pool, tables, lens, starts, block_size, num_tokens):
     return out
 
 
-def attention(pool, q, tables, lens, starts, block_size, scale):
+def attention(pool, q, tables, lens, starts, block_size, scale, bound=False):
     """Causal attention of each sequence's rows over its positions 0 .. their own; rows at
-    negative positions are zeros. Lengths are cut to the table's width and block ids to the pool."""
+    negative positions are zeros. Lengths are cut to the table's width and block ids to the pool.
+
+    With `bound` also how far a kernel may be off that sums in fp32 and rounds probabilities p
+    and outputs o to fp16 (half a step of a value x: 2^-11 |x|). Its weights are off by a factor
+    1 + e each, and their sum with them, so o is off by at most sum_t w_t |e_t| |v_t - o|, with
+    |e| <= 2^-11 (rounded p) + 2 (D + 8) 2^-24 S (a score's fp32 sum of D products and its
+    exponential; S the largest scale * sum |q_i| |k_i|) + (L / 32 + 64) 2^-24 (sums over tokens
+    by chunks of 32, wavefronts and splits); then its own rounding, and fp16's smallest step.
+    """
     rows, hq, d = q.shape
     blocks, _, hkv, _ = pool["k"].shape
     out = np.zeros((rows, hq, d))
+    tol = np.zeros((rows, hq, d))
     for b, n in enumerate(lens):
         n = max(0, min(n, tables.shape[1] * block_size))
         ids = np.clip(tables[b, :-(-n // block_size)], 0, blocks - 1)
@@ -102,5 +111,11 @@ def attention(pool, q, tables, lens, starts, block_size, scale):
                 g = h // (hq // hkv)
                 s = (k[:pos + 1, g] @ q[starts[b] + i, h]) * scale
                 p = np.exp(s - s.max())
-                out[starts[b] + i, h] = (p / p.sum()) @ v[:pos + 1, g]
-    return out
+                w = p / p.sum()
+                o = out[starts[b] + i, h] = w @ v[:pos + 1, g]
+                if bound:
+                    big = (np.abs(k[:pos + 1, g]) @ np.abs(q[starts[b] + i, h])).max() * abs(scale)
+                    e = 2.0 ** -11 + (2 * (d + 8) * big + pos / 32 + 64) * 2.0 ** -24
+                    around = w @ np.abs(v[:pos + 1, g] - o)
+                    tol[starts[b] + i, h] = e * around + 2.0 ** -11 * np.abs(o) + 2.0 ** -24
+    return (out, tol) if bound else out

@@ -63,3 +63,26 @@ def test_python_calls_need_the_gpu():
         qc.paged_kv_write_fp8(rows, rows, *pool)
     with pytest.raises(AssertionError):
         qc.paged_kv_read_fp8(*pool, torch.tensor([0, 1], dtype=torch.int32), 1)
+
+
+def _decode(lib, q=16, k=16, out=16, kstr=POOL, qstr=S([896, 64, 1]), hq=14, hkv=2, d=64, bs=16,
+            blocks=10, width=4, seqs=2, ws=0, nbytes=0):
+    return lib.pa_decode_fp8(q, qstr, k, kstr, 16, POOL, 16, S([2, 1]), 16, S([2, 1]), 16,
+                             S([4, 1]), 16, out, S([896, 64, 1]), seqs, hq, hkv, d, bs, blocks,
+                             width, 0.125, ws, nbytes, None)
+
+
+def test_decode_argument_errors():
+    lib = _native.load()
+    for bad in (dict(q=0), dict(out=0), dict(k=8), dict(hq=15), dict(hkv=0), dict(bs=0), dict(blocks=0),
+                dict(width=0), dict(seqs=-1), dict(kstr=S([2048, 128, 72, 1])),
+                dict(kstr=S([-2048, 128, 64, 1])), dict(kstr=S([2048, 128, 64, 2])),
+                dict(qstr=S([900, 64, 1])), dict(qstr=S([896, 64, 2]))):
+        assert _decode(lib, **bad) == _native.PA_ERR_ARG, bad
+        assert lib.pa_last_error()
+    for bad in (dict(d=48), dict(hq=34), dict(width=2 ** 27)):
+        assert _decode(lib, **bad) == _native.PA_ERR_UNSUPPORTED, bad
+    assert _decode(lib, width=4096) == _native.PA_ERR_WORKSPACE  # long tables are split
+    assert _decode(lib, seqs=0, q=0) == _native.PA_OK
+    assert lib.pa_decode_fp8_workspace_bytes(2, 14, 2, 48, 16, 4) == 0
+    assert lib.pa_decode_fp8_workspace_bytes(1, 14, 2, 64, 16, 4096) > 65536

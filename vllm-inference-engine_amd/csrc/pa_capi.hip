@@ -161,8 +161,6 @@ static int kv_write_args(KVWriteArgs& a, bool& vec, const void* key, const int64
 
 // ---- stream-K schedule: grid size and workspace layout ----
 
-static int device_cus();
-
 // Kv heads per stream-K pair. Two (head_dim <= 64, even kv-head count) fill 14
 // of 16 MFMA columns at group size 7 and halve the tiles and pair segments,
 // which pays when the batch's (sequence, kv head) pairs outnumber the CUs.
@@ -273,7 +271,7 @@ constexpr int kSkFewRanges = 48;
 
 // Compute units of the current device (cached per device; threads that race
 // on the first query store the same value).
-static int device_cus() {
+int device_cus() {
   static std::atomic<int> cache[64];
   int dev = 0;
   if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;

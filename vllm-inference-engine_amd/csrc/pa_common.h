@@ -23,6 +23,9 @@ constexpr int kMaxIds = 512;
 void set_error(const char* fmt, ...) __attribute__((format(printf, 1, 2)));
 void clear_error();
 
+// Compute units of the current device (pa_capi.hip).
+int device_cus();
+
 // Argument bundle of the decode kernels. Element strides; head_dim stride is 1.
 struct DecodeArgs {
   const f16* q;

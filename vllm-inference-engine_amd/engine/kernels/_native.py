@@ -18,7 +18,7 @@ import torch  # noqa: F401  (must be loaded before the HIP library, see above)
 
 LIB_NAME = "libpa_gfx950.so"
 LIB_PATH = Path(__file__).with_name(LIB_NAME)
-ABI_VERSION = 21
+ABI_VERSION = 22
 
 PA_OK = 0
 PA_ERR_ARG = 1
@@ -96,6 +96,10 @@ SIGNATURES: dict[str, tuple] = {
     "pa_kv_read_fp8": (_i32, [
         _vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _vp, _vp, _i64p, _vp,
         _i64p, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _vp]),
+    "pa_decode_fp8_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32, _i32, _i32]),
+    "pa_decode_fp8": (_i32, [
+        _vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _vp, _i64p,
+        _i32, _i32, _i32, _i32, _i32, _i32, _i32, _f32, _vp, _sz, _vp]),
     "pa_verify_drafts_workspace_bytes": (_sz, [_i32, _i32]),
     "pa_verify_drafts_f32": (_i32, [
         _vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _vp,
@@ -230,6 +234,8 @@ WS_SCORES = "scores"
 # "prefill" serves pa_prefill_attention_f16: its counters follow the same
 # zero-between-calls contract as the decode ones, with another layout.
 WS_PREFILL = "prefill"
+# "decode_fp8" serves pa_decode_fp8: arrival counters, then partial records.
+WS_DECODE_FP8 = "decode_fp8"
 # "verify" serves pa_verify_drafts_f32: arrival counters, then sums.
 WS_VERIFY = "verify"
 

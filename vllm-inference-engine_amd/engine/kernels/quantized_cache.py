@@ -26,11 +26,12 @@ from typing import Optional, Tuple
 import torch
 
 from . import _native
-from .paged_attention import _on_device
+from .paged_attention import _on_device, _q_ready
 
 __all__ = [
     "paged_kv_write_fp8",
     "paged_kv_read_fp8",
+    "paged_attention_decode_fp8",
 ]
 
 
@@ -59,6 +60,15 @@ def _check_starts(query_start_loc: torch.Tensor, like: torch.Tensor, num_seqs: i
     _native.same_device(query_start_loc, like)
     assert query_start_loc.dim() == 1 and query_start_loc.shape[0] == num_seqs + 1
     return query_start_loc.contiguous()
+
+
+def _check_queries(q: torch.Tensor, k_cache: torch.Tensor) -> None:
+    assert q.is_cuda and q.dtype == torch.float16
+    _native.same_device(q, k_cache)
+    assert q.dim() == 3 and q.shape[2] == k_cache.shape[3], (
+        f"queries must be [tokens, num_q_heads, {k_cache.shape[3]}], got {tuple(q.shape)}")
+    assert k_cache.shape[2] > 0 and q.shape[1] % k_cache.shape[2] == 0, (
+        f"num_q_heads ({q.shape[1]}) must be divisible by num_kv_heads ({k_cache.shape[2]})")
 
 
 def paged_kv_write_fp8(
@@ -168,3 +178,59 @@ def paged_kv_read_fp8(
             block_tables.shape[1], _native.stream_handle(dev))
     _native.check(status, "pa_kv_read_fp8")
     return key, value
+
+
+_ws_sizes: dict = {}
+# Bytes of the arrival counters at the head of the attention workspaces.
+_COUNTER_BYTES = 65536
+
+
+def paged_attention_decode_fp8(
+    q: torch.Tensor,             # [num_seqs, num_q_heads, head_dim] fp16
+    k_cache: torch.Tensor,       # [num_blocks, block_size, num_kv_heads, head_dim] float8_e4m3fn
+    v_cache: torch.Tensor,
+    k_scale: torch.Tensor,       # [num_blocks, num_kv_heads] fp32
+    v_scale: torch.Tensor,
+    block_tables: torch.Tensor,  # [num_seqs, max_blocks_per_seq] int32
+    seq_lens: torch.Tensor,      # [num_seqs] int32
+    scale: float,
+) -> torch.Tensor:
+    """Batched GQA decode attention over the 8-bit pool: paged_attention_decode_batched on
+    K and V rows = code * scale[block, head].
+
+    The same lengths, tables and refusals: head_dim 32, 64, 128 or 256, query groups of up
+    to 16, seq_lens 0 gives zeros, lengths past the table are cut to it and block ids
+    clamped into the pool. One launch; long contexts are split over workgroups that merge
+    in it, through a per-stream scratch buffer (the graph's own while one is captured).
+    Repeated calls return the same bits.
+    """
+    block_tables, seq_lens = _check_pool(k_cache, v_cache, k_scale, v_scale, block_tables,
+                                         seq_lens)
+    _check_queries(q, k_cache)
+    num_seqs, num_q_heads, head_dim = q.shape
+    assert seq_lens.shape[0] == num_seqs
+    num_blocks, block_size, num_kv_heads, _ = k_cache.shape
+    q = _q_ready(q)
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    if num_seqs == 0 or num_q_heads == 0:
+        return out
+    lib = _native.load()
+    dev = q.device
+    st = _native.strides_of
+    sizes = (num_seqs, num_q_heads, num_kv_heads, head_dim, block_size, block_tables.shape[1])
+    stream = _native.stream_handle(dev)
+    with _on_device(dev):
+        key = ("decode", dev.index, *sizes)
+        nbytes = _ws_sizes.get(key)
+        if nbytes is None:
+            nbytes = _ws_sizes[key] = lib.pa_decode_fp8_workspace_bytes(*sizes)
+        ws, _own = _native.counted_workspace(nbytes, _COUNTER_BYTES, dev, stream,
+                                             _native.WS_DECODE_FP8)
+        status = lib.pa_decode_fp8(
+            q.data_ptr(), st(q), k_cache.data_ptr(), st(k_cache), v_cache.data_ptr(), st(v_cache),
+            k_scale.data_ptr(), st(k_scale), v_scale.data_ptr(), st(v_scale),
+            block_tables.data_ptr(), st(block_tables), seq_lens.data_ptr(),
+            out.data_ptr(), st(out), num_seqs, num_q_heads, num_kv_heads, head_dim, block_size,
+            num_blocks, block_tables.shape[1], float(scale), ws, nbytes, stream)
+    _native.check(status, "pa_decode_fp8")
+    return out
