@@ -62,7 +62,7 @@ enum {
  * pa_decode_rope_prefetch_f16; 19: weight_row_stride of pa_decode_linear_f16, a
  * rotary workspace that never holds queries in the counter region; 20:
  * pa_kv_write_fp8, pa_kv_read_fp8; 21: pa_verify_drafts_f32). pa_abi_version returns the library's. */
-#define PA_ABI_VERSION 22
+#define PA_ABI_VERSION 23
 PA_API int pa_abi_version(void);
 
 /* Message of the last failed call on this thread ("" after a success). */
@@ -551,6 +551,27 @@ PA_API int pa_decode_fp8(const void* q, const int64_t q_strides[3], const void* 
                          int num_kv_heads, int head_dim, int block_size, int num_blocks,
                          int max_blocks_per_seq, float scale, void* workspace,
                          size_t workspace_bytes, void* stream);
+
+/*
+ * Paged prefill attention over the 8-bit pool: pa_prefill_attention_f16 with K and V
+ * rows = code * scale[block, head], for prompts, chunks of them, and a few drafted
+ * tokens per sequence. Same arguments, refusals and workspace
+ * (pa_prefill_attention_workspace_bytes; the two calls may share a buffer on one
+ * stream); cache strides are multiples of 16 bytes. A NaN in a sequence's row makes
+ * the query rows that see it NaN (all of head_dim or a part) and no others.
+ */
+PA_API int pa_prefill_attention_fp8(const void* q, const int64_t q_strides[3],
+                                    const void* k_cache, const int64_t k_strides[4],
+                                    const void* v_cache, const int64_t v_strides[4],
+                                    const float* k_scale, const int64_t k_scale_strides[2],
+                                    const float* v_scale, const int64_t v_scale_strides[2],
+                                    const int32_t* block_tables, const int64_t bt_strides[2],
+                                    const int32_t* seq_lens, const int32_t* query_start_loc,
+                                    int max_query_len, void* out, const int64_t out_strides[3],
+                                    int num_seqs, int num_tokens, int num_q_heads,
+                                    int num_kv_heads, int head_dim, int block_size,
+                                    int num_blocks, int max_blocks_per_seq, float scale,
+                                    void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * Verification of drafted tokens (speculative decoding). No counterpart in the

@@ -86,3 +86,24 @@ def test_decode_argument_errors():
     assert _decode(lib, seqs=0, q=0) == _native.PA_OK
     assert lib.pa_decode_fp8_workspace_bytes(2, 14, 2, 48, 16, 4) == 0
     assert lib.pa_decode_fp8_workspace_bytes(1, 14, 2, 64, 16, 4096) > 65536
+
+
+def _prefill(lib, q=16, k=16, ks=16, kstr=POOL, qstr=S([896, 64, 1]), starts=16, hq=14, d=64,
+             width=4, seqs=2, tokens=9, longest=5, scale=0.125):
+    return lib.pa_prefill_attention_fp8(q, qstr, k, kstr, 16, POOL, ks, S([2, 1]), 16, S([2, 1]), 16,
+                                        S([4, 1]), 16, starts, longest, 16, S([896, 64, 1]), seqs,
+                                        tokens, hq, 2, d, 16, 10, width, scale, None, 0, None)
+
+
+def test_prefill_argument_errors():
+    lib = _native.load()
+    for bad in (dict(q=0), dict(ks=0), dict(k=8), dict(hq=15), dict(width=0), dict(starts=0),
+                dict(kstr=S([2048, 128, 72, 1])), dict(kstr=S([2048, 128, 64, 2])),
+                dict(qstr=S([900, 64, 1])), dict(scale=0.0), dict(scale=float("inf")),
+                dict(longest=-1), dict(seqs=-1)):
+        assert _prefill(lib, **bad) == _native.PA_ERR_ARG, bad
+        assert lib.pa_last_error()
+    assert _prefill(lib, d=48) == _native.PA_ERR_UNSUPPORTED
+    assert _prefill(lib, hq=34) == _native.PA_ERR_UNSUPPORTED
+    assert _prefill(lib, width=4096) == _native.PA_ERR_WORKSPACE
+    assert _prefill(lib, q=0, tokens=0) == _native.PA_OK

@@ -1201,7 +1201,8 @@ size_t pa_prefill_attention_workspace_bytes(int num_seqs, int num_q_heads, int n
                       max_blocks_per_seq, max_query_len).ws_bytes;
 }
 
-int pa_prefill_attention_f16(const void* q, const int64_t q_strides[3], const void* k_cache,
+// Both forms of the prefill attention; k_scale null: the fp16 pool.
+static int prefill_attention(const void* q, const int64_t q_strides[3], const void* k_cache,
                              const int64_t k_strides[4], const void* v_cache,
                              const int64_t v_strides[4], const int32_t* block_tables,
                              const int64_t bt_strides[2], const int32_t* seq_lens,
@@ -1209,8 +1210,9 @@ int pa_prefill_attention_f16(const void* q, const int64_t q_strides[3], const vo
                              const int64_t out_strides[3], int num_seqs, int num_tokens,
                              int num_q_heads, int num_kv_heads, int head_dim, int block_size,
                              int num_blocks, int max_blocks_per_seq, float scale,
-                             void* workspace, size_t workspace_bytes, void* stream) {
-  clear_error();
+                             void* workspace, size_t workspace_bytes, void* stream,
+                             const float* k_scale, const int64_t* k_scale_strides,
+                             const float* v_scale, const int64_t* v_scale_strides) {
   if (num_seqs < 0 || num_tokens < 0 || max_query_len < 0) {
     set_error("num_seqs, num_tokens and max_query_len must be >= 0");
     return PA_ERR_ARG;
@@ -1297,9 +1299,66 @@ int pa_prefill_attention_f16(const void* q, const int64_t q_strides[3], const vo
   const int64_t exist = (int64_t)num_tokens * g / cols + num_seqs;
   if (num_seqs > 1 && num_seqs <= kPfCompactSeqs && exist < plan.col_blocks * num_seqs)
     a.compact = (int)exist;
+  if (k_scale) {
+    a.ks = k_scale;
+    a.ks_sb = k_scale_strides[0];
+    a.ks_sh = k_scale_strides[1];
+    a.vs = v_scale;
+    a.vs_sb = v_scale_strides[0];
+    a.vs_sh = v_scale_strides[1];
+  }
   a.cnt = plan.ws_bytes ? (int*)workspace : nullptr;
   a.recs = plan.ws_bytes ? (float*)((char*)workspace + plan.counter_bytes) : nullptr;
   return finish_launch(launch_prefill_attn(a, head_dim, (hipStream_t)stream));
+}
+
+int pa_prefill_attention_f16(const void* q, const int64_t q_strides[3], const void* k_cache,
+                             const int64_t k_strides[4], const void* v_cache,
+                             const int64_t v_strides[4], const int32_t* block_tables,
+                             const int64_t bt_strides[2], const int32_t* seq_lens,
+                             const int32_t* query_start_loc, int max_query_len, void* out,
+                             const int64_t out_strides[3], int num_seqs, int num_tokens,
+                             int num_q_heads, int num_kv_heads, int head_dim, int block_size,
+                             int num_blocks, int max_blocks_per_seq, float scale,
+                             void* workspace, size_t workspace_bytes, void* stream) {
+  clear_error();
+  return prefill_attention(q, q_strides, k_cache, k_strides, v_cache, v_strides, block_tables,
+                           bt_strides, seq_lens, query_start_loc, max_query_len, out, out_strides,
+                           num_seqs, num_tokens, num_q_heads, num_kv_heads, head_dim, block_size,
+                           num_blocks, max_blocks_per_seq, scale, workspace, workspace_bytes,
+                           stream, nullptr, nullptr, nullptr, nullptr);
+}
+
+int pa_prefill_attention_fp8(const void* q, const int64_t q_strides[3], const void* k_cache,
+                             const int64_t k_strides[4], const void* v_cache,
+                             const int64_t v_strides[4], const float* k_scale,
+                             const int64_t k_scale_strides[2], const float* v_scale,
+                             const int64_t v_scale_strides[2], const int32_t* block_tables,
+                             const int64_t bt_strides[2], const int32_t* seq_lens,
+                             const int32_t* query_start_loc, int max_query_len, void* out,
+                             const int64_t out_strides[3], int num_seqs, int num_tokens,
+                             int num_q_heads, int num_kv_heads, int head_dim, int block_size,
+                             int num_blocks, int max_blocks_per_seq, float scale,
+                             void* workspace, size_t workspace_bytes, void* stream) {
+  clear_error();
+  if (num_seqs > 0 && num_tokens > 0 && max_query_len > 0) {
+    if (!k_scale || !k_scale_strides || !v_scale || !v_scale_strides || !k_strides || !v_strides) {
+      set_error("null pointer argument");
+      return PA_ERR_ARG;
+    }
+    // (In bytes here, where the fp16 pool's checks ask for multiples of 8 elements.)
+    for (int i = 0; i < 3; ++i) {
+      if (k_strides[i] % 16 || v_strides[i] % 16) {
+        set_error("cache strides must be multiples of 16 bytes");
+        return PA_ERR_ARG;
+      }
+    }
+  }
+  return prefill_attention(q, q_strides, k_cache, k_strides, v_cache, v_strides, block_tables,
+                           bt_strides, seq_lens, query_start_loc, max_query_len, out, out_strides,
+                           num_seqs, num_tokens, num_q_heads, num_kv_heads, head_dim, block_size,
+                           num_blocks, max_blocks_per_seq, scale, workspace, workspace_bytes,
+                           stream, k_scale, k_scale_strides, v_scale, v_scale_strides);
 }
 
 int pa_rmsnorm_f16(const void* x, int64_t x_row_stride, const void* residual,

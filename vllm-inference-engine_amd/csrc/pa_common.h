@@ -235,6 +235,12 @@ struct PrefillAttnArgs {
   int compact;
   int* cnt;     // per-column-block arrival counters, zero between launches
   float* recs;  // [seq][kv head][column block][split] records of (D + 2) x columns floats
+  // The 8-bit pool: k and v point to e4m3 codes (strides in bytes), and these to the
+  // scales [num_blocks, kv heads]; ks null for the fp16 pool.
+  const float* ks;
+  int64_t ks_sb, ks_sh;
+  const float* vs;
+  int64_t vs_sb, vs_sh;
 };
 
 // Columns of a prefill workgroup in units of 64 (token, query head) columns:

@@ -25,6 +25,14 @@
 // with fp16 probabilities on K=32 MFMAs, V^T read transposed from LDS -- the
 // operand layouts of the decode kernel, with columns that are (token, head)
 // pairs instead of the heads of one token.
+//
+// The same kernel serves the 8-bit pool (KV8): pieces of K and V rows are then e4m3
+// codes that become fp16 on their way into LDS, times their block's scale, exactly;
+// everything after is the same but for a factor of 2^8 on the probabilities (see
+// `probs`).
+#include <type_traits>
+
+#include "pa_fp8.h"
 #include "pa_tiles.h"
 
 namespace pa {
@@ -86,7 +94,7 @@ __device__ __forceinline__ bool ragged_block(const PrefillAttnArgs& a, int lane,
   return true;
 }
 
-template <int D, int BS, int CG, int NW>
+template <int D, int BS, int CG, int NW, bool KV8>
 __global__ __launch_bounds__(64 * NW) void prefill_attn_kernel(PrefillAttnArgs a) {
   constexpr int COLS = 16 * CG * NW;  // columns per workgroup
   constexpr int KT = prefill_key_tile(D);  // keys per staged tile
@@ -99,11 +107,16 @@ __global__ __launch_bounds__(64 * NW) void prefill_attn_kernel(PrefillAttnArgs a
   // 4096-token prompts of 32 / 8 heads, 83.4 -> 82.6 at 28 / 4 heads and 2048. Up to
   // head_dim 64 (128-key tiles) they would not.
   constexpr int LS = D == 128 ? D + 16 : D + 8;
-  constexpr int CPR = D / 8;          // 16-byte pieces per key row of one head
+  // Elements of a piece, one thread's load: 16 bytes, or 8 where a tile of codes would
+  // not give every thread 16 (head_dim 32).
+  constexpr int PE = !KV8 ? 8 : KT * D / 16 % (64 * NW) == 0 ? 16 : 8;
+  constexpr int CPR = D / PE;         // pieces per key row of one head
   constexpr int PER = KT * CPR / (64 * NW);
   constexpr int BUF = KT * LS;        // halves of one staged K (or V) tile
   static_assert(PER * 64 * NW == KT * CPR, "a tile must split evenly over the workgroup");
   static_assert(NS % 2 == 0, "sub-tiles are paired for the P V products");
+  typedef std::conditional_t<KV8, uint8_t, f16> E;  // what the pool holds
+  typedef unsigned words __attribute__((ext_vector_type(PE * sizeof(E) / 4)));
 
   __shared__ __attribute__((aligned(16))) f16 ks[2 * BUF];
   __shared__ __attribute__((aligned(16))) f16 vs[2 * BUF];
@@ -188,10 +201,11 @@ __global__ __launch_bounds__(64 * NW) void prefill_attn_kernel(PrefillAttnArgs a
   }
 
   const int32_t* btrow = a.bt + (int64_t)b * a.bt_sb;
-  const f16* kbase = a.k + (int64_t)h * a.k_sh;
-  const f16* vbase = a.v + (int64_t)h * a.v_sh;
+  const E* kbase = reinterpret_cast<const E*>(a.k) + (int64_t)h * a.k_sh;
+  const E* vbase = reinterpret_cast<const E*>(a.v) + (int64_t)h * a.v_sh;
   const int bs = BS > 0 ? BS : a.bs;
-  u32x4 kr[PER], vr[PER];
+  words kr[PER], vr[PER];
+  float ksr[PER], vsr[PER];  // KV8: the scales of the pieces' blocks
   int ids[PER];
   // Piece f = 64 NW i + tid of a tile is key row f / CPR, halves (f % CPR) * 8.
   // The block ids of a tile are loaded one tile before its K/V, so a K/V load
@@ -217,14 +231,14 @@ __global__ __launch_bounds__(64 * NW) void prefill_attn_kernel(PrefillAttnArgs a
   // instructions per piece instead of the general form's clamps, divisions
   // and two 64-bit multiply-adds per load.
   constexpr bool FIXED = BS > 0 && KT % BS == 0 && D <= 128;  // at head_dim 256 the bases cost occupancy
-  const f16* kfix[PER];
-  const f16* vfix[PER];
+  const E* kfix[PER];
+  const E* vfix[PER];
   const int32_t* idfix[PER];
   if constexpr (FIXED) {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int f = i * 64 * NW + tid;
-      const uint32_t r = (uint32_t)(f / CPR), c8 = (uint32_t)(f % CPR) * 8;
+      const uint32_t r = (uint32_t)(f / CPR), c8 = (uint32_t)(f % CPR) * PE;
       kfix[i] = kbase + ((r % BS) * k_st + c8);
       vfix[i] = vbase + ((r % BS) * v_st + c8);
       idfix[i] = btrow + (r / BS) * bt_sk;
@@ -244,37 +258,73 @@ __global__ __launch_bounds__(64 * NW) void prefill_attn_kernel(PrefillAttnArgs a
       ids[i] = btrow[(uint32_t)(key / bs) * bt_sk];
     }
   };
+  auto fetch_scales = [&](int i, uint32_t id) {
+    if constexpr (KV8) {
+      ksr[i] = a.ks[(int64_t)id * a.ks_sb + (int64_t)h * a.ks_sh];
+      vsr[i] = a.vs[(int64_t)id * a.vs_sb + (int64_t)h * a.vs_sh];
+    }
+  };
   auto fetch_kv = [&](int kt) {
     if (whole(kt)) {
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
         const uint32_t id = (uint32_t)min(max(ids[i], 0), a.num_blocks - 1);
-        kr[i] = *reinterpret_cast<const u32x4*>(kfix[i] + (uint64_t)id * k_sb);
-        vr[i] = *reinterpret_cast<const u32x4*>(vfix[i] + (uint64_t)id * v_sb);
+        kr[i] = *reinterpret_cast<const words*>(kfix[i] + (uint64_t)id * k_sb);
+        vr[i] = *reinterpret_cast<const words*>(vfix[i] + (uint64_t)id * v_sb);
+        fetch_scales(i, id);
       }
       return;
     }
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int f = i * 64 * NW + tid;
-      const uint32_t c8 = (f % CPR) * 8;
+      const uint32_t c8 = (f % CPR) * PE;
       const int key = min(kt * KT + f / CPR, kmax - 1);
       const uint32_t id = (uint32_t)min(max(ids[i], 0), a.num_blocks - 1);
       const uint32_t off = (uint32_t)(key % bs);
-      kr[i] = *reinterpret_cast<const u32x4*>(kbase + (uint64_t)id * k_sb + (off * k_st + c8));
-      vr[i] = *reinterpret_cast<const u32x4*>(vbase + (uint64_t)id * v_sb + (off * v_st + c8));
+      kr[i] = *reinterpret_cast<const words*>(kbase + (uint64_t)id * k_sb + (off * k_st + c8));
+      vr[i] = *reinterpret_cast<const words*>(vbase + (uint64_t)id * v_sb + (off * v_st + c8));
+      fetch_scales(i, id);
     }
   };
-  auto stash = [&](int buf) {
+  // Tile kt's pieces into its buffer. `crossing`: some column does not see the whole
+  // tile. Its probability of such a key is 0, but 0 times a NaN in the key's V row would
+  // still reach the column, so for the 8-bit pool (whose only non-finite code is NaN) a
+  // NaN in V is moved to the same place in the key's K row: scores of masked keys are
+  // replaced, and the columns that see the key become NaN.
+  auto stash = [&](int buf, bool crossing) {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int f = i * 64 * NW + tid;
       const int r = f / CPR;
-      const int c8 = (f % CPR) * 8;
-      *reinterpret_cast<u32x4*>(&ks[buf * BUF + r * LS + c8]) = kr[i];
-      *reinterpret_cast<u32x4*>(&vs[buf * BUF + r * LS + c8]) = vr[i];
+      const int c8 = (f % CPR) * PE;
+      f16* kd = &ks[buf * BUF + r * LS + c8];
+      f16* vd = &vs[buf * BUF + r * LS + c8];
+      if constexpr (KV8) {
+        if (crossing) {
+#pragma unroll
+          for (int j = 0; j < PE / 4; ++j) {
+            // The top bit of every byte that holds 0x7f or 0xff.
+            const unsigned nan = ((vr[i][j] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+            const unsigned bytes = (nan >> 7) * 0xffu;
+            vr[i][j] &= ~bytes;
+            kr[i][j] |= bytes & 0x7f7f7f7fu;
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < PE / 8; ++j) {
+          *reinterpret_cast<f16x8*>(kd + 8 * j) =
+              fp8::from_codes8(kr[i][2 * j], kr[i][2 * j + 1], ksr[i]);
+          *reinterpret_cast<f16x8*>(vd + 8 * j) =
+              fp8::from_codes8(vr[i][2 * j], vr[i][2 * j + 1], vsr[i]);
+        }
+      } else {
+        *reinterpret_cast<words*>(kd) = kr[i];
+        *reinterpret_cast<words*>(vd) = vr[i];
+      }
     }
   };
+  auto crosses = [&](int kt) { return kt * KT + KT - 1 > pmin; };  // workgroup-uniform
 
   float m_run[CG], l_run[CG];
   f32x4 acc[CG][ND];
@@ -291,7 +341,7 @@ __global__ __launch_bounds__(64 * NW) void prefill_attn_kernel(PrefillAttnArgs a
   fetch_ids(t0);
   fetch_kv(t0);
   fetch_ids(t0 + 1);
-  stash(t0 & 1);
+  stash(t0 & 1, crosses(t0));
   __syncthreads();
   // Every load issued so far (the query fragments included, which the
   // compiler may place after the first tile's loads) is complete before the
@@ -329,7 +379,7 @@ __global__ __launch_bounds__(64 * NW) void prefill_attn_kernel(PrefillAttnArgs a
           sc[cg][s] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[c], qf[cg][c], sc[cg][s], 0, 0, 0);
       }
     }
-    if (kt * KT + KT - 1 > pmin) {  // workgroup-uniform: a tile crossing some column's position
+    if (crosses(kt)) {  // a tile crossing some column's position
 #pragma unroll
       for (int cg = 0; cg < CG; ++cg)
 #pragma unroll
@@ -343,7 +393,10 @@ __global__ __launch_bounds__(64 * NW) void prefill_attn_kernel(PrefillAttnArgs a
     // still -inf) or when a score exceeds it by 16 or more, so that a
     // probability overflows fp16 -- which makes the fp16 denominator sum
     // infinite (or NaN). Probabilities thus stay below 2^16, and most tiles
-    // skip the maxima and the accumulator rescale.
+    // skip the maxima and the accumulator rescale. With the 8-bit pool they carry a
+    // factor of 2^8 (its share is raised from 2^8 over the maximum on): fp16 then keeps
+    // all its bits down to 2^-22 of the maximum instead of 2^-14, at no cost.
+    constexpr float BIAS = KV8 ? 8.f : 0.f;
     f16x8 pb[NS / 2][CG];
     float lt[CG];
     auto probs = [&]() {
@@ -351,7 +404,7 @@ __global__ __launch_bounds__(64 * NW) void prefill_attn_kernel(PrefillAttnArgs a
       for (int cg = 0; cg < CG; ++cg) {
         // A column with no visible key yet keeps m = -inf; any finite offset
         // then gives p = 0 for its -inf scores.
-        const float nm = m_run[cg] == kNegInf ? 0.f : -m_run[cg];
+        const float nm = m_run[cg] == kNegInf ? 0.f : BIAS - m_run[cg];
         lt[cg] = 0.f;
 #pragma unroll
         for (int sp = 0; sp < NS / 2; ++sp) {
@@ -422,7 +475,7 @@ __global__ __launch_bounds__(64 * NW) void prefill_attn_kernel(PrefillAttnArgs a
       }
     }
 
-    if (more) stash((kt + 1) & 1);
+    if (more) stash((kt + 1) & 1, crosses(kt + 1));
     __syncthreads();
   }
 
@@ -560,44 +613,52 @@ __global__ __launch_bounds__(64 * NW) void prefill_attn_kernel(PrefillAttnArgs a
 // so the two forms agree to rounding and mostly bit for bit. At head_dim 128
 // the eight-wavefront form would hold one workgroup per CU (148 VGPRs), so four
 // wavefronts stay.
-template <int D, int BS, int CG>
+template <bool KV8, int D, int BS, int CG>
 static hipError_t launch_prefill_bs(const PrefillAttnArgs& a, int64_t grid, hipStream_t s) {
   if constexpr (D <= 64 && CG == 2) {
     if (a.wave_groups == 1) {
-      hipLaunchKernelGGL((prefill_attn_kernel<D, BS, 1, 8>), dim3((unsigned)grid), dim3(512), 0, s, a);
+      hipLaunchKernelGGL((prefill_attn_kernel<D, BS, 1, 8, KV8>), dim3((unsigned)grid), dim3(512), 0,
+                         s, a);
       return hipGetLastError();
     }
   }
   if (a.wave_groups != CG) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((prefill_attn_kernel<D, BS, CG, 4>), dim3((unsigned)grid), dim3(256), 0, s, a);
+  hipLaunchKernelGGL((prefill_attn_kernel<D, BS, CG, 4, KV8>), dim3((unsigned)grid), dim3(256), 0, s,
+                     a);
   return hipGetLastError();
 }
 
-template <int D, int CG>
+template <bool KV8, int D, int CG>
 static hipError_t launch_prefill_dc(const PrefillAttnArgs& a, hipStream_t s) {
   const int64_t blocks = a.compact ? a.compact : (int64_t)a.col_blocks * a.num_seqs;
   const int64_t grid = blocks * a.max_splits * a.hkv;
-  return a.bs == 16 ? launch_prefill_bs<D, 16, CG>(a, grid, s) : launch_prefill_bs<D, 0, CG>(a, grid, s);
+  return a.bs == 16 ? launch_prefill_bs<KV8, D, 16, CG>(a, grid, s)
+                    : launch_prefill_bs<KV8, D, 0, CG>(a, grid, s);
 }
 
-template <int D>
+template <bool KV8, int D>
 static hipError_t launch_prefill_d(const PrefillAttnArgs& a, hipStream_t s) {
   constexpr int CG = prefill_col_groups(D);
   if constexpr (CG > 1) {
-    if (a.col_groups == 1) return launch_prefill_dc<D, 1>(a, s);
+    if (a.col_groups == 1) return launch_prefill_dc<KV8, D, 1>(a, s);
   }
   if (a.col_groups != CG) return hipErrorInvalidValue;
-  return launch_prefill_dc<D, CG>(a, s);
+  return launch_prefill_dc<KV8, D, CG>(a, s);
+}
+
+template <bool KV8>
+static hipError_t launch_prefill(const PrefillAttnArgs& a, int D, hipStream_t s) {
+  switch (D) {
+    case 32: return launch_prefill_d<KV8, 32>(a, s);
+    case 64: return launch_prefill_d<KV8, 64>(a, s);
+    case 128: return launch_prefill_d<KV8, 128>(a, s);
+    case 256: return launch_prefill_d<KV8, 256>(a, s);
+    default: return hipErrorInvalidValue;
+  }
 }
 
 hipError_t launch_prefill_attn(const PrefillAttnArgs& a, int D, hipStream_t s) {
-  switch (D) {
-    case 32: return launch_prefill_d<32>(a, s);
-    case 64: return launch_prefill_d<64>(a, s);
-    case 128: return launch_prefill_d<128>(a, s);
-    case 256: return launch_prefill_d<256>(a, s);
-    default: return hipErrorInvalidValue;
-  }
+  return a.ks ? launch_prefill<true>(a, D, s) : launch_prefill<false>(a, D, s);
 }
 
 }  // namespace pa

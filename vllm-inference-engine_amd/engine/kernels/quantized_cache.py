@@ -32,6 +32,7 @@ __all__ = [
     "paged_kv_write_fp8",
     "paged_kv_read_fp8",
     "paged_attention_decode_fp8",
+    "paged_attention_prefill_fp8",
 ]
 
 
@@ -181,7 +182,7 @@ def paged_kv_read_fp8(
 
 
 _ws_sizes: dict = {}
-# Bytes of the arrival counters at the head of the attention workspaces.
+# Bytes of the arrival counters at the head of the attention workspaces (16384 ints).
 _COUNTER_BYTES = 65536
 
 
@@ -233,4 +234,60 @@ def paged_attention_decode_fp8(
             out.data_ptr(), st(out), num_seqs, num_q_heads, num_kv_heads, head_dim, block_size,
             num_blocks, block_tables.shape[1], float(scale), ws, nbytes, stream)
     _native.check(status, "pa_decode_fp8")
+    return out
+
+
+def paged_attention_prefill_fp8(
+    q: torch.Tensor,                # [num_tokens, num_q_heads, head_dim] fp16
+    k_cache: torch.Tensor,          # [num_blocks, block_size, num_kv_heads, head_dim] float8_e4m3fn
+    v_cache: torch.Tensor,
+    k_scale: torch.Tensor,          # [num_blocks, num_kv_heads] fp32
+    v_scale: torch.Tensor,
+    block_tables: torch.Tensor,     # [num_seqs, max_blocks_per_seq] int32
+    seq_lens: torch.Tensor,         # [num_seqs] int32: context length after the new tokens
+    query_start_loc: torch.Tensor,  # [num_seqs + 1] int32: first q row of each sequence
+    max_query_len: int,
+    scale: float,
+) -> torch.Tensor:
+    """Causal attention of each sequence's new tokens over the 8-bit pool.
+
+    paged_attention_prefill on K and V rows = code * scale[block, head]: for prompts,
+    chunks of prompts, and the pass over a few drafted tokens per sequence. The new
+    tokens' rows must be in the pool (paged_kv_write_fp8); scale must be positive; rows
+    of q that belong to no sequence, or lie past max_query_len, are not written.
+    """
+    block_tables, seq_lens = _check_pool(k_cache, v_cache, k_scale, v_scale, block_tables,
+                                         seq_lens)
+    _check_queries(q, k_cache)
+    num_tokens, num_q_heads, head_dim = q.shape
+    num_seqs = seq_lens.shape[0]
+    query_start_loc = _check_starts(query_start_loc, k_cache, num_seqs)
+    max_query_len = int(max_query_len)
+    assert 0 <= max_query_len < 2 ** 31
+    num_blocks, block_size, num_kv_heads, _ = k_cache.shape
+    q = _q_ready(q)
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    if num_seqs == 0 or num_tokens == 0 or num_q_heads == 0 or max_query_len == 0:
+        return out
+    lib = _native.load()
+    dev = q.device
+    st = _native.strides_of
+    max_blocks = block_tables.shape[1]
+    sizes = (num_seqs, num_q_heads, num_kv_heads, head_dim, block_size, max_blocks, max_query_len)
+    stream = _native.stream_handle(dev)
+    with _on_device(dev):
+        key = ("prefill", dev.index, *sizes)
+        nbytes = _ws_sizes.get(key)
+        if nbytes is None:
+            nbytes = _ws_sizes[key] = lib.pa_prefill_attention_workspace_bytes(*sizes)
+        ws, _own = _native.counted_workspace(nbytes, _COUNTER_BYTES, dev, stream,
+                                             _native.WS_PREFILL)
+        status = lib.pa_prefill_attention_fp8(
+            q.data_ptr(), st(q), k_cache.data_ptr(), st(k_cache), v_cache.data_ptr(), st(v_cache),
+            k_scale.data_ptr(), st(k_scale), v_scale.data_ptr(), st(v_scale),
+            block_tables.data_ptr(), st(block_tables), seq_lens.data_ptr(),
+            query_start_loc.data_ptr(), max_query_len, out.data_ptr(), st(out),
+            num_seqs, num_tokens, num_q_heads, num_kv_heads, head_dim, block_size, num_blocks,
+            max_blocks, float(scale), ws, nbytes, stream)
+    _native.check(status, "pa_prefill_attention_fp8")
     return out
