@@ -46,16 +46,6 @@ using namespace tiles;
 // A wavefront-uniform value, moved to a scalar register.
 __device__ inline int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
-// The lane index, computed where it is read and opaque to the compiler: the
-// per-lane values a branch derives from it are then formed inside that branch
-// instead of being hoisted out of the segment loop and kept live (in vector
-// registers) through the other branches' streaming loops.
-__device__ inline int fresh_lane() {
-  int l = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
-  asm volatile("" : "+v"(l));
-  return l;
-}
-
 // First workgroup whose range contains tile x of a T-tile list split G ways.
 __host__ __device__ inline int wg_of(int64_t x, int64_t T, int G) {
   return (int)(((x + 1) * G - 1) / T);

@@ -114,6 +114,20 @@ __device__ inline int load_uniform(const int32_t* p) {
   return *(const __attribute__((address_space(4))) int32_t*)p;
 }
 
+// The lane index, computed where it is read and opaque to the compiler: the
+// per-lane values a branch derives from it are then formed inside that branch
+// instead of being hoisted out of the segment loop and kept live (in vector
+// registers) through the other branches' streaming loops.
+__device__ inline int fresh_lane() {
+  int l = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
+  asm volatile("" : "+v"(l));
+  return l;
+}
+
+__device__ inline float load_uniform(const float* p) {
+  return *(const __attribute__((address_space(4))) float*)p;
+}
+
 template <int BS>
 __device__ inline int blk_of(int t, int bs) {
   if constexpr (BS > 0) return t / BS; else return t / bs;
