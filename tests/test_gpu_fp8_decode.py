@@ -47,9 +47,11 @@ def test_matches_oracle(cuda_device, hq, hkv, d, bs):
 
 
 @pytest.mark.parametrize("hq,hkv,d,bs", [(14, 2, 64, 16), (4, 2, 32, 16), (8, 4, 64, 8), (5, 1, 128, 16)])
-def test_many_sequences(cuda_device, hq, hkv, d, bs):
-    """Enough of them that a workgroup takes two kv heads (head_dim 32 and 64)."""
-    lens = [(37 * i) % 211 for i in range(290)]
+@pytest.mark.parametrize("n,longest", [(290, 211), (150, 211), (140, 1500), (40, 2300)])
+def test_many_sequences(cuda_device, hq, hkv, d, bs, n, longest):
+    """Pairs from less than half the compute units to more than all, short and long: enough that a
+    workgroup takes two kv heads (head_dim 32 and 64), whole pairs and ranges."""
+    lens = [(37 * i) % longest for i in range(n)]
     pool = Fp8Pool(lens, hkv, d, bs, seed=3, device=cuda_device, slack=1)
     check(pool, queries(len(lens), hq, d, 4, cuda_device), d ** -0.5)
 

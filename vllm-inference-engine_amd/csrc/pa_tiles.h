@@ -124,10 +124,6 @@ __device__ inline int fresh_lane() {
   return l;
 }
 
-__device__ inline float load_uniform(const float* p) {
-  return *(const __attribute__((address_space(4))) float*)p;
-}
-
 template <int BS>
 __device__ inline int blk_of(int t, int bs) {
   if constexpr (BS > 0) return t / BS; else return t / bs;
