@@ -61,8 +61,10 @@ enum {
  * 16: pa_decode_embed_f16; 17: pa_greedy_f16; 18:
  * pa_decode_rope_prefetch_f16; 19: weight_row_stride of pa_decode_linear_f16, a
  * rotary workspace that never holds queries in the counter region; 20:
- * pa_kv_write_fp8, pa_kv_read_fp8; 21: pa_verify_drafts_f32). pa_abi_version returns the library's. */
-#define PA_ABI_VERSION 23
+ * pa_kv_write_fp8, pa_kv_read_fp8; 21: pa_verify_drafts_f32; 22: pa_decode_fp8; 23:
+ * pa_prefill_attention_fp8; 24: its workspace size). pa_abi_version returns the
+ * library's. */
+#define PA_ABI_VERSION 24
 PA_API int pa_abi_version(void);
 
 /* Message of the last failed call on this thread ("" after a success). */
@@ -555,11 +557,15 @@ PA_API int pa_decode_fp8(const void* q, const int64_t q_strides[3], const void* 
 /*
  * Paged prefill attention over the 8-bit pool: pa_prefill_attention_f16 with K and V
  * rows = code * scale[block, head], for prompts, chunks of them, and a few drafted
- * tokens per sequence. Same arguments, refusals and workspace
- * (pa_prefill_attention_workspace_bytes; the two calls may share a buffer on one
- * stream); cache strides are multiples of 16 bytes. A NaN in a sequence's row makes
+ * tokens per sequence. Same arguments and refusals, and the same contract of the
+ * workspace, sized by its own query (the fp16 and the 8-bit call may share a buffer on
+ * one stream); cache strides are multiples of 16 bytes. A NaN in a sequence's row makes
  * the query rows that see it NaN (all of head_dim or a part) and no others.
  */
+PA_API size_t pa_prefill_attention_fp8_workspace_bytes(int num_seqs, int num_q_heads,
+                                                       int num_kv_heads, int head_dim,
+                                                       int block_size, int max_blocks_per_seq,
+                                                       int max_query_len);
 PA_API int pa_prefill_attention_fp8(const void* q, const int64_t q_strides[3],
                                     const void* k_cache, const int64_t k_strides[4],
                                     const void* v_cache, const int64_t v_strides[4],

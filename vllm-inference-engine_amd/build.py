@@ -56,8 +56,9 @@ HIPCC_FLAGS = [
 # The decode projections keep their accumulators next to the fragments the same
 # way: in the accumulator-register form each tile would be copied out for the
 # sum over the wavefronts.
-# So does the 8-bit decode kernel, whose accumulators are rescaled every chunk.
+# So does the 8-bit attention kernel, whose accumulators are rescaled, too.
 FILE_FLAGS = {
+    "pa_fp8_drafts.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "pa_fp8_decode.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "pa_decode_linear.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "pa_prefill.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1", "-fno-honor-nans"],

@@ -1249,17 +1249,6 @@ static int prefill_attention(const void* q, const int64_t q_strides[3], const vo
     return PA_ERR_UNSUPPORTED;
   }
   const int g = num_q_heads / num_kv_heads;
-  const PrefillPlan plan = prefill_plan(num_seqs, num_q_heads, num_kv_heads, head_dim, block_size,
-                                        max_blocks_per_seq, max_query_len);
-  const int64_t grid = plan.col_blocks * plan.max_splits * num_seqs * num_kv_heads;
-  if (grid > 0x7fffffff || plan.col_blocks > 0x7fffffff) {
-    set_error("%lld workgroups exceed the grid limit", (long long)grid);
-    return PA_ERR_UNSUPPORTED;
-  }
-  if (plan.ws_bytes && (!workspace || workspace_bytes < plan.ws_bytes)) {
-    set_error("workspace of %zu bytes needed, %zu given", plan.ws_bytes, workspace_bytes);
-    return PA_ERR_WORKSPACE;
-  }
   PrefillAttnArgs a{};
   a.q = (const f16*)q;
   a.q_st = q_strides[0];
@@ -1287,10 +1276,32 @@ static int prefill_attention(const void* q, const int64_t q_strides[3], const vo
   a.bs = block_size;
   a.num_blocks = num_blocks;
   a.max_blocks = max_blocks_per_seq;
+  a.scale_log2 = scale * kLog2e;
+  if (k_scale) {
+    a.ks = k_scale;
+    a.ks_sb = k_scale_strides[0];
+    a.ks_sh = k_scale_strides[1];
+    a.vs = v_scale;
+    a.vs_sb = v_scale_strides[0];
+    a.vs_sh = v_scale_strides[1];
+    if (fp8::takes_drafts(head_dim, g, max_query_len))
+      return fp8::prefill_drafts(a, head_dim, max_query_len, workspace, workspace_bytes,
+                                 (hipStream_t)stream);
+  }
+  const PrefillPlan plan = prefill_plan(num_seqs, num_q_heads, num_kv_heads, head_dim, block_size,
+                                        max_blocks_per_seq, max_query_len);
+  const int64_t grid = plan.col_blocks * plan.max_splits * num_seqs * num_kv_heads;
+  if (grid > 0x7fffffff || plan.col_blocks > 0x7fffffff) {
+    set_error("%lld workgroups exceed the grid limit", (long long)grid);
+    return PA_ERR_UNSUPPORTED;
+  }
+  if (plan.ws_bytes && (!workspace || workspace_bytes < plan.ws_bytes)) {
+    set_error("workspace of %zu bytes needed, %zu given", plan.ws_bytes, workspace_bytes);
+    return PA_ERR_WORKSPACE;
+  }
   a.col_blocks = (int)plan.col_blocks;
   a.col_groups = plan.col_groups;
   a.wave_groups = plan.wave_groups;
-  a.scale_log2 = scale * kLog2e;
   a.split_tiles = (int)plan.split_tiles;
   a.max_splits = (int)plan.max_splits;
   // Batches whose sequences are not all max_query_len long: at most one partly
@@ -1299,14 +1310,6 @@ static int prefill_attention(const void* q, const int64_t q_strides[3], const vo
   const int64_t exist = (int64_t)num_tokens * g / cols + num_seqs;
   if (num_seqs > 1 && num_seqs <= kPfCompactSeqs && exist < plan.col_blocks * num_seqs)
     a.compact = (int)exist;
-  if (k_scale) {
-    a.ks = k_scale;
-    a.ks_sb = k_scale_strides[0];
-    a.ks_sh = k_scale_strides[1];
-    a.vs = v_scale;
-    a.vs_sb = v_scale_strides[0];
-    a.vs_sh = v_scale_strides[1];
-  }
   a.cnt = plan.ws_bytes ? (int*)workspace : nullptr;
   a.recs = plan.ws_bytes ? (float*)((char*)workspace + plan.counter_bytes) : nullptr;
   return finish_launch(launch_prefill_attn(a, head_dim, (hipStream_t)stream));
@@ -1327,6 +1330,18 @@ int pa_prefill_attention_f16(const void* q, const int64_t q_strides[3], const vo
                            num_seqs, num_tokens, num_q_heads, num_kv_heads, head_dim, block_size,
                            num_blocks, max_blocks_per_seq, scale, workspace, workspace_bytes,
                            stream, nullptr, nullptr, nullptr, nullptr);
+}
+
+size_t pa_prefill_attention_fp8_workspace_bytes(int num_seqs, int num_q_heads, int num_kv_heads,
+                                                int head_dim, int block_size,
+                                                int max_blocks_per_seq, int max_query_len) {
+  if (num_seqs > 0 && num_kv_heads > 0 && num_q_heads > 0 && num_q_heads % num_kv_heads == 0 &&
+      block_size > 0 && max_blocks_per_seq > 0 && max_query_len > 0 &&
+      fp8::takes_drafts(head_dim, num_q_heads / num_kv_heads, max_query_len))
+    return fp8::drafts_workspace_bytes(num_seqs, num_q_heads, num_kv_heads, head_dim, block_size,
+                                       max_blocks_per_seq, max_query_len);
+  return pa_prefill_attention_workspace_bytes(num_seqs, num_q_heads, num_kv_heads, head_dim,
+                                              block_size, max_blocks_per_seq, max_query_len);
 }
 
 int pa_prefill_attention_fp8(const void* q, const int64_t q_strides[3], const void* k_cache,

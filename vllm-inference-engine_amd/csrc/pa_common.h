@@ -343,6 +343,15 @@ bool plan_handover_supported(const DecodeArgs& a, int D);
 hipError_t launch_kv_write_plan(const DecodeArgs& a, const KVWriteArgs& w, bool vec,
                                 hipStream_t s);
 hipError_t launch_prefill_attn(const PrefillAttnArgs& a, int D, hipStream_t s);
+// The 8-bit pool's form for a few tokens per sequence (pa_fp8_drafts.hip): whether it takes
+// a call, its workspace, and the call (a PA_* status with the message set).
+namespace fp8 {
+bool takes_drafts(int head_dim, int g, int max_query_len);
+size_t drafts_workspace_bytes(int num_seqs, int num_q_heads, int num_kv_heads, int head_dim,
+                              int block_size, int max_blocks, int max_query_len);
+int prefill_drafts(const PrefillAttnArgs& a, int D, int max_query_len, void* workspace,
+                   size_t workspace_bytes, hipStream_t s);
+}  // namespace fp8
 hipError_t launch_rmsnorm(const f16* x, int64_t xs, const f16* res, int64_t rs, f16* sum,
                           int64_t ss, const f16* w, f16* y, int64_t ys, int rows, int H,
                           float eps, hipStream_t s);

@@ -1,0 +1,838 @@
+// Attention over the 8-bit paged pool (gfx950) for one query token per sequence, or a few.
+//
+//   o = sum_t p_t v_t / sum_t p_t,  p_t = 2^(scale log2(e) q.k_t - m),  m the maximum
+//   so far, K and V rows = e4m3 code * scale[block, kv head]
+//
+// Work split. The work is a list of (sequence, group of HG adjacent kv heads) pairs, each
+// of its 32-token chunks plus a fixed cost; a grid of a few workgroups per compute unit
+// takes equal contiguous ranges of it, so every workgroup reads about the same bytes
+// however lengths differ. Each wavefront derives the plan for itself, from the lengths,
+// with lane scans: no memory, no barrier. Where every pair is short a workgroup takes one
+// pair whole and there is no plan. Within a pair's part of its range, a workgroup's four
+// wavefronts take the chunks in turn, each with its own online softmax for the whole
+// query group, and meet in LDS at the end. A pair inside one range is written as fp16
+// there; a pair cut by range boundaries leaves fp32 partial records, and the last of its
+// workgroups to arrive combines them by log-sum-exp in list order (the same bits on
+// every run).
+//
+// Per chunk. K and V codes go from memory straight into LDS (buffer_load ... lds), whole
+// rows of HG heads by neighbouring lanes: no registers are held while they are on their
+// way, which leaves room for sixteen wavefronts per compute unit with 8 KB each in flight
+// (a gather of 2 KB blocks needs about 128 KB per compute unit to reach this memory's
+// rate). From there K is read in the operand layout of S^T = K Q^T and V by transposing
+// reads of bytes (ds_read_b64_tr_b8) in that of O^T += V^T P^T, both
+// v_mfma_f32_16x16x32_f16. Codes become fp16 in v_cvt_scalef32_pk_f16_fp8 with the scale
+// applied, exactly: the products and sums are those of an fp16 cache that holds the same
+// values. All fragments are in registers before the next chunk's loads are issued into
+// the same LDS, and the arithmetic runs under those loads. Each wavefront has its own LDS,
+// without barriers. The 16-byte pieces of a row are permuted by the row's number (by the
+// lanes' addresses when loading), so that neither kind of read meets a bank twice.
+//
+// Probabilities are rounded to fp16 (the denominators sum the rounded ones), scaled by
+// 2^14 so that they keep 11 bits down to 2^-28 of the largest: half a step, 2^-12
+// relative, next to the cache's own rounding of up to 2^-4.
+//
+// A few tokens per sequence (MULTI: drafts to be checked). The (token, query head) columns
+// of one sequence and kv head, token-major, fill up to CB blocks of 16, which share every
+// K and V fragment; a column sees the keys up to its token's position. A NaN in a V row
+// reaches only the columns that see it: where some column does not see the whole chunk,
+// NaN codes are cleared and the probabilities of their tokens become NaN instead.
+#pragma once
+
+#include <type_traits>
+
+#include "pa_fp8.h"
+#include "pa_tiles.h"
+
+namespace pa {
+namespace fp8 {
+
+using namespace tiles;
+
+constexpr int kChunk = 32;  // tokens a wavefront takes at a time
+// The workspace starts with arrival counters at the same place for every call, one per
+// pair of a call that is cut into ranges.
+constexpr int kMaxCounters = 16384;
+constexpr size_t kCounterBytes = (size_t)kMaxCounters * sizeof(int);
+constexpr float kBias = 14.f;  // log2 of the factor on the probabilities
+
+struct DecodeFp8Args {
+  const f16* q;
+  int64_t q_sb, q_sh;
+  const uint8_t* k;
+  int64_t k_sb, k_st, k_sh;
+  const uint8_t* v;
+  int64_t v_sb, v_st, v_sh;
+  const float* ks;
+  int64_t ks_sb, ks_sh;
+  const float* vs;
+  int64_t vs_sb, vs_sh;
+  const int32_t* bt;
+  int64_t bt_sb, bt_sk;
+  const int32_t* lens;
+  f16* out;
+  int64_t o_sb, o_sh;
+  int* cnt;
+  float* recs;
+  int num_seqs, hkv, g, bs, num_blocks, max_blocks;
+  // MULTI: first query row of each sequence, query rows, and the most a sequence may have.
+  const int32_t* qstart;
+  int num_tokens, max_new;
+  int ranged;      // 0: one workgroup per pair, no plan
+  int min_range;   // list positions a range has at least
+  int pair_cost;   // list positions a pair takes beside its chunks
+  int rec_floats;
+  float scale_log2;
+};
+
+// Floats of a partial record: heads x dim accumulators, then maxima and denominators.
+__host__ __device__ inline int record_size(int heads, int D) { return (heads * (D + 2) + 3) & ~3; }
+
+// A T-position list cut into G ranges that differ by one position at most: the first T % G
+// hold T / G + 1. Where range w starts, and the range that holds position x.
+struct Cut {
+  int q, r;
+  __device__ int start(int w) const { return w * q + (w < r ? w : r); }
+  __device__ int of(int x) const {
+    const int head = r * (q + 1);
+    return x < head ? x / (q + 1) : r + (x - head) / q;
+  }
+};
+
+// Lane l's value, in a scalar register.
+__device__ inline float lane_value(float x, int l) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), l));
+}
+
+typedef __attribute__((address_space(3))) void* lds_ptr;
+typedef __attribute__((address_space(1))) const void* global_ptr;
+
+// 16 bytes of every lane from memory into LDS, lane by lane from `to` (uniform) on, with
+// load_tile's cache policy; through a resource, or from a lane's own address.
+__device__ inline void load_to_lds(__amdgpu_buffer_rsrc_t r, uint32_t lane_off, uint8_t* to) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)to, 16, (int)lane_off, 0, 0, 3);
+}
+__device__ inline void load_to_lds(const uint8_t* from, uint8_t* to) {
+  __builtin_amdgcn_global_load_lds((global_ptr)from, (lds_ptr)to, 16, 0, 3);
+}
+
+// Transposing LDS read of bytes: within each group of 16 lanes, lane 2 r + q supplies the
+// address of bytes [8 q, 8 q + 8) of row r of an 8 x 16 block, and lane j receives column j
+// (rows 0 .. 7).
+__device__ inline uint2 lds_read_tr8(const uint8_t* p) {
+  typedef int v2i __attribute__((__vector_size__(8)));
+  auto* lp = (__attribute__((address_space(3))) v2i*)(const_cast<uint8_t*>(p));
+  return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr8_b64_v2i32(lp));
+}
+
+// op over lanes l, l ^ 16, l ^ 32 and l ^ 48, in all four. (The swaps exchange rows of 16 or
+// 32 lanes between two registers: the copy has to be one of its own.)
+template <typename Op>
+__device__ inline float over_groups(float x, Op op) {
+  auto bits = [](float v) { return __builtin_bit_cast(unsigned, v); };
+  auto val = [](unsigned u) { return __builtin_bit_cast(float, u); };
+  unsigned copy = bits(x);
+  asm volatile("" : "+v"(copy));
+  const auto a = __builtin_amdgcn_permlane16_swap(bits(x), copy, false, false);
+  const float y = op(val(a[0]), val(a[1]));
+  copy = bits(y);
+  asm volatile("" : "+v"(copy));
+  const auto b = __builtin_amdgcn_permlane32_swap(bits(y), copy, false, false);
+  return op(val(b[0]), val(b[1]));
+}
+
+// op over the 16 lanes of a row, in all of them (rotations within the row).
+template <typename Op>
+__device__ inline float over_row(float x, Op op) {
+  auto turned = [](float v, auto by) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v),
+                                                                 0x120 + decltype(by)::value, 0xf,
+                                                                 0xf, false));
+  };
+  x = op(x, turned(x, std::integral_constant<int, 8>()));
+  x = op(x, turned(x, std::integral_constant<int, 4>()));
+  x = op(x, turned(x, std::integral_constant<int, 2>()));
+  return op(x, turned(x, std::integral_constant<int, 1>()));
+}
+__device__ inline unsigned or_over_row(unsigned x) {
+  x |= (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x128, 0xf, 0xf, false);
+  x |= (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x124, 0xf, 0xf, false);
+  x |= (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x122, 0xf, 0xf, false);
+  return x | (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x121, 0xf, 0xf, false);
+}
+struct Max {
+  __device__ float operator()(float a, float b) const { return fmaxf(a, b); }
+};
+struct Sum {
+  __device__ float operator()(float a, float b) const { return a + b; }
+};
+
+// The permutation of a row's 16-byte pieces in LDS: piece p of chunk row r lies in slot
+// p ^ swizzle(r) of NP. Eight rows whose same piece is read at once, 0 .. 7 (V) or 0 .. 3
+// and 8 .. 11 (K), then lie in different banks.
+template <int NP>
+__device__ inline int swizzle(int r) {
+  const int f = (r & 3) | (((r >> 2) ^ (r >> 3)) & 1) << 2;
+  return NP >= 8 ? f : NP == 4 ? f >> 1 : f >> 2;
+}
+
+// Wavefronts per SIMD that the registers are kept to.
+constexpr int waves_per_simd(int D, int NW, int CB) {
+  return D == 256 || CB > 1 ? 2 : NW > 4 ? 4 : 3;
+}
+
+// NW: wavefronts of a workgroup. One token per sequence: a block of 16 columns for each of
+// HG heads; MULTI: CB blocks of one head.
+template <int D, int HG, int BS, int NW, int CB, bool MULTI>
+__global__ __launch_bounds__(64 * NW, waves_per_simd(D, NW, CB)) void attend_fp8_kernel(DecodeFp8Args a) {
+  static_assert(MULTI ? HG == 1 : CB == 1, "column blocks of one head, or one of each head");
+  constexpr int NS = HG * CB;  // blocks of 16 columns, each with its online softmax
+  constexpr int kThreads = 64 * NW;
+  constexpr int RB = HG * D;            // bytes of a loaded row
+  constexpr int NP = RB / 16;           // 16-byte pieces of it, one per lane
+  constexpr int RPI = 64 / NP;          // rows per load instruction
+  constexpr int NI = kChunk / RPI;      // load instructions per chunk, for K and for V
+  // Whether an instruction's rows lie in one block: their address is then uniform.
+  constexpr bool UNIFORM = BS > 0 && RPI <= 16;
+  static_assert(BS % 16 == 0, "whole tiles per block, or any block size as 0");
+  constexpr int FB = D >= 64 ? 16 : 8;  // bytes of one lane's K fragment read
+  constexpr int SEG = D / (4 * FB);     // such reads per head and 16-token tile
+  constexpr int NF = FB / 8;            // MFMA operands of one
+  constexpr int NC = D / 32;            // products per score tile
+  constexpr int ND = D / 16;
+  constexpr int D4 = D / 4;
+  constexpr int STAGE = 2 * kChunk * RB;  // bytes per wavefront: K rows, then V rows
+  static_assert(STAGE == HG * 16 * D * 4, "the accumulators take the same room");
+  typedef unsigned frag __attribute__((ext_vector_type(FB / 4)));
+  __shared__ __attribute__((aligned(16))) uint8_t s_stage[NW * STAGE];
+  __shared__ __attribute__((aligned(16))) f32x4 s_part[kThreads];
+  __shared__ float s_m[NW][NS * 16], s_l[NW][NS * 16];
+  // Scales per token where they are not uniform: fp32 of K, fp16 of V.
+  __shared__ float s_ks[UNIFORM ? 1 : NW][HG * kChunk];
+  __shared__ __attribute__((aligned(16))) f16 s_vs[UNIFORM ? 1 : NW][HG * kChunk];
+  __shared__ int s_last;
+
+  const int tid = threadIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lane = tid & 63;
+  const int row = lane & 15;
+  const int grp = lane >> 4;
+  const int bs = BS > 0 ? BS : a.bs;
+  const int groups = a.hkv / HG;
+  const int cap = a.max_blocks * bs;
+  const int last_tile = (cap - 1) / 16;
+  uint8_t* const stage = s_stage + wave * STAGE;
+  // This lane's piece of a loaded row: row lrow of the instruction's. (The swizzle of rows
+  // 8 on differs by 4 from that of the rows before; a row of 16 pieces takes instructions of
+  // four rows, whose swizzles differ by 4 every second one.) Byte offsets, for both.
+  const int lrow = lane / NP;
+  auto piece = [&](int flip) { return ((lane % NP) ^ swizzle<NP>(lrow) ^ flip) * 16; };
+  constexpr int FLIP = NP >= 8 ? 4 : 0;
+  auto lane_offset = [&](int64_t st, int64_t sh, int flip) {
+    const int c = piece(flip);
+    return (uint32_t)(lrow * st + c / D * sh + c % D);
+  };
+  const uint32_t k_lane = lane_offset(a.k_st, a.k_sh, 0), k_flip = lane_offset(a.k_st, a.k_sh, FLIP);
+  const uint32_t v_lane = lane_offset(a.v_st, a.v_sh, 0), v_flip = lane_offset(a.v_st, a.v_sh, FLIP);
+  // Whether instruction i's rows have the flipped swizzle: bits 2 and 3 of i * RPI (those of
+  // lrow are in swizzle(lrow)).
+  auto flipped = [](int i) { return ((i * RPI >> 2) ^ (i * RPI >> 3)) & 1; };
+  constexpr int kAll = 0x7fffffff;
+
+  auto clamped = [&](int n) { return n < 0 ? 0 : (n > cap ? cap : n); };
+  auto chunks_of = [&](int n) { return (clamped(n) + kChunk - 1) / kChunk; };
+
+  // Chunks [c0, c1) of pair (b, group from kv head h0) of a sequence of L tokens (not ranged:
+  // all chunks, of a length found here, while the first ids are on their way). The pair is
+  // spread over nseg workgroups' ranges, from range w0 on; this is its part `seg`.
+  auto segment = [&](int b, int h0, int L, int c0, int c1, int w0, int seg, int nseg) {
+    const int32_t* btrow = a.bt + (int64_t)b * a.bt_sb;
+    // The columns of the pair: its query heads, or times its tokens.
+    int q0 = b, qall = 1, heads = HG * a.g;
+    if constexpr (MULTI) {
+      q0 = min(max(load_uniform(a.qstart + b), 0), a.num_tokens);
+      qall = min(max(load_uniform(a.qstart + b + 1), q0), a.num_tokens) - q0;
+      heads = min(qall, a.max_new) * a.g;
+      if (heads == 0) return;  // (in every workgroup of the pair)
+    }
+    // UNIFORM: the block ids of the chunk's two tiles; else those of the lane's row of each
+    // load, and of token lane % 32 (for the scales).
+    constexpr int NID = UNIFORM ? 2 : NI + 1;
+    int ids[NID];
+    // Clamped to the table's width only, so that ids need no length: a tile past the end
+    // reads some block of the pool and what it reads is masked.
+    auto load_ids = [&](int c) {
+#pragma unroll
+      for (int i = 0; i < NID; ++i) {
+        if constexpr (UNIFORM) {
+          const int at = min(2 * c + i, last_tile);
+          ids[i] = load_uniform(btrow + (int64_t)(at / (BS / 16)) * a.bt_sk);
+        } else {
+          const int t = i < NI ? i * RPI + lrow : lane & 31;
+          ids[i] = btrow[(int64_t)(min(c * kChunk + t, cap - 1) / bs) * a.bt_sk];
+        }
+      }
+    };
+    const int first = c0 + wave;
+    load_ids(first);
+    // Q^T operands: column = query head `row` of a kv head's group, elements in the order
+    // of the K operands; of the scale's sign, so that the largest product has the largest
+    // score.
+    const f16 sign = a.scale_log2 < 0.f ? (f16)-1.f : (f16)1.f;
+    f16x8 qf[NS][NC];
+    int token[NS];  // MULTI: the column's token
+#pragma unroll
+    for (int st = 0; st < NS; ++st) {
+      int64_t at;  // of the query row and head
+      if constexpr (MULTI) {
+        const int col = min(st * 16 + row, heads - 1);
+        token[st] = col / a.g;
+        at = (int64_t)(q0 + token[st]) * a.q_sb + (int64_t)(h0 * a.g + col - token[st] * a.g) * a.q_sh;
+      } else {
+        at = (int64_t)b * a.q_sb + (int64_t)((h0 + st) * a.g + min(row, a.g - 1)) * a.q_sh;
+      }
+#pragma unroll
+      for (int s = 0; s < SEG; ++s)
+#pragma unroll
+        for (int f = 0; f < NF; ++f)
+          qf[st][s * NF + f] =
+              sign * *reinterpret_cast<const f16x8*>(a.q + at + s * 4 * FB + grp * FB + f * 8);
+    }
+    // Issues a chunk's loads. UNIFORM: its scales by one vector load (scalar ones would make
+    // LDS reads wait for their misses), lane t + 2 hg + 4 (0: keys, 1: values) for tile t;
+    // else lane (token, head) those of token lane % 32.
+    float scales = 1.f, vscales = 1.f;
+    auto issue = [&](int c) {
+      if constexpr (UNIFORM) {
+        const int id0 = ids[0], id1 = ids[1];
+        const int64_t id = min(max(lane & 1 ? id1 : id0, 0), a.num_blocks - 1);
+        const int64_t h = h0 + (HG > 1 ? lane >> 1 & 1 : 0);
+        const float* kp = a.ks + id * a.ks_sb + h * a.ks_sh;
+        const float* vp = a.vs + id * a.vs_sb + h * a.vs_sh;
+        scales = *(lane & 4 ? vp : kp);
+      } else {
+        const int64_t id = min(max(ids[NID - 1], 0), a.num_blocks - 1);
+        const int64_t h = h0 + (HG > 1 ? lane >> 5 : 0);
+        scales = a.ks[id * a.ks_sb + h * a.ks_sh];
+        vscales = a.vs[id * a.vs_sb + h * a.vs_sh];
+      }
+      auto load_rows = [&](const uint8_t* base, int64_t sb, int64_t st, int64_t sh, uint32_t plain,
+                           uint32_t flip, uint8_t* to) {
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+          const int64_t id = min(max(ids[UNIFORM ? i * RPI / 16 : i], 0), a.num_blocks - 1);
+          if constexpr (UNIFORM) {
+            const int64_t off = (2 * c + i * RPI / 16) % (BS / 16) * 16 + i * RPI % 16;
+            load_to_lds(tile_rsrc(base + id * sb + off * st + h0 * sh, kAll), flipped(i) ? flip : plain,
+                        to + i * 1024);
+          } else {
+            const int64_t off = (c * kChunk + i * RPI + lrow) % bs;
+            const int p = piece(flipped(i) ? FLIP : 0);
+            load_to_lds(base + id * sb + off * st + (h0 + p / D) * sh + p % D, to + i * 1024);
+          }
+        }
+      };
+      load_rows(a.k, a.k_sb, a.k_st, a.k_sh, k_lane, k_flip, stage);
+      load_rows(a.v, a.v_sb, a.v_st, a.v_sh, v_lane, v_flip, stage + kChunk * RB);
+    };
+
+    if (!a.ranged) {
+      L = clamped(load_uniform(a.lens + b));
+      c1 = (L + kChunk - 1) / kChunk;
+    }
+    // The last position each column sees, and how many all of them see.
+    int last[NS];
+#pragma unroll
+    for (int st = 0; st < NS; ++st) last[st] = MULTI ? L - qall + token[st] : L - 1;
+    const int all_see = MULTI ? L - qall + 1 : L;
+    float m_run[NS], l_run[NS];
+    f32x4 acc[NS][ND];
+#pragma unroll
+    for (int st = 0; st < NS; ++st) {
+      m_run[st] = kNegInf;
+      l_run[st] = 0.f;
+#pragma unroll
+      for (int nd = 0; nd < ND; ++nd) acc[st][nd] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    if (first < c1) {
+      issue(first);
+      load_ids(first + NW);
+    }
+    const float scale = fabsf(a.scale_log2);
+    for (int c = first; c < c1; c += NW) {
+      const int t0 = c * kChunk;
+      const bool whole = t0 + kChunk <= all_see;  // wavefront-uniform: the last may not be
+      // The chunk has landed; all of it into registers. Tile t's score row m is token
+      // 8 (m / 4) + 4 t + m % 4: lane (., grp) then gets the scores of tokens 8 grp .. + 7,
+      // those of its V fragments.
+      __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+      wave_lds_fence();
+      frag kf[2][HG][SEG];
+      uint2 vf[HG][ND];
+      float kfs[2][HG];  // K scales of the lane's fragments
+      float vfs[HG];     // V scale of the lane's tokens,
+      f16x8 vft[HG];     // or one for each
+      if constexpr (UNIFORM) {
+#pragma unroll
+        for (int hg = 0; hg < HG; ++hg) {
+          // (A tile past the end has some block's scale: its codes are cleared below.)
+          const float v0 = lane_value(scales, 2 * hg + 4);
+          const float v1 = t0 + 16 < L ? lane_value(scales, 2 * hg + 5) : 1.f;
+          vfs[hg] = grp < 2 ? v0 : v1;
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            // Score rows 0 .. 7 of either are tokens of the block's first half.
+            const float s0 = lane_value(scales, 2 * hg), s1 = lane_value(scales, 2 * hg + 1);
+            kfs[t][hg] = row < 8 ? s0 : s1;
+          }
+        }
+      } else {
+        const int t = lane & 31, hg = HG > 1 ? lane >> 5 : 0;
+        s_ks[wave][hg * kChunk + t] = scales;
+        s_vs[wave][hg * kChunk + t] = (f16)(t0 + t < L ? vscales : 1.f);
+        wave_lds_fence();
+      }
+#pragma unroll
+      for (int hg = 0; hg < HG; ++hg) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const int r = 8 * (row >> 2) + 4 * t + (row & 3);
+#pragma unroll
+          for (int s = 0; s < SEG; ++s) {
+            const int at = hg * D + s * 4 * FB + grp * FB;  // byte of the row
+            kf[t][hg][s] = *reinterpret_cast<const frag*>(
+                stage + r * RB + ((at / 16) ^ swizzle<NP>(r)) * 16 + at % 16);
+          }
+          if constexpr (!UNIFORM) kfs[t][hg] = s_ks[wave][hg * kChunk + r];
+        }
+        const int r = 8 * grp + (row >> 1);
+        const uint8_t* vp = stage + kChunk * RB + r * RB + (row & 1) * 8;
+#pragma unroll
+        for (int nd = 0; nd < ND; ++nd)
+          vf[hg][nd] = lds_read_tr8(vp + ((hg * ND + nd) ^ swizzle<NP>(r)) * 16);
+        if constexpr (!UNIFORM)
+          vft[hg] = *reinterpret_cast<const f16x8*>(&s_vs[wave][hg * kChunk + 8 * grp]);
+      }
+      wave_lds_fence();
+      __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): nothing reads the LDS any more
+      if (c + NW < c1) {
+        issue(c + NW);
+        load_ids(c + 2 * NW);
+      }
+      unsigned nan_lo = 0, nan_hi = 0;  // MULTI: bit 8 i + 7, token 8 grp + i has a NaN in V
+      if (!whole) {
+        // Codes of rows past the end as 0: 0 * what lies there is never NaN.
+        const int n = L - t0 - 8 * grp;  // the lane's tokens that count
+        const unsigned lo = n >= 4 ? ~0u : n <= 0 ? 0u : (1u << 8 * n) - 1;
+        const unsigned hi = n >= 8 ? ~0u : n <= 4 ? 0u : (1u << 8 * (n - 4)) - 1;
+#pragma unroll
+        for (int hg = 0; hg < HG; ++hg)
+#pragma unroll
+          for (int nd = 0; nd < ND; ++nd) {
+            vf[hg][nd].x &= lo;
+            vf[hg][nd].y &= hi;
+            if constexpr (MULTI) {
+              // The top bit of every byte that holds 0x7f or 0xff.
+              const unsigned x = ((vf[hg][nd].x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+              const unsigned y = ((vf[hg][nd].y & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+              nan_lo |= x;
+              nan_hi |= y;
+              vf[hg][nd].x &= ~((x >> 7) * 0xffu);
+              vf[hg][nd].y &= ~((y >> 7) * 0xffu);
+            }
+          }
+        if constexpr (MULTI) {
+          nan_lo = or_over_row(nan_lo);
+          nan_hi = or_over_row(nan_hi);
+        }
+      }
+#pragma unroll
+      for (int st = 0; st < NS; ++st) {
+        const int hg = MULTI ? 0 : st;
+        float x[2][4];
+        float m = kNegInf;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          f32x4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int i = 0; i < SEG; ++i)
+#pragma unroll
+            for (int f = 0; f < NF; ++f)
+              s = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                  from_codes8(kf[t][hg][i][2 * f], kf[t][hg][i][2 * f + 1], kfs[t][hg]),
+                  qf[st][i * NF + f], s, 0, 0, 0);
+          if (!whole) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (t0 + 8 * grp + 4 * t + r > last[st]) s[r] = kNegInf;
+          }
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            x[t][r] = s[r];
+            m = fmaxf(m, s[r]);
+          }
+        }
+        // (A column that has seen nothing yet stays at -inf, whatever the scale: 0 * -inf
+        // would be NaN.)
+        m = over_groups(m, Max());
+        const float m_new = m == kNegInf ? m_run[st] : fmaxf(m_run[st], m * scale);
+        if (__ballot(m_new > m_run[st]) != 0) {  // wavefront-uniform
+          const float alpha = m_new == kNegInf ? 1.f : fast_exp2(m_run[st] - m_new);
+          l_run[st] *= alpha;
+#pragma unroll
+          for (int nd = 0; nd < ND; ++nd) acc[st][nd] *= alpha;
+          m_run[st] = m_new;
+        }
+        const float off = kBias - m_run[st];
+        f16x8 pb;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            float p = fast_exp2(__builtin_fmaf(x[t][r], scale, off));
+            if (!whole) {
+              if constexpr (MULTI)
+                if ((t ? nan_hi : nan_lo) >> (8 * r + 7) & 1) p = __builtin_nanf("");
+              if (t0 + 8 * grp + 4 * t + r > last[st]) p = 0.f;
+            }
+            pb[4 * t + r] = (f16)p;
+          }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          l_run[st] = __builtin_amdgcn_fdot2(f16x2{pb[2 * i], pb[2 * i + 1]},
+                                             f16x2{(f16)1.f, (f16)1.f}, l_run[st], false);
+        // O^T += V^T P^T: operand index k = 8 grp + i stands for token 8 grp + i on both sides.
+#pragma unroll
+        for (int nd = 0; nd < ND; ++nd) {
+          f16x8 av;
+          if constexpr (UNIFORM)
+            av = from_codes8(vf[hg][nd].x, vf[hg][nd].y, vfs[hg]);
+          else
+            av = from_codes8(vf[hg][nd].x, vf[hg][nd].y, 1.f) * vft[hg];
+          acc[st][nd] = __builtin_amdgcn_mfma_f32_16x16x32_f16(av, pb, acc[st][nd], 0, 0, 0);
+        }
+      }
+    }
+
+    // The wavefronts' states meet in LDS, HG blocks of columns at a time, four elements of
+    // accumulator row r at slot (d / 4) ^ (r & 7). (Lane indices anew: see fresh_lane.)
+    const int lane = fresh_lane();
+    const int tid = wave * 64 + lane, row = lane & 15, grp = lane >> 4;
+    // Part i of a cut pair lies in range w0 + i's slot 0 (the pair began before that range)
+    // or, i = 0, in slot 1.
+    const int64_t rec0 = (int64_t)(2 * w0 + 1) * a.rec_floats;
+    auto record = [&](int i) { return (i ? 2 * i - 1 : 0) * a.rec_floats; };  // from rec0
+    const auto rr = tile_rsrc(a.recs + rec0, (2 * nseg - 1) * a.rec_floats * 4);
+    const int rb = record(seg) * 4;
+    auto out_row = [&](int j) {  // of column j
+      const int t = MULTI ? j / a.g : 0;
+      return a.out + (int64_t)(q0 + t) * a.o_sb + (int64_t)(h0 * a.g + j - t * a.g) * a.o_sh;
+    };
+    float* my_acc = reinterpret_cast<float*>(stage);
+#pragma unroll
+    for (int cb = 0; cb < CB; ++cb) {
+      if (cb * 16 >= heads && MULTI) break;  // workgroup-uniform
+      if (cb) __syncthreads();
+#pragma unroll
+      for (int hg = 0; hg < HG; ++hg) {
+        const int st = MULTI ? cb : hg;
+        const float l = over_groups(l_run[st], Sum());
+        if (grp == 0) {
+          s_m[wave][st * 16 + row] = m_run[st];
+          s_l[wave][st * 16 + row] = l;
+        }
+        if (MULTI || row < a.g) {
+#pragma unroll
+          for (int nd = 0; nd < ND; ++nd)
+            *reinterpret_cast<f32x4*>(my_acc + (hg * 16 + row) * D +
+                                      ((nd * 4 + grp) ^ (row & 7)) * 4) = acc[st][nd];
+        }
+      }
+      __syncthreads();
+      const int count = MULTI ? min(16, heads - cb * 16) : heads;
+      for (int i = tid; i < count * D4; i += kThreads) {
+        const int k = i / D4;
+        const int d = (i - k * D4) * 4;
+        const int r = HG > 1 && k >= a.g ? 16 + k - a.g : k;  // row of the accumulators
+        const int j = cb * 16 + k;
+        float M = s_m[0][cb * 16 + r];
+#pragma unroll
+        for (int w = 1; w < NW; ++w) M = fmaxf(M, s_m[w][cb * 16 + r]);
+        float l = 0.f;
+        f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+          // A state of no maximum holds zeros, or NaN that has to show.
+          const float m = s_m[w][cb * 16 + r];
+          const float f = m == kNegInf ? 1.f : fast_exp2(m - M);
+          l += f * s_l[w][cb * 16 + r];
+          o += f * *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(s_stage + w * STAGE) +
+                                                   r * D + ((d >> 2) ^ (r & 7)) * 4);
+        }
+        if (nseg == 1) {
+          const float inv = l == 0.f ? 0.f : 1.f / l;  // 0: no key at all
+          f16x4 y;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) y[e] = (f16)(o[e] * inv);
+          *reinterpret_cast<f16x4*>(out_row(j) + d) = y;
+        } else {
+          store_coherent16(rr, rb + (j * D + d) * 4, o);
+          if (d == 0) {
+            __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, M), rr,
+                                                  rb + (heads * D + j) * 4, 0, 16);
+            __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, l), rr,
+                                                  rb + (heads * D + heads + j) * 4, 0, 16);
+          }
+        }
+      }
+    }
+    if (nseg == 1) {
+      __syncthreads();  // the next segment stages where this one's states lie
+      return;
+    }
+    int* cnt = a.cnt + (int64_t)b * groups + h0 / HG;
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+    __builtin_amdgcn_s_waitcnt(0);  // the record has landed before the arrival counts
+    __syncthreads();
+    if (tid == 0)
+      s_last = __hip_atomic_fetch_add(cnt, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == nseg - 1;
+    __syncthreads();
+    if (!s_last) return;  // (the next segment writes s_last behind further barriers)
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
+
+    // Merge: every part's maxima and denominators into LDS (batches of parts, as many as
+    // fit), their maximum and sum per head by 16 lanes each, and the accumulators by
+    // threads (item: head and four of its elements; the parts of an item are dealt over as
+    // many threads as there are for it), U parts a round trip, the first ones on their way
+    // before anything else. Part 0 lies apart from the others, which are two records apart.
+    float* s_max = s_m[0];  // (the wavefronts' states are spent)
+    float* s_sum = s_l[0];
+    const int batch = min(nseg, (int)(sizeof(s_stage) / 8) / heads);
+    float* s_pm = reinterpret_cast<float*>(s_stage);
+    float* s_pl = s_pm + heads * batch;
+    const int items = heads * D4;
+    const int parts = items < kThreads ? kThreads / items : 1;
+    const int part = parts > 1 ? tid / items : 0;
+    const int step = 2 * a.rec_floats * 4;  // bytes from part i to part i + 1, i > 0
+    constexpr int U = NW > 4 ? 8 : 16;
+    auto fetch = [&](int i, int j, int d, f32x4 (&y)[U]) {  // past the last part: zeros
+      const int at = (record(i) + j * D + d) * 4;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        y[u] = __builtin_bit_cast(
+            f32x4, __builtin_amdgcn_raw_buffer_load_b128(rr, at, u * parts * step, 16));
+    };
+    // (As above: no maximum, and so zeros or NaN.)
+    auto share = [&](float m, float M) { return m == kNegInf ? 1.f : fast_exp2(m - M); };
+    auto load_ml = [&](int s0, int s1) {
+#pragma unroll 2
+      for (int i = tid; i < heads * (s1 - s0); i += kThreads) {
+        const int j = i / (s1 - s0);
+        const int k = i - j * (s1 - s0);
+        const int at = (record(s0 + k) + heads * D) * 4;
+        s_pm[j * batch + k] = load_coherent4(rr, at + j * 4);
+        s_pl[j * batch + k] = load_coherent4(rr, at + (heads + j) * 4);
+      }
+    };
+#pragma unroll 1
+    for (int base = 0; base < items; base += kThreads) {  // workgroup-uniform
+      const int item = parts > 1 ? tid - part * items : base + tid;
+      const bool live = part < parts && item < items;
+      const int j = live ? item / D4 : 0;
+      const int d = live ? (item - j * D4) * 4 : 0;
+      f32x4 y[U];
+      const f32x4 y0 = load_coherent16(rr, (j * D + d) * 4);
+      fetch(1 + part, j, d, y);
+      if (base == 0) {
+#pragma unroll 1
+        for (int s0 = 0; s0 < nseg; s0 += batch) {
+          const int s1 = min(nseg, s0 + batch);
+          if (s0) __syncthreads();
+          load_ml(s0, s1);
+          __syncthreads();
+#pragma unroll 1
+          for (int jj = tid / 16; jj < heads; jj += kThreads / 16) {
+            const float had = s0 ? s_max[jj] : kNegInf;
+            float M = had;
+            for (int i = row; i < s1 - s0; i += 16) M = fmaxf(M, s_pm[jj * batch + i]);
+            M = over_row(M, Max());
+            float sum = 0.f;
+            for (int i = row; i < s1 - s0; i += 16) sum += s_pl[jj * batch + i] * share(s_pm[jj * batch + i], M);
+            sum = over_row(sum, Sum());
+            if (s0) sum += s_sum[jj] * share(had, M);
+            if (row == 0) {
+              s_max[jj] = M;
+              s_sum[jj] = sum;
+            }
+          }
+        }
+        __syncthreads();
+      }
+      const float M = s_max[j];
+      f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+      for (int s0 = 0; s0 < nseg; s0 += batch) {
+        const int s1 = min(nseg, s0 + batch);
+        if (batch < nseg) {  // the batch's maxima again
+          __syncthreads();
+          load_ml(s0, s1);
+          __syncthreads();
+        }
+        if (live) {
+          const float* pm = s_pm + j * batch - s0;
+          if (s0 == 0 && part == 0) o += share(pm[0], M) * y0;
+#pragma unroll 1
+          for (int i = s0 ? s0 + part : 1 + part; i < s1; i += U * parts) {
+            if (i != 1 + part) fetch(i, j, d, y);
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+              if (i + u * parts < s1) o += share(pm[i + u * parts], M) * y[u];
+          }
+        }
+      }
+      if (parts > 1) {
+        s_part[tid] = o;
+        __syncthreads();
+        if (part == 0)
+          for (int p = 1; p < parts; ++p) o += s_part[item + p * items];
+      }
+      if (live && part == 0) {
+        const float sum = s_sum[j];
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;  // 0: no key at all
+        f16x4 z;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) z[e] = (f16)(o[e] * inv);
+        *reinterpret_cast<f16x4*>(out_row(j) + d) = z;
+      }
+    }
+    if (tid == 0) __hip_atomic_store(cnt, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+  };
+
+  // This workgroup's part of the list: positions [x0, x1); `at` is the first of sequence b.
+  Cut ranges{0, 0};
+  int x0 = 0, x1 = 0, at = 0, b = 0, g0 = 0, w = 0;
+  // Lengths of 256 sequences a time, sequence base + 64 k + lane in lens[k]: read together.
+  constexpr int LK = 4;
+  int lens[LK] = {0, 0, 0, 0}, own[LK], incl[LK];
+  if (a.ranged) {
+    // Each sequence takes groups x (its chunks + pair_cost) positions. (The host sees to it
+    // that 31 bits hold their sum.)
+    auto take = [&](int base) {
+#pragma unroll
+      for (int k = 0; k < LK; ++k) lens[k] = a.lens[min(base + 64 * k + lane, a.num_seqs - 1)];
+#pragma unroll
+      for (int k = 0; k < LK; ++k) {
+        lens[k] = clamped(lens[k]);
+        own[k] = base + 64 * k + lane < a.num_seqs ? groups * (chunks_of(lens[k]) + a.pair_cost) : 0;
+        incl[k] = wave_incl_scan(own[k]);
+      }
+    };
+    int T = 0;
+    for (int base = 0; base < a.num_seqs; base += 64 * LK) {
+      take(base);
+#pragma unroll
+      for (int k = 0; k < LK; ++k) T += __builtin_amdgcn_readlane(incl[k], 63);
+    }
+    const int G = max(1, min((int)gridDim.x, T / a.min_range));
+    if ((int)blockIdx.x >= G) return;
+    w = xcd_order(blockIdx.x, G);
+    ranges = Cut{T / G, T % G};
+    x0 = ranges.start(w);
+    x1 = ranges.start(w + 1);
+    // The sequence that holds x0, and its first position.
+    bool found = false;
+    for (int base = 0; base < a.num_seqs && !found; base += 64 * LK) {
+      if (a.num_seqs > 64 * LK) take(base);
+#pragma unroll
+      for (int k = 0; k < LK; ++k) {
+        const int total = __builtin_amdgcn_readlane(incl[k], 63);
+        if (!found && at + total > x0) {
+          const int l = (int)__builtin_ctzll(__ballot(at + incl[k] > x0));
+          b = base + 64 * k + l;
+          at += __builtin_amdgcn_readlane(incl[k] - own[k], l);
+          found = true;
+        }
+        if (!found) at += total;
+      }
+    }
+  } else {
+    const int pair = xcd_order(blockIdx.x, gridDim.x);
+    b = pair / groups;
+    g0 = pair - b * groups;
+  }
+  for (;;) {
+    int L = 0;
+    if (a.ranged && a.num_seqs <= 64 * LK) {
+#pragma unroll
+      for (int k = 0; k < LK; ++k)
+        if (b / 64 == k) L = __builtin_amdgcn_readlane(lens[k], b % 64);
+    } else if (a.ranged) {
+      L = clamped(load_uniform(a.lens + b));
+    }
+    const int n = (L + kChunk - 1) / kChunk;
+    int c0 = 0, c1 = n, w0 = 0, w1 = 0;
+    if (a.ranged) {
+      // The pair's positions: pair_cost of them, then its chunks.
+      const int span = n + a.pair_cost;
+      for (; g0 < groups && at + span <= x0; ++g0) at += span;
+      if (g0 == groups) {
+        g0 = 0;
+        if (++b == a.num_seqs) return;
+        continue;
+      }
+      if (at >= x1) return;
+      c0 = max(0, min(n, x0 - at - a.pair_cost));
+      c1 = max(0, min(n, x1 - at - a.pair_cost));
+      w0 = ranges.of(at);
+      w1 = ranges.of(at + span - 1);
+      at += span;
+    }
+    segment(b, g0 * HG, L, c0, c1, w0, w - w0, w1 - w0 + 1);
+    if (!a.ranged || at >= x1) return;
+    if (++g0 == groups) {
+      g0 = 0;
+      if (++b == a.num_seqs) return;
+    }
+  }
+}
+
+// ---- launch plan, shared by the two sources that launch the kernel ----
+
+// List positions of 32 tokens: what a pair costs beside its chunks, and the fewest a
+// range takes.
+constexpr int kPairCost = 8;
+constexpr int kMinRange = 16;
+// Tables of at most this many tokens take one workgroup per pair; of the second, where
+// the pairs fill at least half the compute units.
+constexpr int kWholePairs = 1024;
+constexpr int kWholePairsBusy = 2048;
+
+struct DecodePlan {
+  int head_group, waves, ranged, grid, rec_floats;
+  size_t ws_bytes;
+
+  // The launch's part of the arguments.
+  void fill(DecodeFp8Args& a, void* workspace) const {
+    a.cnt = (int*)workspace;
+    a.recs = (float*)((char*)workspace + (ws_bytes ? kCounterBytes : 0));
+    a.ranged = ranged;
+    a.min_range = kMinRange;
+    a.pair_cost = kPairCost;
+    a.rec_floats = rec_floats;
+  }
+};
+
+// For new_tokens query tokens per sequence at most (1: the one-token form).
+DecodePlan decode_plan(int num_seqs, int num_q_heads, int num_kv_heads, int head_dim,
+                       int block_size, int max_blocks, int new_tokens);
+
+// Whether the uniform tiles' loads, which take 31-bit offsets within 16 rows of two heads,
+// serve these strides.
+inline bool near_strides(const DecodeFp8Args& a) {
+  const int64_t most = 1 << 26;
+  return a.k_st < most && a.v_st < most && a.k_sh < most && a.v_sh < most;
+}
+
+}  // namespace fp8
+}  // namespace pa

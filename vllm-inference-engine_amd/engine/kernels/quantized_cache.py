@@ -279,7 +279,7 @@ def paged_attention_prefill_fp8(
         key = ("prefill", dev.index, *sizes)
         nbytes = _ws_sizes.get(key)
         if nbytes is None:
-            nbytes = _ws_sizes[key] = lib.pa_prefill_attention_workspace_bytes(*sizes)
+            nbytes = _ws_sizes[key] = lib.pa_prefill_attention_fp8_workspace_bytes(*sizes)
         ws, _own = _native.counted_workspace(nbytes, _COUNTER_BYTES, dev, stream,
                                              _native.WS_PREFILL)
         status = lib.pa_prefill_attention_fp8(
