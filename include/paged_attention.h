@@ -598,7 +598,8 @@ PA_API int pa_prefill_attention_fp8(const void* q, const int64_t q_strides[3],
  * comparisons in 64 bits; negative weights and NaN count as 0; where rounding or
  * next_u >= 1 leaves no such index, the last index with a weight, and index 0 of a row
  * without any. accepted[b] = n; tokens [num_seqs, max_drafts + 1] int64 contiguous:
- * the n drafts, the next token, then -1. At most 16384 sequences and 64 drafts.
+ * the n drafts, the next token, then -1. At most 16384 sequences, 64 drafts and a
+ * vocabulary of 2^30.
  *
  * Workspace: its first bytes are arrival counters that must be zero before the first
  * call that uses the buffer; every call leaves them zero. One buffer per stream, lent

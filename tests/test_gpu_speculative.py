@@ -42,7 +42,7 @@ def check(*args):
 
 @pytest.mark.parametrize("seqs,k,vocab", [(1, 4, 151936), (7, 3, 32000), (64, 1, 4096), (9, 8, 4097),
                                           (5, 64, 100), (33, 5, 255), (4, 2, 1), (3, 0, 5000),
-                                          (300, 2, 17), (2, 6, 8191)])
+                                          (300, 2, 17), (2, 6, 8191), (2, 2, 600001)])
 def test_matches_oracle(cuda_device, seqs, k, vocab):
     args = case(seqs, k, vocab, seqs * 100 + k, cuda_device)
     check(*args)

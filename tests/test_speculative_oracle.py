@@ -61,8 +61,8 @@ def test_argument_errors_before_launch():
     assert _call(lib, ws=16, nbytes=lib.pa_verify_drafts_workspace_bytes(2, 100) - 1) == \
         _native.PA_ERR_WORKSPACE
     assert _call(lib, seqs=0, target=0) == _native.PA_OK
-    # Counters, then two sums per sequence and 4096 entries of the vocabulary.
-    assert lib.pa_verify_drafts_workspace_bytes(5, 151936) == 16384 * 4 + 5 * 38 * 16
+    # Counters, then two sums per sequence and 1024 entries of the vocabulary.
+    assert lib.pa_verify_drafts_workspace_bytes(5, 151936) == 16384 * 4 + 5 * 149 * 16
     assert lib.pa_verify_drafts_workspace_bytes(16385, 100) == 0
 
 

@@ -13,20 +13,23 @@
 // exact, and sums in any order agree to 2^-40 or better, so the chosen index does
 // not depend on how the row is split.
 //
-// A row of the vocabulary is split over workgroups of kChunk entries. Each finds n
-// for itself (the drafts' entries are a few loads), sums its chunk of w and of p, and
-// leaves the sums in the workspace; the last of a sequence's workgroups finds the
-// chunk in which the cumulative sum crosses u' * total and looks for the index there.
-// Bound by memory: two fp32 rows per sequence, read once (and one chunk twice).
+// A row of the vocabulary is cut into pieces of 1024 entries, one wavefront's work at a
+// time: the sums of w and of p over each piece go to the workspace. The wavefronts of a few
+// workgroups per sequence take the pieces in turn (each decides n for itself: the drafts'
+// entries are a few loads), two pieces in flight; the last of the sequence's workgroups
+// finds the piece in which the cumulative sum crosses u' * total and looks for the index
+// there. Bound by memory: two fp32 rows per sequence, read once (and one piece twice), and
+// for a few sequences by the chain drafts -> their entries -> pieces -> arrival -> sums ->
+// piece.
 #include "../../include/paged_attention.h"
-#include "pa_common.h"
+#include "pa_tiles.h"
 
 namespace pa {
 namespace verify {
 
 constexpr int kThreads = 256;
-constexpr int kPer = 16;  // entries per thread in a chunk
-constexpr int kChunk = kThreads * kPer;
+constexpr int kWaves = kThreads / 64;
+constexpr int kPiece = 1024;  // entries; 16 per lane
 constexpr int kMaxDrafts = 64;  // one per lane of a wavefront
 // The workspace starts with one arrival counter per sequence, at the same place for
 // every call.
@@ -47,14 +50,15 @@ struct Args {
   int64_t* tokens;        // [seqs, k + 1]
   int32_t* accepted;
   int* cnt;
-  double* sums;  // [seqs][chunks][2]: max(p - q, 0), p
-  int seqs, k, vocab, chunks;
+  double* sums;  // [seqs][pieces][2]: max(p - q, 0), p
+  int seqs, k, vocab, pieces;
+  int groups;  // workgroups per sequence
 };
 
 struct Weights {
   const float* p;
   const float* q;      // null: nothing is taken off
-  int64_t certain;     // with q null: the index whose weight is 0, or -1
+  int certain;     // with q null: the index whose weight is 0, or -1
 };
 
 // Weight of entry v. Negative numbers and NaN count as 0.
@@ -63,34 +67,42 @@ __device__ inline double weight(float p, float q) {
   return d > 0.0 ? d : 0.0;
 }
 
+// Sum over a wavefront, in every lane: rotations within rows of 16, then exchanges of rows.
 __device__ inline double wave_sum(double x) {
-#pragma unroll
-  for (int off = 32; off; off >>= 1) x += __shfl_xor(x, off);
-  return x;
+  auto parts = [](double v) { return __builtin_bit_cast(uint2, v); };
+  auto whole = [](unsigned lo, unsigned hi) { return __builtin_bit_cast(double, make_uint2(lo, hi)); };
+#define PA_TURNED(ctrl)                                                                       \
+  whole((unsigned)__builtin_amdgcn_update_dpp(0, (int)parts(x).x, ctrl, 0xf, 0xf, false),     \
+        (unsigned)__builtin_amdgcn_update_dpp(0, (int)parts(x).y, ctrl, 0xf, 0xf, false))
+  x += PA_TURNED(0x128);
+  x += PA_TURNED(0x124);
+  x += PA_TURNED(0x122);
+  x += PA_TURNED(0x121);
+#undef PA_TURNED
+  x += __shfl_xor(x, 16);
+  return x + __shfl_xor(x, 32);
 }
 
-// One thread's entries [v0, v0 + 4) of the chunk: p and q, zeros past the vocabulary.
-template <bool VEC>
-__device__ inline void load4(const Args& a, const Weights& w, int64_t v0, float (&p)[4],
+// One lane's entries [v0, v0 + 4) of a row: p and q, zeros past the vocabulary. WHOLE: there
+// are four, at 16-byte aligned addresses.
+template <bool WHOLE>
+__device__ inline void load4(const Args& a, const Weights& w, int v0, float (&p)[4],
                              float (&q)[4]) {
-  if (VEC && v0 + 4 <= a.vocab) {
+  if constexpr (WHOLE) {
     const float4 x = *reinterpret_cast<const float4*>(w.p + v0);
     p[0] = x.x, p[1] = x.y, p[2] = x.z, p[3] = x.w;
-    if (w.q) {
-      const float4 y = *reinterpret_cast<const float4*>(w.q + v0);
-      q[0] = y.x, q[1] = y.y, q[2] = y.z, q[3] = y.w;
-    } else {
-      q[0] = q[1] = q[2] = q[3] = 0.f;
-    }
+    float4 y = {0.f, 0.f, 0.f, 0.f};
+    if (w.q) y = *reinterpret_cast<const float4*>(w.q + v0);
+    q[0] = y.x, q[1] = y.y, q[2] = y.z, q[3] = y.w;
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const bool in = v0 + i < a.vocab;
+      const bool in = v0 < a.vocab - i;
       p[i] = in ? w.p[v0 + i] : 0.f;
       q[i] = in && w.q ? w.q[v0 + i] : 0.f;
     }
   }
-  if (!w.q) {
+  if (w.certain >= 0) {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       if (v0 + i == w.certain) q[i] = __builtin_huge_valf();
@@ -98,14 +110,13 @@ __device__ inline void load4(const Args& a, const Weights& w, int64_t v0, float 
 }
 
 template <bool VEC>
-__global__ __launch_bounds__(kThreads) void verify_kernel(Args a) {
-  __shared__ double s_sum[2][kThreads / 64];
-  __shared__ double s_before[kThreads / 64];
+__global__ __launch_bounds__(kThreads, 4) void verify_kernel(Args a) {
+  __shared__ double s_before[kWaves];
   __shared__ int s_flag;
   __shared__ int s_best, s_last;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int b = blockIdx.x / a.chunks;
-  const int chunk = blockIdx.x - b * a.chunks;
+  const int b = blockIdx.x / a.groups;
+  const int group = blockIdx.x - b * a.groups;
 
   // Every wavefront decides the drafts for itself, one per lane.
   int k = a.counts ? a.counts[b] : a.k;
@@ -125,113 +136,157 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(Args a) {
   Weights w;
   w.p = a.p + b * a.p_sb + n * a.p_si;
   w.q = n < k && a.q ? a.q + b * a.q_sb + n * a.q_si : nullptr;
-  w.certain = n < k && !a.q ? __shfl(id, n) : -1;
+  // (An id outside the vocabulary is no entry's.)
+  const int own = id >= 0 && id < a.vocab ? (int)id : -1;
+  w.certain = n < k && !a.q ? __builtin_amdgcn_readfirstlane(__shfl(own, n)) : -1;
 
-  const int64_t c0 = (int64_t)chunk * kChunk;
-  double sd = 0.0, sp = 0.0;
+  double* sums = a.sums + (int64_t)b * a.pieces * 2;
+  // One piece: 16 entries per lane, four at a time.
+  auto load_piece = [&](int c, float (&p)[4][4], float (&q)[4][4]) {
+    const int v0 = c * kPiece + lane * 4;
+    if (VEC && c < a.vocab / kPiece) {  // wavefront-uniform
 #pragma unroll
-  for (int j = 0; j < kPer / 4; ++j) {
-    float p[4], q[4];
-    load4<VEC>(a, w, c0 + ((int64_t)j * kThreads + tid) * 4, p, q);
+      for (int j = 0; j < 4; ++j) load4<true>(a, w, v0 + j * 256, p[j], q[j]);
+    } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      sd += weight(p[i], q[i]);
-      sp += weight(p[i], 0.f);
+      for (int j = 0; j < 4; ++j) load4<false>(a, w, v0 + j * 256, p[j], q[j]);
     }
+  };
+  auto sum_piece = [&](int c, const float (&p)[4][4], const float (&q)[4][4]) {
+    double sd = 0.0, sp = 0.0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        sd += weight(p[j][i], q[j][i]);
+        sp += weight(p[j][i], 0.f);
+      }
+    sd = wave_sum(sd);
+    sp = wave_sum(sp);
+    if (lane == 0) {
+      // Device-coherent: the sequence's last workgroup may run on another XCD.
+      __hip_atomic_store(sums + 2 * c, sd, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      __hip_atomic_store(sums + 2 * c + 1, sp, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+  };
+  const int stride = a.groups * kWaves;
+  float p0[4][4], q0[4][4], p1[4][4], q1[4][4];
+  int c = group * kWaves + wave;
+  if (c < a.pieces) load_piece(c, p0, q0);
+  while (c < a.pieces) {  // wavefront-uniform
+    if (c + stride < a.pieces) load_piece(c + stride, p1, q1);
+    sum_piece(c, p0, q0);
+    c += stride;
+    if (c >= a.pieces) break;
+    if (c + stride < a.pieces) load_piece(c + stride, p0, q0);
+    sum_piece(c, p1, q1);
+    c += stride;
   }
-  sd = wave_sum(sd);
-  sp = wave_sum(sp);
-  if (lane == 0) {
-    s_sum[0][wave] = sd;
-    s_sum[1][wave] = sp;
-  }
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+  __builtin_amdgcn_s_waitcnt(0);  // the sums have landed before the arrival counts
   __syncthreads();
-  double* sums = a.sums + (int64_t)b * a.chunks * 2;
-  if (tid == 0) {
-    double x = 0.0, y = 0.0;
-    for (int i = 0; i < kThreads / 64; ++i) {
-      x += s_sum[0][i];
-      y += s_sum[1][i];
-    }
-    // Device-coherent: the sequence's last workgroup may run on another XCD.
-    __hip_atomic_store(sums + 2 * chunk, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    __hip_atomic_store(sums + 2 * chunk + 1, y, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
-    __builtin_amdgcn_s_waitcnt(0);  // the sums have landed before the arrival counts
+  if (tid == 0)
     s_flag = __hip_atomic_fetch_add(a.cnt + b, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
-             a.chunks - 1;
-  }
+             a.groups - 1;
   __syncthreads();
   if (!s_flag) return;
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
 
-  // The chunk of the crossing, by every wavefront: lanes take chunks lane, lane + 64, ...
-  auto chunk_sum = [&](int c, int which) {
-    return c < a.chunks ? __hip_atomic_load(sums + 2 * c + which, __ATOMIC_RELAXED,
-                                            __HIP_MEMORY_SCOPE_AGENT)
-                        : 0.0;
+  // The piece of the crossing, by every wavefront for itself: batches of 256 pieces, four
+  // consecutive ones per lane, both sums of each in one device-coherent read.
+  const auto rs = tiles::tile_rsrc(sums, a.pieces * 16);
+  double x[2][4];  // [whether of p alone][piece]
+  auto take = [&](int first) {  // past the last piece: zeros
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const f32x4 y = tiles::load_coherent16(rs, (first + lane * 4 + i) * 16);
+      typedef double f64x2 __attribute__((ext_vector_type(2)));
+      const f64x2 z = __builtin_bit_cast(f64x2, y);
+      x[0][i] = z[0];
+      x[1][i] = z[1];
+    }
   };
-  double total = 0.0;
-  for (int c = lane; c < a.chunks; c += 64) total += chunk_sum(c, 0);
-  total = wave_sum(total);
-  const bool whole = !(total > 0.0);  // p <= q everywhere: the target's own row
+  double of_diff = 0.0, of_p = 0.0;
+  for (int first = 0; first < a.pieces; first += 256) {
+    take(first);
+    of_diff += wave_sum((x[0][0] + x[0][1]) + (x[0][2] + x[0][3]));
+    of_p += wave_sum((x[1][0] + x[1][1]) + (x[1][2] + x[1][3]));
+  }
+  const bool whole = !(of_diff > 0.0);  // p <= q everywhere: the target's own row
   if (whole) {
     w.q = nullptr;
     w.certain = -1;
-    total = 0.0;
-    for (int c = lane; c < a.chunks; c += 64) total += chunk_sum(c, 1);
-    total = wave_sum(total);
   }
-  const double aim = (double)a.u_next[b] * total;
-  // First chunk whose inclusive sum exceeds aim, and the last with any weight.
+  const double aim = (double)a.u_next[b] * (whole ? of_p : of_diff);
+  // First piece whose inclusive sum exceeds aim, and the last with any weight.
   int at = -1, last = 0;
   double before = 0.0, last_before = 0.0, run = 0.0;
-  for (int c = 0; c < a.chunks && at < 0; c += 64) {
-    const double x = chunk_sum(c + lane, whole);
-    double incl = x;
+  for (int first = 0; first < a.pieces && at < 0; first += 256) {
+    if (a.pieces > 256) take(first);
+    double own4[4], mine = 0.0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      own4[i] = whole ? x[1][i] : x[0][i];
+      mine += own4[i];
+    }
+    double incl = mine;
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
       const double y = __shfl_up(incl, off);
       if (lane >= off) incl += y;
     }
-    incl += run;
-    const uint64_t over = __ballot(x > 0.0 && incl > aim);
-    const uint64_t some = __ballot(x > 0.0);
-    if (over) {
-      const int l = (int)__builtin_ctzll(over);
-      at = c + l;
-      before = __shfl(incl - x, l);
+    double sum = run + (incl - mine);
+    int over = -1, some = -1;
+    double over_before = 0.0, some_before = 0.0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (own4[i] > 0.0) {
+        if (over < 0 && sum + own4[i] > aim) {
+          over = i;
+          over_before = sum;
+        }
+        some = i;
+        some_before = sum;
+      }
+      sum += own4[i];
     }
-    if (some) {
-      const int l = 63 - (int)__builtin_clzll(some);
-      last = c + l;
-      last_before = __shfl(incl - x, l);
+    const uint64_t overs = __ballot(over >= 0), somes = __ballot(some >= 0);
+    if (overs) {
+      const int l = (int)__builtin_ctzll(overs);
+      at = first + 4 * l + __shfl(over, l);
+      before = __shfl(over_before, l);
     }
-    run = __shfl(incl, 63);
+    if (somes) {
+      const int l = 63 - (int)__builtin_clzll(somes);
+      last = first + 4 * l + __shfl(some, l);
+      last_before = __shfl(some_before, l);
+    }
+    run += __shfl(incl, 63);
   }
   if (at < 0) {  // u' * total not below the sum of all, by rounding or u' >= 1
     at = last;
     before = last_before;
   }
 
-  // The index within the chunk: thread t now holds kPer consecutive entries.
+  // The index within the piece: thread t now holds four consecutive entries.
   if (tid == 0) {
     s_best = 0x7fffffff;
     s_last = -1;
   }
-  const int64_t v0 = (int64_t)at * kChunk + (int64_t)tid * kPer;
-  double x[kPer], mine = 0.0;
+  constexpr int kPer = kPiece / kThreads;
+  static_assert(kPer == 4, "one load4 per thread");
+  float ep[4], eq[4];
+  if (VEC && at < a.vocab / kPiece)
+    load4<true>(a, w, at * kPiece + tid * kPer, ep, eq);
+  else
+    load4<false>(a, w, at * kPiece + tid * kPer, ep, eq);
+  double e[kPer], mine = 0.0;
   int mine_last = -1;
 #pragma unroll
-  for (int j = 0; j < kPer / 4; ++j) {
-    float p[4], q[4];
-    load4<VEC>(a, w, v0 + 4 * j, p, q);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[4 * j + i] = weight(p[i], q[i]);
-      mine += x[4 * j + i];
-      if (x[4 * j + i] > 0.0) mine_last = 4 * j + i;
-    }
+  for (int i = 0; i < kPer; ++i) {
+    e[i] = weight(ep[i], eq[i]);
+    mine += e[i];
+    if (e[i] > 0.0) mine_last = i;
   }
   double incl = mine;
 #pragma unroll
@@ -246,8 +301,8 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(Args a) {
   int found = 0x7fffffff;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
-    sum += x[i];
-    if (x[i] > 0.0 && sum > aim && found == 0x7fffffff) found = tid * kPer + i;
+    sum += e[i];
+    if (e[i] > 0.0 && sum > aim && found == 0x7fffffff) found = tid * kPer + i;
   }
   if (found != 0x7fffffff) atomicMin(&s_best, found);
   if (mine_last >= 0) atomicMax(&s_last, tid * kPer + mine_last);
@@ -255,8 +310,8 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(Args a) {
   int64_t* out = a.tokens + (int64_t)b * (a.k + 1);
   if (tid <= a.k) {
     // With no weight anywhere: index 0.
-    const int64_t next = s_best != 0x7fffffff ? (int64_t)at * kChunk + s_best
-                                              : (s_last >= 0 ? (int64_t)at * kChunk + s_last : 0);
+    const int64_t next = s_best != 0x7fffffff ? (int64_t)at * kPiece + s_best
+                                              : (s_last >= 0 ? (int64_t)at * kPiece + s_last : 0);
     out[tid] = tid < n ? a.ids[b * a.i_sb + tid * a.i_si] : (tid == n ? next : -1);
   }
   if (tid == 0) {
@@ -265,7 +320,18 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(Args a) {
   }
 }
 
-static int chunks_of(int vocab) { return (int)(((int64_t)vocab + kChunk - 1) / kChunk); }
+static int pieces_of(int vocab) { return (int)(((int64_t)vocab + kPiece - 1) / kPiece); }
+
+// Workgroups per sequence: one wavefront per piece for a few sequences; for many, as many
+// as fill kWavesPerCu wavefronts per compute unit over all sequences, the pieces dealt in
+// whole rounds.
+constexpr int kWavesPerCu = 8;
+static int groups_of(int num_seqs, int pieces) {
+  const int64_t waves = (int64_t)kWavesPerCu * device_cus() / num_seqs;
+  const int64_t rounds = waves >= pieces ? 1 : (pieces + (waves > 0 ? waves : 1) - 1) / (waves > 0 ? waves : 1);
+  const int64_t per_round = (pieces + rounds - 1) / rounds;
+  return (int)((per_round + kWaves - 1) / kWaves);
+}
 
 }  // namespace verify
 }  // namespace pa
@@ -277,7 +343,7 @@ extern "C" {
 
 size_t pa_verify_drafts_workspace_bytes(int num_seqs, int vocab) {
   if (num_seqs <= 0 || num_seqs > kMaxSeqs || vocab <= 0) return 0;
-  return kCounterBytes + (size_t)num_seqs * chunks_of(vocab) * 2 * sizeof(double);
+  return kCounterBytes + (size_t)num_seqs * pieces_of(vocab) * 2 * sizeof(double);
 }
 
 int pa_verify_drafts_f32(const float* target, const int64_t target_strides[3], const float* draft,
@@ -309,13 +375,18 @@ int pa_verify_drafts_f32(const float* target, const int64_t target_strides[3], c
     set_error("the rows of probabilities need unit vocabulary stride");
     return PA_ERR_ARG;
   }
+  if (vocab > (1 << 30)) {
+    set_error("a vocabulary of %d is not built", vocab);
+    return PA_ERR_UNSUPPORTED;
+  }
   const size_t need = pa_verify_drafts_workspace_bytes(num_seqs, vocab);
   if (!workspace || workspace_bytes < need) {
     set_error("workspace of %zu bytes needed, %zu given", need, workspace_bytes);
     return PA_ERR_WORKSPACE;
   }
-  const int chunks = chunks_of(vocab);
-  const int64_t grid = (int64_t)num_seqs * chunks;
+  const int pieces = pieces_of(vocab);
+  const int groups = groups_of(num_seqs, pieces);
+  const int64_t grid = (int64_t)num_seqs * groups;
   if (grid > 0x7fffffff) {
     set_error("%d sequences of a vocabulary of %d exceed one launch", num_seqs, vocab);
     return PA_ERR_UNSUPPORTED;
@@ -351,7 +422,8 @@ int pa_verify_drafts_f32(const float* target, const int64_t target_strides[3], c
   a.seqs = num_seqs;
   a.k = max_drafts;
   a.vocab = vocab;
-  a.chunks = chunks;
+  a.pieces = pieces;
+  a.groups = groups;
   if (vec)
     verify_kernel<true><<<(unsigned)grid, kThreads, 0, (hipStream_t)stream>>>(a);
   else
