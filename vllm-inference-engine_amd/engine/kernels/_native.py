@@ -164,8 +164,8 @@ def host():
         if ver != ABI_VERSION:
             raise NativeLibraryError(
                 f"{path} has ABI {ver}, the bindings expect {ABI_VERSION}; rebuild it")
-        module.bind({name: ctypes.cast(getattr(lib, name), ctypes.c_void_p).value
-                     for name in module.CALLS})
+        for bind, names in ((module.bind, module.CALLS), (module.bind_fp8, module.CALLS_FP8)):
+            bind({name: ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in names})
         _host = module
     return _host
 
@@ -184,6 +184,41 @@ def direct(name: str, first: torch.Tensor, *args):
     buf = _workspaces.get((index, stream, WS_DECODE))
     if buf is None:
         return None
+    out = getattr(_host or host(), name)(first, *args, buf, stream)
+    if type(out) is int:
+        check(out, name)
+    return out
+
+
+_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", None)
+_no_workspace = torch.empty(0, dtype=torch.uint8)
+
+
+def direct_call(name: str, first: torch.Tensor, *args):
+    """host().<name>(first, *args, stream) on the current stream of first's device, as direct()."""
+    index = first.get_device()
+    if index < 0 or _raw_stream is None:
+        return None
+    out = getattr(_host or host(), name)(first, *args, _raw_stream(index))
+    if type(out) is int:
+        check(out, name)
+    return out
+
+
+def direct_counted(name: str, kind: str, first: torch.Tensor, *args):
+    """host().<name>(first, *args, workspace, stream) with the stream's workspace of this kind.
+
+    None as for direct(), and where the call needs a workspace that is not there, too small,
+    or not to be used: a call under graph capture takes one of the graph's own
+    (counted_workspace).
+    """
+    index = first.get_device()
+    if index < 0 or _raw_stream is None or _capturing is None:
+        return None
+    stream = _raw_stream(index)
+    buf = _workspaces.get((index, stream, kind))
+    if buf is None or _capturing():
+        buf = _no_workspace
     out = getattr(_host or host(), name)(first, *args, buf, stream)
     if type(out) is int:
         check(out, name)

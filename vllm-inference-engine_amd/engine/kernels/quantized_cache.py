@@ -98,6 +98,9 @@ def paged_kv_write_fp8(
     Rows of a written block that lie behind the new ones (tokens taken back) keep
     their codes but not their values. No two sequences may write the same block.
     """
+    if _native.direct_call("write_fp8", key, value, k_cache, v_cache, k_scale, v_scale,
+                           block_tables, seq_lens, query_start_loc):
+        return
     block_tables, seq_lens = _check_pool(k_cache, v_cache, k_scale, v_scale, block_tables,
                                          seq_lens)
     num_seqs = seq_lens.shape[0]
@@ -151,11 +154,15 @@ def paged_kv_read_fp8(
     n_b = seq_lens[b] the whole contexts, one after the other. Exact (each value is an
     fp16 number). Rows without a slot, and rows of no sequence, are zeros.
     """
+    num_tokens = int(num_tokens)
+    out = _native.direct_call("read_fp8", k_cache, v_cache, k_scale, v_scale, block_tables,
+                              seq_lens, query_start_loc, num_tokens)
+    if out is not None:
+        return out
     block_tables, seq_lens = _check_pool(k_cache, v_cache, k_scale, v_scale, block_tables,
                                          seq_lens)
     num_seqs = seq_lens.shape[0]
     query_start_loc = _check_starts(query_start_loc, k_cache, num_seqs)
-    num_tokens = int(num_tokens)
     assert 0 <= num_tokens < 2 ** 31
     num_blocks, block_size, num_kv_heads, head_dim = k_cache.shape
     dev = k_cache.device
@@ -205,6 +212,10 @@ def paged_attention_decode_fp8(
     in it, through a per-stream scratch buffer (the graph's own while one is captured).
     Repeated calls return the same bits.
     """
+    out = _native.direct_counted("decode_fp8", _native.WS_DECODE_FP8, q, k_cache, v_cache,
+                                 k_scale, v_scale, block_tables, seq_lens, float(scale))
+    if out is not None:
+        return out
     block_tables, seq_lens = _check_pool(k_cache, v_cache, k_scale, v_scale, block_tables,
                                          seq_lens)
     _check_queries(q, k_cache)
@@ -256,6 +267,11 @@ def paged_attention_prefill_fp8(
     tokens' rows must be in the pool (paged_kv_write_fp8); scale must be positive; rows
     of q that belong to no sequence, or lie past max_query_len, are not written.
     """
+    out = _native.direct_counted("prefill_fp8", _native.WS_PREFILL, q, k_cache, v_cache, k_scale,
+                                 v_scale, block_tables, seq_lens, query_start_loc,
+                                 int(max_query_len), float(scale))
+    if out is not None:
+        return out
     block_tables, seq_lens = _check_pool(k_cache, v_cache, k_scale, v_scale, block_tables,
                                          seq_lens)
     _check_queries(q, k_cache)

@@ -43,6 +43,10 @@ def verify_drafts(
     drafts and 16384 sequences. Asynchronous on the current stream; no host
     synchronisation; capturable into a HIP graph.
     """
+    out = _native.direct_counted("verify", _native.WS_VERIFY, target_probs, draft_probs, draft_ids,
+                                 accept_u, next_u, num_drafts)
+    if out is not None:
+        return out
     tensors = [target_probs, draft_ids, accept_u, next_u]
     tensors += [t for t in (draft_probs, num_drafts) if t is not None]
     assert all(t.is_cuda for t in tensors), "verify_drafts runs on the GPU only"
