@@ -1363,8 +1363,8 @@ int pa_prefill_attention_fp8(const void* q, const int64_t q_strides[3], const vo
     }
     // (In bytes here, where the fp16 pool's checks ask for multiples of 8 elements.)
     for (int i = 0; i < 3; ++i) {
-      if (k_strides[i] % 16 || v_strides[i] % 16) {
-        set_error("cache strides must be multiples of 16 bytes");
+      if (k_strides[i] % 16 || v_strides[i] % 16 || k_strides[i] < 0 || v_strides[i] < 0) {
+        set_error("cache strides must be non-negative multiples of 16 bytes");
         return PA_ERR_ARG;
       }
     }

@@ -38,7 +38,7 @@ template <>
 struct Piece<true> {
   static constexpr int N = 8;
   f16x8 x;
-  __device__ void load(const uint16_t* p, int64_t) { x = *reinterpret_cast<const f16x8*>(p); }
+  __device__ void load(const uint16_t* p) { x = *reinterpret_cast<const f16x8*>(p); }
   __device__ void store(uint8_t* p, float inv) const {
     float y[8];
 #pragma unroll
@@ -70,7 +70,7 @@ template <>
 struct Piece<false> {
   static constexpr int N = 1;
   f16 x;
-  __device__ void load(const uint16_t* p, int64_t) { x = *reinterpret_cast<const f16*>(p); }
+  __device__ void load(const uint16_t* p) { x = *reinterpret_cast<const f16*>(p); }
   __device__ void store(uint8_t* p, float inv) const {
     *p = (uint8_t)to_codes<false>(in_range((float)x) * inv, 0.f, 0);
   }
@@ -85,13 +85,12 @@ __global__ __launch_bounds__(256) void write_kernel(WriteArgs a) {
   typedef Piece<VEC> P;
   constexpr int HELD = 4;  // pieces per lane kept between the maximum and the codes
   const int lane = threadIdx.x & 63;
-  const int64_t unit = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int unit = (int)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int per_slot = 2 * a.hkv;
-  const int slot = (int)(unit / per_slot);
+  const int slot = unit / per_slot;
   if (slot >= a.slots) return;
-  const int rest = (int)(unit - (int64_t)slot * per_slot);
-  const int c = rest & 1;  // 0: keys, 1: values
-  const int h = rest >> 1;
+  const int c = (unit - slot * per_slot) & 1;  // 0: keys, 1: values
+  const int h = (unit - slot * per_slot) >> 1;
   const Rows& r = a.r;
 
   // Slots are numbered so that sequence b owns those from rows-before-b / bs + 2 b
@@ -104,7 +103,7 @@ __global__ __launch_bounds__(256) void write_kernel(WriteArgs a) {
   if (n <= 0) return;
   const int64_t L = r.lens[b];
   const int64_t from = L - n;  // position of the sequence's first new row
-  const int64_t p0 = from > 0 ? from : 0;
+  const int p0 = from > 0 ? (int)from : 0;
   const int64_t blk = p0 / r.bs + (r.qstart ? slot - (q0 / r.bs + 2 * b) : 0);
   if (blk >= r.max_blocks) return;
   const int64_t lo = blk * r.bs > p0 ? blk * r.bs : p0;
@@ -120,29 +119,44 @@ __global__ __launch_bounds__(256) void write_kernel(WriteArgs a) {
   float* sp = a.scale[c] + (int64_t)id * a.x_sb[c] + (int64_t)h * a.x_sh[c];
   const int e_old = r0 > 0 ? scale_exp(*sp) : kExpMin;
 
+  // This lane's pieces are lane, lane + 64, ...; piece i is piece i % per_row of row
+  // i / per_row. (The host sees to it that 31 bits hold a block's pieces.)
   const int per_row = a.D / P::N;
-  const int64_t pieces = (int64_t)rows * per_row;
-  auto source = [&](int64_t i) {
-    const int64_t row = i / per_row;
-    return src + row * a.s_t[c] + (i - row * per_row) * P::N * a.s_d[c];
+  const int pieces = rows * per_row;
+  struct Place {
+    int row, col;
   };
-  auto target = [&](int64_t i, int first) {
-    const int64_t row = i / per_row;
-    return dst + (first + row) * a.c_st[c] + (i - row * per_row) * P::N;
+  const Place start{lane / per_row, lane % per_row};
+  const int down = 64 / per_row, along = 64 % per_row;
+  auto next = [&](Place& at) {
+    at.row += down;
+    at.col += along;
+    if (at.col >= per_row) {
+      at.col -= per_row;
+      ++at.row;
+    }
+  };
+  auto source = [&](Place at) { return src + at.row * a.s_t[c] + at.col * P::N * a.s_d[c]; };
+  auto target = [&](Place at, int first) {
+    return dst + (first + at.row) * a.c_st[c] + at.col * P::N;
   };
   P held[HELD];
+  Place at[HELD];
   float m = 0.f;
+  Place rest = start;
 #pragma unroll
   for (int k = 0; k < HELD; ++k) {
-    const int64_t i = lane + 64 * k;
-    if (i < pieces) held[k].load(source(i), 0);
+    at[k] = rest;
+    if (lane + 64 * k < pieces) held[k].load(source(rest));
+    next(rest);
   }
 #pragma unroll
   for (int k = 0; k < HELD; ++k)
     if (lane + 64 * k < pieces) m = __builtin_fmaxf(m, held[k].amax());
-  for (int64_t i = lane + 64 * HELD; i < pieces; i += 64) {
+  Place more = rest;
+  for (int i = lane + 64 * HELD; i < pieces; i += 64, next(more)) {
     P x;
-    x.load(source(i), 0);
+    x.load(source(more));
     m = __builtin_fmaxf(m, x.amax());
   }
 #pragma unroll
@@ -152,18 +166,17 @@ __global__ __launch_bounds__(256) void write_kernel(WriteArgs a) {
   const int e = e_old > e_new ? e_old : e_new;
   if (r0 > 0 && e > e_old) {
     const float shift = exp2i(e_old - e);
-    for (int64_t i = lane; i < (int64_t)r0 * per_row; i += 64) P::recode(target(i, 0), shift);
+    more = start;
+    for (int i = lane; i < r0 * per_row; i += 64, next(more)) P::recode(target(more, 0), shift);
   }
   const float inv = exp2i(-e);
 #pragma unroll
-  for (int k = 0; k < HELD; ++k) {
-    const int64_t i = lane + 64 * k;
-    if (i < pieces) held[k].store(target(i, r0), inv);
-  }
-  for (int64_t i = lane + 64 * HELD; i < pieces; i += 64) {
+  for (int k = 0; k < HELD; ++k)
+    if (lane + 64 * k < pieces) held[k].store(target(at[k], r0), inv);
+  for (int i = lane + 64 * HELD; i < pieces; i += 64, next(rest)) {
     P x;
-    x.load(source(i), 0);
-    x.store(target(i, r0), inv);
+    x.load(source(rest));
+    x.store(target(rest, r0), inv);
   }
   if (lane == 0) *sp = exp2i(e);
 }
@@ -330,11 +343,13 @@ int pa_kv_write_fp8(const void* key, const int64_t key_strides[3], const void* v
   a.D = head_dim;
   const int64_t slots =
       query_start_loc ? (int64_t)num_tokens / block_size + 2 * (int64_t)num_seqs : num_seqs;
-  const int64_t grid = (slots * num_kv_heads * 2 + 3) / 4;
-  if (slots > 0x7fffffff || grid > 0x7fffffff) {
-    set_error("%lld blocks of %d kv heads exceed one launch", (long long)slots, num_kv_heads);
+  // (Also in the kernel's 31-bit counts of units and of a block's values.)
+  if (slots > 0x3ffffff0 || slots * num_kv_heads > 0x3ffffff0 || (int64_t)block_size * head_dim > 0x7fffff00) {
+    set_error("%lld blocks of %d kv heads, %d rows of %d values each, exceed one launch",
+              (long long)slots, num_kv_heads, block_size, head_dim);
     return PA_ERR_UNSUPPORTED;
   }
+  const int64_t grid = (slots * num_kv_heads * 2 + 3) / 4;
   a.slots = (int)slots;
   if (vec)
     write_kernel<true><<<(unsigned)grid, 256, 0, (hipStream_t)stream>>>(a);

@@ -9,6 +9,9 @@
 namespace pa {
 namespace fp8 {
 
+// (Calls take the same workspaces as the prefill kernel's.)
+static_assert(kCounterBytes == kPfCounterBytes, "counters, and nothing else, where it has its own");
+
 // Columns of a sequence and kv head that the registers hold: four blocks of 16, or two at
 // head_dim 128 (four would spill 91 registers there).
 static int most_columns(int D) { return D <= 64 ? 64 : 32; }

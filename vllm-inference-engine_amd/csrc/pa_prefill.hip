@@ -404,7 +404,7 @@ __global__ __launch_bounds__(64 * NW) void prefill_attn_kernel(PrefillAttnArgs a
       for (int cg = 0; cg < CG; ++cg) {
         // A column with no visible key yet keeps m = -inf; any finite offset
         // then gives p = 0 for its -inf scores.
-        const float nm = m_run[cg] == kNegInf ? 0.f : BIAS - m_run[cg];
+        const float nm = m_run[cg] == kNegInf ? 0.f : KV8 ? BIAS - m_run[cg] : -m_run[cg];
         lt[cg] = 0.f;
 #pragma unroll
         for (int sp = 0; sp < NS / 2; ++sp) {
