@@ -16,7 +16,7 @@ DecodePlan decode_plan(int num_seqs, int num_q_heads, int num_kv_heads, int head
   const int64_t pairs = (int64_t)num_seqs * (num_kv_heads / p.head_group);
   const int64_t cap = (int64_t)max_blocks * block_size;
   const bool few = p.head_group == 1 && pairs <= n;
-  p.waves = few && head_dim <= 128 && !multi ? 8 : 4;
+  p.waves = few && head_dim <= 128 ? 8 : 4;
   const int64_t whole = 2 * pairs >= n ? kWholePairsBusy : kWholePairs;
   p.ranged = cap > whole && pairs <= kMaxCounters &&
              pairs * ((cap + kChunk - 1) / kChunk + kPairCost) < 0x7fffffff;
@@ -25,7 +25,7 @@ DecodePlan decode_plan(int num_seqs, int num_q_heads, int num_kv_heads, int head
     // One workgroup per compute unit, or two of many pairs; no more ranges than the longest
     // lengths fill.
     const int64_t most = pairs * ((cap + kChunk - 1) / kChunk + kPairCost) / kMinRange;
-    const int want = (few && !multi ? 1 : 2) * n;
+    const int want = (few ? 1 : 2) * n;
     p.grid = (int)(most < want ? (most < 1 ? 1 : most) : want);
     const int heads = num_q_heads / num_kv_heads * p.head_group * (multi ? new_tokens : 1);
     p.rec_floats = record_size(heads, head_dim);

@@ -27,21 +27,28 @@ size_t drafts_workspace_bytes(int num_seqs, int num_q_heads, int num_kv_heads, i
                      max_query_len).ws_bytes;
 }
 
-template <int D, int CB>
-static hipError_t launch_drafts_cb(const DecodeFp8Args& a, unsigned grid, hipStream_t s) {
+template <int D, int CB, int NW>
+static hipError_t launch_drafts_nw(const DecodeFp8Args& a, unsigned grid, hipStream_t s) {
   if (a.bs == 16 && near_strides(a))
-    attend_fp8_kernel<D, 1, 16, 4, CB, true><<<grid, 256, 0, s>>>(a);
+    attend_fp8_kernel<D, 1, 16, NW, CB, true><<<grid, 64 * NW, 0, s>>>(a);
   else
-    attend_fp8_kernel<D, 1, 0, 4, CB, true><<<grid, 256, 0, s>>>(a);
+    attend_fp8_kernel<D, 1, 0, NW, CB, true><<<grid, 64 * NW, 0, s>>>(a);
   return hipGetLastError();
 }
 
-static hipError_t launch_drafts(const DecodeFp8Args& a, int D, unsigned grid, hipStream_t s) {
+template <int D, int CB>
+static hipError_t launch_drafts_cb(const DecodeFp8Args& a, const DecodePlan& p, hipStream_t s) {
+  const unsigned grid = (unsigned)p.grid;
+  return p.waves == 8 ? launch_drafts_nw<D, CB, 8>(a, grid, s)
+                      : launch_drafts_nw<D, CB, 4>(a, grid, s);
+}
+
+static hipError_t launch_drafts(const DecodeFp8Args& a, int D, const DecodePlan& p, hipStream_t s) {
   const bool two = a.max_new * a.g <= 32;
   switch (D) {
-    case 32: return two ? launch_drafts_cb<32, 2>(a, grid, s) : launch_drafts_cb<32, 4>(a, grid, s);
-    case 64: return two ? launch_drafts_cb<64, 2>(a, grid, s) : launch_drafts_cb<64, 4>(a, grid, s);
-    case 128: return launch_drafts_cb<128, 2>(a, grid, s);
+    case 32: return two ? launch_drafts_cb<32, 2>(a, p, s) : launch_drafts_cb<32, 4>(a, p, s);
+    case 64: return two ? launch_drafts_cb<64, 2>(a, p, s) : launch_drafts_cb<64, 4>(a, p, s);
+    case 128: return launch_drafts_cb<128, 2>(a, p, s);
     default: return hipErrorInvalidValue;
   }
 }
@@ -98,7 +105,7 @@ int prefill_drafts(const PrefillAttnArgs& p, int D, int max_query_len, void* wor
   a.max_new = max_query_len;
   a.scale_log2 = p.scale_log2;
   plan.fill(a, workspace);
-  const hipError_t e = launch_drafts(a, D, (unsigned)plan.grid, s);
+  const hipError_t e = launch_drafts(a, D, plan, s);
   if (e == hipSuccess) return PA_OK;
   set_error("HIP launch failed: %s", hipGetErrorString(e));
   return PA_ERR_HIP;
