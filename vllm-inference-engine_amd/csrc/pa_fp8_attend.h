@@ -167,6 +167,15 @@ struct Sum {
   __device__ float operator()(float a, float b) const { return a + b; }
 };
 
+// A uniform value in scalar registers of its own from here on. (The arguments come in blocks
+// of sixteen registers; what loops use straight from them keeps whole blocks alive, which
+// then come back lane by lane from vector registers at every use.)
+template <typename T>
+__device__ inline T pinned(T x) {
+  asm volatile("" : "+s"(x));
+  return x;
+}
+
 // The permutation of a row's 16-byte pieces in LDS: piece p of chunk row r lies in slot
 // p ^ swizzle(r) of NP. Eight rows whose same piece is read at once, 0 .. 7 (V) or 0 .. 3
 // and 8 .. 11 (K), then lie in different banks.
@@ -201,8 +210,9 @@ __global__ __launch_bounds__(64 * NW, waves_per_simd(D, NW, CB)) void attend_fp8
   constexpr int NC = D / 32;            // products per score tile
   constexpr int ND = D / 16;
   constexpr int D4 = D / 4;
-  constexpr int STAGE = 2 * kChunk * RB;  // bytes per wavefront: K rows, then V rows
-  static_assert(STAGE == HG * 16 * D * 4, "the accumulators take the same room");
+  // Bytes per wavefront: K rows, then V rows; at the end its accumulators.
+  constexpr int STAGE = NS * 16 * D * 4;
+  static_assert(STAGE >= 2 * kChunk * RB, "the accumulators take the larger room");
   typedef unsigned frag __attribute__((ext_vector_type(FB / 4)));
   __shared__ __attribute__((aligned(16))) uint8_t s_stage[NW * STAGE];
   __shared__ __attribute__((aligned(16))) f32x4 s_part[kThreads];
@@ -246,7 +256,18 @@ __global__ __launch_bounds__(64 * NW, waves_per_simd(D, NW, CB)) void attend_fp8
   // all chunks, of a length found here, while the first ids are on their way). The pair is
   // spread over nseg workgroups' ranges, from range w0 on; this is its part `seg`.
   auto segment = [&](int b, int h0, int L, int c0, int c1, int w0, int seg, int nseg) {
-    const int32_t* btrow = a.bt + (int64_t)b * a.bt_sb;
+    const int32_t* const btrow = pinned(a.bt + (int64_t)b * a.bt_sb);
+    const int64_t bt_sk = pinned(a.bt_sk);
+    const uint8_t* const kbase = pinned(a.k + h0 * a.k_sh);
+    const uint8_t* const vbase = pinned(a.v + h0 * a.v_sh);
+    const int64_t k_sb = pinned(a.k_sb), v_sb = pinned(a.v_sb);
+    const int64_t k_st = pinned(a.k_st), v_st = pinned(a.v_st);
+    const int last_id = pinned(a.num_blocks - 1);
+    // The scale that the lane loads of each chunk: see issue().
+    const int shead = UNIFORM ? (HG > 1 ? lane >> 1 & 1 : 0) : (HG > 1 ? lane >> 5 : 0);
+    const bool of_v = UNIFORM && (lane & 4);
+    const float* const sbase = (of_v ? a.vs : a.ks) + (h0 + shead) * (of_v ? a.vs_sh : a.ks_sh);
+    const int64_t s_sb = of_v ? a.vs_sb : a.ks_sb;
     // The columns of the pair: its query heads, or times its tokens.
     int q0 = b, qall = 1, heads = HG * a.g;
     if constexpr (MULTI) {
@@ -266,10 +287,10 @@ __global__ __launch_bounds__(64 * NW, waves_per_simd(D, NW, CB)) void attend_fp8
       for (int i = 0; i < NID; ++i) {
         if constexpr (UNIFORM) {
           const int at = min(2 * c + i, last_tile);
-          ids[i] = load_uniform(btrow + (int64_t)(at / (BS / 16)) * a.bt_sk);
+          ids[i] = load_uniform(btrow + (int64_t)(at / (BS / 16)) * bt_sk);
         } else {
           const int t = i < NI ? i * RPI + lrow : lane & 31;
-          ids[i] = btrow[(int64_t)(min(c * kChunk + t, cap - 1) / bs) * a.bt_sk];
+          ids[i] = btrow[(int64_t)(min(c * kChunk + t, cap - 1) / bs) * bt_sk];
         }
       }
     };
@@ -303,37 +324,34 @@ __global__ __launch_bounds__(64 * NW, waves_per_simd(D, NW, CB)) void attend_fp8
     // else lane (token, head) those of token lane % 32.
     float scales = 1.f, vscales = 1.f;
     auto issue = [&](int c) {
+      auto block = [&](int id) { return (int64_t)min(max(id, 0), last_id); };
       if constexpr (UNIFORM) {
         const int id0 = ids[0], id1 = ids[1];
-        const int64_t id = min(max(lane & 1 ? id1 : id0, 0), a.num_blocks - 1);
-        const int64_t h = h0 + (HG > 1 ? lane >> 1 & 1 : 0);
-        const float* kp = a.ks + id * a.ks_sb + h * a.ks_sh;
-        const float* vp = a.vs + id * a.vs_sb + h * a.vs_sh;
-        scales = *(lane & 4 ? vp : kp);
+        scales = sbase[block(lane & 1 ? id1 : id0) * s_sb];
       } else {
-        const int64_t id = min(max(ids[NID - 1], 0), a.num_blocks - 1);
-        const int64_t h = h0 + (HG > 1 ? lane >> 5 : 0);
-        scales = a.ks[id * a.ks_sb + h * a.ks_sh];
-        vscales = a.vs[id * a.vs_sb + h * a.vs_sh];
+        const int64_t id = block(ids[NID - 1]);
+        scales = sbase[id * s_sb];
+        vscales = a.vs[id * a.vs_sb + (h0 + shead) * a.vs_sh];
       }
+      uint8_t* const to = s_stage + pinned(wave * STAGE);  // (nor are 2 NI places kept)
       auto load_rows = [&](const uint8_t* base, int64_t sb, int64_t st, int64_t sh, uint32_t plain,
                            uint32_t flip, uint8_t* to) {
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
-          const int64_t id = min(max(ids[UNIFORM ? i * RPI / 16 : i], 0), a.num_blocks - 1);
+          const int64_t id = block(ids[UNIFORM ? i * RPI / 16 : i]);
           if constexpr (UNIFORM) {
             const int64_t off = (2 * c + i * RPI / 16) % (BS / 16) * 16 + i * RPI % 16;
-            load_to_lds(tile_rsrc(base + id * sb + off * st + h0 * sh, kAll), flipped(i) ? flip : plain,
+            load_to_lds(tile_rsrc(base + id * sb + off * st, kAll), flipped(i) ? flip : plain,
                         to + i * 1024);
           } else {
             const int64_t off = (c * kChunk + i * RPI + lrow) % bs;
             const int p = piece(flipped(i) ? FLIP : 0);
-            load_to_lds(base + id * sb + off * st + (h0 + p / D) * sh + p % D, to + i * 1024);
+            load_to_lds(base + id * sb + off * st + p / D * sh + p % D, to + i * 1024);
           }
         }
       };
-      load_rows(a.k, a.k_sb, a.k_st, a.k_sh, k_lane, k_flip, stage);
-      load_rows(a.v, a.v_sb, a.v_st, a.v_sh, v_lane, v_flip, stage + kChunk * RB);
+      load_rows(kbase, k_sb, k_st, a.k_sh, k_lane, k_flip, to);
+      load_rows(vbase, v_sb, v_st, a.v_sh, v_lane, v_flip, to + kChunk * RB);
     };
 
     if (!a.ranged) {
@@ -514,8 +532,8 @@ __global__ __launch_bounds__(64 * NW, waves_per_simd(D, NW, CB)) void attend_fp8
       }
     }
 
-    // The wavefronts' states meet in LDS, HG blocks of columns at a time, four elements of
-    // accumulator row r at slot (d / 4) ^ (r & 7). (Lane indices anew: see fresh_lane.)
+    // The wavefronts' states meet in LDS, four elements of accumulator row r at slot
+    // (d / 4) ^ (r & 7). (Lane indices anew: see fresh_lane.)
     const int lane = fresh_lane();
     const int tid = wave * 64 + lane, row = lane & 15, grp = lane >> 4;
     // Part i of a cut pair lies in range w0 + i's slot 0 (the pair began before that range)
@@ -530,59 +548,52 @@ __global__ __launch_bounds__(64 * NW, waves_per_simd(D, NW, CB)) void attend_fp8
     };
     float* my_acc = reinterpret_cast<float*>(stage);
 #pragma unroll
-    for (int cb = 0; cb < CB; ++cb) {
-      if (cb * 16 >= heads && MULTI) break;  // workgroup-uniform
-      if (cb) __syncthreads();
-#pragma unroll
-      for (int hg = 0; hg < HG; ++hg) {
-        const int st = MULTI ? cb : hg;
-        const float l = over_groups(l_run[st], Sum());
-        if (grp == 0) {
-          s_m[wave][st * 16 + row] = m_run[st];
-          s_l[wave][st * 16 + row] = l;
-        }
-        if (MULTI || row < a.g) {
-#pragma unroll
-          for (int nd = 0; nd < ND; ++nd)
-            *reinterpret_cast<f32x4*>(my_acc + (hg * 16 + row) * D +
-                                      ((nd * 4 + grp) ^ (row & 7)) * 4) = acc[st][nd];
-        }
+    for (int st = 0; st < NS; ++st) {
+      const float l = over_groups(l_run[st], Sum());
+      if (grp == 0) {
+        s_m[wave][st * 16 + row] = m_run[st];
+        s_l[wave][st * 16 + row] = l;
       }
-      __syncthreads();
-      const int count = MULTI ? min(16, heads - cb * 16) : heads;
-      for (int i = tid; i < count * D4; i += kThreads) {
-        const int k = i / D4;
-        const int d = (i - k * D4) * 4;
-        const int r = HG > 1 && k >= a.g ? 16 + k - a.g : k;  // row of the accumulators
-        const int j = cb * 16 + k;
-        float M = s_m[0][cb * 16 + r];
+      if (MULTI ? st * 16 + row < heads : row < a.g) {
 #pragma unroll
-        for (int w = 1; w < NW; ++w) M = fmaxf(M, s_m[w][cb * 16 + r]);
-        float l = 0.f;
-        f32x4 o = {0.f, 0.f, 0.f, 0.f};
+        for (int nd = 0; nd < ND; ++nd)
+          *reinterpret_cast<f32x4*>(my_acc + (st * 16 + row) * D +
+                                    ((nd * 4 + grp) ^ (row & 7)) * 4) = acc[st][nd];
+      }
+    }
+    __syncthreads();
+#pragma unroll 1
+    for (int i = tid; i < heads * D4; i += kThreads) {
+      const int j = i / D4;
+      const int d = (i - j * D4) * 4;
+      const int r = HG > 1 && j >= a.g ? 16 + j - a.g : j;  // row of the accumulators
+      float M = s_m[0][r];
 #pragma unroll
-        for (int w = 0; w < NW; ++w) {
-          // A state of no maximum holds zeros, or NaN that has to show.
-          const float m = s_m[w][cb * 16 + r];
-          const float f = m == kNegInf ? 1.f : fast_exp2(m - M);
-          l += f * s_l[w][cb * 16 + r];
-          o += f * *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(s_stage + w * STAGE) +
-                                                   r * D + ((d >> 2) ^ (r & 7)) * 4);
-        }
-        if (nseg == 1) {
-          const float inv = l == 0.f ? 0.f : 1.f / l;  // 0: no key at all
-          f16x4 y;
+      for (int w = 1; w < NW; ++w) M = fmaxf(M, s_m[w][r]);
+      float l = 0.f;
+      f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int e = 0; e < 4; ++e) y[e] = (f16)(o[e] * inv);
-          *reinterpret_cast<f16x4*>(out_row(j) + d) = y;
-        } else {
-          store_coherent16(rr, rb + (j * D + d) * 4, o);
-          if (d == 0) {
-            __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, M), rr,
-                                                  rb + (heads * D + j) * 4, 0, 16);
-            __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, l), rr,
-                                                  rb + (heads * D + heads + j) * 4, 0, 16);
-          }
+      for (int w = 0; w < NW; ++w) {
+        // A state of no maximum holds zeros, or NaN that has to show.
+        const float m = s_m[w][r];
+        const float f = m == kNegInf ? 1.f : fast_exp2(m - M);
+        l += f * s_l[w][r];
+        o += f * *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(s_stage + w * STAGE) +
+                                                 r * D + ((d >> 2) ^ (r & 7)) * 4);
+      }
+      if (nseg == 1) {
+        const float inv = l == 0.f ? 0.f : 1.f / l;  // 0: no key at all
+        f16x4 y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = (f16)(o[e] * inv);
+        *reinterpret_cast<f16x4*>(out_row(j) + d) = y;
+      } else {
+        store_coherent16(rr, rb + (j * D + d) * 4, o);
+        if (d == 0) {
+          __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, M), rr,
+                                                rb + (heads * D + j) * 4, 0, 16);
+          __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, l), rr,
+                                                rb + (heads * D + heads + j) * 4, 0, 16);
         }
       }
     }
