@@ -187,7 +187,7 @@ __device__ inline int swizzle(int r) {
 
 // Wavefronts per SIMD that the registers are kept to.
 constexpr int waves_per_simd(int D, int NW, int CB) {
-  return D == 256 || CB > 1 ? 2 : NW > 4 ? 4 : 3;
+  return D == 256 || CB > 1 || NW > 4 ? 2 : 3;
 }
 
 // NW: wavefronts of a workgroup. One token per sequence: a block of 16 columns for each of
@@ -464,62 +464,84 @@ __global__ __launch_bounds__(64 * NW, waves_per_simd(D, NW, CB)) void attend_fp8
           nan_hi = or_over_row(nan_hi);
         }
       }
+      // Every step for all blocks of columns: their chains of dependent instructions overlap.
+      // (Block st is of head st, or all are of one head.)
+      constexpr int CPH = MULTI ? NS : 1;  // blocks per head
+      f32x4 s[NS][2];
 #pragma unroll
-      for (int st = 0; st < NS; ++st) {
-        const int hg = MULTI ? 0 : st;
-        float x[2][4];
-        float m = kNegInf;
+      for (int hg = 0; hg < HG; ++hg)
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          f32x4 s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int i = 0; i < SEG; ++i)
+          for (int cb = 0; cb < CPH; ++cb) s[hg * CPH + cb][t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int f = 0; f < NF; ++f)
-              s = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                  from_codes8(kf[t][hg][i][2 * f], kf[t][hg][i][2 * f + 1], kfs[t][hg]),
-                  qf[st][i * NF + f], s, 0, 0, 0);
-          if (!whole) {
+          for (int i = 0; i < NC; ++i) {
+            const frag& w = kf[t][hg][i / NF];
+            const f16x8 kk = from_codes8(w[i % NF * 2], w[i % NF * 2 + 1], kfs[t][hg]);
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-              if (t0 + 8 * grp + 4 * t + r > last[st]) s[r] = kNegInf;
-          }
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            x[t][r] = s[r];
-            m = fmaxf(m, s[r]);
+            for (int cb = 0; cb < CPH; ++cb)
+              s[hg * CPH + cb][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                  kk, qf[hg * CPH + cb][i], s[hg * CPH + cb][t], 0, 0, 0);
           }
         }
+      auto unseen = [&](int st, int t, int r) { return t0 + 8 * grp + 4 * t + r > last[st]; };
+      if (!whole) {
+#pragma unroll
+        for (int st = 0; st < NS; ++st)
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (unseen(st, i / 4, i % 4)) s[st][i / 4][i % 4] = kNegInf;
+      }
+      float m_new[NS];
+      bool grown = false;
+#pragma unroll
+      for (int st = 0; st < NS; ++st) {
+        float m = s[st][0][0];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) m = fmaxf(m, s[st][i / 4][i % 4]);
         // (A column that has seen nothing yet stays at -inf, whatever the scale: 0 * -inf
         // would be NaN.)
         m = over_groups(m, Max());
-        const float m_new = m == kNegInf ? m_run[st] : fmaxf(m_run[st], m * scale);
-        if (__ballot(m_new > m_run[st]) != 0) {  // wavefront-uniform
-          const float alpha = m_new == kNegInf ? 1.f : fast_exp2(m_run[st] - m_new);
+        m_new[st] = m == kNegInf ? m_run[st] : fmaxf(m_run[st], m * scale);
+        grown |= m_new[st] > m_run[st];
+      }
+      if (__ballot(grown) != 0) {  // wavefront-uniform
+#pragma unroll
+        for (int st = 0; st < NS; ++st) {
+          const float alpha = m_new[st] == kNegInf ? 1.f : fast_exp2(m_run[st] - m_new[st]);
           l_run[st] *= alpha;
 #pragma unroll
           for (int nd = 0; nd < ND; ++nd) acc[st][nd] *= alpha;
-          m_run[st] = m_new;
+          m_run[st] = m_new[st];
         }
+      }
+      f16x8 pb[NS];
+#pragma unroll
+      for (int st = 0; st < NS; ++st) {
         const float off = kBias - m_run[st];
-        f16x8 pb;
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int i = 0; i < 8; ++i)
+          pb[st][i] = (f16)fast_exp2(__builtin_fmaf(s[st][i / 4][i % 4], scale, off));
+      }
+      if (!whole) {
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            float p = fast_exp2(__builtin_fmaf(x[t][r], scale, off));
-            if (!whole) {
-              if constexpr (MULTI)
-                if ((t ? nan_hi : nan_lo) >> (8 * r + 7) & 1) p = __builtin_nanf("");
-              if (t0 + 8 * grp + 4 * t + r > last[st]) p = 0.f;
-            }
-            pb[4 * t + r] = (f16)p;
+        for (int st = 0; st < NS; ++st)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            if constexpr (MULTI)
+              if ((i / 4 ? nan_hi : nan_lo) >> (8 * (i % 4) + 7) & 1) pb[st][i] = (f16)__builtin_nanf("");
+            if (unseen(st, i / 4, i % 4)) pb[st][i] = (f16)0.f;
           }
+      }
+#pragma unroll
+      for (int st = 0; st < NS; ++st)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          l_run[st] = __builtin_amdgcn_fdot2(f16x2{pb[2 * i], pb[2 * i + 1]},
+          l_run[st] = __builtin_amdgcn_fdot2(f16x2{pb[st][2 * i], pb[st][2 * i + 1]},
                                              f16x2{(f16)1.f, (f16)1.f}, l_run[st], false);
-        // O^T += V^T P^T: operand index k = 8 grp + i stands for token 8 grp + i on both sides.
+      // O^T += V^T P^T: operand index k = 8 grp + i stands for token 8 grp + i on both sides.
+#pragma unroll
+      for (int hg = 0; hg < HG; ++hg)
 #pragma unroll
         for (int nd = 0; nd < ND; ++nd) {
           f16x8 av;
@@ -527,9 +549,11 @@ __global__ __launch_bounds__(64 * NW, waves_per_simd(D, NW, CB)) void attend_fp8
             av = from_codes8(vf[hg][nd].x, vf[hg][nd].y, vfs[hg]);
           else
             av = from_codes8(vf[hg][nd].x, vf[hg][nd].y, 1.f) * vft[hg];
-          acc[st][nd] = __builtin_amdgcn_mfma_f32_16x16x32_f16(av, pb, acc[st][nd], 0, 0, 0);
+#pragma unroll
+          for (int cb = 0; cb < CPH; ++cb)
+            acc[hg * CPH + cb][nd] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                av, pb[hg * CPH + cb], acc[hg * CPH + cb][nd], 0, 0, 0);
         }
-      }
     }
 
     // The wavefronts' states meet in LDS, four elements of accumulator row r at slot
