@@ -649,7 +649,9 @@ __global__ __launch_bounds__(64 * NW, waves_per_simd(D, NW, CB)) void attend_fp8
     const int parts = items < kThreads ? kThreads / items : 1;
     const int part = parts > 1 ? tid / items : 0;
     const int step = 2 * a.rec_floats * 4;  // bytes from part i to part i + 1, i > 0
-    constexpr int U = NW > 4 ? 8 : 16;
+    // U parts a round trip, for each of IPT items of a thread.
+    constexpr int IPT = MULTI && NW == 4 ? 4 : 1;
+    constexpr int U = NW > 4 ? 8 : 16 / IPT;
     auto fetch = [&](int i, int j, int d, f32x4 (&y)[U]) {  // past the last part: zeros
       const int at = (record(i) + j * D + d) * 4;
 #pragma unroll
@@ -670,14 +672,23 @@ __global__ __launch_bounds__(64 * NW, waves_per_simd(D, NW, CB)) void attend_fp8
       }
     };
 #pragma unroll 1
-    for (int base = 0; base < items; base += kThreads) {  // workgroup-uniform
-      const int item = parts > 1 ? tid - part * items : base + tid;
-      const bool live = part < parts && item < items;
-      const int j = live ? item / D4 : 0;
-      const int d = live ? (item - j * D4) * 4 : 0;
-      f32x4 y[U];
-      const f32x4 y0 = load_coherent16(rr, (j * D + d) * 4);
-      fetch(1 + part, j, d, y);
+    for (int base = 0; base < items; base += IPT * kThreads) {  // workgroup-uniform
+      bool live[IPT];
+      int j[IPT], d[IPT];
+      f32x4 y0[IPT], y[IPT][U];
+#pragma unroll
+      for (int k = 0; k < IPT; ++k) {
+        if (base + k * kThreads >= items) {  // workgroup-uniform
+          live[k] = false;
+          continue;
+        }
+        const int item = parts > 1 ? tid - part * items : base + k * kThreads + tid;
+        live[k] = part < parts && item < items;
+        j[k] = live[k] ? item / D4 : 0;
+        d[k] = live[k] ? (item - j[k] * D4) * 4 : 0;
+        y0[k] = load_coherent16(rr, (j[k] * D + d[k]) * 4);
+        fetch(1 + part, j[k], d[k], y[k]);
+      }
       if (base == 0) {
 #pragma unroll 1
         for (int s0 = 0; s0 < nseg; s0 += batch) {
@@ -703,8 +714,9 @@ __global__ __launch_bounds__(64 * NW, waves_per_simd(D, NW, CB)) void attend_fp8
         }
         __syncthreads();
       }
-      const float M = s_max[j];
-      f32x4 o = {0.f, 0.f, 0.f, 0.f};
+      f32x4 o[IPT];
+#pragma unroll
+      for (int k = 0; k < IPT; ++k) o[k] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
       for (int s0 = 0; s0 < nseg; s0 += batch) {
         const int s1 = min(nseg, s0 + batch);
@@ -713,31 +725,36 @@ __global__ __launch_bounds__(64 * NW, waves_per_simd(D, NW, CB)) void attend_fp8
           load_ml(s0, s1);
           __syncthreads();
         }
-        if (live) {
-          const float* pm = s_pm + j * batch - s0;
-          if (s0 == 0 && part == 0) o += share(pm[0], M) * y0;
+#pragma unroll
+        for (int k = 0; k < IPT; ++k) {
+          if (!live[k]) continue;
+          const float M = s_max[j[k]];
+          const float* pm = s_pm + j[k] * batch - s0;
+          if (s0 == 0 && part == 0) o[k] += share(pm[0], M) * y0[k];
 #pragma unroll 1
           for (int i = s0 ? s0 + part : 1 + part; i < s1; i += U * parts) {
-            if (i != 1 + part) fetch(i, j, d, y);
+            if (i != 1 + part) fetch(i, j[k], d[k], y[k]);
 #pragma unroll
             for (int u = 0; u < U; ++u)
-              if (i + u * parts < s1) o += share(pm[i + u * parts], M) * y[u];
+              if (i + u * parts < s1) o[k] += share(pm[i + u * parts], M) * y[k][u];
           }
         }
       }
       if (parts > 1) {
-        s_part[tid] = o;
+        s_part[tid] = o[0];
         __syncthreads();
         if (part == 0)
-          for (int p = 1; p < parts; ++p) o += s_part[item + p * items];
+          for (int p = 1; p < parts; ++p) o[0] += s_part[tid + p * items];
       }
-      if (live && part == 0) {
-        const float sum = s_sum[j];
+#pragma unroll
+      for (int k = 0; k < IPT; ++k) {
+        if (!live[k] || part != 0) continue;
+        const float sum = s_sum[j[k]];
         const float inv = sum == 0.f ? 0.f : 1.f / sum;  // 0: no key at all
         f16x4 z;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) z[e] = (f16)(o[e] * inv);
-        *reinterpret_cast<f16x4*>(out_row(j) + d) = z;
+        for (int e = 0; e < 4; ++e) z[e] = (f16)(o[k][e] * inv);
+        *reinterpret_cast<f16x4*>(out_row(j[k]) + d[k]) = z;
       }
     }
     if (tid == 0) __hip_atomic_store(cnt, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -819,11 +836,12 @@ __global__ __launch_bounds__(64 * NW, waves_per_simd(D, NW, CB)) void attend_fp8
       if (at >= x1) return;
       c0 = max(0, min(n, x0 - at - a.pair_cost));
       c1 = max(0, min(n, x1 - at - a.pair_cost));
-      w0 = ranges.of(at);
-      w1 = ranges.of(at + span - 1);
+      // The ranges that hold chunks of it (of no chunks: the one that holds its start).
+      w0 = ranges.of(at + (n ? a.pair_cost : 0));
+      w1 = n ? ranges.of(at + span - 1) : w0;
       at += span;
     }
-    segment(b, g0 * HG, L, c0, c1, w0, w - w0, w1 - w0 + 1);
+    if (w >= w0 && w <= w1) segment(b, g0 * HG, L, c0, c1, w0, w - w0, w1 - w0 + 1);
     if (!a.ranged || at >= x1) return;
     if (++g0 == groups) {
       g0 = 0;
@@ -836,7 +854,7 @@ __global__ __launch_bounds__(64 * NW, waves_per_simd(D, NW, CB)) void attend_fp8
 
 // List positions of 32 tokens: what a pair costs beside its chunks, and the fewest a
 // range takes.
-constexpr int kPairCost = 8;
+constexpr int kPairCost = 16;
 constexpr int kMinRange = 16;
 // Tables of at most this many tokens take one workgroup per pair; of the second, where
 // the pairs fill at least half the compute units.
