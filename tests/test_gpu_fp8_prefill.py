@@ -69,6 +69,22 @@ def test_drafts(cuda_device, hq, hkv, d, bs):
     check(pool, queries(sum(new), hq, d, 2, cuda_device), new, d ** -0.5)
 
 
+@pytest.mark.parametrize("longest", [60, 2540])
+@pytest.mark.parametrize("most", [1, 3, 9])
+@pytest.mark.parametrize("seqs", [20, 40, 140, 290])
+@pytest.mark.parametrize("hq,hkv,d", [(14, 2, 64), (4, 2, 32), (6, 3, 128)])
+def test_drafts_of_many_sequences(cuda_device, hq, hkv, d, seqs, most, longest):
+    """One token each at most, and more, for pair counts around the compute units', tables of
+    whole pairs and of ranges."""
+    g = torch.Generator().manual_seed(seqs + most)
+    new = torch.randint(0, most + 1, (seqs,), generator=g).tolist()
+    new[seqs // 2] = most
+    lens = [n + int(x) for n, x in zip(new, torch.randint(0, 50, (seqs,), generator=g))]
+    lens[1], new[1] = longest, 1
+    pool = Fp8Pool(lens, hkv, d, 16, seed=seqs, device=cuda_device)
+    check(pool, queries(sum(new), hq, d, 3, cuda_device), new, d ** -0.5)
+
+
 def test_split_keys(cuda_device):
     """One long context: its keys are split over workgroups; the same bits every time."""
     pool = Fp8Pool([9000], 2, 64, 16, seed=3, device=cuda_device)

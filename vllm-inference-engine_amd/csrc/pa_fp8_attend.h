@@ -4,29 +4,35 @@
 //   so far, K and V rows = e4m3 code * scale[block, kv head]
 //
 // Work split. The work is a list of (sequence, group of HG adjacent kv heads) pairs, each
-// of its 32-token chunks plus a fixed cost; a grid of a few workgroups per compute unit
+// of its 32-token chunks plus a fixed cost; a grid of one or two workgroups per compute unit
 // takes equal contiguous ranges of it, so every workgroup reads about the same bytes
 // however lengths differ. Each wavefront derives the plan for itself, from the lengths,
-// with lane scans: no memory, no barrier. Where every pair is short a workgroup takes one
-// pair whole and there is no plan. Within a pair's part of its range, a workgroup's four
-// wavefronts take the chunks in turn, each with its own online softmax for the whole
-// query group, and meet in LDS at the end. A pair inside one range is written as fp16
+// with lane scans: no memory, no barrier (1.3 us). Where every pair is short a workgroup
+// takes one pair whole and there is no plan. Within a pair's part of its range, a
+// workgroup's wavefronts take the chunks in turn, each with its own online softmax for the
+// whole query group, and meet in LDS at the end. A pair inside one range is written as fp16
 // there; a pair cut by range boundaries leaves fp32 partial records, and the last of its
 // workgroups to arrive combines them by log-sum-exp in list order (the same bits on
 // every run).
 //
 // Per chunk. K and V codes go from memory straight into LDS (buffer_load ... lds), whole
 // rows of HG heads by neighbouring lanes: no registers are held while they are on their
-// way, which leaves room for sixteen wavefronts per compute unit with 8 KB each in flight
-// (a gather of 2 KB blocks needs about 128 KB per compute unit to reach this memory's
-// rate). From there K is read in the operand layout of S^T = K Q^T and V by transposing
-// reads of bytes (ds_read_b64_tr_b8) in that of O^T += V^T P^T, both
-// v_mfma_f32_16x16x32_f16. Codes become fp16 in v_cvt_scalef32_pk_f16_fp8 with the scale
-// applied, exactly: the products and sums are those of an fp16 cache that holds the same
-// values. All fragments are in registers before the next chunk's loads are issued into
-// the same LDS, and the arithmetic runs under those loads. Each wavefront has its own LDS,
-// without barriers. The 16-byte pieces of a row are permuted by the row's number (by the
-// lanes' addresses when loading), so that neither kind of read meets a bank twice.
+// way, and eight wavefronts per compute unit have 8 KB each in flight. From there K is read
+// in the operand layout of S^T = K Q^T and V by transposing reads of bytes
+// (ds_read_b64_tr_b8) in that of O^T += V^T P^T, both v_mfma_f32_16x16x32_f16. Codes become
+// fp16 in v_cvt_scalef32_pk_f16_fp8 with the scale applied, exactly: the products and sums
+// are those of an fp16 cache that holds the same values. All fragments are in registers
+// before the next chunk's loads are issued into the same LDS, and the arithmetic runs under
+// those loads. Each wavefront has its own LDS, without barriers. The 16-byte pieces of a row
+// are permuted by the row's number (by the lanes' addresses when loading), so that neither
+// kind of read meets a bank twice.
+//
+// Bounds on MI355X (head_dim 64, 14 / 2 heads, block 16, unless stated). 256 sequences of
+// 1.2M tokens in all (316 MB): memory, 62.5 us, 5.1 TB/s, where a gather of such 2 KB blocks
+// alone reaches 6.3. 8 sequences of 1k to 8k at 32 / 8 heads of 128 (73 MB): 22.8 us, of
+// which the streaming takes about 12; the rest is the chain launch -> plan -> first ids ->
+// first chunk, and meeting, arrival and merge. One sequence: chains alone, 14.3 us at 24001
+// tokens (4.5 of them the merge of 47 parts) and 6.0 at 300 tokens.
 //
 // Probabilities are rounded to fp16 (the denominators sum the rounded ones), scaled by
 // 2^14 so that they keep 11 bits down to 2^-28 of the largest: half a step, 2^-12
@@ -36,7 +42,9 @@
 // of one sequence and kv head, token-major, fill up to CB blocks of 16, which share every
 // K and V fragment; a column sees the keys up to its token's position. A NaN in a V row
 // reaches only the columns that see it: where some column does not see the whole chunk,
-// NaN codes are cleared and the probabilities of their tokens become NaN instead.
+// NaN codes are cleared and the probabilities of their tokens become NaN instead. 16
+// sequences of 0.3k to 4k tokens and 5 drafts at 32 / 8 heads of 128 (90 MB): 30 us, about 14
+// of them streaming.
 #pragma once
 
 #include <type_traits>
@@ -185,7 +193,8 @@ __device__ inline int swizzle(int r) {
   return NP >= 8 ? f : NP == 4 ? f >> 1 : f >> 2;
 }
 
-// Wavefronts per SIMD that the registers are kept to.
+// Wavefronts per SIMD that the registers are kept to. (A workgroup of eight is its compute
+// unit's only one, and spills nothing then: blocks of 8 tokens 36.8 -> 26.2 us.)
 constexpr int waves_per_simd(int D, int NW, int CB) {
   return D == 256 || CB > 1 || NW > 4 ? 2 : 3;
 }
@@ -852,12 +861,17 @@ __global__ __launch_bounds__(64 * NW, waves_per_simd(D, NW, CB)) void attend_fp8
 
 // ---- launch plan, shared by the two sources that launch the kernel ----
 
-// List positions of 32 tokens: what a pair costs beside its chunks, and the fewest a
-// range takes.
+// List positions of 32 tokens: what a pair costs beside its chunks (its beginning, meeting,
+// arrival and merge), and the fewest a range takes. Measured on MI355X at 8 / 16 / 32: the
+// cost, 256 x ~4.6k tokens 66.8 / 64.4 / 67.1 us, 16 x 5 drafts 33.8 / 33.6 / 34.6, 20 x 4
+// drafts at head_dim 64 17.5 / 15.3 / 15.2, 64 x 5 drafts of up to 4k 74.5 / 79.0 / 78.9; the
+// range, one sequence of 24001 tokens 17.9 / 15.9 / 17.4, 8 of 1k to 8k 25.2 / 24.6 / 24.6.
 constexpr int kPairCost = 16;
 constexpr int kMinRange = 16;
 // Tables of at most this many tokens take one workgroup per pair; of the second, where
-// the pairs fill at least half the compute units.
+// the pairs fill at least half the compute units. Whole pairs against ranges, measured: 8 x
+// 1024 tokens at 32 / 8 heads 12.5 against 15.2 us, 8 x 2k 19.5 against 15.8; 64 x 2k at 14 / 2
+// heads 13.4 against 16.5, 512 x 2k 33.3 against 40.1, 64 x 5 drafts of up to 4k 77 against 68.
 constexpr int kWholePairs = 1024;
 constexpr int kWholePairsBusy = 2048;
 
@@ -876,7 +890,7 @@ struct DecodePlan {
   }
 };
 
-// For new_tokens query tokens per sequence at most (1: the one-token form).
+// For the form of up to new_tokens query tokens per sequence, or 0: the one-token form.
 DecodePlan decode_plan(int num_seqs, int num_q_heads, int num_kv_heads, int head_dim,
                        int block_size, int max_blocks, int new_tokens);
 
