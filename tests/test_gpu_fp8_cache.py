@@ -227,6 +227,7 @@ def test_offsets_past_32_bits(cuda_device):
     assert torch.equal(key, want)
 
 
+@torch.inference_mode()  # as every capture among these tests: torch's generator state may be one of it
 def test_on_another_stream_and_in_a_graph(cuda_device):
     """A captured write and read, replayed on changing rows with eager work between."""
     lens, new = [50, 20, 128], [3, 20, 1]

@@ -122,6 +122,7 @@ def test_emitted_tokens_follow_the_target(cuda_device, draft_given):
     assert np.abs(got - p).max() <= 2 / 64
 
 
+@torch.inference_mode()  # as every capture among these tests: torch's generator state may be one of it
 def test_two_graphs_and_eager_calls_share_nothing(cuda_device):
     """Two captured calls of other sizes, replayed in turn and at once on two streams, with eager
     calls between."""

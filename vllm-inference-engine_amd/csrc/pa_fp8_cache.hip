@@ -12,8 +12,11 @@
 // One wavefront takes one (block, kv head, cache): the maximum is a reduction over
 // its lanes, no other wavefront reads or writes that scale or those rows, and the
 // fp16 rows are read once (up to 256 pieces of 16 bytes stay in registers between
-// the maximum and the codes). Bound by memory at prompts, by the chain length ->
-// table entry -> scale -> store at single tokens.
+// the maximum and the codes; each lane finds its pieces by steps, not divisions: prompts
+// 18.2 -> 16.2 us). Bound by memory at prompts, by the chain length -> table entry -> scale ->
+// store at single tokens. On MI355X: four prompts of 9.6k rows in all at 8 heads of 128 (59
+// MB) 15.3 us, 3.9 TB/s; a decode step's row for each of 128 sequences at 2 heads of 64 4.4
+// us, little more than a launch.
 #include "../../include/paged_attention.h"
 #include "pa_fp8.h"
 
@@ -185,7 +188,11 @@ __global__ __launch_bounds__(256) void write_kernel(WriteArgs a) {
 // block are found once (16 lanes, the first row's sequence by a wavefront search and
 // the others' from there) and kept in LDS; then the threads take 16-code pieces of
 // the rows' keys and values. Rows without a slot are written as zeros. Bound by
-// memory: one byte read and two written per value.
+// memory: one byte read and two written per value. On MI355X 37.5k rows at 8 heads of 128
+// (231 MB) in 57.7 us, 4.0 TB/s where a large copy reaches 4.75; 8192 rows at 2 heads of 64
+// (6.3 MB) in 5.4. Two, four or eight pieces per
+// thread on their way at a time (54.1 us for 51.9 in a graph), and stores past the caches
+// (54.5), were slower than one piece after the other in many workgroups.
 constexpr int kReadRows = 16;
 
 template <bool VEC>

