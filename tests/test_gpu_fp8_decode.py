@@ -56,6 +56,20 @@ def test_many_sequences(cuda_device, hq, hkv, d, bs, n, longest):
     check(pool, queries(len(lens), hq, d, 4, cuda_device), d ** -0.5)
 
 
+@pytest.mark.parametrize("hq,hkv,d", [(14, 2, 64), (4, 2, 32), (8, 2, 128), (3, 1, 256)])
+@pytest.mark.parametrize("n", [3, 90, 257, 700])
+def test_ranges_of_mostly_empty_sequences(cuda_device, hq, hkv, d, n):
+    """A long sequence among short and empty ones: range boundaries fall on what a pair costs
+    beside its chunks, and the lengths are read in several turns."""
+    g = torch.Generator().manual_seed(n)
+    lens = torch.randint(0, 45, (n,), generator=g).tolist()
+    lens[n // 3], lens[n - 1], lens[0] = 2700, 1333, 0
+    pool = Fp8Pool(lens, hkv, d, 16, seed=n, device=cuda_device, slack=1)
+    q = queries(n, hq, d, 5, cuda_device)
+    out = check(pool, q, d ** -0.5)
+    assert torch.equal(paged_attention_decode_fp8(q, *pool.args(), d ** -0.5), out)
+
+
 @pytest.mark.parametrize("hq,hkv,d,bs,lens", [
     (14, 2, 64, 16, [24001]), (8, 1, 128, 16, [9000, 5, 0, 4097]), (16, 2, 256, 32, [5000, 260]),
     (2, 2, 64, 8, [3000, 2999, 1]), (4, 2, 32, 7, [2500])])
