@@ -68,20 +68,41 @@ __device__ inline double weight(float p, float q) {
   return d > 0.0 ? d : 0.0;
 }
 
-// Sum over a wavefront, in every lane: rotations within rows of 16, then exchanges of rows.
+// x of another lane of the row of 16 (a data-parallel-primitive control word), 0 where there
+// is none.
+template <int CTRL>
+__device__ inline double row_lane(double x) {
+  const uint2 v = __builtin_bit_cast(uint2, x);
+  return __builtin_bit_cast(
+      double, make_uint2((unsigned)__builtin_amdgcn_update_dpp(0, (int)v.x, CTRL, 0xf, 0xf, false),
+                         (unsigned)__builtin_amdgcn_update_dpp(0, (int)v.y, CTRL, 0xf, 0xf, false)));
+}
+
+// Lane l's x, l uniform.
+__device__ inline double lane_of(double x, int l) {
+  const uint2 v = __builtin_bit_cast(uint2, x);
+  return __builtin_bit_cast(double, make_uint2((unsigned)__builtin_amdgcn_readlane((int)v.x, l),
+                                               (unsigned)__builtin_amdgcn_readlane((int)v.y, l)));
+}
+
+// Sum over a wavefront, in every lane: rotations within rows of 16, then the rows.
 __device__ inline double wave_sum(double x) {
-  auto parts = [](double v) { return __builtin_bit_cast(uint2, v); };
-  auto whole = [](unsigned lo, unsigned hi) { return __builtin_bit_cast(double, make_uint2(lo, hi)); };
-#define PA_TURNED(ctrl)                                                                       \
-  whole((unsigned)__builtin_amdgcn_update_dpp(0, (int)parts(x).x, ctrl, 0xf, 0xf, false),     \
-        (unsigned)__builtin_amdgcn_update_dpp(0, (int)parts(x).y, ctrl, 0xf, 0xf, false))
-  x += PA_TURNED(0x128);
-  x += PA_TURNED(0x124);
-  x += PA_TURNED(0x122);
-  x += PA_TURNED(0x121);
-#undef PA_TURNED
-  x += __shfl_xor(x, 16);
-  return x + __shfl_xor(x, 32);
+  x += row_lane<0x128>(x);
+  x += row_lane<0x124>(x);
+  x += row_lane<0x122>(x);
+  x += row_lane<0x121>(x);
+  return (lane_of(x, 0) + lane_of(x, 16)) + (lane_of(x, 32) + lane_of(x, 48));
+}
+
+// Sums over the lanes up to each: shifts within rows of 16, then the rows before.
+__device__ inline double wave_scan(double x, int lane) {
+  x += row_lane<0x111>(x);
+  x += row_lane<0x112>(x);
+  x += row_lane<0x114>(x);
+  x += row_lane<0x118>(x);
+  const double r0 = lane_of(x, 15), r1 = lane_of(x, 31), r2 = lane_of(x, 47);
+  const double before = lane < 16 ? 0.0 : lane < 32 ? r0 : lane < 48 ? r0 + r1 : (r0 + r1) + r2;
+  return before + x;
 }
 
 // One lane's entries [v0, v0 + 4) of a row: p and q, zeros past the vocabulary. WHOLE: there
@@ -112,9 +133,8 @@ __device__ inline void load4(const Args& a, const Weights& w, int v0, float (&p)
 
 template <bool VEC>
 __global__ __launch_bounds__(kThreads, 4) void verify_kernel(Args a) {
-  __shared__ double s_before[kWaves];
-  __shared__ int s_flag;
-  __shared__ int s_best, s_last;
+  __shared__ double s_sum[kWaves];
+  __shared__ int s_flag, s_found[kWaves], s_some[kWaves];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int b = blockIdx.x / a.groups;
   const int group = blockIdx.x - b * a.groups;
@@ -230,12 +250,7 @@ __global__ __launch_bounds__(kThreads, 4) void verify_kernel(Args a) {
       own4[i] = whole ? x[1][i] : x[0][i];
       mine += own4[i];
     }
-    double incl = mine;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const double y = __shfl_up(incl, off);
-      if (lane >= off) incl += y;
-    }
+    const double incl = wave_scan(mine, lane);
     double sum = run + (incl - mine);
     int over = -1, some = -1;
     double over_before = 0.0, some_before = 0.0;
@@ -254,15 +269,15 @@ __global__ __launch_bounds__(kThreads, 4) void verify_kernel(Args a) {
     const uint64_t overs = __ballot(over >= 0), somes = __ballot(some >= 0);
     if (overs) {
       const int l = (int)__builtin_ctzll(overs);
-      at = first + 4 * l + __shfl(over, l);
-      before = __shfl(over_before, l);
+      at = first + 4 * l + __builtin_amdgcn_readlane(over, l);
+      before = lane_of(over_before, l);
     }
     if (somes) {
       const int l = 63 - (int)__builtin_clzll(somes);
-      last = first + 4 * l + __shfl(some, l);
-      last_before = __shfl(some_before, l);
+      last = first + 4 * l + __builtin_amdgcn_readlane(some, l);
+      last_before = lane_of(some_before, l);
     }
-    run += __shfl(incl, 63);
+    run += lane_of(incl, 63);
   }
   if (at < 0) {  // u' * total not below the sum of all, by rounding or u' >= 1
     at = last;
@@ -270,10 +285,6 @@ __global__ __launch_bounds__(kThreads, 4) void verify_kernel(Args a) {
   }
 
   // The index within the piece: thread t now holds four consecutive entries.
-  if (tid == 0) {
-    s_best = 0x7fffffff;
-    s_last = -1;
-  }
   constexpr int kPer = kPiece / kThreads;
   static_assert(kPer == 4, "one load4 per thread");
   float ep[4], eq[4];
@@ -282,38 +293,46 @@ __global__ __launch_bounds__(kThreads, 4) void verify_kernel(Args a) {
   else
     load4<false>(a, w, at * kPiece + tid * kPer, ep, eq);
   double e[kPer], mine = 0.0;
-  int mine_last = -1;
+  int some = -1;  // the thread's last entry with any weight
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     e[i] = weight(ep[i], eq[i]);
     mine += e[i];
-    if (e[i] > 0.0) mine_last = i;
+    if (e[i] > 0.0) some = i;
   }
-  double incl = mine;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const double y = __shfl_up(incl, off);
-    if (lane >= off) incl += y;
-  }
-  if (lane == 63) s_before[wave] = incl;
+  const double incl = wave_scan(mine, lane);
+  if (lane == 63) s_sum[wave] = incl;
   __syncthreads();
   double sum = before + (incl - mine);
-  for (int i = 0; i < wave; ++i) sum += s_before[i];
-  int found = 0x7fffffff;
+  for (int i = 0; i < wave; ++i) sum += s_sum[i];
+  int found = -1;  // and the first whose sum exceeds aim
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     sum += e[i];
-    if (e[i] > 0.0 && sum > aim && found == 0x7fffffff) found = tid * kPer + i;
+    if (e[i] > 0.0 && sum > aim && found < 0) found = i;
   }
-  if (found != 0x7fffffff) atomicMin(&s_best, found);
-  if (mine_last >= 0) atomicMax(&s_last, tid * kPer + mine_last);
+  // Per wavefront the first of the ones and the last of the others, or -1.
+  const uint64_t founds = __ballot(found >= 0), somes = __ballot(some >= 0);
+  const int fl = founds ? (int)__builtin_ctzll(founds) : 0;
+  const int sl = somes ? 63 - (int)__builtin_clzll(somes) : 0;
+  const int fi = __builtin_amdgcn_readlane(found, fl), si = __builtin_amdgcn_readlane(some, sl);
+  if (lane == 0) {
+    s_found[wave] = founds ? (wave * 64 + fl) * kPer + fi : -1;
+    s_some[wave] = somes ? (wave * 64 + sl) * kPer + si : -1;
+  }
   __syncthreads();
   int64_t* out = a.tokens + (int64_t)b * (a.k + 1);
   if (tid <= a.k) {
-    // With no weight anywhere: index 0.
-    const int64_t next = s_best != 0x7fffffff ? (int64_t)at * kPiece + s_best
-                                              : (s_last >= 0 ? (int64_t)at * kPiece + s_last : 0);
-    out[tid] = tid < n ? a.ids[b * a.i_sb + tid * a.i_si] : (tid == n ? next : -1);
+    int best = -1, spare = -1;
+#pragma unroll
+    for (int i = kWaves - 1; i >= 0; --i) {
+      best = s_found[i] >= 0 ? s_found[i] : best;
+      spare = spare >= 0 ? spare : s_some[i];
+    }
+    if (best < 0) best = spare;
+    // With no weight anywhere: index 0. (Lane i of the first wavefront holds id i.)
+    const int64_t next = best >= 0 ? (int64_t)at * kPiece + best : 0;
+    out[tid] = tid < n ? id : (tid == n ? next : -1);
   }
   if (tid == 0) {
     a.accepted[b] = n;
