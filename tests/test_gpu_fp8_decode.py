@@ -72,7 +72,8 @@ def test_ranges_of_mostly_empty_sequences(cuda_device, hq, hkv, d, n):
 
 @pytest.mark.parametrize("hq,hkv,d,bs,lens", [
     (14, 2, 64, 16, [24001]), (8, 1, 128, 16, [9000, 5, 0, 4097]), (16, 2, 256, 32, [5000, 260]),
-    (2, 2, 64, 8, [3000, 2999, 1]), (4, 2, 32, 7, [2500])])
+    (2, 2, 64, 8, [3000, 2999, 1]), (4, 2, 32, 7, [2500]),
+    (16, 1, 32, 16, [90000])])  # (the last: more parts of a pair than the merge takes at once)
 def test_long_contexts_are_split(cuda_device, hq, hkv, d, bs, lens):
     pool = Fp8Pool(lens, hkv, d, bs, seed=5, device=cuda_device)
     q = queries(len(lens), hq, d, 6, cuda_device)

@@ -94,6 +94,14 @@ def test_split_keys(cuda_device):
         assert torch.equal(run(pool, q, [6], 0.125), out)
 
 
+def test_more_parts_than_a_merge_takes_at_once(cuda_device):
+    pool = Fp8Pool([90000], 1, 32, 16, seed=4, device=cuda_device)
+    q = queries(4, 16, 32, 5, cuda_device)
+    out = check(pool, q, [4], 0.2)
+    for _ in range(3):
+        assert torch.equal(run(pool, q, [4], 0.2), out)
+
+
 @pytest.mark.parametrize("scale", [4.0, 1e-3])
 def test_peaked_and_flat(cuda_device, scale):
     pool = Fp8Pool([500, 40], 2, 64, 16, seed=5, device=cuda_device)

@@ -645,7 +645,7 @@ __global__ __launch_bounds__(64 * NW, waves_per_simd(D, NW, CB)) void attend_fp8
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
 
     // Merge: every part's maxima and denominators into LDS (batches of parts, as many as
-    // fit), their maximum and sum per head by 16 lanes each, and the accumulators by
+    // fit), their maximum, sum and shares per head by 16 lanes each, and the accumulators by
     // threads (item: head and four of its elements; the parts of an item are dealt over as
     // many threads as there are for it), U parts a round trip, the first ones on their way
     // before anything else. Part 0 lies apart from the others, which are two records apart.
@@ -725,7 +725,11 @@ __global__ __launch_bounds__(64 * NW, waves_per_simd(D, NW, CB)) void attend_fp8
             for (int i = row; i < s1 - s0; i += 16) M = fmaxf(M, s_pm[jj * batch + i]);
             M = over_row(M, Max());
             float sum = 0.f;
-            for (int i = row; i < s1 - s0; i += 16) sum += s_pl[jj * batch + i] * share(s_pm[jj * batch + i], M);
+            for (int i = row; i < s1 - s0; i += 16) {
+              const float f = share(s_pm[jj * batch + i], M);
+              sum += s_pl[jj * batch + i] * f;
+              s_pm[jj * batch + i] = f;
+            }
             sum = over_row(sum, Sum());
             if (s0) sum += s_sum[jj] * share(had, M);
             if (row == 0) {
@@ -742,23 +746,28 @@ __global__ __launch_bounds__(64 * NW, waves_per_simd(D, NW, CB)) void attend_fp8
 #pragma unroll 1
       for (int s0 = 0; s0 < nseg; s0 += batch) {
         const int s1 = min(nseg, s0 + batch);
-        if (batch < nseg) {  // the batch's maxima again
+        if (batch < nseg) {  // the batch's shares, of the maxima over all batches
           __syncthreads();
           load_ml(tid, s0, s1);
+          __syncthreads();
+          for (int i = tid; i < heads * (s1 - s0); i += kThreads) {
+            const int j = i / (s1 - s0);
+            float& x = s_pm[j * batch + i - j * (s1 - s0)];
+            x = share(x, s_max[j]);
+          }
           __syncthreads();
         }
 #pragma unroll
         for (int k = 0; k < IPT; ++k) {
           if (!live[k]) continue;
-          const float M = s_max[j[k]];
           const float* pm = s_pm + j[k] * batch - s0;
-          if (s0 == 0 && part == 0) o[k] += share(pm[0], M) * y0[k];
+          if (s0 == 0 && part == 0) o[k] += pm[0] * y0[k];
 #pragma unroll 1
           for (int i = s0 ? s0 + part : 1 + part; i < s1; i += U * parts) {
             if (i != 1 + part) fetch(i, j[k], d[k], y[k]);
 #pragma unroll
             for (int u = 0; u < U; ++u)
-              if (i + u * parts < s1) o[k] += share(pm[i + u * parts], M) * y[k][u];
+              if (i + u * parts < s1) o[k] += pm[i + u * parts] * y[k][u];
           }
         }
       }
