@@ -28,11 +28,11 @@
 // kind of read meets a bank twice.
 //
 // Bounds on MI355X (head_dim 64, 14 / 2 heads, block 16, unless stated). 256 sequences of
-// 1.2M tokens in all (316 MB): memory, 62.5 us, 5.1 TB/s, where a gather of such 2 KB blocks
-// alone reaches 6.3. 8 sequences of 1k to 8k at 32 / 8 heads of 128 (73 MB): 22.8 us, of
+// 1.2M tokens in all (316 MB): memory, 61.7 us, 5.1 TB/s, where a gather of such 2 KB blocks
+// alone reaches 6.3. 8 sequences of 1k to 8k at 32 / 8 heads of 128 (73 MB): 22.4 us, of
 // which the streaming takes about 12; the rest is the chain launch -> plan -> first ids ->
-// first chunk, and meeting, arrival and merge. One sequence: chains alone, 14.3 us at 24001
-// tokens (4.5 of them the merge of 47 parts) and 6.0 at 300 tokens.
+// first chunk, and meeting, arrival and merge. One sequence: chains alone, 13.2 us at 24001
+// tokens (3.7 of them the merge of 47 parts) and 5.7 at 300 tokens.
 //
 // Probabilities are rounded to fp16 (the denominators sum the rounded ones), scaled by
 // 2^14 so that they keep 11 bits down to 2^-28 of the largest: half a step, 2^-12
