@@ -56,7 +56,7 @@ def test_many_sequences(cuda_device, hq, hkv, d, bs, n, longest):
     check(pool, queries(len(lens), hq, d, 4, cuda_device), d ** -0.5)
 
 
-@pytest.mark.parametrize("hq,hkv,d", [(14, 2, 64), (4, 2, 32), (8, 2, 128), (3, 1, 256)])
+@pytest.mark.parametrize("hq,hkv,d", [(14, 2, 64), (32, 2, 64), (64, 4, 32), (4, 2, 32), (8, 2, 128), (3, 1, 256)])
 @pytest.mark.parametrize("n", [3, 90, 257, 700])
 def test_ranges_of_mostly_empty_sequences(cuda_device, hq, hkv, d, n):
     """A long sequence among short and empty ones: range boundaries fall on what a pair costs

@@ -11,10 +11,17 @@ DecodePlan decode_plan(int num_seqs, int num_q_heads, int num_kv_heads, int head
   DecodePlan p{};
   const int n = device_cus();
   const bool multi = new_tokens > 0;
-  p.head_group = !multi && head_dim <= 64 && num_kv_heads % 2 == 0 &&
-                         (int64_t)num_seqs * num_kv_heads > n ? 2 : 1;
-  const int64_t pairs = (int64_t)num_seqs * (num_kv_heads / p.head_group);
   const int64_t cap = (int64_t)max_blocks * block_size;
+  // Two kv heads per pair read rows of twice the bytes and halve the merges. Measured on
+  // MI355X at 14 / 2 heads of 64, one head against two, (sequence, head) pairs more than
+  // compute units: 256 x ~4.6k tokens 106 against 66 us, 140 x 4k 33.6 against 25.8 (300 x 1k
+  // 16.3 against 16.7); fewer, in ranges: 128 x 4k 29.9 against 24.7, 64 x 4k 19.7 against
+  // 19.8, 8 x 4k 13.2 against 15.2, and 12 x 4k at 16 heads 36.7 against 24.7; fewer, as whole
+  // pairs: 100 x 2k 13.9 against 19.5.
+  const int64_t total = (int64_t)num_seqs * num_kv_heads;
+  p.head_group = !multi && head_dim <= 64 && num_kv_heads % 2 == 0 &&
+                         (total > n || (2 * total > n && cap > kWholePairsBusy)) ? 2 : 1;
+  const int64_t pairs = total / p.head_group;
   // Few pairs: one workgroup of eight wavefronts per compute unit, which halves the parts of
   // a merge, instead of two of four. Measured on MI355X: one sequence of 24001 tokens 16.5
   // against 18.4 us, of 300 5.9 against 6.8; 4 x 5 drafts of 8k 31.5 against 33.5.
