@@ -661,12 +661,12 @@ __global__ __launch_bounds__(64 * NW, waves_per_simd(D, NW, CB)) void attend_fp8
     // U parts a round trip, for each of IPT items of a thread.
     constexpr int IPT = MULTI && NW == 4 ? 4 : 1;
     constexpr int U = NW > 4 ? 8 : 16 / IPT;
-    auto fetch = [&](int i, int j, int d, f32x4 (&y)[U]) {  // past the last part: zeros
+    // Past the last part: zeros. (By the lane's offset, whole: a scalar offset's part in the
+    // check against the resource's end is not specified.)
+    auto fetch = [&](int i, int j, int d, f32x4 (&y)[U]) {
       const int at = (record(i) + j * D + d) * 4;
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        y[u] = __builtin_bit_cast(
-            f32x4, __builtin_amdgcn_raw_buffer_load_b128(rr, at, u * parts * step, 16));
+      for (int u = 0; u < U; ++u) y[u] = load_coherent16(rr, at + u * parts * step);
     };
     // (As above: no maximum, and so zeros or NaN.)
     auto share = [&](float m, float M) { return m == kNegInf ? 1.f : fast_exp2(m - M); };

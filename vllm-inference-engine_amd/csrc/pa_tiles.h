@@ -60,7 +60,10 @@ __device__ inline u32x4 load_stream(const f16* p) {
 // past the end of the work is issued with bytes = 0 instead of being skipped:
 // the loop then has no branches around its loads, and the compiler's count of
 // loads in flight stays exact (a skipped load on one path would force every
-// wait to assume the shorter path and drain the pipeline).
+// wait to assume the shorter path and drain the pipeline). Where a resource ends
+// before some of what is asked of it, the whole offset goes into the lane's
+// operand, which is what the end is specified to be compared with; a uniform
+// offset only where the resource is empty or covers all of it.
 __device__ inline __amdgpu_buffer_rsrc_t tile_rsrc(const void* base, int bytes) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, bytes, 0x00020000);
 }
