@@ -574,18 +574,19 @@ __global__ __launch_bounds__(64 * NW) void prefill_attn_kernel(PrefillAttnArgs a
             m[k] = in ? load_coherent4(rr, rb + cl * 4) : kNegInf;
             l[k] = in ? load_coherent4(rr, rb + (COLS + cl) * 4) : 0.f;
           }
-          // A split that saw no key of this column has m = -inf and l = 0.
+          // A split without a maximum for this column saw none of its keys and holds
+          // zeros, or saw nothing but NaN, which has to show.
           float mn = Mr;
 #pragma unroll
           for (int k = 0; k < MS; ++k) mn = fmaxf(mn, m[k]);
-          if (mn == kNegInf) continue;
-          const float al = Mr == kNegInf ? 0.f : fast_exp2(Mr - mn);
+          const float al = Mr == kNegInf ? 1.f : fast_exp2(Mr - mn);
           L *= al;
 #pragma unroll
           for (int i = 0; i < DPT / 4; ++i) v[i] *= al;
 #pragma unroll
           for (int k = 0; k < MS; ++k) {
-            const float w = m[k] == kNegInf ? 0.f : fast_exp2(m[k] - mn);
+            const bool in = sp + k < nsplit;
+            const float w = !in ? 0.f : m[k] == kNegInf ? 1.f : fast_exp2(m[k] - mn);
             L += l[k] * w;
 #pragma unroll
             for (int i = 0; i < DPT / 4; ++i) v[i] += w * pt[k][i];
