@@ -39,3 +39,43 @@ def test_nan_in_the_first_keys_only(cuda_device, new, spoiled):
     out = attend(pool, q, new, 0.125)
     assert torch.equal(out[:, :7], base[:, :7]) and base.isfinite().all()
     assert out[:, 7:].isnan().all()
+
+
+def sharp(pool, q, scale):
+    """Where one score lies so far above a row's others that fp32 sums of the products cannot
+    mistake it and the others' weights are 0 -- [sequences, heads], nearly everywhere -- and that
+    key's V row, which is then the output, exactly."""
+    rows, where = [], []
+    k, v = ((getattr(pool, c).double() * getattr(pool, c + "_scale").double()[:, None, :, None])
+            for c in ("k", "v"))
+    group = q.shape[1] // pool.hkv
+    for b, n in enumerate(pool.lens):
+        ids = torch.from_numpy(pool.tables[b].astype(np.int64))
+        keys, values = (x[ids].reshape(-1, pool.hkv, pool.d)[:n].repeat_interleave(group, 1).transpose(0, 1)
+                        for x in (k, v))
+        x = q[b].double().cpu()[:, :, None]
+        top = (keys @ x)[..., 0].mul(scale).topk(min(2, n), dim=1)
+        size = (keys.abs() @ x.abs()).amax() * abs(scale)
+        far = 100 + 2 * (pool.d + 8) * size * 2.0 ** -24
+        where.append(top.values[:, 0] - top.values[:, -1] > (far if n > 1 else -1))
+        rows.append(values[torch.arange(len(values)), top.indices[:, 0]])
+    where = torch.stack(where)
+    assert where.double().mean() > 0.98
+    return where, torch.stack(rows).half()
+
+
+@pytest.mark.parametrize("seqs", [2, 300])
+@pytest.mark.parametrize("several,scale,hq,hkv,d,bs", [
+    (several, scale, *shape) for several, scale in [(False, 0.125), (False, -0.125), (False, 16.0), (True, 16.0)]
+    for shape in [(14, 2, 64, 16), (4, 2, 64, 8), (8, 2, 128, 16), (3, 1, 256, 16)][:3 if several else 4]])
+def test_scores_of_many_millions(cuda_device, several, scale, hq, hkv, d, bs, seqs):
+    """Scores beyond what fp32 holds to one unit: the largest one's weight is still 1."""
+    lens = [1 + (97 * i) % 290 for i in range(seqs)]
+    lens[1] = 2500
+    pool = Fp8Pool(lens, hkv, d, bs, seed=hq + d, device=cuda_device)
+    pool.k_scale = pool.k_scale * 2.0 ** 12
+    pool.dks = pool.k_scale.to(cuda_device)
+    q = queries(seqs, hq, d, 4, cuda_device, std=2000.0)
+    where, rows = sharp(pool, q, scale)
+    out = attend(pool, q, [1] * seqs if several else None, scale).cpu()
+    assert out.isfinite().all() and torch.equal(out[where], rows[where])

@@ -1,6 +1,6 @@
 // Attention over the 8-bit paged pool (gfx950) for one query token per sequence, or a few.
 //
-//   o = sum_t p_t v_t / sum_t p_t,  p_t = 2^(scale log2(e) q.k_t - m),  m the maximum
+//   o = sum_t p_t v_t / sum_t p_t,  p_t = 2^(scale log2(e) (q.k_t - m)),  m the maximum
 //   so far, K and V rows = e4m3 code * scale[block, kv head]
 //
 // Work split. The work is a list of (sequence, group of HG adjacent kv heads) pairs, each
@@ -508,16 +508,16 @@ __global__ __launch_bounds__(64 * NW, waves_per_simd(D, NW, CB)) void attend_fp8
         float m = s[st][0][0];
 #pragma unroll
         for (int i = 1; i < 8; ++i) m = fmaxf(m, s[st][i / 4][i % 4]);
-        // (A column that has seen nothing yet stays at -inf, whatever the scale: 0 * -inf
-        // would be NaN.)
-        m = over_groups(m, Max());
-        m_new[st] = m == kNegInf ? m_run[st] : fmaxf(m_run[st], m * scale);
+        m_new[st] = fmaxf(m_run[st], over_groups(m, Max()));
         grown |= m_new[st] > m_run[st];
       }
       if (__ballot(grown) != 0) {  // wavefront-uniform
 #pragma unroll
         for (int st = 0; st < NS; ++st) {
-          const float alpha = m_new[st] == kNegInf ? 1.f : fast_exp2(m_run[st] - m_new[st]);
+          // (Nothing seen yet: 0, whatever the scale; 0 * -inf would be NaN.)
+          const float alpha = m_new[st] == kNegInf ? 1.f
+                              : m_run[st] == kNegInf ? 0.f
+                                                     : fast_exp2((m_run[st] - m_new[st]) * scale);
           l_run[st] *= alpha;
 #pragma unroll
           for (int nd = 0; nd < ND; ++nd) acc[st][nd] *= alpha;
@@ -527,10 +527,11 @@ __global__ __launch_bounds__(64 * NW, waves_per_simd(D, NW, CB)) void attend_fp8
       f16x8 pb[NS];
 #pragma unroll
       for (int st = 0; st < NS; ++st) {
-        const float off = kBias - m_run[st];
+        // (Scaled after the subtraction: products of many millions, which fp32 holds to some
+        // units only, still give the largest one's probability.)
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-          pb[st][i] = (f16)fast_exp2(__builtin_fmaf(s[st][i / 4][i % 4], scale, off));
+          pb[st][i] = (f16)fast_exp2(__builtin_fmaf(s[st][i / 4][i % 4] - m_run[st], scale, kBias));
       }
       if (!whole) {
 #pragma unroll
@@ -584,7 +585,7 @@ __global__ __launch_bounds__(64 * NW, waves_per_simd(D, NW, CB)) void attend_fp8
     for (int st = 0; st < NS; ++st) {
       const float l = over_groups(l_run[st], Sum());
       if (grp == 0) {
-        s_m[wave][st * 16 + row] = m_run[st];
+        s_m[wave][st * 16 + row] = m_run[st] == kNegInf ? kNegInf : m_run[st] * scale;
         s_l[wave][st * 16 + row] = l;
       }
       if (MULTI ? st * 16 + row < heads : row < a.g) {
