@@ -18,12 +18,13 @@ def queries(n, hq, d, seed, device, std=1.0):
     return x.half().to(device)
 
 
-def attend(pool, q, new, scale):
-    """`new` tokens per sequence through the several-token call, or None: the decode call."""
+def attend(pool, q, new, scale, longest=None):
+    """`new` tokens per sequence through the several-token call (of up to `longest`), or None: the
+    decode call."""
     if new is None:
         return paged_attention_decode_fp8(q, *pool.args(), scale)
-    return paged_attention_prefill_fp8(q, *pool.args(), int32(starts_of(new), pool.device), max(new),
-                                       scale)
+    return paged_attention_prefill_fp8(q, *pool.args(), int32(starts_of(new), pool.device),
+                                       longest or max(new), scale)
 
 
 @pytest.mark.parametrize("new", [None, [4], [40], [300]])
@@ -78,4 +79,19 @@ def test_scores_of_many_millions(cuda_device, several, scale, hq, hkv, d, bs, se
     q = queries(seqs, hq, d, 4, cuda_device, std=2000.0)
     where, rows = sharp(pool, q, scale)
     out = attend(pool, q, [1] * seqs if several else None, scale).cpu()
+    assert out.isfinite().all() and torch.equal(out[where], rows[where])
+
+
+@pytest.mark.parametrize("seqs", [2, 300])
+@pytest.mark.parametrize("hq,hkv,d,bs", [(14, 2, 64, 16), (4, 2, 32, 8), (8, 2, 128, 16), (3, 1, 256, 16)])
+def test_scores_of_many_millions_in_a_call_for_prompts(cuda_device, hq, hkv, d, bs, seqs):
+    """The same in the kernel that takes calls of up to 100 tokens per sequence."""
+    lens = [1 + (97 * i) % 290 for i in range(seqs)]
+    lens[1] = 2500
+    pool = Fp8Pool(lens, hkv, d, bs, seed=hq + d, device=cuda_device)
+    pool.k_scale = pool.k_scale * 2.0 ** 12
+    pool.dks = pool.k_scale.to(cuda_device)
+    q = queries(seqs, hq, d, 4, cuda_device, std=2000.0)
+    where, rows = sharp(pool, q, 64.0)
+    out = attend(pool, q, [1] * seqs, 64.0, longest=100).cpu()
     assert out.isfinite().all() and torch.equal(out[where], rows[where])

@@ -397,7 +397,11 @@ __global__ __launch_bounds__(64 * NW) void prefill_attn_kernel(PrefillAttnArgs a
     // infinite (or NaN). Probabilities thus stay below 2^16, and most tiles
     // skip the maxima and the accumulator rescale. With the 8-bit pool they carry a
     // factor of 2^8 (its share is raised from 2^8 over the maximum on): fp16 then keeps
-    // all its bits down to 2^-22 of the maximum instead of 2^-14, at no cost.
+    // all its bits down to 2^-22 of the maximum instead of 2^-14, at no cost. Their maxima
+    // are of the raw scores, which are scaled after the subtraction: products of many
+    // millions, which fp32 holds to some units only, still give the largest one's
+    // probability. (One more instruction a score: 8 x (2048 + 512) tokens at 14 / 2 heads of 64
+    // 60.9 -> 61.7 us in a graph, 32 / 8 heads of 128 172.6 -> 174.0.)
     constexpr float BIAS = KV8 ? 8.f : 0.f;
     f16x8 pb[NS / 2][CG];
     float lt[CG];
@@ -406,15 +410,18 @@ __global__ __launch_bounds__(64 * NW) void prefill_attn_kernel(PrefillAttnArgs a
       for (int cg = 0; cg < CG; ++cg) {
         // A column with no visible key yet keeps m = -inf; any finite offset
         // then gives p = 0 for its -inf scores.
-        const float nm = m_run[cg] == kNegInf ? 0.f : KV8 ? BIAS - m_run[cg] : -m_run[cg];
+        const float nm = m_run[cg] == kNegInf ? 0.f : -m_run[cg];
+        auto prob = [&](float x) {
+          return (f16)fast_exp2(KV8 ? __builtin_fmaf(x + nm, a.scale_log2, BIAS)
+                                    : __builtin_fmaf(x, a.scale_log2, nm));
+        };
         lt[cg] = 0.f;
 #pragma unroll
         for (int sp = 0; sp < NS / 2; ++sp) {
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            pb[sp][cg][r] = (f16)fast_exp2(__builtin_fmaf(sc[cg][2 * sp][r], a.scale_log2, nm));
-            pb[sp][cg][4 + r] =
-                (f16)fast_exp2(__builtin_fmaf(sc[cg][2 * sp + 1][r], a.scale_log2, nm));
+            pb[sp][cg][r] = prob(sc[cg][2 * sp][r]);
+            pb[sp][cg][4 + r] = prob(sc[cg][2 * sp + 1][r]);
           }
 #pragma unroll
           for (int i = 0; i < 4; ++i)
@@ -431,7 +438,8 @@ __global__ __launch_bounds__(64 * NW) void prefill_attn_kernel(PrefillAttnArgs a
               (__builtin_bit_cast(uint32_t, lt[cg]) & 0x7f800000u) == 0x7f800000u;
     if (__builtin_amdgcn_ballot_w64(redo) != 0) {  // wavefront-uniform
       // Maxima in the exp2 domain (the scale is positive, so it commutes
-      // with the maximum), raise, rescale, recompute.
+      // with the maximum), of the 8-bit pool's raw scores; raise, rescale,
+      // recompute.
 #pragma unroll
       for (int cg = 0; cg < CG; ++cg) {
         float m = kNegInf;
@@ -442,10 +450,12 @@ __global__ __launch_bounds__(64 * NW) void prefill_attn_kernel(PrefillAttnArgs a
         }
         m = fmaxf(m, __shfl_xor(m, 16));
         m = fmaxf(m, __shfl_xor(m, 32));
-        const float m_new = fmaxf(m_run[cg], m * a.scale_log2);
+        const float m_new = fmaxf(m_run[cg], KV8 ? m : m * a.scale_log2);
         // A column with no visible key yet (only in a split after the first)
         // stays at -inf, and -inf - -inf would make its alpha NaN.
-        const float alpha = m_new == kNegInf ? 1.f : fast_exp2(m_run[cg] - m_new);
+        const float alpha = m_new == kNegInf ? 1.f
+                                             : fast_exp2((m_run[cg] - m_new) *
+                                                         (KV8 ? a.scale_log2 : 1.f));
         l_run[cg] *= alpha;
 #pragma unroll
         for (int nd = 0; nd < ND; ++nd) acc[cg][nd] *= alpha;
@@ -521,8 +531,8 @@ __global__ __launch_bounds__(64 * NW) void prefill_attn_kernel(PrefillAttnArgs a
     for (int cg = 0; cg < CG; ++cg) {
       const int cl = (wave * CG + cg) * 16 + row;
       if (grp == 0) {
-        __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, m_run[cg]), rr,
-                                              rb + cl * 4, 0, 16);
+        const float m = KV8 ? m_run[cg] * a.scale_log2 : m_run[cg];
+        __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, m), rr, rb + cl * 4, 0, 16);
         __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, lsum[cg]), rr,
                                               rb + (COLS + cl) * 4, 0, 16);
       }
