@@ -509,7 +509,8 @@ PA_API int pa_decode_batched_noalloc_f16(const void* q, const int64_t q_strides[
  *
  * pa_kv_read_fp8: the same rows' values as fp16 into key / value [num_tokens,
  * num_kv_heads, head_dim] (unit head_dim stride; exact for the scales above);
- * zeros for rows without a slot and rows of no sequence.
+ * zeros for rows without a slot and rows of no sequence (num_seqs 0: all of them, and
+ * nothing else is asked of the arguments; with a null key or value there is nothing to do).
  */
 PA_API int pa_kv_write_fp8(const void* key, const int64_t key_strides[3], const void* value,
                            const int64_t value_strides[3], void* k_cache,

@@ -8,6 +8,7 @@ import pytest
 import torch
 
 from _fp8_pool import Fp8Pool, int32, starts_of
+from engine.kernels import _native
 from engine.kernels.quantized_cache import paged_attention_decode_fp8, paged_attention_prefill_fp8
 
 pytestmark = pytest.mark.gpu
@@ -95,3 +96,23 @@ def test_scores_of_many_millions_in_a_call_for_prompts(cuda_device, hq, hkv, d, 
     where, rows = sharp(pool, q, 64.0)
     out = attend(pool, q, [1] * seqs, 64.0, longest=100).cpu()
     assert out.isfinite().all() and torch.equal(out[where], rows[where])
+
+
+@pytest.mark.parametrize("d", [64, 5])
+def test_read_of_no_sequence_through_the_c_abi(cuda_device, d):
+    """All rows are rows of no sequence: zeros, whatever the other arguments are."""
+    lib, st = _native.load(), _native.strides_of
+    pool = Fp8Pool([20], 2, d, 16, seed=3, device=cuda_device)
+    starts = int32([0], cuda_device)
+    real = (pool.dk.data_ptr(), st(pool.dk), pool.dv.data_ptr(), st(pool.dv), pool.dks.data_ptr(),
+            st(pool.dks), pool.dvs.data_ptr(), st(pool.dvs), pool.dt.data_ptr(), st(pool.dt),
+            pool.dl.data_ptr(), starts.data_ptr())
+    for args, bs, blocks, width in ((real, 16, pool.blocks, pool.dt.shape[1]), ((None,) * 12, 0, 0, 0)):
+        wide = [torch.full((40, 2, d), 7.0, dtype=torch.float16, device=cuda_device) for _ in range(2)]
+        rows = [x[1:38] for x in wide]
+        status = lib.pa_kv_read_fp8(
+            *args, rows[0].data_ptr(), st(rows[0]), rows[1].data_ptr(), st(rows[1]), 0, 37, 2, d, bs,
+            blocks, width, _native.stream_handle(cuda_device))
+        assert status == _native.PA_OK
+        for x in wide:
+            assert not x[1:38].any() and (x[:1] == 7).all() and (x[38:] == 7).all()

@@ -206,14 +206,14 @@ __global__ __launch_bounds__(256) void read_kernel(ReadArgs a) {
   if (threadIdx.x < 64) {
     int b = wave_search(r.num_seqs, first, lane, [&](int i) { return row_start(r, i); });
     if (lane < rows) {
-      const int t = first + lane;
-      while (b + 1 < r.num_seqs && row_start(r, b + 1) <= t) ++b;
-      const int q0 = row_start(r, b), q1 = row_start(r, b + 1);
       int id = -1, off = 0;
-      if (t >= q0 && t < q1) {
+      if (r.num_seqs > 0) {
+        const int t = first + lane;
+        while (b + 1 < r.num_seqs && row_start(r, b + 1) <= t) ++b;
+        const int q0 = row_start(r, b), q1 = row_start(r, b + 1);
         const int64_t pos = (int64_t)r.lens[b] - (q1 - q0) + (t - q0);
         const int64_t blk = pos / r.bs;
-        if (pos >= 0 && blk < r.max_blocks) {
+        if (t >= q0 && t < q1 && pos >= 0 && blk < r.max_blocks) {
           id = r.bt[(int64_t)b * r.bt_sb + blk * r.bt_sk];
           if (id >= r.num_blocks) id = -1;
           off = (int)(pos - blk * r.bs);
@@ -379,19 +379,29 @@ int pa_kv_read_fp8(const void* k_cache, const int64_t k_strides[4], const void* 
     set_error("num_seqs (%d) and num_tokens (%d) must be >= 0", num_seqs, num_tokens);
     return PA_ERR_ARG;
   }
-  if (num_seqs == 0 || num_tokens == 0) return PA_OK;
-  if (!key || !value || !k_cache || !v_cache || !k_scale || !v_scale || !key_strides ||
-      !value_strides || !k_strides || !v_strides || !k_scale_strides || !v_scale_strides ||
-      !query_start_loc) {
+  // Rows of no sequence are zeros, without any sequence too; of the other arguments nothing
+  // is then asked (tables of no rows have null pointers).
+  const bool none = num_seqs == 0;
+  if (num_tokens == 0 ||
+      (none && (!key || !value || !key_strides || !value_strides || num_kv_heads <= 0 || head_dim <= 0)))
+    return PA_OK;
+  if (!none && (!key || !value || !k_cache || !v_cache || !k_scale || !v_scale || !key_strides ||
+                !value_strides || !k_strides || !v_strides || !k_scale_strides ||
+                !v_scale_strides || !query_start_loc)) {
     set_error("null pointer argument");
     return PA_ERR_ARG;
   }
   ReadArgs a{};
-  const int rc = rows_args(a.r, block_tables, bt_strides, seq_lens, query_start_loc, num_seqs,
-                           num_tokens, num_kv_heads, head_dim, block_size, num_blocks,
-                           max_blocks_per_seq);
-  if (rc) return rc;
-  if (k_strides[3] != 1 || v_strides[3] != 1 || key_strides[2] != 1 || value_strides[2] != 1) {
+  if (none) {
+    a.r.num_tokens = num_tokens;
+  } else {
+    const int rc = rows_args(a.r, block_tables, bt_strides, seq_lens, query_start_loc, num_seqs,
+                             num_tokens, num_kv_heads, head_dim, block_size, num_blocks,
+                             max_blocks_per_seq);
+    if (rc) return rc;
+  }
+  if ((!none && (k_strides[3] != 1 || v_strides[3] != 1)) || key_strides[2] != 1 ||
+      value_strides[2] != 1) {
     set_error("the head_dim stride of the caches, key and value must be 1");
     return PA_ERR_ARG;
   }
@@ -399,12 +409,13 @@ int pa_kv_read_fp8(const void* k_cache, const int64_t k_strides[4], const void* 
     set_error("%d kv heads x head_dim %d is not built", num_kv_heads, head_dim);
     return PA_ERR_UNSUPPORTED;
   }
-  const void* cache[2] = {k_cache, v_cache};
-  const float* scale[2] = {k_scale, v_scale};
+  const int64_t no_strides[4] = {};
+  const void* cache[2] = {none ? nullptr : k_cache, none ? nullptr : v_cache};
+  const float* scale[2] = {none ? nullptr : k_scale, none ? nullptr : v_scale};
   void* out[2] = {key, value};
   const int64_t* os[2] = {key_strides, value_strides};
-  const int64_t* cs[2] = {k_strides, v_strides};
-  const int64_t* xs[2] = {k_scale_strides, v_scale_strides};
+  const int64_t* cs[2] = {none ? no_strides : k_strides, none ? no_strides : v_strides};
+  const int64_t* xs[2] = {none ? no_strides : k_scale_strides, none ? no_strides : v_scale_strides};
   bool vec = head_dim % 16 == 0;
   for (int i = 0; i < 2; ++i) {
     a.cache[i] = (const uint8_t*)cache[i];
