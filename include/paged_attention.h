@@ -484,7 +484,8 @@ PA_API int pa_decode_batched_noalloc_f16(const void* q, const int64_t q_strides[
  * pool's layout [num_blocks, block_size, num_kv_heads, head_dim] (strides in
  * elements, which are bytes here, unit head_dim stride); k_scale and v_scale are
  * fp32 [num_blocks, num_kv_heads], any strides: a value is code * scale[block, head].
- * Scales are powers of two from 2^-15 to 2^8, as pa_kv_write_fp8 leaves them.
+ * Scales are powers of two from 2^-15 to 2^8, as pa_kv_write_fp8 leaves them; of a
+ * scale between two powers every call takes the lower one.
  *
  * Sequences and rows. num_tokens rows belong to num_seqs sequences: sequence b
  * owns rows query_start_loc[b] .. query_start_loc[b + 1] - 1 (n_b rows; int32

@@ -9,7 +9,11 @@ import torch
 
 from _fp8_pool import Fp8Pool, int32, starts_of
 from engine.kernels import _native
-from engine.kernels.quantized_cache import paged_attention_decode_fp8, paged_attention_prefill_fp8
+from engine.kernels.quantized_cache import (
+    paged_attention_decode_fp8,
+    paged_attention_prefill_fp8,
+    paged_kv_read_fp8,
+)
 
 pytestmark = pytest.mark.gpu
 
@@ -116,3 +120,22 @@ def test_read_of_no_sequence_through_the_c_abi(cuda_device, d):
         assert status == _native.PA_OK
         for x in wide:
             assert not x[1:38].any() and (x[:1] == 7).all() and (x[38:] == 7).all()
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(14, 2, 64), (4, 2, 32), (8, 2, 128), (3, 1, 256)])
+@pytest.mark.parametrize("bs", [5, 8, 16, 32, 48])
+def test_scales_count_by_their_exponent(cuda_device, hq, hkv, d, bs):
+    """A pool whose scales are no powers of two gives what the next lower powers give, whatever the
+    block size and the call."""
+    lens = [300, 2, 2500]
+    pool = Fp8Pool(lens, hkv, d, bs, seed=5, device=cuda_device)
+    calls = [(None, None), ([2, 1, 3], 4), ([2, 1, 3], 100)]
+    qs = [queries(sum(new or [1] * 3), hq, d, 6, cuda_device) for new, _ in calls]
+    base = [attend(pool, q, new, 0.125, most) for q, (new, most) in zip(qs, calls)]
+    starts = int32(starts_of(lens), cuda_device)
+    rows = paged_kv_read_fp8(*pool.args(), starts, sum(lens))
+    pool.dks, pool.dvs = pool.dks * 1.5, pool.dvs * 1.9375
+    for q, (new, most), want in zip(qs, calls, base):
+        assert torch.equal(attend(pool, q, new, 0.125, most), want)
+    for got, want in zip(paged_kv_read_fp8(*pool.args(), starts, sum(lens)), rows):
+        assert torch.equal(got, want)

@@ -107,6 +107,11 @@ struct Cut {
   }
 };
 
+// The power of two that conversions of codes take from a scale: its exponent alone.
+__device__ inline float power_of(float scale) {
+  return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, scale) & 0x7f800000u);
+}
+
 // Lane l's value, in a scalar register.
 __device__ inline float lane_value(float x, int l) {
   return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), l));
@@ -416,7 +421,7 @@ __global__ __launch_bounds__(64 * NW, waves_per_simd(D, NW, CB)) void attend_fp8
       } else {
         const int t = lane & 31, hg = HG > 1 ? lane >> 5 : 0;
         s_ks[wave][hg * kChunk + t] = scales;
-        s_vs[wave][hg * kChunk + t] = (f16)(t0 + t < L ? vscales : 1.f);
+        s_vs[wave][hg * kChunk + t] = (f16)(t0 + t < L ? power_of(vscales) : 1.f);
         wave_lds_fence();
       }
 #pragma unroll
