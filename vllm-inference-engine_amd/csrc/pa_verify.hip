@@ -52,7 +52,7 @@ struct Args {
   int32_t* accepted;
   int* cnt;
   double* sums;  // [seqs][pieces][2]: max(p - q, 0), p
-  int seqs, k, vocab, pieces;
+  int k, vocab, pieces;
   int groups;  // workgroups per sequence
 };
 
@@ -440,7 +440,6 @@ int pa_verify_drafts_f32(const float* target, const int64_t target_strides[3], c
   a.accepted = accepted;
   a.cnt = (int*)workspace;
   a.sums = (double*)((char*)workspace + kCounterBytes);
-  a.seqs = num_seqs;
   a.k = max_drafts;
   a.vocab = vocab;
   a.pieces = pieces;
