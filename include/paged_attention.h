@@ -597,9 +597,10 @@ PA_API int pa_prefill_attention_fp8(const void* q, const int64_t q_strides[3],
  * cumulative weight exceeds next_u times the sum of weights; the weights are
  * max(target[n] - draft[n], 0) for n < d (target[n] with draft_ids[n] left out where
  * draft is NULL), and target[n] for n = d or where those are all 0. Products, sums and
- * comparisons in 64 bits; negative weights and NaN count as 0; where rounding or
- * next_u >= 1 leaves no such index, the last index with a weight, and index 0 of a row
- * without any. accepted[b] = n; tokens [num_seqs, max_drafts + 1] int64 contiguous:
+ * comparisons in 64 bits; negative weights and NaN count as 0; where rounding or a
+ * next_u of 1 and more or NaN leaves no such index, the last index with a weight, and
+ * index 0 of a row without any; an accept_u of NaN rejects. (Where next_u times the sum
+ * lies within about 2^-40 of the sum of a border, the neighbour may be taken.) accepted[b] = n; tokens [num_seqs, max_drafts + 1] int64 contiguous:
  * the n drafts, the next token, then -1. At most 16384 sequences, 64 drafts and a
  * vocabulary of 2^30.
  *

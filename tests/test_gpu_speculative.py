@@ -171,3 +171,19 @@ def test_refusals(cuda_device):
                       torch.zeros(1, 65, device=cuda_device), nxt[:1])
     tokens, accepted = verify_drafts(p[:0], q[:0], ids[:0], u[:0], nxt[:0])
     assert tokens.shape == (0, 4) and accepted.shape == (0,)
+
+
+@pytest.mark.parametrize("vocab", [100, 9000, 600001])
+@pytest.mark.parametrize("draft_given", [True, False])
+def test_random_numbers_that_are_none(cuda_device, vocab, draft_given):
+    """NaN: the draft is rejected, and the last index with a weight follows."""
+    p, q, ids, u, nxt = case(6, 3, vocab, 9, cuda_device, off=0.3)
+    q, nan = q if draft_given else None, float("nan")
+    u = u * 0.01
+    u[0, 0] = u[1, 2] = nan
+    nxt[0] = nxt[2] = nan
+    p[2, :, vocab * 2 // 3:] = 0.0
+    p[3, :, vocab // 2:] = 0.0
+    nxt[3] = 1.0
+    want = check(p, q, ids, u, nxt)
+    assert want[1][0] == 0 and want[1][1] <= 2

@@ -10,8 +10,9 @@
 // u' * (sum of all). The tokens so made follow the target's distribution.
 //
 // All sums and products are in 64 bits: the products of two fp32 numbers are then
-// exact, and sums in any order agree to 2^-40 or better, so the chosen index does
-// not depend on how the row is split.
+// exact, and sums in any order agree to 2^-40 of the whole or better. The chosen index is
+// that of the definition except where u' * (sum of all) lies that near to a cumulative
+// sum: there the neighbour with a weight may be taken.
 //
 // A row of the vocabulary is cut into pieces of 1024 entries, one wavefront's work at a
 // time: the sums of w and of p over each piece go to the workspace. The wavefronts of a few

@@ -38,8 +38,9 @@ def verify_drafts(
     of the draw if it is not. A row of tokens holds the accepted drafts, the next token,
     then -1.
 
-    The rows need not sum to 1. Sums and products are in 64 bits; negative numbers and
-    NaN count as no weight; an id outside the vocabulary is not accepted. At most 64
+    The rows need not sum to 1. Sums and products are in 64 bits; a negative weight or
+    NaN counts as none; an id outside the vocabulary is not accepted, nor one whose random
+    number is NaN; a next_u of 1 and more or NaN takes the last index with a weight. At most 64
     drafts and 16384 sequences. Asynchronous on the current stream; no host
     synchronisation; capturable into a HIP graph.
     """
