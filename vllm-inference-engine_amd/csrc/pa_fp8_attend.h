@@ -28,10 +28,10 @@
 // kind of read meets a bank twice.
 //
 // Bounds on MI355X (head_dim 64, 14 / 2 heads, block 16, unless stated). 256 sequences of
-// 1.2M tokens in all (316 MB): memory, 61.7 us, 5.1 TB/s, where a gather of such 2 KB blocks
-// alone reaches 6.3. 8 sequences of 1k to 8k at 32 / 8 heads of 128 (73 MB): 22.4 us, of
+// 1.2M tokens in all (316 MB): memory, 62.4 us, 5.1 TB/s, where a gather of such 2 KB blocks
+// alone reaches 6.3. 8 sequences of 1k to 8k at 32 / 8 heads of 128 (73 MB): 22.3 us, of
 // which the streaming takes about 12; the rest is the chain launch -> plan -> first ids ->
-// first chunk, and meeting, arrival and merge. One sequence: chains alone, 13.2 us at 24001
+// first chunk, and meeting, arrival and merge. One sequence: chains alone, 13.1 us at 24001
 // tokens (3.7 of them the merge of 47 parts) and 5.7 at 300 tokens.
 //
 // Probabilities are rounded to fp16 (the denominators sum the rounded ones), scaled by
@@ -43,7 +43,7 @@
 // K and V fragment; a column sees the keys up to its token's position. A NaN in a V row
 // reaches only the columns that see it: where some column does not see the whole chunk,
 // NaN codes are cleared and the probabilities of their tokens become NaN instead. 16
-// sequences of 0.3k to 4k tokens and 5 drafts at 32 / 8 heads of 128 (90 MB): 30 us, about 14
+// sequences of 0.3k to 4k tokens and 5 drafts at 32 / 8 heads of 128 (90 MB): 30.9 us, about 14
 // of them streaming.
 #pragma once
 
@@ -199,7 +199,9 @@ __device__ inline int swizzle(int r) {
 }
 
 // Wavefronts per SIMD that the registers are kept to. (A workgroup of eight is its compute
-// unit's only one, and spills nothing then: blocks of 8 tokens 36.8 -> 26.2 us.)
+// unit's only one, and spills no vector registers then. Every form keeps about 90 to 150
+// scalar registers in lanes of vector ones; of four wavefronts, two heads of 64 in blocks of
+// other sizes than 16 and 32 alone spill vector registers, 6.)
 constexpr int waves_per_simd(int D, int NW, int CB) {
   return D == 256 || CB > 1 || NW > 4 ? 2 : 3;
 }
@@ -692,7 +694,7 @@ __global__ __launch_bounds__(64 * NW, waves_per_simd(D, NW, CB)) void attend_fp8
       for (int i = from; i < heads * (s1 - s0); i += kThreads) keep_ml(i, s0, s1, fetch_ml(i, s0, s1));
     };
     // The first ones before the accumulators: maxima and sums are formed while those are on
-    // their way (24001 tokens 15.9 -> 14.9 us). Not where it costs spills: at one token in
+    // their way (1 us of 24001 tokens, when it was added). Not where it costs spills: at one token in
     // workgroups of four (316 MB: 65.5 -> 69.2).
     constexpr bool EARLY = MULTI || NW > 4;
     const int early = EARLY ? min(nseg, batch) : 0;
@@ -891,15 +893,16 @@ __global__ __launch_bounds__(64 * NW, waves_per_simd(D, NW, CB)) void attend_fp8
 
 // List positions of 32 tokens: what a pair costs beside its chunks (its beginning, meeting,
 // arrival and merge), and the fewest a range takes. Measured on MI355X at 8 / 16 / 32: the
-// cost, 256 x ~4.6k tokens 66.8 / 64.4 / 67.1 us, 16 x 5 drafts 33.8 / 33.6 / 34.6, 20 x 4
-// drafts at head_dim 64 17.5 / 15.3 / 15.2, 64 x 5 drafts of up to 4k 74.5 / 79.0 / 78.9; the
-// range, one sequence of 24001 tokens 17.9 / 15.9 / 17.4, 8 of 1k to 8k 25.2 / 24.6 / 24.6.
+// cost, 256 x ~4.6k tokens 62.3 / 62.3 / 64.8 us, 16 x 5 drafts 31.7 / 31.2 / 32.8, 20 x 4
+// drafts at head_dim 64 15.6 / 13.4 / 13.3, 64 x 5 drafts of up to 4k 72.5 / 76.9 / 76.9; the
+// range, one sequence of 24001 tokens 15.1 / 13.3 / 14.4, 8 of 1k to 8k 22.6 / 22.8 / 22.5.
 constexpr int kPairCost = 16;
 constexpr int kMinRange = 16;
 // Tables of at most this many tokens take one workgroup per pair; of the second, where
 // the pairs fill at least half the compute units. Whole pairs against ranges, measured: 8 x
-// 1024 tokens at 32 / 8 heads 12.5 against 15.2 us, 8 x 2k 19.5 against 15.8; 64 x 2k at 14 / 2
-// heads 13.4 against 16.5, 512 x 2k 33.3 against 40.1, 64 x 5 drafts of up to 4k 77 against 68.
+// 1024 tokens at 32 / 8 heads 12.5 against 13.5 us, 8 x 2k 20.1 against 14.3; at 14 / 2 heads
+// 128 x 1088 10.6 against 16.8, 64 x 2k 14.0 against 16.0, 512 x 2k 34.4 against 40.1; 64 x 5
+// drafts of up to 4k 79.6 against 76.8.
 constexpr int kWholePairs = 1024;
 constexpr int kWholePairsBusy = 2048;
 

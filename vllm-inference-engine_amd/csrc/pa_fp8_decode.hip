@@ -14,17 +14,20 @@ DecodePlan decode_plan(int num_seqs, int num_q_heads, int num_kv_heads, int head
   const int64_t cap = (int64_t)max_blocks * block_size;
   // Two kv heads per pair read rows of twice the bytes and halve the merges. Measured on
   // MI355X at 14 / 2 heads of 64, one head against two, (sequence, head) pairs more than
-  // compute units: 256 x ~4.6k tokens 106 against 66 us, 140 x 4k 33.6 against 25.8 (300 x 1k
-  // 16.3 against 16.7); fewer, in ranges: 128 x 4k 29.9 against 24.7, 64 x 4k 19.7 against
-  // 19.8, 8 x 4k 13.2 against 15.2, and 12 x 4k at 16 heads 36.7 against 24.7; fewer, as whole
-  // pairs: 100 x 2k 13.9 against 19.5.
+  // compute units: 256 x ~4.6k tokens 103.7 against 62.2 us, 140 x 4k 34.0 against 25.0 (300 x
+  // 1k 17.7 against 18.1); fewer, in ranges: 128 x 4k 28.8 against 23.6, 64 x 4k 18.7 against
+  // 18.2, 8 x 4k 12.0 against 14.4, and 12 x 4k at 16 heads 35.8 against 22.7; fewer, as whole
+  // pairs: 100 x 2k 14.4 against 17.8.
   const int64_t total = (int64_t)num_seqs * num_kv_heads;
   p.head_group = !multi && head_dim <= 64 && num_kv_heads % 2 == 0 &&
                          (total > n || (2 * total > n && cap > kWholePairsBusy)) ? 2 : 1;
   const int64_t pairs = total / p.head_group;
   // Few pairs: one workgroup of eight wavefronts per compute unit, which halves the parts of
-  // a merge, instead of two of four. Measured on MI355X: one sequence of 24001 tokens 16.5
-  // against 18.4 us, of 300 5.9 against 6.8; 4 x 5 drafts of 8k 31.5 against 33.5.
+  // a merge, instead of two of four. Measured on MI355X: one sequence of 24001 tokens 13.5
+  // against 15.2 us, of 300 6.5 against 6.9; 4 x 5 drafts of 8k 25.1 against 29.4. One range
+  // per compute unit also at head_dim 256, of four wavefronts there, against two: at 16 / 2
+  // heads 8 x 8k 19.8 for either, 32 x 8k 38.9 against 41.6, 4 x 32k 35.2 against 40.9, 100 x 4k
+  // 55.2 against 58.9.
   const bool few = p.head_group == 1 && pairs <= n;
   p.waves = few && head_dim <= 128 ? 8 : 4;
   const int64_t whole = 2 * pairs >= n ? kWholePairsBusy : kWholePairs;

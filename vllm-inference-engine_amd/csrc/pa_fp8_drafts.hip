@@ -3,7 +3,7 @@
 // The prefill kernel stages K and V once per 64 or 128 columns of tokens x query heads; with
 // a few columns it spends its time on the ones that are not there, and on key ranges too
 // few to fill the GPU: 16 sequences of 0.3k to 4k tokens and 5 drafts at 32 / 8 heads of 128
-// took 62 us there, and take 31 here (MI355X).
+// take 59 us there and 31 here (MI355X).
 #include "../../include/paged_attention.h"
 #include "pa_fp8_attend.h"
 
@@ -15,8 +15,10 @@ static_assert(kCounterBytes == kPfCounterBytes, "counters, and nothing else, whe
 
 // Columns of a sequence and kv head that the registers hold: four blocks of 16, or two at
 // head_dim 128 (four would spill 91 registers there). At the full number the prefill kernel
-// against this one on MI355X: 100 x 9 tokens on up to 4k at 14 / 2 heads of 64 53.8 against 37.0
-// us, 16 x 9 20.0 against 19.7, 16 x 8 at 32 / 8 heads of 128 64.2 against 35.1.
+// against this one on MI355X: 100 x 9 tokens on up to 4k at 14 / 2 heads of 64 53.2 against 36.4
+// us, 16 x 9 18.2 for either, 16 x 8 at 32 / 8 heads of 128 59.8 against 32.9. What it costs to
+// be past it: 16 sequences of 0.3k to 4k tokens at 28 / 4 heads of 128 take 21.7 us with 4 tokens
+// each (28 columns) and 40.7 with 5 (35).
 static int most_columns(int D) { return D <= 64 ? 64 : 32; }
 
 bool takes_drafts(int head_dim, int g, int max_query_len) {
@@ -30,6 +32,9 @@ size_t drafts_workspace_bytes(int num_seqs, int num_q_heads, int num_kv_heads, i
                      max_query_len).ws_bytes;
 }
 
+// (Blocks of 32 tokens take the general form: 16 x 5 drafts at 32 / 8 heads of 128 34.0 us where
+// blocks of 16 take 30.9 and the prefill kernel 64.4, 64 x 4 at 14 / 2 heads of 64 23.8 for 20.2
+// and 38.0.)
 template <int D, int CB, int NW>
 static hipError_t launch_drafts_nw(const DecodeFp8Args& a, unsigned grid, hipStream_t s) {
   if (a.bs == 16 && near_strides(a))

@@ -30,7 +30,7 @@
 // codes that become fp16 on their way into LDS, times their block's scale, exactly;
 // everything after is the same but for a factor of 2^8 on the probabilities (see
 // `probs`). What bounds it is the same too, the issue of softmax and MFMAs: 8 x (2048 + 512)
-// tokens at 14 / 2 heads of 64 take 55.5 us, 609 TFLOP/s of products (a large fp16 matrix
+// tokens at 14 / 2 heads of 64 take 56.5 us, 599 TFLOP/s of products (a large fp16 matrix
 // product reaches 1181).
 #include <type_traits>
 
@@ -401,7 +401,7 @@ __global__ __launch_bounds__(64 * NW) void prefill_attn_kernel(PrefillAttnArgs a
     // are of the raw scores, which are scaled after the subtraction: products of many
     // millions, which fp32 holds to some units only, still give the largest one's
     // probability. (One more instruction a score: 8 x (2048 + 512) tokens at 14 / 2 heads of 64
-    // 60.9 -> 61.7 us in a graph, 32 / 8 heads of 128 172.6 -> 174.0.)
+    // 60.9 -> 61.7 us in a graph, at 32 / 8 heads of 128 172.6 -> 174.0.)
     constexpr float BIAS = KV8 ? 8.f : 0.f;
     f16x8 pb[NS / 2][CG];
     float lt[CG];

@@ -21,7 +21,7 @@
 // finds the piece in which the cumulative sum crosses u' * total and looks for the index
 // there. Bound by memory: two fp32 rows per sequence, read once (and one piece twice), and
 // for a few sequences by the chain drafts -> their entries -> pieces -> arrival -> sums ->
-// piece. On MI355X with 4 drafts and a vocabulary of 151936: 64 sequences (78 MB) 17.2 us, 4.5
+// piece. On MI355X with 4 drafts and a vocabulary of 151936: 64 sequences (78 MB) 16.7 us, 4.7
 // TB/s; one 6.1 us.
 #include "../../include/paged_attention.h"
 #include "pa_tiles.h"
@@ -345,8 +345,7 @@ static int pieces_of(int vocab) { return (int)(((int64_t)vocab + kPiece - 1) / k
 
 // Workgroups per sequence: one wavefront per piece for a few sequences; for many, as many
 // as fill kWavesPerCu wavefronts per compute unit over all sequences, the pieces dealt in
-// whole rounds. (64 sequences at 4 / 8 / 12 / 16 on MI355X: 20.0 / 19.6 / 20.4 / 20.9 us in a
-// graph.)
+// whole rounds. (64 sequences at 4 / 8 / 12 / 16 on MI355X: 18.0 / 17.0 / 18.0 / 18.6 us.)
 constexpr int kWavesPerCu = 8;
 static int groups_of(int num_seqs, int pieces) {
   const int64_t waves = (int64_t)kWavesPerCu * device_cus() / num_seqs;

@@ -10,9 +10,11 @@ A value is code * scale[block, head]. Scales are powers of two from 2^-15 to 2^8
 as paged_kv_write_fp8 leaves them (of a scale between two powers every call takes the
 lower one: a pool coded with others has to be coded again): every value is then an
 fp16 number, and a block whose scale grows as it fills is coded again without a
-second rounding (but for codes that fall below e4m3's normal range). A fresh pool needs no initial values:
-a write that begins a block sets its scale. Half the bytes of the fp16 pool (plus
-8 bytes per block and head), for a rounding of at most 2^-4 of each value.
+second rounding (but for codes that fall below e4m3's normal range). A fresh pool
+needs no initial values: a write that begins a block sets its scale. Half the bytes of
+the fp16 pool (plus 8 bytes per block and head), for a rounding of at most 2^-4 of each
+value, or for values below 2^-6 times their scale of 2^-10 times it (once more where
+they are coded again).
 
 Several tokens per sequence are described as for paged_attention_prefill: sequence
 b owns rows query_start_loc[b] .. query_start_loc[b + 1] - 1 of a packed row list,
