@@ -201,7 +201,7 @@ __device__ inline int swizzle(int r) {
 // Wavefronts per SIMD that the registers are kept to. (A workgroup of eight is its compute
 // unit's only one, and spills no vector registers then. Every form keeps about 90 to 150
 // scalar registers in lanes of vector ones; of four wavefronts, two heads of 64 in blocks of
-// other sizes than 16 and 32 alone spill vector registers, 6.)
+// other sizes than 16 and 32 alone spill vector registers, 7.)
 constexpr int waves_per_simd(int D, int NW, int CB) {
   return D == 256 || CB > 1 || NW > 4 ? 2 : 3;
 }
@@ -694,8 +694,8 @@ __global__ __launch_bounds__(64 * NW, waves_per_simd(D, NW, CB)) void attend_fp8
       for (int i = from; i < heads * (s1 - s0); i += kThreads) keep_ml(i, s0, s1, fetch_ml(i, s0, s1));
     };
     // The first ones before the accumulators: maxima and sums are formed while those are on
-    // their way (1 us of 24001 tokens, when it was added). Not where it costs spills: at one token in
-    // workgroups of four (316 MB: 65.5 -> 69.2).
+    // their way (1 us of 24001 tokens, when it was added). Not where it costs spills: at one
+    // token in workgroups of four (316 MB: 65.5 -> 69.2 in a graph).
     constexpr bool EARLY = MULTI || NW > 4;
     const int early = EARLY ? min(nseg, batch) : 0;
     float2 ml0 = {0.f, 0.f};

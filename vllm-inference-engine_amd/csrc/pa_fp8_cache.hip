@@ -13,10 +13,10 @@
 // its lanes, no other wavefront reads or writes that scale or those rows, and the
 // fp16 rows are read once (up to 256 pieces of 16 bytes stay in registers between
 // the maximum and the codes; each lane finds its pieces by steps, not divisions: prompts
-// 18.2 -> 16.2 us in a graph). Bound by memory at prompts, by the chain length -> table entry -> scale ->
-// store at single tokens. On MI355X: four prompts of 9.6k rows in all at 8 heads of 128 (59
-// MB) 15.4 us, 3.8 TB/s; a decode step's row for each of 128 sequences at 2 heads of 64 4.3
-// us, little more than a launch.
+// 18.2 -> 16.2 us in a graph). Bound by memory at prompts, by the chain length -> table
+// entry -> scale -> store at single tokens. On MI355X: four prompts of 9.6k rows in all at
+// 8 heads of 128 (59 MB) 15.4 us, 3.8 TB/s; a decode step's row for each of 128 sequences at 2
+// heads of 64 4.3 us, little more than a launch.
 #include "../../include/paged_attention.h"
 #include "pa_fp8.h"
 
