@@ -31,11 +31,11 @@ own = False
 DEVICE = "cuda"
 FP8 = torch.float8_e4m3fn
 TYPES = {"fp16": torch.float16, "bf16": torch.bfloat16, "fp32": torch.float32}
-# Every drawn case stays within about the listed ones' bytes and operations, and for the
-# decode's plain form within about the listed ones' padded table rows.
+# Every drawn case stays within about the listed ones' bytes, operations and, for the
+# attention's plain form, padded table rows and scores.
 MOST_BYTES = 320e6
-MOST_FLOPS = 6e10
-MOST_PADDED = 2.7e8
+MOST_FLOPS = 4.5e10
+MOST_PADDED = 5.5e8
 # A drawn pool has at most about the largest listed one's bytes.
 MOST_POOL = 700e6
 
@@ -145,7 +145,7 @@ def draw(rng):
             lens, _ = _lens(case)
             if sum(lens) * kv_heads * dim * 4 > MOST_POOL:
                 continue
-            if kind == "decode" and len(lens) * max(lens) * kv_heads * dim > MOST_PADDED:
+            if len(lens) * max(lens) * (kv_heads * dim + heads * min(new, max(lens))) > MOST_PADDED:
                 continue
         w = work(case)
         if w["bytes"] <= MOST_BYTES and w["flops"] <= MOST_FLOPS:
@@ -319,7 +319,7 @@ def run(s):
     if own:
         return _run_own(kind, s)
     return {"sample": _sample_plain, "probs": _probs_plain, "copy": _copy_plain,
-            "decode": _decode_plain, "prefill": _prefill_plain}[kind](s)
+            "decode": _attention, "prefill": _attention}[kind](s)
 
 
 @functools.cache
@@ -393,67 +393,44 @@ def _copy_plain(s):
     return s["caches"]
 
 
-def _scores(s, qk, pos, keys):
-    """Scores from the products [.., rows, heads, keys]; pos [.., rows, 1, 1], keys [keys]."""
-    c = s["case"]
-    x = qk.mul_(s["scale"])
-    if c["softcap"]:
-        x = torch.tanh(x.div_(c["softcap"])).mul_(c["softcap"])
-    if s["slopes"] is not None:
-        x -= s["slopes"][:, None] * (pos - keys).abs().float()
-    return x
-
-
-def _decode_plain(s):
+def _attention(s):
+    """Both attentions, padded to the longest context and the most new tokens."""
     c = s["case"]
     n, hkv, d, g = c["seqs"], c["kv_heads"], c["dim"], c["heads"] // c["kv_heads"]
     ids = s["tables"].long()
-    width = ids.shape[1] * c["block"]
-    keys = torch.arange(width, device=DEVICE)
-    pos = s["seq_lens"].long()[:, None, None] - 1
+    width, most = ids.shape[1] * c["block"], s["most"]
+    start = s["start"].long()
+    new = start[1:] - start[:-1]
+    # [n, kv heads, most * g, d] queries; rows past a sequence's new tokens repeat its last one.
+    at = torch.minimum(torch.arange(most, device=DEVICE)[None, :] + start[:-1, None],
+                       start[1:, None] - 1)
+    pos = (s["seq_lens"].long() - new - start[:-1])[:, None] + at
+    q = s["q"].float()[at].view(n, most, hkv, g, d).transpose(1, 2).reshape(n, hkv, most * g, d)
     k = s["k"][ids].float().view(n, width, hkv, d).permute(0, 2, 3, 1).contiguous()
-    x = torch.matmul(s["q"].float().view(n, hkv, g, d), k).view(n, hkv * g, width)
+    x = torch.matmul(q, k).mul_(s["scale"]).view(n, hkv, most, g, width)
     del k
-    x = _scores(s, x, pos, keys)
-    hidden = keys > pos
+    if c["softcap"]:
+        x.div_(c["softcap"]).tanh_().mul_(c["softcap"])
+    keys = torch.arange(width, device=DEVICE)
+    if s["slopes"] is not None:
+        away = (pos[:, None, :, None, None] - keys).abs_().float()
+        x -= s["slopes"].view(hkv, 1, g, 1) * away
+        del away
+    end = pos + 1 if s["key_ends"] is None else s["key_ends"].long()[at]
+    first = torch.zeros_like(pos) if s["key_starts"] is None else s["key_starts"].long()[at]
     if c["window"]:
-        hidden = hidden | (keys <= pos - c["window"])
-    x.masked_fill_(hidden, -math.inf)
+        first = torch.maximum(first, pos - c["window"] + 1)
+    hidden = (keys >= end[:, :, None]) | (keys < first[:, :, None])
+    x.masked_fill_(hidden[:, None, :, None, :], -math.inf)
     p = x.sub_(x.amax(dim=-1, keepdim=True)).exp_()
-    total = p.sum(dim=-1, keepdim=True)
+    total = p.sum(dim=-1)[..., None]
     v = s["v"][ids].float().view(n, width, hkv, d).transpose(1, 2).contiguous()
-    out = torch.matmul(p.view(n, hkv, g, width), v).view(n, hkv * g, d) / total
-    return {"out": out.half()}
-
-
-def _prefill_plain(s):
-    c = s["case"]
-    hkv, d, g, bs = c["kv_heads"], c["dim"], c["heads"] // c["kv_heads"], c["block"]
-    lens, new = _lens(c)
-    out, at = [], 0
-    for b, (n, rows) in enumerate(zip(lens, new)):
-        ids = s["tables"][b, :-(-n // bs)].long()
-        k = s["k"][ids].view(-1, hkv, d)[:n].float()
-        v = s["v"][ids].view(-1, hkv, d)[:n].float()
-        q = s["q"][at:at + rows].float().view(rows, hkv, g, d).permute(1, 0, 2, 3)
-        x = torch.matmul(q.reshape(hkv, rows * g, d), k.permute(1, 2, 0).contiguous())
-        keys = torch.arange(n, device=DEVICE)
-        pos = torch.arange(n - rows, n, device=DEVICE)
-        x = x.view(hkv, rows, g, n).transpose(0, 1).reshape(rows, hkv * g, n)
-        x = _scores(s, x, pos[:, None, None], keys)
-        end = pos + 1 if s["key_ends"] is None else s["key_ends"][at:at + rows].long()
-        first = torch.zeros_like(pos) if s["key_starts"] is None else s["key_starts"][at:at + rows].long()
-        if c["window"]:
-            first = torch.maximum(first, pos - c["window"] + 1)
-        hidden = (keys[None, :] >= end[:, None]) | (keys[None, :] < first[:, None])
-        x.masked_fill_(hidden[:, None, :], -math.inf)
-        p = x.sub_(x.amax(dim=-1, keepdim=True)).exp_()
-        total = p.sum(dim=-1, keepdim=True)
-        p = p.view(rows, hkv, g, n).transpose(0, 1).reshape(hkv, rows * g, n)
-        o = torch.matmul(p, v.transpose(0, 1).contiguous()).view(hkv, rows, g, d)
-        out.append((o.transpose(0, 1).reshape(rows, hkv * g, d) / total).half())
-        at += rows
-    return {"out": torch.cat(out)}
+    out = torch.matmul(p.view(n, hkv, most * g, width), v).view(n, hkv, most, g, d) / total
+    out = out.permute(0, 2, 1, 3, 4).reshape(n * most, hkv * g, d).half()
+    if n * most == s["q"].shape[0]:
+        return {"out": out}
+    real = torch.arange(most, device=DEVICE)[None, :] < new[:, None]
+    return {"out": out[real.reshape(-1)]}
 
 
 # ---- work --------------------------------------------------------------------------
