@@ -62,9 +62,10 @@ enum {
  * pa_decode_rope_prefetch_f16; 19: weight_row_stride of pa_decode_linear_f16, a
  * rotary workspace that never holds queries in the counter region; 20:
  * pa_kv_write_fp8, pa_kv_read_fp8; 21: pa_verify_drafts_f32; 22: pa_decode_fp8; 23:
- * pa_prefill_attention_fp8; 24: its workspace size). pa_abi_version returns the
+ * pa_prefill_attention_fp8; 24: its workspace size; 25: pa_copy_blocks; 26:
+ * pa_sample_tokens, pa_sampling_probs). pa_abi_version returns the
  * library's. */
-#define PA_ABI_VERSION 24
+#define PA_ABI_VERSION 26
 PA_API int pa_abi_version(void);
 
 /* Message of the last failed call on this thread ("" after a success). */
@@ -616,6 +617,63 @@ PA_API int pa_verify_drafts_f32(const float* target, const int64_t target_stride
                                 const float* next_u, const int32_t* num_drafts, int64_t* tokens,
                                 int32_t* accepted, int num_seqs, int max_drafts, int vocab,
                                 void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Copies of pool blocks: t[dst_blocks[i]] = t[src_blocks[i]] for every tensor t and pair i,
+ * bit for bit. No counterpart in the reference, which refuses to write a block that is
+ * shared (engine/kernels/paged_attention_integration.py:587-592). tensors, block_strides
+ * and block_bytes are host arrays of num_tensors entries: the address of block 0, the
+ * bytes from block to block (at least block_bytes) and the contiguous bytes of one.
+ * src_blocks and dst_blocks are device arrays of num_pairs ids, their strides in elements;
+ * pairs with an id outside [0, num_blocks) are skipped. A destination must be in no other
+ * pair. One launch for up to 96 tensors.
+ */
+PA_API int pa_copy_blocks(void* const* tensors, const int64_t* block_strides,
+                          const int64_t* block_bytes, int num_tensors, const int32_t* src_blocks,
+                          int64_t src_stride, const int32_t* dst_blocks, int64_t dst_stride,
+                          int num_pairs, int num_blocks, void* stream);
+
+/*
+ * Sampling from logits. No counterpart in the reference, whose decode step selects
+ * greedily (engine/kernels/paged_attention_integration.py:636-651). logits are
+ * [num_seqs, rows_per_seq, vocab] of type PA_F16, PA_BF16 or PA_F32, strides in elements
+ * (the vocabulary's 1). Settings are per sequence, contiguous, or NULL: the value beside
+ * them for all. For a row z with maximum m:
+ *   - weights w = exp((z - m) / temperature). A temperature that is not above 0 keeps the
+ *     first of the largest logits alone. NaN logits count as -inf, whose weight is 0; beside a
+ *     logit of +inf all finite ones weigh 0.
+ *   - the order is by z, largest first, equal ones (both zeros, too) by index.
+ *   - top_k (<= 0: off): the first top_k stay.
+ *   - top_p (not below 1, NaN: off): of those, the shortest beginning whose weight is at
+ *     least top_p times their sum, one entry at least.
+ *   - min_p (<= 0, NaN: off; at most 1): of those, the entries with w >= min_p.
+ * pa_sample_tokens: tokens[num_seqs][rows_per_seq] (contiguous) = the first index, in the
+ * vocabulary's order, whose cumulative weight of kept entries exceeds u[seq][row] times
+ * their sum; the last one with a weight where there is none (u of 1 and more, NaN), index 0
+ * of a row without any weight. pa_sampling_probs: probs[num_seqs][rows_per_seq][vocab]
+ * (contiguous) = w / sum for kept entries, 0 for others and for a row without any weight.
+ * Weights are computed in 64 bits and summed as whole numbers of 2^-44: a token drawn never
+ * weighs less than 2^-45, and one is exchanged for its neighbour only where u times the sum
+ * lies within 2^-44 per entry of a border. At most 16384 rows of 2^19 logits.
+ *
+ * Workspace: its first bytes are arrival counters that must be zero before the first
+ * call that uses the buffer; every call leaves them zero. One buffer per stream, lent
+ * to nothing else but these two.
+ */
+enum { PA_F16 = 0, PA_BF16 = 1, PA_F32 = 2 };
+PA_API size_t pa_sample_workspace_bytes(int num_seqs, int rows_per_seq, int vocab);
+PA_API int pa_sample_tokens(const void* logits, int dtype, const int64_t logits_strides[3],
+                            const float* u, const int64_t u_strides[2], const float* temperature,
+                            float temperature_all, const int32_t* top_k, int top_k_all,
+                            const float* top_p, float top_p_all, const float* min_p,
+                            float min_p_all, int64_t* tokens, int num_seqs, int rows_per_seq,
+                            int vocab, void* workspace, size_t workspace_bytes, void* stream);
+PA_API int pa_sampling_probs(const void* logits, int dtype, const int64_t logits_strides[3],
+                             const float* temperature, float temperature_all,
+                             const int32_t* top_k, int top_k_all, const float* top_p,
+                             float top_p_all, const float* min_p, float min_p_all, float* probs,
+                             int num_seqs, int rows_per_seq, int vocab, void* workspace,
+                             size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

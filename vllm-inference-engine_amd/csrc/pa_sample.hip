@@ -1,0 +1,1296 @@
+// Sampling from logits: temperature, top-k, top-p and min-p, by given random numbers (gfx950).
+//
+// A row's weights are w = exp((z - max z) / T). Its entries are ordered by z, largest first,
+// equal ones by index; the first top_k stay, of them the shortest beginning that weighs
+// top_p of their sum, of those the ones with w >= min_p. The token is the first index whose
+// cumulative kept weight exceeds u times the sum; or the row of probabilities is written.
+//
+// A row is read once, in pieces of 1024 entries by wavefronts of several workgroups: the
+// maximum of each cell of 128 entries, of each piece, and where the settings need the whole
+// sum, the piece's sum of weights go to the workspace. The last of the row's workgroups to
+// arrive decides. It does not sort. The cells' maxima give a lower bound on what can be
+// kept: for top-k, the k-th largest of them (k entries at least reach it); for min-p its
+// own logit; for top-p, entries below (1 - p) / vocab of the sum, which together weigh less
+// than 1 - p. Only cells that reach the bound are read again, and their entries above it
+// listed: tens to hundreds for usual settings. A short list is ranked by comparing all
+// with all; a longer one by radix passes over the logits' bits with counts and weights; one
+// that does not fit LDS (flat distributions) is first narrowed by counts and weights per
+// interval of logits, to the interval in which the border lies.
+//
+// Weights and sums. w is computed in 64 bits (2^-45 relative) and summed as whole numbers of
+// 2^-44: sums do not depend on the order, so that LDS atomics may form them, and the 2^19
+// entries that a row may have cannot overflow 64 bits. (Sums of whole pieces, formed while
+// the row is read, are in 64-bit floating point in a fixed order.) The token differs from the
+// definition's only where u times the sum lies within about 2^-44 per entry of a border.
+#include "../../include/paged_attention.h"
+#include "pa_tiles.h"
+
+namespace pa {
+namespace sample {
+
+constexpr int kThreads = 512;
+constexpr int kWaves = kThreads / 64;
+constexpr int kPiece = 1024;  // entries of a wavefront's step, 16 per lane
+constexpr int kCell = 128;    // entries of 16 lanes, eight each
+constexpr int kMaxVocab = 1 << 19;
+constexpr int kMaxPieces = kMaxVocab / kPiece;
+constexpr int kMaxCells = kMaxVocab / kCell;
+// The workspace starts with one arrival counter per row, at the same place for every call.
+constexpr int kMaxRows = 16384;
+constexpr size_t kCounterBytes = (size_t)kMaxRows * sizeof(int);
+constexpr int kList = 2048;   // listed entries
+constexpr int kShort = 256;   // of them, ranked by comparing all with all
+constexpr int kBins = 1024;
+constexpr uint32_t kDead = 0x007fffffu;  // order key of -inf; NaN counts as -inf
+constexpr double kUnit = 17592186044416.0;  // 2^44
+
+typedef unsigned long long u64;
+
+// What the deciding workgroup leaves for the launch that writes probabilities.
+struct Decision {
+  float max;
+  uint32_t key;   // kept: order keys above this one,
+  int last;       // or equal to it up to this index
+  float min_p;
+  double c;       // log2(e) / T
+  double sum;
+};
+
+struct Piece {
+  float max, pad;
+  double sum;
+};
+
+struct Args {
+  const void* logits;
+  int64_t s_seq, s_row;  // elements from sequence to sequence and row to row
+  int rows, each, vocab;
+  const float* temperature;  // per sequence, or null: t_all
+  const int32_t* top_k;
+  const float* top_p;
+  const float* min_p;
+  float t_all, p_all, m_all;
+  int k_all;
+  const float* u;  // per row, strides; null: decisions for the probabilities
+  int64_t u_seq, u_row;
+  int64_t* tokens;
+  float* probs;
+  int* cnt;
+  char* records;  // per row: Decision, pieces, cells
+  int row_bytes, pieces, cells, groups;
+};
+
+__host__ __device__ inline int row_record(int pieces, int cells) {
+  return (int)sizeof(Decision) + pieces * (int)sizeof(Piece) + (cells + 3) / 4 * 16;
+}
+
+// ---- entries -----------------------------------------------------------------------
+
+// Logits in memory at any alignment of their own.
+struct Half {
+  typedef uint16_t E;
+  static constexpr E kLow = 0xfc00;  // -inf
+  __device__ static float get(E x) { return (float)__builtin_bit_cast(f16, x); }
+};
+struct Brain {
+  typedef uint16_t E;
+  static constexpr E kLow = 0xff80;
+  __device__ static float get(E x) { return __builtin_bit_cast(float, (uint32_t)x << 16); }
+};
+struct Single {
+  typedef uint32_t E;
+  static constexpr E kLow = 0xff800000u;
+  __device__ static float get(E x) { return __builtin_bit_cast(float, x); }
+};
+
+// Eight entries as they lie in memory; the floats they stand for, NaN as -inf.
+template <typename T>
+struct Eight {
+  typedef typename T::E E;
+  typedef E words __attribute__((ext_vector_type(8), aligned(sizeof(E))));
+  words w;
+
+  // Entries v0 .. v0 + 7 of a row of eight and more. A lane whose entries reach past the end
+  // gets the row's last eight, those before v0 as -inf, and is told where they begin.
+  __device__ __forceinline__ int load(const E* row, int v0, int vocab) {
+    const int at = min(v0, vocab - 8);
+    w = *reinterpret_cast<const words*>(row + at);
+    if (at != v0) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = at + i < v0 ? T::kLow : w[i];
+    }
+    return at;
+  }
+  __device__ __forceinline__ float operator[](int i) const { return fmaxf(T::get(w[i]), kNegInf); }
+};
+
+// Unsigned numbers in the logits' order; both zeros are one.
+__device__ inline uint32_t order_key(float z) {
+  const uint32_t b = __builtin_bit_cast(uint32_t, z + 0.f);
+  return b ^ ((uint32_t)((int)b >> 31) | 0x80000000u);
+}
+__device__ inline float of_key(uint32_t k) {
+  return __builtin_bit_cast(float, k & 0x80000000u ? k ^ 0x80000000u : ~k);
+}
+
+// 2^d for d <= 0, to 2^-45 relative: the whole part by the exponent, the rest by a polynomial
+// through 2^f at the ten Chebyshev nodes of [-1/2, 1/2]. Below -1060 and for NaN as good as 0.
+__device__ inline double exp2_of(double d) {
+  d = fmax(d, -1060.0);
+  const double n = __builtin_rint(d);
+  const double f = d - n;
+  double p = 1.0212097549811005e-07;
+  p = __builtin_fma(p, f, 1.3259945262689143e-06);
+  p = __builtin_fma(p, f, 1.5252640059770786e-05);
+  p = __builtin_fma(p, f, 0.00015403432339553542);
+  p = __builtin_fma(p, f, 0.001333355825801874);
+  p = __builtin_fma(p, f, 0.009618129195951041);
+  p = __builtin_fma(p, f, 0.05550410866428854);
+  p = __builtin_fma(p, f, 0.24022650695631514);
+  p = __builtin_fma(p, f, 0.6931471805599526);
+  p = __builtin_fma(p, f, 1.000000000000014);
+  return __builtin_amdgcn_ldexp(p, (int)n);
+}
+
+// Weight of z next to the maximum m: 1 at the maximum, whatever the temperature (a maximum
+// of +inf too, beside which all others weigh nothing).
+__device__ inline double weight(float z, float m, double c) {
+  return z == m ? 1.0 : exp2_of(((double)z - (double)m) * c);
+}
+__device__ inline u64 units(double w) { return (u64)(w * kUnit + 0.5); }
+
+// ---- sums over lanes ---------------------------------------------------------------
+
+template <int CTRL>
+__device__ inline double row_lane(double x) {
+  const uint2 v = __builtin_bit_cast(uint2, x);
+  return __builtin_bit_cast(
+      double, make_uint2((unsigned)__builtin_amdgcn_update_dpp(0, (int)v.x, CTRL, 0xf, 0xf, false),
+                         (unsigned)__builtin_amdgcn_update_dpp(0, (int)v.y, CTRL, 0xf, 0xf, false)));
+}
+template <int CTRL>
+__device__ inline u64 row_lane(u64 x) {
+  return __builtin_bit_cast(u64, row_lane<CTRL>(__builtin_bit_cast(double, x)));
+}
+template <typename X>
+__device__ inline X lane_of(X x, int l) {  // of 64 bits, l uniform
+  const uint2 v = __builtin_bit_cast(uint2, x);
+  return __builtin_bit_cast(X, make_uint2((unsigned)__builtin_amdgcn_readlane((int)v.x, l),
+                                          (unsigned)__builtin_amdgcn_readlane((int)v.y, l)));
+}
+// Over a wavefront, in every lane: rotations within rows of 16, then the rows.
+template <typename X>
+__device__ inline X wave_sum(X x) {
+  x += row_lane<0x128>(x);
+  x += row_lane<0x124>(x);
+  x += row_lane<0x122>(x);
+  x += row_lane<0x121>(x);
+  return (lane_of(x, 0) + lane_of(x, 16)) + (lane_of(x, 32) + lane_of(x, 48));
+}
+// Over the lanes up to each.
+__device__ inline u64 wave_scan(u64 x, int lane) {
+  x += row_lane<0x111>(x);
+  x += row_lane<0x112>(x);
+  x += row_lane<0x114>(x);
+  x += row_lane<0x118>(x);
+  const u64 r0 = lane_of(x, 15), r1 = lane_of(x, 31), r2 = lane_of(x, 47);
+  return x + (lane < 16 ? 0 : lane < 32 ? r0 : lane < 48 ? r0 + r1 : r0 + r1 + r2);
+}
+// Maximum over rows of 16 lanes, in all of them.
+__device__ inline float row_max(float x) {
+  auto turned = [](float v, auto by) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v),
+                                                                 0x120 + decltype(by)::value, 0xf,
+                                                                 0xf, false));
+  };
+  x = fmaxf(x, turned(x, std::integral_constant<int, 8>()));
+  x = fmaxf(x, turned(x, std::integral_constant<int, 4>()));
+  x = fmaxf(x, turned(x, std::integral_constant<int, 2>()));
+  return fmaxf(x, turned(x, std::integral_constant<int, 1>()));
+}
+__device__ inline float wave_max_of_rows(float x) {  // x: equal within rows of 16
+  auto at = [&](int l) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), l));
+  };
+  return fmaxf(fmaxf(at(0), at(16)), fmaxf(at(32), at(48)));
+}
+
+// ---- settings ----------------------------------------------------------------------
+
+struct Settings {
+  double c;      // log2(e) / T
+  int k;         // entries that top-k keeps, 0: all
+  float p;       // top-p, 1: off
+  float min_p;   // 0: off
+  bool whole;    // the sum over all entries is needed
+  bool filtered;
+};
+
+__device__ inline Settings settings_of(const Args& a, int seq) {
+  Settings s;
+  const float t = a.temperature ? a.temperature[seq] : a.t_all;
+  s.k = a.top_k ? a.top_k[seq] : a.k_all;
+  s.p = a.top_p ? a.top_p[seq] : a.p_all;
+  s.min_p = a.min_p ? a.min_p[seq] : a.m_all;
+  if (s.k <= 0 || s.k >= a.vocab) s.k = 0;
+  if (!(s.p < 1.f)) s.p = 1.f;
+  s.min_p = s.min_p > 0.f ? fminf(s.min_p, 1.f) : 0.f;
+  if (!(t > 0.f)) {  // greedy: the first of the largest
+    s.c = 1.0;
+    s.k = 1;
+    s.p = 1.f;
+    s.min_p = 0.f;
+  } else {
+    s.c = 1.4426950408889634 / (double)t;
+    if (s.p <= 0.f) {  // the first alone, too
+      s.k = 1;
+      s.p = 1.f;
+    }
+  }
+  s.filtered = s.k > 0 || s.p < 1.f || s.min_p > 0.f;
+  s.whole = !s.filtered || (s.k == 0 && s.p < 1.f);
+  return s;
+}
+
+// ---- the deciding workgroup ---------------------------------------------------------
+
+struct Shared {
+  uint32_t key[kList];
+  int idx[kList];
+  union {
+    struct {
+      u64 w[kBins];
+      uint32_t n[kBins];
+    } bin;
+    uint16_t cells[kMaxCells];
+    struct {
+      u64 w[kShort];
+      u64 order[kShort];
+    } brief;
+  };
+  u64 psum[kMaxPieces];
+  int pcount[kMaxPieces];
+  u64 part[kWaves];
+  int count;
+  uint32_t found_key;
+  int found, found2;
+  u64 found_w;
+};
+
+// The entries that are still in question: those in interval `bin` of the logits' line (of
+// scale 0: all are in interval 0), with these leading bits of their key. What lies above is
+// kept for sure.
+struct Range {
+  uint32_t floor;  // keys below are out of the question
+  float lo, scale;
+  int bin;
+  uint32_t mask, bits;
+  __device__ int bin_of(float z) const {
+    const float t = (z - lo) * scale;
+    return t > 0.f ? (t < (float)(kBins - 1) ? (int)t : kBins - 1) : 0;
+  }
+  // 0: no, 1: in question, 2: kept
+  __device__ int place(float z, uint32_t key) const {
+    if (key < floor) return 0;
+    const int b = bin_of(z);
+    if (b != bin) return b > bin ? 2 : 0;
+    const uint32_t x = key & mask;
+    return x == bits ? 1 : x > bits ? 2 : 0;
+  }
+};
+
+template <typename T>
+struct Decider {
+  typedef typename T::E E;
+  const Args& a;
+  Shared& sh;
+  const E* row;
+  Settings s;
+  float m;
+  int tid, lane, wave;
+  int listed_cells;  // -1: all pieces are read
+
+  // f(x, v0) for entries v0 .. v0 + 7 of every lane, by whole wavefronts: 512 entries a time,
+  // kAhead times read before the first is looked at.
+  static constexpr int kAhead = 4;
+  template <typename F>
+  __device__ __forceinline__ void each_entry(F f) {
+    const bool dense = listed_cells < 0;
+    const int steps = dense ? (a.vocab + 511) / 512 : (listed_cells + 3) / 4;
+    for (int i0 = wave; i0 < steps; i0 += kWaves * kAhead) {  // wavefront-uniform
+      Eight<T> x[kAhead];
+      int v0[kAhead];
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        const int i = i0 + j * kWaves;
+        v0[j] = a.vocab;
+        if (dense)
+          v0[j] = i * 512 + lane * 8;
+        else if (i * 4 + (lane >> 4) < listed_cells)
+          v0[j] = (int)sh.cells[i * 4 + (lane >> 4)] * kCell + (lane & 15) * 8;
+        if (i < steps) v0[j] = x[j].load(row, v0[j], a.vocab);
+      }
+      // (One copy of f's code.)
+#pragma unroll 1
+      for (int j = 0; j < kAhead && i0 + j * kWaves < steps; ++j) {
+        Eight<T> y;
+        int v;
+        switch (j) {
+          case 0: y = x[0], v = v0[0]; break;
+          case 1: y = x[1], v = v0[1]; break;
+          case 2: y = x[2], v = v0[2]; break;
+          default: y = x[3], v = v0[3]; break;
+        }
+        f(y, v);
+      }
+    }
+  }
+
+  // Sum over the workgroup, in every thread.
+  __device__ __forceinline__ u64 block_sum(u64 x) {
+    x = wave_sum(x);
+    __syncthreads();
+    if (lane == 0) sh.part[wave] = x;
+    __syncthreads();
+    u64 t = 0;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) t += sh.part[i];
+    return t;
+  }
+
+  __device__ __forceinline__ float block_max(float x) {
+    x = wave_max_of_rows(row_max(x));
+    __syncthreads();
+    if (lane == 0) sh.part[wave] = (u64)__builtin_bit_cast(uint32_t, x);
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) x = fmaxf(x, __builtin_bit_cast(float, (uint32_t)sh.part[i]));
+    return x;
+  }
+
+  // The smallest key that the k-th largest of the cells' maxima can have, to 16 bits.
+  __device__ __forceinline__ uint32_t cell_bound(const __amdgpu_buffer_rsrc_t& rc, int k) {
+    if (k > a.cells) return 0;
+    constexpr int PER = kMaxCells / kThreads;
+    static_assert(PER == 8, "two loads of four per thread");
+    uint32_t keys[PER];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int c0 = (j * kThreads + tid) * 4;
+      if (j * kThreads * 4 >= a.cells) {  // uniform
+#pragma unroll
+        for (int i = 0; i < 4; ++i) keys[j * 4 + i] = 0;
+        continue;
+      }
+      const f32x4 y = tiles::load_coherent16(rc, c0 * 4);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) keys[j * 4 + i] = c0 + i < a.cells ? order_key(y[i]) : 0;
+    }
+    uint32_t prefix = 0;
+    int left = k;
+#pragma unroll
+    for (int pass = 0; pass < 2; ++pass) {
+      for (int i = tid; i < 256; i += kThreads) sh.bin.n[i] = 0;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const uint32_t x = keys[i];
+        if (x != 0 && (pass == 0 || x >> 24 == prefix))
+          atomicAdd(&sh.bin.n[pass == 0 ? x >> 24 : (x >> 16) & 255], 1u);
+      }
+      __syncthreads();
+      if (wave == 0) {
+        // Lane l: bins 255 - 4 l down to 252 - 4 l.
+        int own[4], mine = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mine += own[i] = (int)sh.bin.n[255 - 4 * lane - i];
+        const int incl = tiles::wave_incl_scan(mine);
+        int sum = incl - mine, hit = -1, before = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (hit < 0 && sum + own[i] >= left) {
+            hit = 255 - 4 * lane - i;
+            before = sum;
+          }
+          sum += own[i];
+        }
+        const uint64_t hits = __ballot(hit >= 0);
+        if (hits && lane == (int)__builtin_ctzll(hits)) {
+          sh.found = hit;
+          sh.found2 = left - before;
+        }
+      }
+      __syncthreads();
+      prefix = prefix << 8 | (uint32_t)sh.found;
+      left = sh.found2;
+      __syncthreads();
+    }
+    return prefix << 16;
+  }
+
+  // Lists the cells whose maximum reaches the bound; whether few enough are listed.
+  __device__ __forceinline__ bool list_cells(const __amdgpu_buffer_rsrc_t& rc, uint32_t floor) {
+    if (tid == 0) sh.count = 0;
+    __syncthreads();
+    for (int base = 0; base < a.cells; base += kThreads * 4) {  // uniform
+      const int c0 = base + tid * 4;
+      const f32x4 y = tiles::load_coherent16(rc, c0 * 4);
+      bool in[4];
+      int mine = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) mine += in[i] = c0 + i < a.cells && order_key(y[i]) >= floor;
+      const int incl = tiles::wave_incl_scan(mine);
+      int at = 0;
+      if (lane == 63 && incl) at = atomicAdd(&sh.count, incl);
+      at = __builtin_amdgcn_readlane(at, 63) + incl - mine;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (in[i]) sh.cells[at++] = (uint16_t)(c0 + i);
+    }
+    __syncthreads();
+    const int n = sh.count;
+    __syncthreads();
+    listed_cells = n;
+    return n * 4 <= a.cells || a.cells <= 64;
+  }
+
+  // Lists the entries in question; how many there are (more than kList: not all listed).
+  __device__ __forceinline__ int list_entries(const Range& r) {
+    if (tid == 0) sh.count = 0;
+    __syncthreads();
+    each_entry([&](const Eight<T>& x, int v0) __attribute__((always_inline)) {
+      unsigned in = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) in |= (unsigned)(r.place(x[i], order_key(x[i])) == 1) << i;
+      if (__ballot(in != 0) == 0) return;
+      const int mine = __builtin_popcount(in);
+      const int incl = tiles::wave_incl_scan(mine);
+      int at = 0;
+      if (lane == 63) at = atomicAdd(&sh.count, incl);
+      at = __builtin_amdgcn_readlane(at, 63) + incl - mine;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (in >> i & 1) {
+          if (at < kList) {
+            sh.key[at] = order_key(x[i]);
+            sh.idx[at] = v0 + i;
+          }
+          ++at;
+        }
+    });
+    __syncthreads();
+    const int n = sh.count;
+    __syncthreads();
+    return n;
+  }
+
+  // Of the bins' counts and weights, from the last bin down: the first at which k entries
+  // or a weight of `aim` are reached, in sh.found (-1: none), and what lies above it in
+  // sh.found2 and sh.found_w. (k 0 or aim ~0: no such limit.)
+  __device__ __forceinline__ void walk_bins(int bins, int have, u64 have_w, int k, u64 aim) {
+    __syncthreads();
+    if (wave == 0) {
+      const int per = bins / 64;
+      int mine = 0;
+      u64 mine_w = 0;
+      for (int i = 0; i < per; ++i) {
+        const int b = bins - 1 - lane * per - i;
+        mine += (int)sh.bin.n[b];
+        mine_w += sh.bin.w[b];
+      }
+      int sum = have + tiles::wave_incl_scan(mine) - mine;
+      u64 sum_w = have_w + wave_scan(mine_w, lane) - mine_w;
+      int hit = -1, before = 0;
+      u64 before_w = 0;
+      for (int i = 0; i < per; ++i) {
+        const int b = bins - 1 - lane * per - i;
+        const int n = (int)sh.bin.n[b];
+        const u64 w = sh.bin.w[b];
+        if (hit < 0 && n > 0 && ((k > 0 && sum + n >= k) || sum_w + w >= aim)) {
+          hit = b;
+          before = sum;
+          before_w = sum_w;
+        }
+        sum += n;
+        sum_w += w;
+      }
+      const uint64_t hits = __ballot(hit >= 0);
+      if (hits ? lane == (int)__builtin_ctzll(hits) : lane == 0) {
+        sh.found = hit;
+        sh.found2 = before;
+        sh.found_w = before_w;
+      }
+    }
+    __syncthreads();
+  }
+
+  // Where the kept ones end: keys above `key`, and of those equal to it `ties`; `count` and
+  // `w` of the entries above it. ties -1: everything down to the bound is kept.
+  struct Cut {
+    uint32_t key;
+    int ties, all;  // kept ones of that key, and all of it
+    int above;
+    u64 above_w;
+    Range range;    // in which the listed entries lie (narrowed where they did not fit)
+    bool in_list;   // the entries of range are listed
+    int n;
+  };
+
+  // First k entries (0: no such limit), or the shortest beginning that weighs aim, of the
+  // entries from `floor` on, n of them (all listed if they fit).
+  __device__ __forceinline__ Cut cut(uint32_t floor, int n, int k, u64 aim) {
+    Cut c{};
+    c.range = Range{floor, 0.f, 0.f, 0, 0, 0};
+    c.n = n;
+    bool none = false;
+    if (n > kList) {
+      // Narrowed by intervals of the line of logits first; if more than fit are in one, by
+      // the bits of their keys.
+      listed_cells = -1;
+      c.range.lo = floor > kDead ? of_key(floor) : (float)((double)m - 46.0 / s.c);
+      const float width = m - c.range.lo;
+      c.range.scale = width > 0.f && width < 3e38f ? (float)kBins / width : 0.f;
+      int shift = 32;
+      bool first = c.range.scale > 0.f;
+      c.range.bin = 0;
+      for (;;) {
+        // A round: the bins of what is in question.
+        for (int i = tid; i < kBins; i += kThreads) {
+          sh.bin.n[i] = 0;
+          sh.bin.w[i] = 0;
+        }
+        __syncthreads();
+        const int low = first ? 0 : shift > 10 ? shift - 10 : 0;
+        const int bits = first ? 10 : shift - low;
+        each_entry([&](const Eight<T>& x, int) __attribute__((always_inline)) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const uint32_t key = order_key(x[i]);
+            if (first ? key >= floor : c.range.place(x[i], key) == 1) {
+              const int b = first ? c.range.bin_of(x[i]) : (int)((key >> low) & ((1u << bits) - 1));
+              atomicAdd(&sh.bin.n[b], 1u);
+              atomicAdd(&sh.bin.w[b], units(weight(x[i], m, s.c)));
+            }
+          }
+        });
+        walk_bins(kBins, c.above, c.above_w, k, aim);
+        int b = sh.found;
+        if (b < 0) {  // the limit is not reached
+          none = true;
+          // On with the lowest bin that holds anything: what lies above it is kept for sure.
+          if (tid == 0) sh.count = kBins - 1;
+          __syncthreads();
+          for (int i = tid; i < kBins; i += kThreads)
+            if (sh.bin.n[i] != 0) atomicMin(&sh.count, i);
+          __syncthreads();
+          b = sh.count;
+          u64 w = 0;
+          int above = 0;
+          for (int i = b + 1 + tid; i < kBins; i += kThreads) {
+            w += sh.bin.w[i];
+            above += (int)sh.bin.n[i];
+          }
+          c.above += (int)block_sum((u64)above);
+          c.above_w += block_sum(w);
+        } else {
+          c.above = sh.found2;
+          c.above_w = sh.found_w;
+        }
+        const int held = (int)sh.bin.n[b];
+        if (first) {
+          c.range.bin = b;
+          first = false;
+        } else {
+          shift = low;
+          c.range.bits |= (uint32_t)b << low;
+          c.range.mask = low == 0 ? ~0u : ~((1u << low) - 1);
+        }
+        __syncthreads();
+        if (c.range.mask == ~0u) {  // equal logits alone
+          c.key = c.range.bits;
+          c.all = held;
+          finish(c, none, k, aim);
+          return c;
+        }
+        if (held <= kList) break;
+      }
+      c.n = list_entries(c.range);
+    }
+    c.in_list = true;
+    // Radix passes over the list.
+    uint32_t prefix = 0;
+    for (int shift = 24; shift >= 0; shift -= 8) {
+      for (int i = tid; i < 256; i += kThreads) {
+        sh.bin.n[i] = 0;
+        sh.bin.w[i] = 0;
+      }
+      __syncthreads();
+      for (int i = tid; i < c.n; i += kThreads) {
+        const uint32_t key = sh.key[i];
+        if (shift == 24 || key >> (shift + 8) == prefix) {
+          atomicAdd(&sh.bin.n[key >> shift & 255], 1u);
+          atomicAdd(&sh.bin.w[key >> shift & 255], units(weight(of_key(key), m, s.c)));
+        }
+      }
+      walk_bins(256, c.above, c.above_w, k, aim);
+      if (sh.found < 0) {  // the limit is not reached (in the first pass, if at all)
+        c.key = c.range.floor;
+        c.ties = -1;
+        c.all = 0;
+        __syncthreads();
+        return c;
+      }
+      prefix = prefix << 8 | (uint32_t)sh.found;
+      c.above = sh.found2;
+      c.above_w = sh.found_w;
+      c.all = (int)sh.bin.n[sh.found];
+      __syncthreads();
+    }
+    c.key = prefix;
+    finish(c, false, k, aim);
+    return c;
+  }
+
+  // How many of the equal logits at the border are kept.
+  __device__ __forceinline__ void finish(Cut& c, bool none, int k, u64 aim) {
+    if (none) {
+      c.ties = c.all;
+      return;
+    }
+    int t = c.all;
+    if (k > 0) t = min(t, k - c.above);
+    const u64 w = units(weight(of_key(c.key), m, s.c));
+    if (aim != ~0ull && w > 0) {
+      const u64 need = aim > c.above_w ? (aim - c.above_w + w - 1) / w : 0;
+      if (need < (u64)t) t = (int)need;
+    }
+    c.ties = t > 0 ? t : (c.above > 0 ? 0 : 1);
+  }
+
+  // The index up to which entries of key c.key are kept.
+  __device__ __forceinline__ int last_tie(const Cut& c) {
+    if (c.ties < 0 || c.ties >= c.all) return 0x7fffffff;
+    if (c.ties == 0) return -1;
+    for (int i = tid; i < kMaxPieces; i += kThreads) sh.pcount[i] = 0;
+    __syncthreads();
+    if (c.in_list) {
+      for (int i = tid; i < c.n; i += kThreads)
+        if (sh.key[i] == c.key) atomicAdd(&sh.pcount[sh.idx[i] / kPiece], 1);
+    } else {
+      each_entry([&](const Eight<T>& x, int v0) __attribute__((always_inline)) {
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) n += order_key(x[i]) == c.key;
+        if (n) atomicAdd(&sh.pcount[(v0 + 7) / kPiece], n);
+      });
+    }
+    __syncthreads();
+    if (wave == 0) {
+      // Lane l: pieces 8 l .. 8 l + 7.
+      constexpr int PER = kMaxPieces / 64;
+      int own[PER], mine = 0;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) mine += own[i] = sh.pcount[lane * PER + i];
+      int sum = tiles::wave_incl_scan(mine) - mine, hit = -1, before = 0;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        if (hit < 0 && sum + own[i] >= c.ties) {
+          hit = lane * PER + i;
+          before = sum;
+        }
+        sum += own[i];
+      }
+      const uint64_t hits = __ballot(hit >= 0);
+      const int l = (int)__builtin_ctzll(hits);  // (the kept ones are among all)
+      const int piece = __builtin_amdgcn_readlane(hit, l);
+      int left = c.ties - __builtin_amdgcn_readlane(before, l);
+      int found = -1;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        Eight<T> x;
+        const int v0 = x.load(row, piece * kPiece + j * 512 + lane * 8, a.vocab);
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) n += order_key(x[i]) == c.key;
+        const int incl = tiles::wave_incl_scan(n);
+        int run = incl - n;
+        int at = -1;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (order_key(x[i]) == c.key && ++run == left) at = v0 + i;
+        const uint64_t got = __ballot(at >= 0);
+        if (got && found < 0) found = __builtin_amdgcn_readlane(at, (int)__builtin_ctzll(got));
+        left -= __builtin_amdgcn_readlane(incl, 63);
+      }
+      if (lane == 0) sh.found = found;
+    }
+    __syncthreads();
+    const int last = sh.found;
+    __syncthreads();
+    return last;
+  }
+
+  // Weight of a kept entry, or 0.
+  __device__ __forceinline__ u64 kept_units(float z, int v, uint32_t key_above, int last) const {
+    const uint32_t key = order_key(z);
+    if (key <= kDead || key < key_above || (key == key_above && v > last)) return 0;
+    const double w = weight(z, m, s.c);
+    return w >= (double)s.min_p ? units(w) : 0;
+  }
+
+  // The first index whose cumulative kept weight exceeds u times the sum, of the pieces'
+  // kept weights in psum. The last with any weight where there is none.
+  __device__ __forceinline__ void draw(int r, uint32_t key_above, int last, u64 sum) {
+    __syncthreads();
+    if (wave != 0) return;
+    const int seq = r / a.each;
+    const float u = a.u[seq * a.u_seq + (r - seq * a.each) * a.u_row];
+    const double aim = (double)u * (double)sum;
+    constexpr int PER = kMaxPieces / 64;
+    u64 own[PER], mine = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) mine += own[i] = lane * PER + i < a.pieces ? sh.psum[lane * PER + i] : 0;
+    u64 run = wave_scan(mine, lane) - mine;
+    int hit = -1, some = -1;
+    u64 hit_before = 0, some_before = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      if (own[i] > 0) {
+        if (hit < 0 && (double)(run + own[i]) > aim) {
+          hit = lane * PER + i;
+          hit_before = run;
+        }
+        some = lane * PER + i;
+        some_before = run;
+      }
+      run += own[i];
+    }
+    const uint64_t hits = __ballot(hit >= 0), somes = __ballot(some >= 0);
+    int64_t token = 0;
+    if (hits || somes) {
+      const int l = hits ? (int)__builtin_ctzll(hits) : 63 - (int)__builtin_clzll(somes);
+      const int piece = __builtin_amdgcn_readlane(hits ? hit : some, l);
+      u64 before = lane_of(hits ? hit_before : some_before, l);
+      int found = -1, spare = -1;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        Eight<T> x;
+        const int v0 = x.load(row, piece * kPiece + j * 512 + lane * 8, a.vocab);
+        u64 w[8], mine = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) mine += w[i] = kept_units(x[i], v0 + i, key_above, last);
+        const u64 incl = wave_scan(mine, lane);
+        u64 run = before + incl - mine;
+        int at = -1, any = -1;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (w[i] > 0) {
+            run += w[i];
+            if (at < 0 && (double)run > aim) at = v0 + i;
+            any = v0 + i;
+          }
+        const uint64_t ats = __ballot(at >= 0), anys = __ballot(any >= 0);
+        if (ats && found < 0) found = __builtin_amdgcn_readlane(at, (int)__builtin_ctzll(ats));
+        if (anys) spare = __builtin_amdgcn_readlane(any, 63 - (int)__builtin_clzll(anys));
+        before += lane_of(incl, 63);
+      }
+      token = found >= 0 ? found : spare >= 0 ? spare : 0;
+    }
+    if (lane == 0) a.tokens[r] = token;
+  }
+
+  __device__ __forceinline__ void leave(int r, uint32_t key, int last, u64 sum) {
+    if (tid == 0) {
+      Decision d;
+      d.max = m;
+      d.key = key;
+      d.last = last;
+      d.min_p = s.min_p;
+      d.c = s.c;
+      d.sum = (double)sum / kUnit;
+      *reinterpret_cast<Decision*>(a.records + (int64_t)r * a.row_bytes) = d;
+    }
+  }
+
+  // No entry has a weight.
+  __device__ __forceinline__ void nothing(int r) {
+    if (!a.u)
+      leave(r, ~0u, -1, 0);
+    else if (tid == 0)
+      a.tokens[r] = 0;
+  }
+
+  // The logit at which a weight is `share` of the maximum's, a little less for the rounding.
+  __device__ __forceinline__ uint32_t floor_of(double share) const {
+    const double z = (double)m + log2(share) / s.c;
+    const double lo = z - 1e-6 * (fabs((double)m) + fabs(z)) - 1e-30;
+    return lo > -3.4e38 ? order_key((float)lo) : 0;  // (NaN too: no bound)
+  }
+
+  __device__ __forceinline__ void decide(int r) {
+    char* const rec = a.records + (int64_t)r * a.row_bytes;
+    const auto rp = tiles::tile_rsrc(rec + sizeof(Decision), a.pieces * (int)sizeof(Piece));
+    const auto rc = tiles::tile_rsrc(rec + sizeof(Decision) + a.pieces * sizeof(Piece),
+                                     (a.cells + 3) / 4 * 16);
+    listed_cells = -1;
+    // Each thread its piece; maximum and sum of all.
+    static_assert(kMaxPieces == kThreads, "one piece per thread");
+    const f32x4 y = tiles::load_coherent16(rp, tid * 16);
+    typedef double f64x2 __attribute__((ext_vector_type(2)));
+    const float pm = tid < a.pieces ? y[0] : kNegInf;
+    const double ps = tid < a.pieces ? __builtin_bit_cast(f64x2, y)[1] : 0.0;
+    m = block_max(pm);
+    if (m == kNegInf) {
+      nothing(r);
+      return;
+    }
+    u64 whole = 0;
+    if (s.whole) {
+      // (A piece none of whose entries has a unit of weight counts as nothing.)
+      const double top = weight(pm, m, s.c);
+      const u64 w = pm == kNegInf || units(top) == 0 ? 0 : units(ps * top);
+      if (tid < a.pieces) sh.psum[tid] = w;
+      whole = block_sum(w);
+    }
+    if (!s.filtered) {
+      if (a.u)
+        draw(r, 0, 0x7fffffff, whole);
+      else
+        leave(r, 0, 0x7fffffff, whole);
+      return;
+    }
+    uint32_t floor = 0;
+    if (s.k == 1)
+      floor = order_key(m);
+    else if (s.k > 0)
+      floor = cell_bound(rc, s.k);
+    else if (s.p < 1.f)
+      floor = floor_of((1.0 - (double)s.p) * ((double)whole / kUnit) / a.vocab);
+    if (s.min_p > 0.f && (s.k == 0 || s.p == 1.f)) floor = max(floor, floor_of((double)s.min_p));
+    floor = max(m == -kNegInf ? order_key(m) : floor, kDead + 1);
+    if (!list_cells(rc, floor)) listed_cells = -1;
+    const int n = list_entries(Range{floor, 0.f, 0.f, 0, 0, 0});
+    if (n <= kShort) {
+      brief(r, n, whole);
+      return;
+    }
+    uint32_t key = floor;  // with min-p alone, all from the bound on are kept but for their weight
+    int last = 0x7fffffff;
+    if (s.k > 0 || s.p < 1.f) {
+      // (With top-k and top-p, the former's cut gives the sum for the latter's.)
+      u64 aim = ~0ull, total = whole;
+      Cut c;
+#pragma unroll 1
+      for (int pass = s.k > 0 && s.p < 1.f ? 0 : 1; pass < 2; ++pass) {
+        if (pass == 1 && s.p < 1.f) aim = (u64)ceil((double)s.p * (double)total);
+        c = cut(floor, n, s.k, aim);
+        if (pass == 0)
+          total = c.ties < 0 ? c.above_w + everything(c.n)
+                             : c.above_w + (u64)c.ties * units(weight(of_key(c.key), m, s.c));
+      }
+      key = c.key;
+      last = last_tie(c);
+    }
+    // The kept weights of the pieces.
+    for (int i = tid; i < kMaxPieces; i += kThreads) sh.psum[i] = 0;
+    __syncthreads();
+    if (n <= kList) {
+      for (int i = tid; i < n; i += kThreads) {
+        const u64 w = kept_units(of_key(sh.key[i]), sh.idx[i], key, last);
+        if (w) atomicAdd(&sh.psum[sh.idx[i] / kPiece], w);
+      }
+    } else {
+      listed_cells = -1;
+      each_entry([&](const Eight<T>& x, int v0) __attribute__((always_inline)) {
+        u64 w = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w += kept_units(x[i], v0 + i, key, last);
+        w = wave_sum(w);
+        if (lane == 0 && w) atomicAdd(&sh.psum[(v0 + 7) / kPiece], w);
+      });
+    }
+    __syncthreads();
+    const u64 sum = block_sum(sh.psum[tid]);
+    if (a.u)
+      draw(r, key, last, sum);
+    else
+      leave(r, key, last, sum);
+  }
+
+  // Weight of all listed entries.
+  __device__ __forceinline__ u64 everything(int n) {
+    u64 w = 0;
+    for (int i = tid; i < n; i += kThreads) w += units(weight(of_key(sh.key[i]), m, s.c));
+    return block_sum(w);
+  }
+
+  // A row of at most kShort entries, one per thread.
+  __device__ __forceinline__ void decide_short(int r) {
+    const float z = tid < a.vocab ? fmaxf(T::get(row[tid]), kNegInf) : kNegInf;
+    m = block_max(z);
+    if (m == kNegInf) {
+      nothing(r);
+      return;
+    }
+    if (tid < a.vocab) {
+      sh.key[tid] = order_key(z);
+      sh.idx[tid] = tid;
+    }
+    const u64 whole = block_sum(z == kNegInf ? 0 : units(weight(z, m, s.c)));
+    brief(r, a.vocab, whole);
+  }
+
+  // The end for at most kShort listed entries, one per thread.
+  __device__ __forceinline__ void brief(int r, int n, u64 whole) {
+    u64 order = 0, w = 0;
+    uint32_t key = 0;
+    int v = 0;
+    if (tid < n) {
+      key = sh.key[tid];
+      v = sh.idx[tid];
+      order = (u64)key << 32 | (uint32_t)~v;
+      w = units(weight(of_key(key), m, s.c));
+      sh.brief.order[tid] = order;
+      sh.brief.w[tid] = w;
+    }
+    __syncthreads();
+    int rank = 0;
+    u64 before = 0;
+    if (tid < n)
+      for (int i = 0; i < n; ++i) {
+        const bool first = sh.brief.order[i] > order;
+        rank += first;
+        before += first ? sh.brief.w[i] : 0;
+      }
+    bool kept = tid < n && key > kDead && (s.k == 0 || rank < s.k);
+    if (s.p < 1.f) {
+      u64 total = whole;
+      if (s.k > 0) total = block_sum(kept ? w : 0);
+      const u64 aim = (u64)ceil((double)s.p * (double)total);
+      kept = kept && (rank == 0 || before < aim);
+    }
+    if (kept && s.min_p > 0.f) kept = weight(of_key(key), m, s.c) >= (double)s.min_p;
+    const u64 sum = block_sum(kept ? w : 0);
+    if (!a.u) {
+      // The last kept one in the order.
+      if (tid == 0) sh.count = 0;
+      __syncthreads();
+      if (kept) atomicMax(&sh.count, rank);
+      __syncthreads();
+      if (kept && rank == sh.count) {
+        sh.found_key = key;
+        sh.found = v;
+      }
+      __syncthreads();
+      leave(r, sh.found_key, sh.found, sum);
+      return;
+    }
+    // By the index now.
+    __syncthreads();
+    if (tid < n) sh.brief.w[tid] = kept ? w : 0;
+    if (tid == 0) {
+      sh.found = 0x7fffffff;
+      sh.found2 = -1;
+    }
+    __syncthreads();
+    const int seq = r / a.each;
+    const double aim = (double)a.u[seq * a.u_seq + (r - seq * a.each) * a.u_row] * (double)sum;
+    if (kept && w > 0) {
+      u64 run = 0;
+      for (int i = 0; i < n; ++i) run += sh.idx[i] <= v ? sh.brief.w[i] : 0;
+      if ((double)run > aim) atomicMin(&sh.found, v);
+      atomicMax(&sh.found2, v);
+    }
+    __syncthreads();
+    if (tid == 0) a.tokens[r] = sh.found != 0x7fffffff ? sh.found : sh.found2;
+  }
+};
+
+template <typename T>
+__global__ __launch_bounds__(kThreads, 4) void sample_kernel(Args a) {
+  __shared__ Shared sh;
+  __shared__ int s_last;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r = blockIdx.x / a.groups;
+  const int group = blockIdx.x - r * a.groups;
+  const int seq = r / a.each;
+  const typename T::E* row = (const typename T::E*)a.logits + seq * a.s_seq +
+                             (int64_t)(r - seq * a.each) * a.s_row;
+  const Settings s = settings_of(a, seq);
+  if (a.vocab <= kShort) {
+    Decider<T>{a, sh, row, s, 0.f, tid, lane, wave, -1}.decide_short(r);
+    return;
+  }
+  char* const rec = a.records + (int64_t)r * a.row_bytes;
+  Piece* const pieces = reinterpret_cast<Piece*>(rec + sizeof(Decision));
+  float* const cells = reinterpret_cast<float*>(rec + sizeof(Decision) + a.pieces * sizeof(Piece));
+
+  auto take = [&](int p, Eight<T> (&x)[2]) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) x[j].load(row, p * kPiece + j * 512 + lane * 8, a.vocab);
+  };
+  auto reduce = [&](int p, const Eight<T> (&w)[2]) {
+    float x[2][8];
+    float mp = kNegInf;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[j][i] = w[j][i];
+      float y = fmaxf(fmaxf(fmaxf(x[j][0], x[j][1]), fmaxf(x[j][2], x[j][3])),
+                      fmaxf(fmaxf(x[j][4], x[j][5]), fmaxf(x[j][6], x[j][7])));
+      y = row_max(y);
+      const int c = p * (kPiece / kCell) + j * 4 + (lane >> 4);
+      // Device-coherent, as all that the deciding workgroup reads: it may run on another XCD.
+      if ((lane & 15) == 0 && c < a.cells) tiles::store_coherent(cells + c, y);
+      mp = fmaxf(mp, y);
+    }
+    mp = wave_max_of_rows(mp);
+    double sum = 0.0;
+    if (s.whole && mp != kNegInf) {  // wavefront-uniform
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum += weight(x[j][i], mp, s.c);
+      sum = wave_sum(sum);
+    }
+    if (lane == 0) {
+      tiles::store_coherent(&pieces[p].max, mp);
+      __hip_atomic_store(&pieces[p].sum, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+  };
+  const int stride = a.groups * kWaves;
+  Eight<T> x0[2], x1[2];
+  int p = group * kWaves + wave;
+  if (p < a.pieces) take(p, x0);
+  while (p < a.pieces) {  // wavefront-uniform
+    if (p + stride < a.pieces) take(p + stride, x1);
+    reduce(p, x0);
+    p += stride;
+    if (p >= a.pieces) break;
+    if (p + stride < a.pieces) take(p + stride, x0);
+    reduce(p, x1);
+    p += stride;
+  }
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+  __builtin_amdgcn_s_waitcnt(0);  // the records have landed before the arrival counts
+  __syncthreads();
+  if (tid == 0)
+    s_last = __hip_atomic_fetch_add(a.cnt + r, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
+             a.groups - 1;
+  __syncthreads();
+  if (!s_last) return;
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
+  Decider<T> d{a, sh, row, s, 0.f, tid, lane, wave, -1};
+  d.decide(r);
+  if (tid == 0) __hip_atomic_store(a.cnt + r, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// Probabilities of one piece per wavefront.
+template <typename T>
+__global__ __launch_bounds__(256) void probs_kernel(Args a) {
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t item = (int64_t)blockIdx.x * 4 + wave;
+  const int r = (int)(item / a.pieces), p = (int)(item - (int64_t)r * a.pieces);
+  if (r >= a.rows) return;
+  const int seq = r / a.each;
+  const typename T::E* row = (const typename T::E*)a.logits + seq * a.s_seq +
+                             (int64_t)(r - seq * a.each) * a.s_row;
+  const Decision d = *reinterpret_cast<const Decision*>(a.records + (int64_t)r * a.row_bytes);
+  float* out = a.probs + (int64_t)r * a.vocab;
+  const double inv = d.sum > 0.0 ? 1.0 / d.sum : 0.0;
+  if (a.vocab <= kShort) {  // (one piece)
+    for (int v = lane; v < a.vocab; v += 64) {
+      const float z = fmaxf(T::get(row[v]), kNegInf);
+      const uint32_t key = order_key(z);
+      const double w = weight(z, d.max, d.c);
+      out[v] = key > kDead && (key > d.key || (key == d.key && v <= d.last)) && w >= (double)d.min_p
+                   ? (float)(w * inv) : 0.f;
+    }
+    return;
+  }
+  Eight<T> x[2];
+  int at[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) at[j] = x[j].load(row, p * kPiece + j * 512 + lane * 8, a.vocab);
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int v0 = at[j];
+    float y[8];
+    bool in[8], any = false;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t key = order_key(x[j][i]);
+      in[i] = key > kDead && (key > d.key || (key == d.key && v0 + i <= d.last));
+      any |= in[i];
+      y[i] = 0.f;
+    }
+    if (__ballot(any) != 0) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const double w = weight(x[j][i], d.max, d.c);
+        if (in[i] && w >= (double)d.min_p) y[i] = (float)(w * inv);
+      }
+    }
+    typedef float quad __attribute__((ext_vector_type(4), aligned(4)));
+    const int first = p * kPiece + j * 512 + lane * 8;
+    if (first == v0) {
+      *reinterpret_cast<quad*>(out + v0) = quad{y[0], y[1], y[2], y[3]};
+      *reinterpret_cast<quad*>(out + v0 + 4) = quad{y[4], y[5], y[6], y[7]};
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (v0 + i >= first) out[v0 + i] = y[i];
+    }
+  }
+}
+
+static int pieces_of(int vocab) { return (vocab + kPiece - 1) / kPiece; }
+static int cells_of(int vocab) { return (vocab + kCell - 1) / kCell; }
+
+// Workgroups per row: one wavefront per piece for a few rows; for many, as many as fill
+// kWavesPerCu wavefronts per compute unit over all rows, the pieces dealt in whole rounds.
+constexpr int kWavesPerCu = 16;
+static int groups_of(int rows, int pieces) {
+  int64_t waves = (int64_t)kWavesPerCu * device_cus() / rows;
+  if (waves < 1) waves = 1;
+  const int64_t rounds = (pieces + waves - 1) / waves;
+  const int64_t per_round = (pieces + rounds - 1) / rounds;
+  return (int)((per_round + kWaves - 1) / kWaves);
+}
+
+static int run(const Args& a, int dtype, hipStream_t stream) {
+  const unsigned grid = (unsigned)((int64_t)a.rows * a.groups);
+  switch (dtype) {
+    case PA_F16: sample_kernel<Half><<<grid, kThreads, 0, stream>>>(a); break;
+    case PA_BF16: sample_kernel<Brain><<<grid, kThreads, 0, stream>>>(a); break;
+    default: sample_kernel<Single><<<grid, kThreads, 0, stream>>>(a); break;
+  }
+  hipError_t e = hipGetLastError();
+  if (e == hipSuccess && a.probs) {
+    const unsigned wgs = (unsigned)(((int64_t)a.rows * a.pieces + 3) / 4);
+    switch (dtype) {
+      case PA_F16: probs_kernel<Half><<<wgs, 256, 0, stream>>>(a); break;
+      case PA_BF16: probs_kernel<Brain><<<wgs, 256, 0, stream>>>(a); break;
+      default: probs_kernel<Single><<<wgs, 256, 0, stream>>>(a); break;
+    }
+    e = hipGetLastError();
+  }
+  if (e == hipSuccess) return PA_OK;
+  set_error("HIP launch failed: %s", hipGetErrorString(e));
+  return PA_ERR_HIP;
+}
+
+}  // namespace sample
+}  // namespace pa
+
+using namespace pa;
+using namespace pa::sample;
+
+extern "C" {
+
+size_t pa_sample_workspace_bytes(int num_seqs, int rows_per_seq, int vocab) {
+  const int64_t rows = (int64_t)num_seqs * rows_per_seq;
+  if (num_seqs <= 0 || rows_per_seq <= 0 || rows > kMaxRows || vocab <= 0 || vocab > kMaxVocab) return 0;
+  return kCounterBytes + (size_t)rows * row_record(pieces_of(vocab), cells_of(vocab));
+}
+
+static int start(Args& a, const void* logits, int dtype, const int64_t* strides, int num_seqs,
+                 int rows_per_seq, int vocab, const float* temperature, float temperature_all,
+                 const int32_t* top_k, int top_k_all, const float* top_p, float top_p_all,
+                 const float* min_p, float min_p_all, const void* out, void* workspace,
+                 size_t workspace_bytes) {
+  clear_error();
+  if (num_seqs < 0 || rows_per_seq < 0 || vocab <= 0) {
+    set_error("num_seqs (%d) and rows_per_seq (%d) must be >= 0, vocab (%d) positive", num_seqs,
+              rows_per_seq, vocab);
+    return PA_ERR_ARG;
+  }
+  if (dtype != PA_F16 && dtype != PA_BF16 && dtype != PA_F32) {
+    set_error("unknown type of logits %d", dtype);
+    return PA_ERR_ARG;
+  }
+  if (num_seqs == 0 || rows_per_seq == 0) return PA_OK;
+  if ((int64_t)num_seqs * rows_per_seq > kMaxRows || vocab > kMaxVocab) {
+    set_error("at most %d rows of %d logits, %d x %d of %d given", kMaxRows, kMaxVocab, num_seqs,
+              rows_per_seq, vocab);
+    return PA_ERR_UNSUPPORTED;
+  }
+  if (!logits || !strides || !out) {
+    set_error("null pointer argument");
+    return PA_ERR_ARG;
+  }
+  if (strides[2] != 1 && vocab > 1) {
+    set_error("the rows of logits need unit vocabulary stride");
+    return PA_ERR_ARG;
+  }
+  if ((uintptr_t)logits % (dtype == PA_F32 ? 4 : 2)) {
+    set_error("logits must be aligned to their type");
+    return PA_ERR_ARG;
+  }
+  const size_t need = pa_sample_workspace_bytes(num_seqs, rows_per_seq, vocab);
+  if (!workspace || workspace_bytes < need) {
+    set_error("workspace of %zu bytes needed, %zu given", need, workspace_bytes);
+    return PA_ERR_WORKSPACE;
+  }
+  a.logits = logits;
+  a.s_seq = strides[0];
+  a.s_row = strides[1];
+  a.rows = num_seqs * rows_per_seq;
+  a.each = rows_per_seq;
+  a.vocab = vocab;
+  a.temperature = temperature;
+  a.t_all = temperature_all;
+  a.top_k = top_k;
+  a.k_all = top_k_all;
+  a.top_p = top_p;
+  a.p_all = top_p_all;
+  a.min_p = min_p;
+  a.m_all = min_p_all;
+  a.pieces = pieces_of(vocab);
+  a.cells = cells_of(vocab);
+  a.groups = groups_of(a.rows, a.pieces);
+  a.row_bytes = row_record(a.pieces, a.cells);
+  a.cnt = (int*)workspace;
+  a.records = (char*)workspace + kCounterBytes;
+  return PA_OK;
+}
+
+int pa_sample_tokens(const void* logits, int dtype, const int64_t logits_strides[3],
+                     const float* u, const int64_t u_strides[2], const float* temperature,
+                     float temperature_all, const int32_t* top_k, int top_k_all,
+                     const float* top_p, float top_p_all, const float* min_p, float min_p_all,
+                     int64_t* tokens, int num_seqs, int rows_per_seq, int vocab, void* workspace,
+                     size_t workspace_bytes, void* stream) {
+  Args a{};
+  const int status = start(a, logits, dtype, logits_strides, num_seqs, rows_per_seq, vocab,
+                           temperature, temperature_all, top_k, top_k_all, top_p, top_p_all, min_p,
+                           min_p_all, tokens, workspace, workspace_bytes);
+  if (status != PA_OK || a.rows == 0) return status;
+  if (!u || !u_strides) {
+    set_error("null pointer argument");
+    return PA_ERR_ARG;
+  }
+  a.u = u;
+  a.u_seq = u_strides[0];
+  a.u_row = u_strides[1];
+  a.tokens = tokens;
+  return run(a, dtype, (hipStream_t)stream);
+}
+
+int pa_sampling_probs(const void* logits, int dtype, const int64_t logits_strides[3],
+                      const float* temperature, float temperature_all, const int32_t* top_k,
+                      int top_k_all, const float* top_p, float top_p_all, const float* min_p,
+                      float min_p_all, float* probs, int num_seqs, int rows_per_seq, int vocab,
+                      void* workspace, size_t workspace_bytes, void* stream) {
+  Args a{};
+  const int status = start(a, logits, dtype, logits_strides, num_seqs, rows_per_seq, vocab,
+                           temperature, temperature_all, top_k, top_k_all, top_p, top_p_all, min_p,
+                           min_p_all, probs, workspace, workspace_bytes);
+  if (status != PA_OK || a.rows == 0) return status;
+  a.probs = probs;
+  return run(a, dtype, (hipStream_t)stream);
+}
+
+}  // extern "C"

@@ -18,7 +18,7 @@ import torch  # noqa: F401  (must be loaded before the HIP library, see above)
 
 LIB_NAME = "libpa_gfx950.so"
 LIB_PATH = Path(__file__).with_name(LIB_NAME)
-ABI_VERSION = 24
+ABI_VERSION = 26
 
 PA_OK = 0
 PA_ERR_ARG = 1
@@ -108,6 +108,15 @@ SIGNATURES: dict[str, tuple] = {
     "pa_verify_drafts_f32": (_i32, [
         _vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _vp,
         _sz, _vp]),
+    "pa_copy_blocks": (_i32, [
+        ctypes.POINTER(ctypes.c_void_p), _i64p, _i64p, _i32, _vp, _i64, _vp, _i64, _i32, _i32, _vp]),
+    "pa_sample_workspace_bytes": (_sz, [_i32, _i32, _i32]),
+    "pa_sample_tokens": (_i32, [
+        _vp, _i32, _i64p, _vp, _i64p, _vp, _f32, _vp, _i32, _vp, _f32, _vp, _f32, _vp, _i32, _i32,
+        _i32, _vp, _sz, _vp]),
+    "pa_sampling_probs": (_i32, [
+        _vp, _i32, _i64p, _vp, _f32, _vp, _i32, _vp, _f32, _vp, _f32, _vp, _i32, _i32, _i32, _vp, _sz,
+        _vp]),
 }
 
 _lib = None
@@ -164,7 +173,8 @@ def host():
         if ver != ABI_VERSION:
             raise NativeLibraryError(
                 f"{path} has ABI {ver}, the bindings expect {ABI_VERSION}; rebuild it")
-        for bind, names in ((module.bind, module.CALLS), (module.bind_fp8, module.CALLS_FP8)):
+        for bind, names in ((module.bind, module.CALLS), (module.bind_fp8, module.CALLS_FP8),
+                            (module.bind_sampled, module.CALLS_SAMPLED)):
             bind({name: ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in names})
         _host = module
     return _host
@@ -230,6 +240,11 @@ def i64_array(values) -> ctypes.Array:
     return (ctypes.c_int64 * len(vals))(*vals)
 
 
+def pointer_array(addresses) -> ctypes.Array:
+    vals = list(addresses)
+    return (ctypes.c_void_p * len(vals))(*vals)
+
+
 _arrays: dict[tuple, ctypes.Array] = {}
 
 
@@ -277,6 +292,8 @@ WS_PREFILL = "prefill"
 WS_DECODE_FP8 = "decode_fp8"
 # "verify" serves pa_verify_drafts_f32: arrival counters, then sums.
 WS_VERIFY = "verify"
+# "sample" serves pa_sample_tokens and pa_sampling_probs: arrival counters, then records.
+WS_SAMPLE = "sample"
 
 
 # Buffers replaced by larger ones. A HIP graph captured with an older buffer's

@@ -55,11 +55,19 @@ using Obj = py::handle;
   X(pa_verify_drafts_workspace_bytes)         \
   X(pa_verify_drafts_f32)
 
+// Those of sampled and forked decoding (bind_sampled).
+#define PA_HOST_CALLS_SAMPLED(X) \
+  X(pa_copy_blocks)              \
+  X(pa_sample_workspace_bytes)   \
+  X(pa_sample_tokens)            \
+  X(pa_sampling_probs)
+
 // The loaded library's entry points (bind).
 struct Api {
 #define PA_HOST_MEMBER(name) decltype(&::name) name;
   PA_HOST_CALLS(PA_HOST_MEMBER)
   PA_HOST_CALLS_FP8(PA_HOST_MEMBER)
+  PA_HOST_CALLS_SAMPLED(PA_HOST_MEMBER)
 #undef PA_HOST_MEMBER
 } api;
 
@@ -71,6 +79,10 @@ void bind(const py::dict& addresses) {
 
 void bind_fp8(const py::dict& addresses) {
   PA_HOST_CALLS_FP8(PA_HOST_BIND)
+}
+
+void bind_sampled(const py::dict& addresses) {
+  PA_HOST_CALLS_SAMPLED(PA_HOST_BIND)
 }
 #undef PA_HOST_BIND
 
@@ -486,21 +498,173 @@ py::object verify(Obj p_, Obj q_, Obj ids_, Obj u_, Obj next_, Obj counts_, Obj 
   return status == PA_ERR_HIP ? py::object(py::int_(status)) : py::object(py::none());
 }
 
+// ---- pool blocks ----
+
+py::object copy_blocks(Obj src_, Obj dst_, const py::list& caches, int64_t stream) {
+  const Tensor* t[2];
+  if (!unpack({src_, dst_}, t)) return py::none();
+  const Tensor &src = *t[0], &dst = *t[1];
+  const c10::Device dev = src.device();
+  if (!plain(src, at::kInt, dev) || !plain(dst, at::kInt, dev) || !current(dev) || src.dim() != 1 ||
+      dst.dim() != 1 || src.size(0) != dst.size(0))
+    return py::none();
+  constexpr size_t most = 1024;
+  const size_t n = caches.size();
+  if (n == 0 || n > most) return py::none();
+  void* bases[most];
+  int64_t strides[most], bytes[most], blocks = 0;
+  for (size_t i = 0; i < n; ++i) {
+    const Tensor* c[1];
+    if (!unpack({caches[i]}, c)) return py::none();
+    const Tensor& x = *c[0];
+    if (!plain(x, x.scalar_type(), dev) || x.dim() < 1) return py::none();
+    if (i == 0) blocks = x.size(0);
+    if (x.size(0) != blocks || blocks <= 0) return py::none();
+    int64_t inner = 1;  // elements of a block, which lie side by side
+    for (int64_t d = x.dim() - 1; d > 0; --d) {
+      if (x.size(d) != 1 && x.stride(d) != inner) return py::none();
+      inner *= x.size(d);
+    }
+    const int64_t step = blocks > 1 ? x.stride(0) : inner;
+    if (step < inner) return py::none();
+    bases[i] = x.data_ptr();
+    strides[i] = step * x.element_size();
+    bytes[i] = inner * x.element_size();
+  }
+  if (src.size(0) > 0x7fffffff || blocks > 0x7fffffff) return py::none();
+  int status;
+  {
+    py::gil_scoped_release release;
+    status = api.pa_copy_blocks(bases, strides, bytes, (int)n, (const int32_t*)src.data_ptr(),
+                                src.stride(0), (const int32_t*)dst.data_ptr(), dst.stride(0),
+                                (int)src.size(0), (int)blocks, (void*)stream);
+  }
+  if (status == PA_OK) return py::bool_(true);
+  return status == PA_ERR_HIP ? py::object(py::int_(status)) : py::object(py::none());
+}
+
+// ---- sampling ----
+
+// A setting of each sequence, or a number for all.
+template <typename T>
+struct Setting {
+  const T* each = nullptr;
+  T all = 0;
+
+  bool fill(Obj x, int64_t seqs, c10::Device dev) {
+    constexpr bool whole = std::is_same_v<T, int>;
+    if (PyLong_CheckExact(x.ptr())) {
+      int overflow = 0;
+      const long long v = PyLong_AsLongLongAndOverflow(x.ptr(), &overflow);
+      if (overflow || v < -0x7fffffffLL || v > 0x7fffffffLL) return false;
+      all = (T)v;
+      return true;
+    }
+    if (PyFloat_CheckExact(x.ptr())) {
+      all = (T)PyFloat_AS_DOUBLE(x.ptr());
+      return !whole;
+    }
+    const Tensor* t[1];
+    if (!unpack({x}, t)) return false;
+    if (!plain(*t[0], whole ? at::kInt : at::kFloat, dev) || !packed(*t[0]) || t[0]->size(0) != seqs)
+      return false;
+    each = (const T*)t[0]->data_ptr();
+    return true;
+  }
+};
+
+// Logits [seqs, vocab] or [seqs, rows, vocab] and their settings.
+struct Logits {
+  int64_t seqs, rows, vocab, st[3];
+  int type;
+  Setting<float> temperature, top_p, min_p;
+  Setting<int> top_k;
+
+  bool fill(const Tensor& x, Obj t, Obj k, Obj p, Obj m) {
+    const c10::Device dev = x.device();
+    if (x.scalar_type() == at::kHalf) type = PA_F16;
+    else if (x.scalar_type() == at::kBFloat16) type = PA_BF16;
+    else if (x.scalar_type() == at::kFloat) type = PA_F32;
+    else return false;
+    if (!plain(x, x.scalar_type(), dev) || !current(dev) || (x.dim() != 2 && x.dim() != 3)) return false;
+    seqs = x.size(0);
+    rows = x.dim() == 3 ? x.size(1) : 1;
+    vocab = x.size(-1);
+    for (int64_t n : {seqs, rows, vocab})
+      if (n <= 0 || n > 0x7fffffff) return false;
+    st[0] = x.stride(0);
+    st[1] = x.dim() == 3 ? x.stride(1) : 0;
+    st[2] = x.stride(-1);
+    return st[2] == 1 && temperature.fill(t, seqs, dev) && top_k.fill(k, seqs, dev) &&
+           top_p.fill(p, seqs, dev) && min_p.fill(m, seqs, dev);
+  }
+};
+
+py::object sample(Obj logits_, Obj u_, Obj t_, Obj k_, Obj p_, Obj m_, Obj ws_, int64_t stream) {
+  const Tensor* t[3];
+  if (!unpack({logits_, u_, ws_}, t)) return py::none();
+  const Tensor &x = *t[0], &u = *t[1];
+  Logits c;
+  if (!c.fill(x, t_, k_, p_, m_) || !plain(u, at::kFloat, x.device()) || u.dim() != x.dim() - 1 ||
+      u.size(0) != c.seqs || (u.dim() == 2 && u.size(1) != c.rows))
+    return py::none();
+  const int64_t us[2] = {u.stride(0), u.dim() == 2 ? u.stride(1) : 0};
+  const size_t need = api.pa_sample_workspace_bytes(c.seqs, c.rows, c.vocab);
+  void* wp;
+  if (!workspace(*t[2], x.device(), need, wp)) return py::none();
+  const Tensor tokens = at::empty(u.sizes(), u.options().dtype(at::kLong));
+  int status;
+  {
+    py::gil_scoped_release release;
+    status = api.pa_sample_tokens(
+        x.data_ptr(), c.type, c.st, (const float*)u.data_ptr(), us, c.temperature.each,
+        c.temperature.all, c.top_k.each, c.top_k.all, c.top_p.each, c.top_p.all, c.min_p.each,
+        c.min_p.all, (int64_t*)tokens.data_ptr(), c.seqs, c.rows, c.vocab, wp, need, (void*)stream);
+  }
+  return done(status, tokens);
+}
+
+py::object probabilities(Obj logits_, Obj t_, Obj k_, Obj p_, Obj m_, Obj ws_, int64_t stream) {
+  const Tensor* t[2];
+  if (!unpack({logits_, ws_}, t)) return py::none();
+  const Tensor& x = *t[0];
+  Logits c;
+  if (!c.fill(x, t_, k_, p_, m_)) return py::none();
+  const size_t need = api.pa_sample_workspace_bytes(c.seqs, c.rows, c.vocab);
+  void* wp;
+  if (!workspace(*t[1], x.device(), need, wp)) return py::none();
+  const Tensor probs = at::empty(x.sizes(), x.options().dtype(at::kFloat));
+  int status;
+  {
+    py::gil_scoped_release release;
+    status = api.pa_sampling_probs(
+        x.data_ptr(), c.type, c.st, c.temperature.each, c.temperature.all, c.top_k.each, c.top_k.all,
+        c.top_p.each, c.top_p.all, c.min_p.each, c.min_p.all, (float*)probs.data_ptr(), c.seqs,
+        c.rows, c.vocab, wp, need, (void*)stream);
+  }
+  return done(status, probs);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_pa_host, m) {
-  py::list calls, calls_fp8;
+  py::list calls, calls_fp8, calls_sampled;
 #define PA_HOST_NAME(name) calls.append(#name);
   PA_HOST_CALLS(PA_HOST_NAME)
 #undef PA_HOST_NAME
 #define PA_HOST_NAME(name) calls_fp8.append(#name);
   PA_HOST_CALLS_FP8(PA_HOST_NAME)
 #undef PA_HOST_NAME
+#define PA_HOST_NAME(name) calls_sampled.append(#name);
+  PA_HOST_CALLS_SAMPLED(PA_HOST_NAME)
+#undef PA_HOST_NAME
   m.attr("ABI_VERSION") = PA_ABI_VERSION;  // of the argument lists compiled in here
   m.attr("CALLS") = py::tuple(calls);
   m.attr("CALLS_FP8") = py::tuple(calls_fp8);
+  m.attr("CALLS_SAMPLED") = py::tuple(calls_sampled);
   m.def("bind", &bind);
   m.def("bind_fp8", &bind_fp8);
+  m.def("bind_sampled", &bind_sampled);
   m.def("decode", &decode);
   m.def("kv_write_decode", &kv_write_decode);
   m.def("rope_decode", &rope_decode);
@@ -509,4 +673,7 @@ PYBIND11_MODULE(_pa_host, m) {
   m.def("decode_fp8", &decode_fp8);
   m.def("prefill_fp8", &prefill_fp8);
   m.def("verify", &verify);
+  m.def("copy_blocks", &copy_blocks);
+  m.def("sample", &sample);
+  m.def("probabilities", &probabilities);
 }
