@@ -63,9 +63,10 @@ enum {
  * rotary workspace that never holds queries in the counter region; 20:
  * pa_kv_write_fp8, pa_kv_read_fp8; 21: pa_verify_drafts_f32; 22: pa_decode_fp8; 23:
  * pa_prefill_attention_fp8; 24: its workspace size; 25: pa_copy_blocks; 26:
- * pa_sample_tokens, pa_sampling_probs). pa_abi_version returns the
+ * pa_sample_tokens, pa_sampling_probs; 27: pa_decode_scored_f16,
+ * pa_prefill_attention_scored_f16). pa_abi_version returns the
  * library's. */
-#define PA_ABI_VERSION 26
+#define PA_ABI_VERSION 27
 PA_API int pa_abi_version(void);
 
 /* Message of the last failed call on this thread ("" after a success). */
@@ -617,6 +618,62 @@ PA_API int pa_verify_drafts_f32(const float* target, const int64_t target_stride
                                 const float* next_u, const int32_t* num_drafts, int64_t* tokens,
                                 int32_t* accepted, int num_seqs, int max_drafts, int vocab,
                                 void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Attention whose scores are capped, biased by distance, or limited to a window or to an
+ * interval of keys. No counterpart in the reference, whose kernels compute plain causal
+ * scores (engine/kernels/paged_attention.py:508-698). For a query row at position p of head h
+ * and key j:
+ *   s = scale q.k_j,  s = softcap tanh(s / softcap) where softcap > 0,
+ *   s -= slopes[h] |p - j| where slopes is not NULL (fp32 per query head, slope_stride apart),
+ * and out = softmax(s) v over the keys the row sees. window > 0: no key before p - window + 1.
+ * A row that sees no key is zeros. What lies in keys that a row does not see, NaN too, never
+ * reaches it; a NaN or an infinity in a V row makes the rows that see it NaN or infinite (all of
+ * head_dim or a part). scale is positive, softcap 0 or positive, both finite.
+ *
+ * pa_decode_scored_f16: one query row per sequence, at p = seq_lens[b] - 1, as
+ * pa_decode_batched_f16 (lengths, tables and block ids out of range are treated alike): keys
+ * max(key_starts[b], p - window + 1, 0) .. p; key_starts int32 [num_seqs] or NULL. head_dim 32,
+ * 64, 128 or 256, query groups up to 16, any block size; cache strides are non-negative
+ * multiples of 8 elements. Its workspace (0 bytes: none needed) begins with arrival counters
+ * that must be zero before the first call that uses the buffer; every call leaves them zero.
+ * One buffer per stream, lent to nothing else.
+ *
+ * pa_prefill_attention_scored_f16: several rows per sequence, as pa_prefill_attention_f16. Query
+ * row t sees keys from max(key_starts[t], p - window + 1, 0) on and before key_ends[t]
+ * (seq_lens[b] at most); key_starts and key_ends int32 [num_tokens], NULL: 0 and p + 1. Packed
+ * documents give every row its document's first key; a prefix that is seen as a whole gives
+ * its rows its end. Rows whose position is negative see nothing. The contract of the workspace
+ * is pa_prefill_attention_f16's, which may share it, sized by its own query (has_key_ends:
+ * whether key_ends is given).
+ */
+PA_API size_t pa_decode_scored_workspace_bytes(int num_seqs, int num_q_heads, int num_kv_heads,
+                                               int head_dim, int block_size,
+                                               int max_blocks_per_seq, int window);
+PA_API int pa_decode_scored_f16(const void* q, const int64_t q_strides[3], const void* k_cache,
+                                const int64_t k_strides[4], const void* v_cache,
+                                const int64_t v_strides[4], const int32_t* block_tables,
+                                const int64_t bt_strides[2], const int32_t* seq_lens, void* out,
+                                const int64_t out_strides[3], int num_seqs, int num_q_heads,
+                                int num_kv_heads, int head_dim, int block_size, int num_blocks,
+                                int max_blocks_per_seq, float scale, float softcap,
+                                const float* slopes, int64_t slope_stride, int window,
+                                const int32_t* key_starts, void* workspace,
+                                size_t workspace_bytes, void* stream);
+PA_API size_t pa_prefill_attention_scored_workspace_bytes(int num_seqs, int num_q_heads,
+                                                          int num_kv_heads, int head_dim,
+                                                          int block_size, int max_blocks_per_seq,
+                                                          int max_query_len, int window,
+                                                          int has_key_ends);
+PA_API int pa_prefill_attention_scored_f16(
+    const void* q, const int64_t q_strides[3], const void* k_cache, const int64_t k_strides[4],
+    const void* v_cache, const int64_t v_strides[4], const int32_t* block_tables,
+    const int64_t bt_strides[2], const int32_t* seq_lens, const int32_t* query_start_loc,
+    int max_query_len, void* out, const int64_t out_strides[3], int num_seqs, int num_tokens,
+    int num_q_heads, int num_kv_heads, int head_dim, int block_size, int num_blocks,
+    int max_blocks_per_seq, float scale, float softcap, const float* slopes, int64_t slope_stride,
+    int window, const int32_t* key_starts, const int32_t* key_ends, void* workspace,
+    size_t workspace_bytes, void* stream);
 
 /*
  * Copies of pool blocks: t[dst_blocks[i]] = t[src_blocks[i]] for every tensor t and pair i,

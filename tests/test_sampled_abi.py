@@ -93,3 +93,49 @@ def test_fork_without_a_partial_block():
     assert fork_block_table(BlockTable(seq_id=1, block_size=4), alloc, [], 1)[0].num_tokens == 0
     with pytest.raises(AssertionError):
         fork_block_table(BlockTable(seq_id=1, block_size=4, num_tokens=3), alloc, [], 1)
+
+
+POOL = S([2048, 128, 64, 1])
+
+
+def _decode(lib, q=16, k=16, out=16, kstr=POOL, qstr=S([896, 64, 1]), hq=14, hkv=2, d=64, bs=16, blocks=10,
+            width=4, seqs=2, scale=0.125, softcap=0.0, window=0, ws=0, nbytes=0):
+    return lib.pa_decode_scored_f16(q, qstr, k, kstr, 16, POOL, 16, S([4, 1]), 16, out, S([896, 64, 1]), seqs,
+                                    hq, hkv, d, bs, blocks, width, scale, softcap, None, 1, window, None, ws,
+                                    nbytes, None)
+
+
+def _prefill(lib, q=16, k=16, out=16, kstr=POOL, qstr=S([896, 64, 1]), hq=14, hkv=2, d=64, bs=16, blocks=10,
+             width=4, seqs=2, scale=0.125, softcap=0.0, window=0, ws=0, nbytes=0):
+    return lib.pa_prefill_attention_scored_f16(q, qstr, k, kstr, 16, POOL, 16, S([4, 1]), 16, 16, 9, out,
+                                               S([896, 64, 1]), seqs, 9, hq, hkv, d, bs, blocks, width, scale,
+                                               softcap, None, 1, window, None, None, ws, nbytes, None)
+
+
+@pytest.mark.parametrize("call", [_decode, _prefill])
+def test_scored_attention_argument_errors(call):
+    lib = _native.load()
+    nan, inf = float("nan"), float("inf")
+    for bad in (dict(q=0), dict(out=0), dict(k=8), dict(hq=15), dict(hkv=0), dict(bs=0), dict(blocks=0),
+                dict(width=0), dict(seqs=-1), dict(kstr=S([2048, 128, 60, 1])), dict(kstr=S([2048, 128, 64, 2])),
+                dict(qstr=S([900, 64, 1])), dict(qstr=S([896, 64, 2])), dict(scale=0.0), dict(scale=-1.0),
+                dict(scale=nan), dict(scale=inf), dict(softcap=-1.0), dict(softcap=nan), dict(softcap=inf),
+                dict(window=-1)):
+        assert call(lib, **bad) == _native.PA_ERR_ARG, bad
+        assert lib.pa_last_error()
+    for bad in (dict(hq=34), dict(d=48, qstr=S([896, 64, 1])), dict(width=2 ** 28)):
+        assert call(lib, **bad) == _native.PA_ERR_UNSUPPORTED, bad
+    assert call(lib, q=0, seqs=0) == _native.PA_OK
+
+
+def test_scored_attention_workspace():
+    lib = _native.load()
+    # Windows and short tables need none; what a window bounds needs no more than the table.
+    decode = lib.pa_decode_scored_workspace_bytes
+    assert decode(4, 14, 2, 64, 16, 32, 0) == 0 and decode(4, 14, 2, 64, 16, 2048, 512) == 0
+    assert decode(4, 14, 2, 64, 16, 2048, 0) >= decode(4, 14, 2, 64, 16, 2048, 4096) > 65536
+    assert decode(4, 34, 2, 64, 16, 2048, 0) == 0
+    prefill = lib.pa_prefill_attention_scored_workspace_bytes
+    assert prefill(1, 14, 2, 64, 16, 512, 64, 0, 0) == lib.pa_prefill_attention_workspace_bytes(
+        1, 14, 2, 64, 16, 512, 64)
+    assert prefill(1, 14, 2, 64, 16, 512, 64, 100, 0) < prefill(1, 14, 2, 64, 16, 512, 64, 100, 1)

@@ -60,8 +60,10 @@ HIPCC_FLAGS = [
 FILE_FLAGS = {
     "pa_fp8_drafts.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "pa_fp8_decode.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    "pa_scored_decode.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "pa_decode_linear.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "pa_prefill.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1", "-fno-honor-nans"],
+    "pa_prefill_scored.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1", "-fno-honor-nans"],
 }
 
 

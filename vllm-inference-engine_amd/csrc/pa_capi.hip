@@ -366,8 +366,9 @@ constexpr int64_t kPrefillFewBlocks = 64;
 // workspace then holds the fixed counter region (kPfCounterBytes, one counter
 // per column block, zero between launches) and a record of (head_dim + 2) x
 // cols floats per split.
+// cap: the most tokens a column block's keys can span.
 static PrefillPlan prefill_plan(int num_seqs, int num_q_heads, int num_kv_heads, int head_dim,
-                                int block_size, int max_blocks, int max_query_len) {
+                                int64_t cap, int max_query_len) {
   PrefillPlan p;
   const int g = num_q_heads / num_kv_heads;
   p.col_groups = prefill_col_groups(head_dim);
@@ -377,7 +378,7 @@ static PrefillPlan prefill_plan(int num_seqs, int num_q_heads, int num_kv_heads,
   const int cols = 64 * p.col_groups;
   p.col_blocks = blocks_for(p.col_groups);
   const int kt = prefill_key_tile(head_dim);
-  const int64_t max_tiles = ((int64_t)max_blocks * block_size + kt - 1) / kt;
+  const int64_t max_tiles = (cap + kt - 1) / kt;
   const int64_t base = p.col_blocks * num_seqs * num_kv_heads;
   // The kernel keeps two workgroups per CU resident (one at head_dim 256, for
   // LDS); splitting pays only while the column blocks fill less than about
@@ -412,7 +413,7 @@ static PrefillPlan prefill_plan(int num_seqs, int num_q_heads, int num_kv_heads,
   if (head_dim > 64)
     p.wave_groups = p.col_groups;
   else if (p.col_groups == 2 &&
-           ((p.max_splits == 1 && 2 * (int64_t)max_query_len <= (int64_t)max_blocks * block_size) ||
+           ((p.max_splits == 1 && 2 * (int64_t)max_query_len <= cap) ||
             (p.max_splits > 1 && head_dim == 64 && p.split_tiles >= kPrefillLongPieceTiles)))
     p.wave_groups = 2;
   if (p.max_splits > 1) {
@@ -421,6 +422,22 @@ static PrefillPlan prefill_plan(int num_seqs, int num_q_heads, int num_kv_heads,
                  (size_t)base * p.max_splits * cols * (head_dim + 2) * sizeof(float);
   }
   return p;
+}
+
+int check_scores(float scale, float softcap, int window) {
+  if (!(scale > 0.f) || scale == __builtin_huge_valf()) {
+    set_error("scale must be positive and finite");
+    return PA_ERR_ARG;
+  }
+  if (!(softcap >= 0.f) || softcap == __builtin_huge_valf()) {
+    set_error("softcap must be 0 (none) or positive and finite");
+    return PA_ERR_ARG;
+  }
+  if (window < 0) {
+    set_error("window must be 0 (none) or positive");
+    return PA_ERR_ARG;
+  }
+  return PA_OK;
 }
 
 }  // namespace pa
@@ -1197,11 +1214,30 @@ size_t pa_prefill_attention_workspace_bytes(int num_seqs, int num_q_heads, int n
       block_size <= 0 || max_blocks_per_seq <= 0 || max_query_len <= 0 ||
       !supported_head_dim(head_dim))
     return 0;
-  return prefill_plan(num_seqs, num_q_heads, num_kv_heads, head_dim, block_size,
-                      max_blocks_per_seq, max_query_len).ws_bytes;
+  return prefill_plan(num_seqs, num_q_heads, num_kv_heads, head_dim,
+                      (int64_t)max_blocks_per_seq * block_size, max_query_len).ws_bytes;
 }
 
-// Both forms of the prefill attention; k_scale null: the fp16 pool.
+// Most tokens that the keys of a column block span: the table's, or with a window (and no
+// ends of the caller's) the window's and the block's own.
+static int64_t scored_span(int block_size, int max_blocks, int head_dim, int window, bool ends) {
+  const int64_t cap = (int64_t)max_blocks * block_size;
+  if (window <= 0 || ends) return cap;
+  const int64_t span = (int64_t)window + 64 * prefill_col_groups(head_dim) + prefill_key_tile(head_dim);
+  return span < cap ? span : cap;
+}
+
+// What the scored form adds.
+struct ScoredInputs {
+  float softcap;
+  const float* slopes;
+  int64_t slope_stride;
+  int window;
+  const int32_t* starts;
+  const int32_t* ends;
+};
+
+// All forms of the prefill attention; k_scale null: the fp16 pool; scored null: plain scores.
 static int prefill_attention(const void* q, const int64_t q_strides[3], const void* k_cache,
                              const int64_t k_strides[4], const void* v_cache,
                              const int64_t v_strides[4], const int32_t* block_tables,
@@ -1212,7 +1248,8 @@ static int prefill_attention(const void* q, const int64_t q_strides[3], const vo
                              int num_blocks, int max_blocks_per_seq, float scale,
                              void* workspace, size_t workspace_bytes, void* stream,
                              const float* k_scale, const int64_t* k_scale_strides,
-                             const float* v_scale, const int64_t* v_scale_strides) {
+                             const float* v_scale, const int64_t* v_scale_strides,
+                             const ScoredInputs* scored) {
   if (num_seqs < 0 || num_tokens < 0 || max_query_len < 0) {
     set_error("num_seqs, num_tokens and max_query_len must be >= 0");
     return PA_ERR_ARG;
@@ -1288,8 +1325,11 @@ static int prefill_attention(const void* q, const int64_t q_strides[3], const vo
       return fp8::prefill_drafts(a, head_dim, max_query_len, workspace, workspace_bytes,
                                  (hipStream_t)stream);
   }
-  const PrefillPlan plan = prefill_plan(num_seqs, num_q_heads, num_kv_heads, head_dim, block_size,
-                                        max_blocks_per_seq, max_query_len);
+  const int64_t span =
+      scored ? scored_span(block_size, max_blocks_per_seq, head_dim, scored->window, scored->ends)
+             : (int64_t)max_blocks_per_seq * block_size;
+  const PrefillPlan plan =
+      prefill_plan(num_seqs, num_q_heads, num_kv_heads, head_dim, span, max_query_len);
   const int64_t grid = plan.col_blocks * plan.max_splits * num_seqs * num_kv_heads;
   if (grid > 0x7fffffff || plan.col_blocks > 0x7fffffff) {
     set_error("%lld workgroups exceed the grid limit", (long long)grid);
@@ -1312,6 +1352,20 @@ static int prefill_attention(const void* q, const int64_t q_strides[3], const vo
     a.compact = (int)exist;
   a.cnt = plan.ws_bytes ? (int*)workspace : nullptr;
   a.recs = plan.ws_bytes ? (float*)((char*)workspace + plan.counter_bytes) : nullptr;
+  if (scored) {
+    PrefillScoredArgs sa{};
+    static_cast<PrefillAttnArgs&>(sa) = a;
+    const ScoreForm f = score_form(scale, scored->softcap);
+    sa.cap_log2 = f.cap_log2;
+    sa.cap_out = f.cap_out;
+    sa.cap_in = f.cap_in;
+    sa.slopes = scored->slopes;
+    sa.slope_s = scored->slope_stride;
+    sa.window = scored->window;
+    sa.starts = scored->starts;
+    sa.ends = scored->ends;
+    return finish_launch(launch_prefill_scored(sa, head_dim, (hipStream_t)stream));
+  }
   return finish_launch(launch_prefill_attn(a, head_dim, (hipStream_t)stream));
 }
 
@@ -1329,7 +1383,48 @@ int pa_prefill_attention_f16(const void* q, const int64_t q_strides[3], const vo
                            bt_strides, seq_lens, query_start_loc, max_query_len, out, out_strides,
                            num_seqs, num_tokens, num_q_heads, num_kv_heads, head_dim, block_size,
                            num_blocks, max_blocks_per_seq, scale, workspace, workspace_bytes,
-                           stream, nullptr, nullptr, nullptr, nullptr);
+                           stream, nullptr, nullptr, nullptr, nullptr, nullptr);
+}
+
+size_t pa_prefill_attention_scored_workspace_bytes(int num_seqs, int num_q_heads, int num_kv_heads,
+                                                   int head_dim, int block_size,
+                                                   int max_blocks_per_seq, int max_query_len,
+                                                   int window, int has_key_ends) {
+  if (num_seqs <= 0 || num_kv_heads <= 0 || num_q_heads <= 0 || num_q_heads % num_kv_heads ||
+      block_size <= 0 || max_blocks_per_seq <= 0 || max_query_len <= 0 ||
+      !supported_head_dim(head_dim))
+    return 0;
+  return prefill_plan(num_seqs, num_q_heads, num_kv_heads, head_dim,
+                      scored_span(block_size, max_blocks_per_seq, head_dim, window, has_key_ends),
+                      max_query_len).ws_bytes;
+}
+
+int pa_prefill_attention_scored_f16(const void* q, const int64_t q_strides[3], const void* k_cache,
+                                    const int64_t k_strides[4], const void* v_cache,
+                                    const int64_t v_strides[4], const int32_t* block_tables,
+                                    const int64_t bt_strides[2], const int32_t* seq_lens,
+                                    const int32_t* query_start_loc, int max_query_len, void* out,
+                                    const int64_t out_strides[3], int num_seqs, int num_tokens,
+                                    int num_q_heads, int num_kv_heads, int head_dim, int block_size,
+                                    int num_blocks, int max_blocks_per_seq, float scale,
+                                    float softcap, const float* slopes, int64_t slope_stride,
+                                    int window, const int32_t* key_starts, const int32_t* key_ends,
+                                    void* workspace, size_t workspace_bytes, void* stream) {
+  clear_error();
+  if (num_seqs > 0 && num_tokens > 0 && max_query_len > 0) {
+    const int rc = check_scores(scale, softcap, window);
+    if (rc) return rc;
+    if (block_size > 0 && (int64_t)max_blocks_per_seq * block_size > 0x7fffffff - 4096) {
+      set_error("tables of 2^31 tokens are not built");
+      return PA_ERR_UNSUPPORTED;
+    }
+  }
+  const ScoredInputs s{softcap, slopes, slope_stride, window, key_starts, key_ends};
+  return prefill_attention(q, q_strides, k_cache, k_strides, v_cache, v_strides, block_tables,
+                           bt_strides, seq_lens, query_start_loc, max_query_len, out, out_strides,
+                           num_seqs, num_tokens, num_q_heads, num_kv_heads, head_dim, block_size,
+                           num_blocks, max_blocks_per_seq, scale, workspace, workspace_bytes,
+                           stream, nullptr, nullptr, nullptr, nullptr, &s);
 }
 
 size_t pa_prefill_attention_fp8_workspace_bytes(int num_seqs, int num_q_heads, int num_kv_heads,
@@ -1373,7 +1468,7 @@ int pa_prefill_attention_fp8(const void* q, const int64_t q_strides[3], const vo
                            bt_strides, seq_lens, query_start_loc, max_query_len, out, out_strides,
                            num_seqs, num_tokens, num_q_heads, num_kv_heads, head_dim, block_size,
                            num_blocks, max_blocks_per_seq, scale, workspace, workspace_bytes,
-                           stream, k_scale, k_scale_strides, v_scale, v_scale_strides);
+                           stream, k_scale, k_scale_strides, v_scale, v_scale_strides, nullptr);
 }
 
 int pa_rmsnorm_f16(const void* x, int64_t x_row_stride, const void* residual,

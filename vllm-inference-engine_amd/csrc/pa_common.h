@@ -243,6 +243,33 @@ struct PrefillAttnArgs {
   int64_t vs_sb, vs_sh;
 };
 
+// A score scale x, or softcap * tanh(scale x / softcap), in the exp2 domain: scale_log2 x, or
+// cap_log2 + cap_out / (1 + 2^(cap_in x)); cap_log2 0: no cap.
+struct ScoreForm {
+  float scale_log2, cap_log2, cap_out, cap_in;
+};
+inline ScoreForm score_form(float scale, float softcap) {
+  ScoreForm f{scale * kLog2e, 0.f, 0.f, 0.f};
+  if (softcap > 0.f) {
+    f.cap_log2 = softcap * kLog2e;
+    f.cap_out = -2.f * f.cap_log2;
+    f.cap_in = (float)(2.0 * 1.4426950408889634 * (double)scale / (double)softcap);
+  }
+  return f;
+}
+// Whether scale, softcap and window can be taken: an error code, or PA_OK (pa_capi.hip).
+int check_scores(float scale, float softcap, int window);
+
+// And of the form with capped, biased and masked scores.
+struct PrefillScoredArgs : PrefillAttnArgs {
+  float cap_log2, cap_out, cap_in;  // see ScoreForm
+  const float* slopes;    // per query head, or null
+  int64_t slope_s;
+  int window;             // keys that a row sees back from its position, 0: all
+  const int32_t* starts;  // per query row: its first key, or null: 0
+  const int32_t* ends;    // and the end of its keys, or null: up to its position
+};
+
 // Columns of a prefill workgroup in units of 64 (token, query head) columns:
 // two (128 columns) below head_dim 256, where the registers allow it. At head_dim
 // 128 the kernel runs them as four wavefronts of two groups of 16 (each K and V
@@ -343,6 +370,7 @@ bool plan_handover_supported(const DecodeArgs& a, int D);
 hipError_t launch_kv_write_plan(const DecodeArgs& a, const KVWriteArgs& w, bool vec,
                                 hipStream_t s);
 hipError_t launch_prefill_attn(const PrefillAttnArgs& a, int D, hipStream_t s);
+hipError_t launch_prefill_scored(const PrefillScoredArgs& a, int D, hipStream_t s);
 // The 8-bit pool's form for a few tokens per sequence (pa_fp8_drafts.hip): whether it takes
 // a call, its workspace, and the call (a PA_* status with the message set).
 namespace fp8 {

@@ -18,7 +18,7 @@ import torch  # noqa: F401  (must be loaded before the HIP library, see above)
 
 LIB_NAME = "libpa_gfx950.so"
 LIB_PATH = Path(__file__).with_name(LIB_NAME)
-ABI_VERSION = 26
+ABI_VERSION = 27
 
 PA_OK = 0
 PA_ERR_ARG = 1
@@ -108,6 +108,15 @@ SIGNATURES: dict[str, tuple] = {
     "pa_verify_drafts_f32": (_i32, [
         _vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _vp,
         _sz, _vp]),
+    "pa_decode_scored_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32, _i32, _i32, _i32]),
+    "pa_decode_scored_f16": (_i32, [
+        _vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _vp, _i64p, _i32, _i32, _i32, _i32, _i32,
+        _i32, _i32, _f32, _f32, _vp, _i64, _i32, _vp, _vp, _sz, _vp]),
+    "pa_prefill_attention_scored_workspace_bytes": (
+        _sz, [_i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32]),
+    "pa_prefill_attention_scored_f16": (_i32, [
+        _vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _vp, _i32, _vp, _i64p, _i32, _i32, _i32,
+        _i32, _i32, _i32, _i32, _i32, _f32, _f32, _vp, _i64, _i32, _vp, _vp, _vp, _sz, _vp]),
     "pa_copy_blocks": (_i32, [
         ctypes.POINTER(ctypes.c_void_p), _i64p, _i64p, _i32, _vp, _i64, _vp, _i64, _i32, _i32, _vp]),
     "pa_sample_workspace_bytes": (_sz, [_i32, _i32, _i32]),
@@ -292,6 +301,9 @@ WS_PREFILL = "prefill"
 WS_DECODE_FP8 = "decode_fp8"
 # "verify" serves pa_verify_drafts_f32: arrival counters, then sums.
 WS_VERIFY = "verify"
+# "decode_scored" serves pa_decode_scored_f16: arrival counters, then partial records.
+# (pa_prefill_attention_scored_f16 takes the "prefill" workspace.)
+WS_DECODE_SCORED = "decode_scored"
 # "sample" serves pa_sample_tokens and pa_sampling_probs: arrival counters, then records.
 WS_SAMPLE = "sample"
 

@@ -56,11 +56,15 @@ using Obj = py::handle;
   X(pa_verify_drafts_f32)
 
 // Those of sampled and forked decoding (bind_sampled).
-#define PA_HOST_CALLS_SAMPLED(X) \
-  X(pa_copy_blocks)              \
-  X(pa_sample_workspace_bytes)   \
-  X(pa_sample_tokens)            \
-  X(pa_sampling_probs)
+#define PA_HOST_CALLS_SAMPLED(X)                 \
+  X(pa_copy_blocks)                              \
+  X(pa_sample_workspace_bytes)                   \
+  X(pa_sample_tokens)                            \
+  X(pa_sampling_probs)                           \
+  X(pa_decode_scored_workspace_bytes)            \
+  X(pa_decode_scored_f16)                        \
+  X(pa_prefill_attention_scored_workspace_bytes) \
+  X(pa_prefill_attention_scored_f16)
 
 // The loaded library's entry points (bind).
 struct Api {
@@ -498,6 +502,109 @@ py::object verify(Obj p_, Obj q_, Obj ids_, Obj u_, Obj next_, Obj counts_, Obj 
   return status == PA_ERR_HIP ? py::object(py::int_(status)) : py::object(py::none());
 }
 
+// ---- scored attention ----
+
+// Packed int32 (or fp32) entries, or None.
+bool entries(Obj x, const Tensor* (&t)[1], c10::ScalarType type, int64_t n, c10::Device dev) {
+  if (x.is_none()) {
+    t[0] = nullptr;
+    return true;
+  }
+  return unpack({x}, t) && plain(*t[0], type, dev) && packed(*t[0]) && t[0]->size(0) == n;
+}
+template <typename T>
+const T* data(const Tensor* t) { return t ? (const T*)t->data_ptr() : nullptr; }
+
+// (A window of the table's length or more is none.)
+int window_of(int64_t window, const Call& c) { return window < c.width * c.bs ? (int)window : 0; }
+
+py::object decode_scored(Obj q_, Obj k_, Obj v_, Obj bt_, Obj lens_, double scale, double softcap,
+                         Obj slopes_, int64_t window, Obj starts_, Obj ws_, int64_t stream) {
+  const Tensor* t[6];
+  const Tensor *slopes[1], *starts[1];
+  if (!unpack({q_, k_, v_, bt_, lens_, ws_}, t)) return py::none();
+  const Tensor &q = *t[0], &k = *t[1], &v = *t[2], &bt = *t[3], &lens = *t[4];
+  Call c;
+  int64_t qs[3];
+  if (!c.fill(q, k, v, bt, lens) || q.dim() != 3 || !rows3(q, c.n, c.hq, c.d, qs) ||
+      !rows16(q, qs) || !packed(lens) || window < 0 ||
+      !entries(slopes_, slopes, at::kFloat, c.hq, q.device()) ||
+      !entries(starts_, starts, at::kInt, c.n, q.device()))
+    return py::none();
+  const int win = window_of(window, c);
+  const size_t need =
+      api.pa_decode_scored_workspace_bytes(c.n, c.hq, c.hkv, c.d, c.bs, c.width, win);
+  void* wp;
+  if (!workspace(*t[5], q.device(), need, wp)) return py::none();
+  const Tensor out = at::empty({c.n, c.hq, c.d}, q.options());
+  const int64_t os[3] = {c.hq * c.d, c.d, 1};
+  int status;
+  {
+    py::gil_scoped_release release;
+    status = api.pa_decode_scored_f16(
+        q.data_ptr(), qs, k.data_ptr(), c.ks, v.data_ptr(), c.vs, (const int32_t*)bt.data_ptr(),
+        c.bts, (const int32_t*)lens.data_ptr(), out.data_ptr(), os, c.n, c.hq, c.hkv, c.d, c.bs,
+        c.blocks, c.width, (float)scale, (float)softcap, data<float>(slopes[0]), 1, win,
+        data<int32_t>(starts[0]), wp, need, (void*)stream);
+  }
+  return done(status, out);
+}
+
+py::object prefill_scored(Obj q_, Obj k_, Obj v_, Obj bt_, Obj lens_, Obj start_, int64_t most,
+                          double scale, double softcap, Obj slopes_, int64_t window, Obj starts_,
+                          Obj ends_, Obj ws_, int64_t stream) {
+  const Tensor* t[7];
+  const Tensor *slopes[1], *starts[1], *ends[1];
+  if (!unpack({q_, k_, v_, bt_, lens_, start_, ws_}, t)) return py::none();
+  const Tensor &q = *t[0], &k = *t[1], &v = *t[2], &bt = *t[3], &lens = *t[4];
+  const c10::Device dev = q.device();
+  if (!plain(q, at::kHalf, dev) || !plain(k, at::kHalf, dev) || !plain(v, at::kHalf, dev) ||
+      !plain(bt, at::kInt, dev) || !plain(lens, at::kInt, dev) || !current(dev) || q.dim() != 3 ||
+      k.dim() != 4 || k.sizes() != v.sizes() || bt.dim() != 2 || !packed(lens))
+    return py::none();
+  Call c;
+  c.n = lens.size(0);
+  c.hq = q.size(1);
+  c.blocks = k.size(0);
+  c.bs = k.size(1);
+  c.hkv = k.size(2);
+  c.d = k.size(3);
+  c.width = bt.size(1);
+  const int64_t rows = q.size(0);
+  for (int64_t x : {c.n, c.hq, c.hkv, c.d, c.bs, c.blocks, c.width, rows, most})
+    if (x <= 0 || x > 0x7fffffff) return py::none();
+  int64_t qs[3];
+  if (c.hq % c.hkv || bt.size(0) != c.n || !starts_of(*t[5], c.n, dev) ||
+      !rows3(q, rows, c.hq, c.d, qs) || !rows16(q, qs) || window < 0 ||
+      !entries(slopes_, slopes, at::kFloat, c.hq, dev) ||
+      !entries(starts_, starts, at::kInt, rows, dev) || !entries(ends_, ends, at::kInt, rows, dev))
+    return py::none();
+  for (int i = 0; i < 4; ++i) {
+    c.ks[i] = k.stride(i);
+    c.vs[i] = v.stride(i);
+  }
+  c.bts[0] = bt.stride(0);
+  c.bts[1] = bt.stride(1);
+  const int win = window_of(window, c);
+  const size_t need = api.pa_prefill_attention_scored_workspace_bytes(
+      c.n, c.hq, c.hkv, c.d, c.bs, c.width, most, win, ends[0] != nullptr);
+  void* wp;
+  if (!workspace(*t[6], dev, need, wp)) return py::none();
+  const Tensor out = at::empty({rows, c.hq, c.d}, q.options());
+  const int64_t os[3] = {c.hq * c.d, c.d, 1};
+  int status;
+  {
+    py::gil_scoped_release release;
+    status = api.pa_prefill_attention_scored_f16(
+        q.data_ptr(), qs, k.data_ptr(), c.ks, v.data_ptr(), c.vs, (const int32_t*)bt.data_ptr(),
+        c.bts, (const int32_t*)lens.data_ptr(), (const int32_t*)t[5]->data_ptr(), most,
+        out.data_ptr(), os, c.n, rows, c.hq, c.hkv, c.d, c.bs, c.blocks, c.width, (float)scale,
+        (float)softcap, data<float>(slopes[0]), 1, win, data<int32_t>(starts[0]),
+        data<int32_t>(ends[0]), wp, need, (void*)stream);
+  }
+  return done(status, out);
+}
+
 // ---- pool blocks ----
 
 py::object copy_blocks(Obj src_, Obj dst_, const py::list& caches, int64_t stream) {
@@ -673,6 +780,8 @@ PYBIND11_MODULE(_pa_host, m) {
   m.def("decode_fp8", &decode_fp8);
   m.def("prefill_fp8", &prefill_fp8);
   m.def("verify", &verify);
+  m.def("decode_scored", &decode_scored);
+  m.def("prefill_scored", &prefill_scored);
   m.def("copy_blocks", &copy_blocks);
   m.def("sample", &sample);
   m.def("probabilities", &probabilities);
