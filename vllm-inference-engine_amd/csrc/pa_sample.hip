@@ -13,9 +13,11 @@
 // own logit; for top-p, entries below (1 - p) / vocab of the sum, which together weigh less
 // than 1 - p. Only cells that reach the bound are read again, and their entries above it
 // listed: tens to hundreds for usual settings. A short list is ranked by comparing all
-// with all; a longer one by radix passes over the logits' bits with counts and weights; one
-// that does not fit LDS (flat distributions) is first narrowed by counts and weights per
-// interval of logits, to the interval in which the border lies.
+// with all; a longer one by radix passes over the logits' bits with counts and weights.
+// Where more are listed than fit LDS (flat distributions), two more launches share the row
+// among workgroups again: the first adds up counts and weights per interval of logits and finds
+// the interval in which the border lies, the second lists its entries, sums what lies above it
+// per piece, and decides. (Rows without such a list leave those launches at once.)
 //
 // Weights and sums. w is computed in 64 bits (2^-45 relative) and summed as whole numbers of
 // 2^-44: sums do not depend on the order, so that LDS atomics may form them, and the 2^19
@@ -40,13 +42,16 @@ constexpr int kMaxRows = 16384;
 constexpr size_t kCounterBytes = (size_t)kMaxRows * sizeof(int);
 constexpr int kList = 2048;   // listed entries
 constexpr int kShort = 256;   // of them, ranked by comparing all with all
-constexpr int kBins = 1024;
+constexpr int kBins = 2048;
+// Pieces that a workgroup looks through by itself, though most of them reach the bound.
+constexpr int kAlonePieces = 32;
+constexpr int kMaxShared = 2048;  // rows with an area to be shared by
 constexpr uint32_t kDead = 0x007fffffu;  // order key of -inf; NaN counts as -inf
 constexpr double kUnit = 17592186044416.0;  // 2^44
 
+// What the deciding workgroup leaves for the launch that writes probabilities.
 typedef unsigned long long u64;
 
-// What the deciding workgroup leaves for the launch that writes probabilities.
 struct Decision {
   float max;
   uint32_t key;   // kept: order keys above this one,
@@ -58,7 +63,33 @@ struct Decision {
 
 struct Piece {
   float max, pad;
-  double sum;
+  double sum;  // (of a shared row in the end: the kept weight, in units)
+};
+
+// A row whose list does not fit, between the launches that share it.
+enum { kDecided = 0, kCount = 1, kCollect = 2, kKeepAll = 3, kAlone = 4 };
+struct alignas(16) Shared_row {
+  int mode;
+  float max;
+  uint32_t floor;   // keys below are out of the question
+  float lo, scale;  // the intervals of the logits' line,
+  int bin;          // and the one with the border
+  int above;        // entries above it, and their weight
+  int listed;       // entries of it
+  u64 above_w, aim, whole;
+};
+// Its bins, and then its list.
+struct Area {
+  union {
+    struct {
+      u64 w[2048];
+      uint32_t n[2048];
+    } bin;
+    struct {
+      uint32_t key[2048];
+      int idx[2048];
+    } list;
+  };
 };
 
 struct Args {
@@ -76,12 +107,16 @@ struct Args {
   int64_t* tokens;
   float* probs;
   int* cnt;
-  char* records;  // per row: Decision, pieces, cells
+  char* records;  // per row: Decision, Shared_row, pieces, cells
+  Area* areas;    // of the first `shared_rows` rows
   int row_bytes, pieces, cells, groups;
+  int shared_rows, shared_groups;
 };
 
+constexpr int kHead = sizeof(Decision) + sizeof(Shared_row);
+static_assert(sizeof(Decision) % 16 == 0 && sizeof(Shared_row) % 16 == 0, "16-byte reads behind them");
 __host__ __device__ inline int row_record(int pieces, int cells) {
-  return (int)sizeof(Decision) + pieces * (int)sizeof(Piece) + (cells + 3) / 4 * 16;
+  return kHead + pieces * (int)sizeof(Piece) + (cells + 3) / 4 * 16;
 }
 
 // ---- entries -----------------------------------------------------------------------
@@ -133,12 +168,13 @@ __device__ inline float of_key(uint32_t k) {
   return __builtin_bit_cast(float, k & 0x80000000u ? k ^ 0x80000000u : ~k);
 }
 
-// 2^d for d <= 0, to 2^-45 relative: the whole part by the exponent, the rest by a polynomial
-// through 2^f at the ten Chebyshev nodes of [-1/2, 1/2]. Below -1060 and for NaN as good as 0.
+// 2^d for -1000 <= d <= 0, to 2^-45 relative: the whole part, by an addition that leaves it in
+// the low bits, goes to the exponent; the rest by the polynomial through 2^f at the ten Chebyshev
+// nodes of [-1/2, 1/2], its constant rounded to 1: the largest weighs exactly that.
 __device__ inline double exp2_of(double d) {
-  d = fmax(d, -1060.0);
-  const double n = __builtin_rint(d);
-  const double f = d - n;
+  constexpr double kWhole = 6755399441055744.0;  // 1.5 * 2^52
+  const double t = d + kWhole;
+  const double f = d - (t - kWhole);
   double p = 1.0212097549811005e-07;
   p = __builtin_fma(p, f, 1.3259945262689143e-06);
   p = __builtin_fma(p, f, 1.5252640059770786e-05);
@@ -148,15 +184,27 @@ __device__ inline double exp2_of(double d) {
   p = __builtin_fma(p, f, 0.05550410866428854);
   p = __builtin_fma(p, f, 0.24022650695631514);
   p = __builtin_fma(p, f, 0.6931471805599526);
-  p = __builtin_fma(p, f, 1.000000000000014);
-  return __builtin_amdgcn_ldexp(p, (int)n);
+  p = __builtin_fma(p, f, 1.0);
+  uint2 b = __builtin_bit_cast(uint2, p);
+  b.y += __builtin_bit_cast(uint2, t).x << 20;
+  return __builtin_bit_cast(double, b);
 }
 
-// Weight of z next to the maximum m: 1 at the maximum, whatever the temperature (a maximum
-// of +inf too, beside which all others weigh nothing).
-__device__ inline double weight(float z, float m, double c) {
-  return z == m ? 1.0 : exp2_of(((double)z - (double)m) * c);
-}
+// The weight of z next to a maximum m: 2^(c (z - m)), c = log2(e) / T; as good as 0 from 2^-1000
+// down and for z = -inf. Where m is +inf the entries of +inf alone count: they are told by
+// comparing, and weigh 1.
+struct Scale {
+  double m, c, low;
+  bool top_only;
+  __device__ Scale() {}
+  __device__ Scale(float max, double per_logit) {
+    top_only = max == -kNegInf;
+    m = top_only ? 0.0 : (double)max;
+    c = top_only ? 0.0 : per_logit;
+    low = top_only ? 0.0 : -1000.0;
+  }
+  __device__ double weight(float z) const { return exp2_of(fmax(((double)z - m) * c, low)); }
+};
 __device__ inline u64 units(double w) { return (u64)(w * kUnit + 0.5); }
 
 // ---- sums over lanes ---------------------------------------------------------------
@@ -264,13 +312,14 @@ struct Shared {
     } bin;
     uint16_t cells[kMaxCells];
     struct {
-      u64 w[kShort];
-      u64 order[kShort];
+      ulonglong2 entry[kShort];  // order or index, weight
+      u64 more[kShort];
     } brief;
   };
   u64 psum[kMaxPieces];
   int pcount[kMaxPieces];
   u64 part[kWaves];
+  int part_n[kWaves];
   int count;
   uint32_t found_key;
   int found, found2;
@@ -306,9 +355,18 @@ struct Decider {
   Shared& sh;
   const E* row;
   Settings s;
-  float m;
   int tid, lane, wave;
-  int listed_cells;  // -1: all pieces are read
+  float m = kNegInf;      // the row's maximum
+  Scale sc;               // and its weights
+  int listed_cells = -1;  // -1: all pieces are read
+
+  __device__ Decider(const Args& a_, Shared& sh_, const E* row_, const Settings& s_, int tid_, int lane_,
+                     int wave_)
+      : a(a_), sh(sh_), row(row_), s(s_), tid(tid_), lane(lane_), wave(wave_) {}
+  __device__ __forceinline__ void set_max(float x) {
+    m = x;
+    sc = Scale(x, s.c);
+  }
 
   // f(x, v0) for entries v0 .. v0 + 7 of every lane, by whole wavefronts: 512 entries a time,
   // kAhead times read before the first is looked at.
@@ -485,41 +543,65 @@ struct Decider {
   }
 
   // Of the bins' counts and weights, from the last bin down: the first at which k entries
-  // or a weight of `aim` are reached, in sh.found (-1: none), and what lies above it in
-  // sh.found2 and sh.found_w. (k 0 or aim ~0: no such limit.)
-  __device__ __forceinline__ void walk_bins(int bins, int have, u64 have_w, int k, u64 aim) {
+  // or a weight of `aim` are reached, in sh.found (-1: none), and what lies above it (then:
+  // all) in sh.found2 and sh.found_w. (k 0 or aim ~0: no such limit.)
+  // BINS: each thread BINS / kThreads neighbouring ones, the last threads the first bins.
+  template <int BINS>
+  __device__ __forceinline__ void walk_bins(int have, u64 have_w, int k, u64 aim) {
+    constexpr int PER = BINS > kThreads ? BINS / kThreads : 1;
+    static_assert(PER * kThreads >= BINS && BINS % 64 == 0, "whole wavefronts of bins");
     __syncthreads();
-    if (wave == 0) {
-      const int per = bins / 64;
-      int mine = 0;
-      u64 mine_w = 0;
-      for (int i = 0; i < per; ++i) {
-        const int b = bins - 1 - lane * per - i;
-        mine += (int)sh.bin.n[b];
-        mine_w += sh.bin.w[b];
+    const int b0 = BINS - 1 - tid * PER;  // and down from there
+    const bool live = tid * PER < BINS;
+    int own[PER], mine = 0;
+    u64 own_w[PER], mine_w = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      mine += own[i] = live ? (int)sh.bin.n[b0 - i] : 0;
+      mine_w += own_w[i] = live ? sh.bin.w[b0 - i] : 0;
+    }
+    const int incl = tiles::wave_incl_scan(mine);
+    const u64 incl_w = wave_scan(mine_w, lane);
+    if (lane == 63) {
+      sh.part[wave] = incl_w;
+      sh.part_n[wave] = incl;
+    }
+    if (tid == 0) sh.found = 0x7fffffff;
+    __syncthreads();
+    int sum = have + incl - mine;
+    u64 sum_w = have_w + incl_w - mine_w;
+    int all = have;
+    u64 all_w = have_w;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) {
+      if (i < wave) {
+        sum += sh.part_n[i];
+        sum_w += sh.part[i];
       }
-      int sum = have + tiles::wave_incl_scan(mine) - mine;
-      u64 sum_w = have_w + wave_scan(mine_w, lane) - mine_w;
-      int hit = -1, before = 0;
-      u64 before_w = 0;
-      for (int i = 0; i < per; ++i) {
-        const int b = bins - 1 - lane * per - i;
-        const int n = (int)sh.bin.n[b];
-        const u64 w = sh.bin.w[b];
-        if (hit < 0 && n > 0 && ((k > 0 && sum + n >= k) || sum_w + w >= aim)) {
-          hit = b;
-          before = sum;
-          before_w = sum_w;
-        }
-        sum += n;
-        sum_w += w;
+      all += sh.part_n[i];
+      all_w += sh.part[i];
+    }
+    int hit = -1, before = 0;
+    u64 before_w = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      if (hit < 0 && own[i] > 0 && ((k > 0 && sum + own[i] >= k) || sum_w + own_w[i] >= aim)) {
+        hit = b0 - i;
+        before = sum;
+        before_w = sum_w;
       }
-      const uint64_t hits = __ballot(hit >= 0);
-      if (hits ? lane == (int)__builtin_ctzll(hits) : lane == 0) {
-        sh.found = hit;
-        sh.found2 = before;
-        sh.found_w = before_w;
-      }
+      sum += own[i];
+      sum_w += own_w[i];
+    }
+    const uint64_t hits = __ballot(hit >= 0);
+    if (hits && lane == (int)__builtin_ctzll(hits)) atomicMin(&sh.found, tid);
+    __syncthreads();
+    const int first = sh.found;
+    __syncthreads();
+    if (tid == (first == 0x7fffffff ? 0 : first)) {
+      sh.found = hit;
+      sh.found2 = hit < 0 ? all : before;
+      sh.found_w = hit < 0 ? all_w : before_w;
     }
     __syncthreads();
   }
@@ -536,109 +618,32 @@ struct Decider {
     int n;
   };
 
-  // First k entries (0: no such limit), or the shortest beginning that weighs aim, of the
-  // entries from `floor` on, n of them (all listed if they fit).
-  __device__ __forceinline__ Cut cut(uint32_t floor, int n, int k, u64 aim) {
-    Cut c{};
-    c.range = Range{floor, 0.f, 0.f, 0, 0, 0};
-    c.n = n;
-    bool none = false;
-    if (n > kList) {
-      // Narrowed by intervals of the line of logits first; if more than fit are in one, by
-      // the bits of their keys.
-      listed_cells = -1;
-      c.range.lo = floor > kDead ? of_key(floor) : (float)((double)m - 46.0 / s.c);
-      const float width = m - c.range.lo;
-      c.range.scale = width > 0.f && width < 3e38f ? (float)kBins / width : 0.f;
-      int shift = 32;
-      bool first = c.range.scale > 0.f;
-      c.range.bin = 0;
-      for (;;) {
-        // A round: the bins of what is in question.
-        for (int i = tid; i < kBins; i += kThreads) {
-          sh.bin.n[i] = 0;
-          sh.bin.w[i] = 0;
-        }
-        __syncthreads();
-        const int low = first ? 0 : shift > 10 ? shift - 10 : 0;
-        const int bits = first ? 10 : shift - low;
-        each_entry([&](const Eight<T>& x, int) __attribute__((always_inline)) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const uint32_t key = order_key(x[i]);
-            if (first ? key >= floor : c.range.place(x[i], key) == 1) {
-              const int b = first ? c.range.bin_of(x[i]) : (int)((key >> low) & ((1u << bits) - 1));
-              atomicAdd(&sh.bin.n[b], 1u);
-              atomicAdd(&sh.bin.w[b], units(weight(x[i], m, s.c)));
-            }
-          }
-        });
-        walk_bins(kBins, c.above, c.above_w, k, aim);
-        int b = sh.found;
-        if (b < 0) {  // the limit is not reached
-          none = true;
-          // On with the lowest bin that holds anything: what lies above it is kept for sure.
-          if (tid == 0) sh.count = kBins - 1;
-          __syncthreads();
-          for (int i = tid; i < kBins; i += kThreads)
-            if (sh.bin.n[i] != 0) atomicMin(&sh.count, i);
-          __syncthreads();
-          b = sh.count;
-          u64 w = 0;
-          int above = 0;
-          for (int i = b + 1 + tid; i < kBins; i += kThreads) {
-            w += sh.bin.w[i];
-            above += (int)sh.bin.n[i];
-          }
-          c.above += (int)block_sum((u64)above);
-          c.above_w += block_sum(w);
-        } else {
-          c.above = sh.found2;
-          c.above_w = sh.found_w;
-        }
-        const int held = (int)sh.bin.n[b];
-        if (first) {
-          c.range.bin = b;
-          first = false;
-        } else {
-          shift = low;
-          c.range.bits |= (uint32_t)b << low;
-          c.range.mask = low == 0 ? ~0u : ~((1u << low) - 1);
-        }
-        __syncthreads();
-        if (c.range.mask == ~0u) {  // equal logits alone
-          c.key = c.range.bits;
-          c.all = held;
-          finish(c, none, k, aim);
-          return c;
-        }
-        if (held <= kList) break;
-      }
-      c.n = list_entries(c.range);
-    }
+  // Where the kept ones end: the first k entries (0: no such limit), or the shortest beginning
+  // that weighs aim, of what c.range and c.above stand for, all c.n entries in question listed.
+  __device__ __forceinline__ void cut_list(Cut& c, int k, u64 aim) {
     c.in_list = true;
     // Radix passes over the list.
     uint32_t prefix = 0;
+#pragma unroll 1
     for (int shift = 24; shift >= 0; shift -= 8) {
       for (int i = tid; i < 256; i += kThreads) {
         sh.bin.n[i] = 0;
         sh.bin.w[i] = 0;
       }
       __syncthreads();
+#pragma unroll 1
       for (int i = tid; i < c.n; i += kThreads) {
         const uint32_t key = sh.key[i];
         if (shift == 24 || key >> (shift + 8) == prefix) {
           atomicAdd(&sh.bin.n[key >> shift & 255], 1u);
-          atomicAdd(&sh.bin.w[key >> shift & 255], units(weight(of_key(key), m, s.c)));
+          atomicAdd(&sh.bin.w[key >> shift & 255], units(sc.weight(of_key(key))));
         }
       }
-      walk_bins(256, c.above, c.above_w, k, aim);
+      walk_bins<256>(c.above, c.above_w, k, aim);
       if (sh.found < 0) {  // the limit is not reached (in the first pass, if at all)
-        c.key = c.range.floor;
-        c.ties = -1;
-        c.all = 0;
+        keep_all(c);
         __syncthreads();
-        return c;
+        return;
       }
       prefix = prefix << 8 | (uint32_t)sh.found;
       c.above = sh.found2;
@@ -647,19 +652,122 @@ struct Decider {
       __syncthreads();
     }
     c.key = prefix;
-    finish(c, false, k, aim);
-    return c;
+    finish(c, k, aim);
+  }
+
+  // The same for at most kShort listed entries, by their places in the order; `last` too.
+  __device__ __forceinline__ void cut_brief(Cut& c, int k, u64 aim, int& last) {
+    const int e = tid & (kShort - 1);
+    u64 order = 0, w = 0;
+    if (e < c.n) {
+      order = (u64)sh.key[e] << 32 | (uint32_t)~sh.idx[e];
+      w = units(sc.weight(of_key(sh.key[e])));
+    }
+    if (tid < kShort) sh.brief.entry[e] = ulonglong2{order, w};
+    if (tid == 0) sh.count = -1;
+    __syncthreads();
+    const u64 first = places(c.n, order);
+    const int rank = (int)(first >> 53);
+    const u64 before = c.above_w + (first & ((1ull << 53) - 1));
+    const bool kept = tid < c.n && (k == 0 || c.above + rank < k) &&
+                      (before < aim || (c.above == 0 && rank == 0));
+    if (kept) atomicMax(&sh.count, rank);
+    __syncthreads();
+    if (kept && rank == sh.count) {
+      sh.found_key = sh.key[e];
+      sh.found = sh.idx[e];
+    }
+    __syncthreads();
+    if (sh.count < 0) {  // none of them (none listed)
+      keep_all(c);
+      last = 0x7fffffff;
+    } else {
+      c.key = sh.found_key;
+      last = sh.found;
+    }
+    __syncthreads();
+  }
+
+  // Everything down to the bound is kept.
+  __device__ __forceinline__ void keep_all(Cut& c) {
+    c.key = c.range.floor;
+    c.ties = -1;
+    c.all = 0;
+  }
+
+  // The intervals of the logits' line from the bound to the maximum.
+  __device__ __forceinline__ void lay_bins(Range& r) {
+    r.lo = r.floor > kDead + 1 ? of_key(r.floor) : (float)((double)m - 46.0 / s.c);
+    const float width = m - r.lo;
+    r.scale = width > 0.f && width < 3e38f ? (float)kBins / width : 0.f;
+  }
+
+  // The same of all entries from c.range.floor on, more than fit the list: by this workgroup
+  // alone, narrowed by intervals first and then, if more than fit are in one, by the bits of
+  // their keys.
+  __device__ __forceinline__ void cut_alone(Cut& c, int k, u64 aim) {
+    listed_cells = -1;
+    lay_bins(c.range);
+    int shift = 32;
+    bool first = c.range.scale > 0.f;
+#pragma unroll 1
+    for (;;) {
+      // A round: the bins of what is in question.
+      for (int i = tid; i < kBins; i += kThreads) {
+        sh.bin.n[i] = 0;
+        sh.bin.w[i] = 0;
+      }
+      __syncthreads();
+      const int low = first ? 0 : shift > 10 ? shift - 10 : 0;
+      const int bits = first ? 10 : shift - low;
+      each_entry([&](const Eight<T>& x, int) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const uint32_t key = order_key(x[i]);
+          if (first ? key >= c.range.floor : c.range.place(x[i], key) == 1) {
+            const int b = first ? c.range.bin_of(x[i]) : (int)((key >> low) & ((1u << bits) - 1));
+            atomicAdd(&sh.bin.n[b], 1u);
+            atomicAdd(&sh.bin.w[b], units(sc.weight(x[i])));
+          }
+        }
+      });
+      walk_bins<kBins>(c.above, c.above_w, k, aim);
+      const int b = sh.found;
+      c.above = sh.found2;
+      c.above_w = sh.found_w;
+      if (b < 0) {  // the limit is not reached (in the first round, if at all)
+        c.n = 0;
+        keep_all(c);
+        __syncthreads();
+        return;
+      }
+      const int held = (int)sh.bin.n[b];
+      if (first) {
+        c.range.bin = b;
+        first = false;
+      } else {
+        shift = low;
+        c.range.bits |= (uint32_t)b << low;
+        c.range.mask = low == 0 ? ~0u : ~((1u << low) - 1);
+      }
+      __syncthreads();
+      if (c.range.mask == ~0u) {  // equal logits alone
+        c.key = c.range.bits;
+        c.all = held;
+        finish(c, k, aim);
+        return;
+      }
+      if (held <= kList) break;
+    }
+    c.n = list_entries(c.range);
+    cut_list(c, k, aim);
   }
 
   // How many of the equal logits at the border are kept.
-  __device__ __forceinline__ void finish(Cut& c, bool none, int k, u64 aim) {
-    if (none) {
-      c.ties = c.all;
-      return;
-    }
+  __device__ __forceinline__ void finish(Cut& c, int k, u64 aim) {
     int t = c.all;
     if (k > 0) t = min(t, k - c.above);
-    const u64 w = units(weight(of_key(c.key), m, s.c));
+    const u64 w = units(sc.weight(of_key(c.key)));
     if (aim != ~0ull && w > 0) {
       const u64 need = aim > c.above_w ? (aim - c.above_w + w - 1) / w : 0;
       if (need < (u64)t) t = (int)need;
@@ -734,7 +842,7 @@ struct Decider {
   __device__ __forceinline__ u64 kept_units(float z, int v, uint32_t key_above, int last) const {
     const uint32_t key = order_key(z);
     if (key <= kDead || key < key_above || (key == key_above && v > last)) return 0;
-    const double w = weight(z, m, s.c);
+    const double w = sc.weight(z);
     return w >= (double)s.min_p ? units(w) : 0;
   }
 
@@ -827,78 +935,40 @@ struct Decider {
     return lo > -3.4e38 ? order_key((float)lo) : 0;  // (NaN too: no bound)
   }
 
-  __device__ __forceinline__ void decide(int r) {
-    char* const rec = a.records + (int64_t)r * a.row_bytes;
-    const auto rp = tiles::tile_rsrc(rec + sizeof(Decision), a.pieces * (int)sizeof(Piece));
-    const auto rc = tiles::tile_rsrc(rec + sizeof(Decision) + a.pieces * sizeof(Piece),
-                                     (a.cells + 3) / 4 * 16);
-    listed_cells = -1;
-    // Each thread its piece; maximum and sum of all.
-    static_assert(kMaxPieces == kThreads, "one piece per thread");
-    const f32x4 y = tiles::load_coherent16(rp, tid * 16);
-    typedef double f64x2 __attribute__((ext_vector_type(2)));
-    const float pm = tid < a.pieces ? y[0] : kNegInf;
-    const double ps = tid < a.pieces ? __builtin_bit_cast(f64x2, y)[1] : 0.0;
-    m = block_max(pm);
-    if (m == kNegInf) {
-      nothing(r);
-      return;
+  // The first of the largest logits: of the first cell whose maximum is the row's.
+  __device__ __forceinline__ void first_of_largest(int r, const __amdgpu_buffer_rsrc_t& rc) {
+    const uint32_t top = order_key(m);
+    int c = 0x7fffffff;
+    for (int base = 0; base < a.cells; base += kThreads * 4) {  // uniform
+      const int c0 = base + tid * 4;
+      const f32x4 y = tiles::load_coherent16(rc, c0 * 4);
+#pragma unroll
+      for (int i = 3; i >= 0; --i)
+        if (c0 + i < a.cells && order_key(y[i]) == top) c = min(c, c0 + i);
     }
-    u64 whole = 0;
-    if (s.whole) {
-      // (A piece none of whose entries has a unit of weight counts as nothing.)
-      const double top = weight(pm, m, s.c);
-      const u64 w = pm == kNegInf || units(top) == 0 ? 0 : units(ps * top);
-      if (tid < a.pieces) sh.psum[tid] = w;
-      whole = block_sum(w);
-    }
-    if (!s.filtered) {
-      if (a.u)
-        draw(r, 0, 0x7fffffff, whole);
-      else
-        leave(r, 0, 0x7fffffff, whole);
-      return;
-    }
-    uint32_t floor = 0;
-    if (s.k == 1)
-      floor = order_key(m);
-    else if (s.k > 0)
-      floor = cell_bound(rc, s.k);
-    else if (s.p < 1.f)
-      floor = floor_of((1.0 - (double)s.p) * ((double)whole / kUnit) / a.vocab);
-    if (s.min_p > 0.f && (s.k == 0 || s.p == 1.f)) floor = max(floor, floor_of((double)s.min_p));
-    floor = max(m == -kNegInf ? order_key(m) : floor, kDead + 1);
-    if (!list_cells(rc, floor)) listed_cells = -1;
-    const int n = list_entries(Range{floor, 0.f, 0.f, 0, 0, 0});
-    if (n <= kShort) {
-      brief(r, n, whole);
-      return;
-    }
-    uint32_t key = floor;  // with min-p alone, all from the bound on are kept but for their weight
-    int last = 0x7fffffff;
-    if (s.k > 0 || s.p < 1.f) {
-      // (With top-k and top-p, the former's cut gives the sum for the latter's.)
-      u64 aim = ~0ull, total = whole;
-      Cut c;
-#pragma unroll 1
-      for (int pass = s.k > 0 && s.p < 1.f ? 0 : 1; pass < 2; ++pass) {
-        if (pass == 1 && s.p < 1.f) aim = (u64)ceil((double)s.p * (double)total);
-        c = cut(floor, n, s.k, aim);
-        if (pass == 0)
-          total = c.ties < 0 ? c.above_w + everything(c.n)
-                             : c.above_w + (u64)c.ties * units(weight(of_key(c.key), m, s.c));
-      }
-      key = c.key;
-      last = last_tie(c);
-    }
-    // The kept weights of the pieces.
+    if (tid == 0) sh.found = 0x7fffffff;
+    __syncthreads();
+    if (c != 0x7fffffff) atomicMin(&sh.found, c);
+    __syncthreads();
+    if (wave != 0) return;
+    const int v0 = sh.found * kCell;
+    const int v1 = v0 + lane, v2 = v0 + 64 + lane;
+    const uint64_t low = __ballot(v1 < a.vocab && order_key(T::get(row[min(v1, a.vocab - 1)])) == top);
+    const uint64_t high = __ballot(v2 < a.vocab && order_key(T::get(row[min(v2, a.vocab - 1)])) == top);
+    const int v = v0 + (low ? (int)__builtin_ctzll(low) : 64 + (high ? (int)__builtin_ctzll(high) : 0));
+    if (!a.u)
+      leave(r, top, v, (u64)kUnit);
+    else if (lane == 0)
+      a.tokens[r] = v;
+  }
+
+  // What is kept of a row: keys above `key`, or equal to it up to index `last`; `in_list`: all of
+  // it is among the n listed entries, else the row is read again. Its token or its decision.
+  __device__ __forceinline__ void conclude(int r, uint32_t key, int last, bool in_list, int n) {
     for (int i = tid; i < kMaxPieces; i += kThreads) sh.psum[i] = 0;
     __syncthreads();
-    if (n <= kList) {
-      for (int i = tid; i < n; i += kThreads) {
-        const u64 w = kept_units(of_key(sh.key[i]), sh.idx[i], key, last);
-        if (w) atomicAdd(&sh.psum[sh.idx[i] / kPiece], w);
-      }
+    if (in_list) {
+      add_listed(key, last, n);
     } else {
       listed_cells = -1;
       each_entry([&](const Eight<T>& x, int v0) __attribute__((always_inline)) {
@@ -909,6 +979,19 @@ struct Decider {
         if (lane == 0 && w) atomicAdd(&sh.psum[(v0 + 7) / kPiece], w);
       });
     }
+    sum_up(r, key, last);
+  }
+
+  // The kept ones of the list, into their pieces' sums.
+  __device__ __forceinline__ void add_listed(uint32_t key, int last, int n) {
+#pragma unroll 1
+    for (int i = tid; i < n; i += kThreads) {
+      const u64 w = kept_units(of_key(sh.key[i]), sh.idx[i], key, last);
+      if (w) atomicAdd(&sh.psum[sh.idx[i] / kPiece], w);
+    }
+  }
+
+  __device__ __forceinline__ void sum_up(int r, uint32_t key, int last) {
     __syncthreads();
     const u64 sum = block_sum(sh.psum[tid]);
     if (a.u)
@@ -917,51 +1000,380 @@ struct Decider {
       leave(r, key, last, sum);
   }
 
+  // The whole way of a row whose list does not fit, by this workgroup alone.
+  __device__ __forceinline__ void alone(int r, uint32_t floor, u64 whole) {
+    // (With top-k and top-p, the former's cut gives the sum for the latter's.)
+    u64 aim = ~0ull, total = whole;
+    Cut c;
+#pragma unroll 1
+    for (int pass = s.k > 0 && s.p < 1.f ? 0 : 1; pass < 2; ++pass) {
+      if (pass == 1 && s.p < 1.f) aim = (u64)ceil((double)s.p * (double)total);
+      c = Cut{};
+      c.range = Range{floor, 0.f, 0.f, 0, 0, 0};
+      cut_alone(c, s.k, aim);
+      if (pass == 0) total = weight_to(c);
+    }
+    conclude(r, c.key, last_tie(c), false, 0);
+  }
+
+  // Weight of the entries up to a cut.
+  __device__ __forceinline__ u64 weight_to(const Cut& c) {
+    if (c.ties < 0) return c.above_w + everything(c.n);
+    return c.above_w + (u64)c.ties * units(sc.weight(of_key(c.key)));
+  }
+
+  __device__ __forceinline__ void decide(int r) {
+    char* const rec = a.records + (int64_t)r * a.row_bytes;
+    Shared_row* const state = reinterpret_cast<Shared_row*>(rec + sizeof(Decision));
+    const auto rp = tiles::tile_rsrc(rec + kHead, a.pieces * (int)sizeof(Piece));
+    const auto rc = tiles::tile_rsrc(rec + kHead + a.pieces * sizeof(Piece), (a.cells + 3) / 4 * 16);
+    if (tid == 0) state->mode = kDecided;  // (unless the row is shared, below)
+    // Each thread its piece; maximum and sum of all.
+    static_assert(kMaxPieces == kThreads, "one piece per thread");
+    const f32x4 y = tiles::load_coherent16(rp, tid * 16);
+    typedef double f64x2 __attribute__((ext_vector_type(2)));
+    const float pm = tid < a.pieces ? y[0] : kNegInf;
+    const double ps = tid < a.pieces ? __builtin_bit_cast(f64x2, y)[1] : 0.0;
+    set_max(block_max(pm));
+    if (m == kNegInf) {
+      nothing(r);
+      return;
+    }
+    if (s.k == 1) {
+      first_of_largest(r, rc);
+      return;
+    }
+    u64 whole = 0;
+    if (s.whole) {
+      // (A piece none of whose entries has a unit of weight counts as nothing.)
+      const double top = sc.top_only ? (pm == m ? 1.0 : 0.0) : sc.weight(pm);
+      const u64 w = pm == kNegInf || units(top) == 0 ? 0 : units(ps * top);
+      if (tid < a.pieces) sh.psum[tid] = w;
+      whole = block_sum(w);
+    }
+    const uint32_t lowest = sc.top_only ? order_key(m) : kDead + 1;  // key with a weight
+    if (!s.filtered) {
+      if (a.u)
+        draw(r, lowest, 0x7fffffff, whole);
+      else
+        leave(r, lowest, 0x7fffffff, whole);
+      return;
+    }
+    uint32_t floor = lowest;
+    if (s.k > 0)
+      floor = cell_bound(rc, s.k);
+    else if (s.p < 1.f)
+      floor = floor_of((1.0 - (double)s.p) * ((double)whole / kUnit) / a.vocab);
+    if (s.min_p > 0.f && (s.k == 0 || s.p == 1.f)) floor = max(floor, floor_of((double)s.min_p));
+    floor = max(floor, lowest);
+    // (Where most cells of a long row reach the bound, its entries are not even counted here:
+    // they are nearly always too many, and one workgroup takes 25 us for 150,000.)
+    const bool few = list_cells(rc, floor);
+    if (!few) listed_cells = -1;
+    const int n = few || a.pieces <= kAlonePieces || r >= a.shared_rows
+                      ? list_entries(Range{floor, 0.f, 0.f, 0, 0, 0}) : kList + 1;
+    if (n <= kShort) {
+      brief(r, n, whole);
+      return;
+    }
+    const bool limited = s.k > 0 || s.p < 1.f;  // (with min-p alone, only the weights decide)
+    if (n > kList) {
+      // Shared by several workgroups in the next launches. Top-k and top-p together would take
+      // two cuts, and areas may have run out: then by one alone.
+      Cut c{};
+      c.range.floor = floor;
+      lay_bins(c.range);
+      const bool counted = c.range.scale > 0.f && !(s.k > 0 && s.p < 1.f);
+      const int mode = r >= a.shared_rows || (limited && !counted) ? kAlone
+                       : limited ? kCount : kKeepAll;
+      if (mode == kCount) {
+        Area& area = a.areas[r];
+        for (int i = tid; i < kBins; i += kThreads) {
+          area.bin.w[i] = 0;
+          area.bin.n[i] = 0;
+        }
+      }
+      if (tid == 0) {
+        Shared_row x{};
+        x.mode = mode;
+        x.max = m;
+        x.floor = floor;
+        x.lo = c.range.lo;
+        x.scale = c.range.scale;
+        x.aim = s.p < 1.f ? (u64)ceil((double)s.p * (double)whole) : ~0ull;
+        x.whole = whole;
+        *state = x;
+      }
+      return;
+    }
+    uint32_t key = floor;
+    int last = 0x7fffffff;
+    if (limited) {
+      u64 aim = ~0ull, total = whole;
+      Cut c;
+#pragma unroll 1
+      for (int pass = s.k > 0 && s.p < 1.f ? 0 : 1; pass < 2; ++pass) {
+        if (pass == 1 && s.p < 1.f) aim = (u64)ceil((double)s.p * (double)total);
+        c = Cut{};
+        c.range = Range{floor, 0.f, 0.f, 0, 0, 0};
+        c.n = n;
+        cut_list(c, s.k, aim);
+        if (pass == 0) total = weight_to(c);
+      }
+      key = c.key;
+      last = last_tie(c);
+    }
+    conclude(r, key, last, true, n);
+  }
+
+  // ---- a row shared by workgroups: the launch that counts, and the one that ends it ----
+
+  __device__ __forceinline__ static Range range_of(const Shared_row& x) {
+    return Range{x.floor, x.lo, x.scale, x.bin, 0, 0};
+  }
+
+  // f(x, v0) for this workgroup's pieces, with the piece's number, by whole wavefronts.
+  template <typename F>
+  __device__ __forceinline__ void each_piece(int group, F f) {
+    const int stride = a.shared_groups * kWaves;
+#pragma unroll 1
+    for (int p = group * kWaves + wave; p < a.pieces; p += stride) {  // wavefront-uniform
+      Eight<T> x[2];
+      int v0[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) v0[j] = x[j].load(row, p * kPiece + j * 512 + lane * 8, a.vocab);
+      f(p, x, v0);
+    }
+  }
+
+  // Counts (with top-k) or weights (with top-p) per interval into the row's bins.
+  __device__ __forceinline__ void count(int r, int group, const Shared_row& state) {
+    for (int i = tid; i < kBins; i += kThreads) {
+      sh.bin.n[i] = 0;
+      sh.bin.w[i] = 0;
+    }
+    __syncthreads();
+    const Range range = range_of(state);
+    each_piece(group, [&](int, const Eight<T> (&x)[2], const int (&)[2]) __attribute__((always_inline)) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        if (s.k > 0) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float z = x[j][i];
+            if (order_key(z) >= range.floor) atomicAdd(&sh.bin.n[range.bin_of(z)], 1u);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float z = x[j][i];
+            const u64 w = units(sc.weight(z));
+            if (order_key(z) >= range.floor) atomicAdd(&sh.bin.w[range.bin_of(z)], w);
+          }
+        }
+      }
+    });
+    __syncthreads();
+    Area& area = a.areas[r];
+    for (int i = tid; i < kBins; i += kThreads) {
+      if (s.k > 0) {
+        const uint32_t n = sh.bin.n[i];
+        if (n) __hip_atomic_fetch_add(&area.bin.n[i], n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      } else {
+        const u64 w = sh.bin.w[i];
+        if (w) __hip_atomic_fetch_add(&area.bin.w[i], w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      }
+    }
+  }
+
+  // All of the row's bins: the interval with the border.
+  __device__ __forceinline__ void find_bin(int r, Shared_row* state) {
+    Area& area = a.areas[r];
+    for (int i = tid; i < kBins; i += kThreads) {
+      const u64 w = __hip_atomic_load(&area.bin.w[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      const uint32_t n = __hip_atomic_load(&area.bin.n[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      sh.bin.w[i] = w;
+      sh.bin.n[i] = s.k > 0 ? n : w > 0;  // (how many weigh it is not counted: some)
+    }
+    walk_bins<kBins>(0, 0, s.k, state->aim);
+    if (tid == 0) {
+      state->mode = sh.found < 0 ? kKeepAll : kCollect;
+      state->bin = sh.found;
+      state->above = sh.found2;
+      state->above_w = sh.found_w;
+    }
+  }
+
+  // The entries of the border's interval into the row's list, and what is kept above it into
+  // the pieces' sums.
+  __device__ __forceinline__ void collect(int r, int group, Shared_row* state, Piece* pieces) {
+    const bool all = state->mode == kKeepAll;
+    const Range range = all ? Range{state->floor, 0.f, 0.f, -1, 0, 0} : range_of(*state);
+    if (tid == 0) sh.count = 0;
+    __syncthreads();
+    each_piece(group, [&](int p, const Eight<T> (&x)[2], const int (&v0)[2]) __attribute__((always_inline)) {
+      u64 w = 0;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        unsigned in = 0, over = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int at = range.place(x[j][i], order_key(x[j][i]));
+          in |= (unsigned)(at == 1) << i;
+          over |= (unsigned)(at == 2) << i;
+        }
+        if (__ballot(over != 0) != 0) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const double y = sc.weight(x[j][i]);
+            w += (over >> i & 1) && y >= (double)s.min_p ? units(y) : 0;
+          }
+        }
+        if (__ballot(in != 0) != 0) {
+          const int mine = __builtin_popcount(in);
+          const int incl = tiles::wave_incl_scan(mine);
+          int at = 0;
+          if (lane == 63) at = atomicAdd(&sh.count, incl);
+          at = __builtin_amdgcn_readlane(at, 63) + incl - mine;
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (in >> i & 1) {
+              if (at < kList) {
+                sh.key[at] = order_key(x[j][i]);
+                sh.idx[at] = v0[j] + i;
+              }
+              ++at;
+            }
+        }
+      }
+      w = wave_sum(w);
+      if (lane == 0)
+        __hip_atomic_store(reinterpret_cast<u64*>(&pieces[p].sum), w, __ATOMIC_RELAXED,
+                           __HIP_MEMORY_SCOPE_AGENT);
+    });
+    __syncthreads();
+    const int n = sh.count;
+    if (n > 0) {  // uniform
+      if (tid == 0)
+        sh.found = __hip_atomic_fetch_add(&state->listed, n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      __syncthreads();
+      Area& area = a.areas[r];
+      for (int i = tid; i < min(n, kList - sh.found); i += kThreads) {
+        __hip_atomic_store(&area.list.key[sh.found + i], sh.key[i], __ATOMIC_RELAXED,
+                           __HIP_MEMORY_SCOPE_AGENT);
+        __hip_atomic_store(&area.list.idx[sh.found + i], sh.idx[i], __ATOMIC_RELAXED,
+                           __HIP_MEMORY_SCOPE_AGENT);
+      }
+    }
+  }
+
+  // The end of a shared row, of all workgroups' lists and sums.
+  __device__ __forceinline__ void end(int r, Shared_row* state, Piece* pieces) {
+    const bool all = state->mode == kKeepAll;
+    Cut c{};
+    c.range = range_of(*state);
+    c.above = state->above;
+    c.above_w = state->above_w;
+    keep_all(c);
+    int last = 0x7fffffff;
+    if (!all) {
+      c.n = __hip_atomic_load(&state->listed, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      if (c.n > kList) {  // many equal logits, or nearly
+        alone(r, state->floor, state->whole);
+        return;
+      }
+      const Area& area = a.areas[r];
+      for (int i = tid; i < c.n; i += kThreads) {
+        sh.key[i] = __hip_atomic_load(&area.list.key[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        sh.idx[i] = __hip_atomic_load(&area.list.idx[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      }
+      __syncthreads();
+      if (c.n <= kShort) {
+        cut_brief(c, s.k, state->aim, last);
+      } else {
+        cut_list(c, s.k, state->aim);
+        last = last_tie(c);
+      }
+    }
+    sh.psum[tid] = tid < a.pieces
+                       ? __hip_atomic_load(reinterpret_cast<const u64*>(&pieces[tid].sum),
+                                           __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)
+                       : 0;
+    __syncthreads();
+    if (!all) add_listed(c.key, last, c.n);
+    sum_up(r, c.key, last);
+  }
+
   // Weight of all listed entries.
   __device__ __forceinline__ u64 everything(int n) {
     u64 w = 0;
-    for (int i = tid; i < n; i += kThreads) w += units(weight(of_key(sh.key[i]), m, s.c));
+    for (int i = tid; i < n; i += kThreads) w += units(sc.weight(of_key(sh.key[i])));
     return block_sum(w);
   }
 
   // A row of at most kShort entries, one per thread.
   __device__ __forceinline__ void decide_short(int r) {
     const float z = tid < a.vocab ? fmaxf(T::get(row[tid]), kNegInf) : kNegInf;
-    m = block_max(z);
+    set_max(block_max(z));
     if (m == kNegInf) {
       nothing(r);
       return;
     }
+    const bool out = z == kNegInf || (sc.top_only && z != m);
     if (tid < a.vocab) {
-      sh.key[tid] = order_key(z);
+      sh.key[tid] = out ? kDead : order_key(z);
       sh.idx[tid] = tid;
     }
-    const u64 whole = block_sum(z == kNegInf ? 0 : units(weight(z, m, s.c)));
+    const u64 whole = block_sum(out ? 0 : units(sc.weight(z)));
     brief(r, a.vocab, whole);
   }
 
-  // The end for at most kShort listed entries, one per thread.
+  // The sum over the n entries in sh.brief of what f makes of each, for entry tid % kShort: half
+  // by thread tid of the first kShort, which get it, half by its partner.
+  template <typename F>
+  __device__ __forceinline__ u64 over_brief(int n, F f) {
+    static_assert(kThreads == 2 * kShort, "two threads per entry");
+    const int half = (n + 15) / 16 * 8;  // (behind the n there are entries that add nothing)
+    const int from = tid < kShort ? 0 : half;
+    u64 x = 0;
+    if ((tid & (kShort - 1)) < ((n + 63) & ~63)) {  // wavefront-uniform
+#pragma unroll 1
+      for (int i = from; i < from + half; i += 8)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x += f(sh.brief.entry[i + j]);
+    }
+    if (tid >= kShort) sh.brief.more[tid - kShort] = x;
+    __syncthreads();
+    if (tid < kShort) x += sh.brief.more[tid];
+    return x;
+  }
+
+  // How many of the entries in sh.brief come before `order`, times 2^53, and their weight.
+  // (Weights of 2^44 at most: 256 of them leave room for their number in the same sum.)
+  __device__ __forceinline__ u64 places(int n, u64 order) {
+    return over_brief(n, [&](ulonglong2 x) __attribute__((always_inline)) {
+      return x.x > order ? x.y + (1ull << 53) : 0;
+    });
+  }
+
+  // The end for at most kShort listed entries, one per thread of the first half: every entry's
+  // place in the order and the weight before it.
   __device__ __forceinline__ void brief(int r, int n, u64 whole) {
+    const int e = tid & (kShort - 1);
     u64 order = 0, w = 0;
     uint32_t key = 0;
     int v = 0;
-    if (tid < n) {
-      key = sh.key[tid];
-      v = sh.idx[tid];
+    if (e < n) {
+      key = sh.key[e];
+      v = sh.idx[e];
       order = (u64)key << 32 | (uint32_t)~v;
-      w = units(weight(of_key(key), m, s.c));
-      sh.brief.order[tid] = order;
-      sh.brief.w[tid] = w;
+      w = units(sc.weight(of_key(key)));
     }
+    if (tid < kShort) sh.brief.entry[e] = ulonglong2{order, w};
     __syncthreads();
-    int rank = 0;
-    u64 before = 0;
-    if (tid < n)
-      for (int i = 0; i < n; ++i) {
-        const bool first = sh.brief.order[i] > order;
-        rank += first;
-        before += first ? sh.brief.w[i] : 0;
-      }
+    const u64 first = places(n, order);
+    const int rank = (int)(first >> 53);
+    const u64 before = first & ((1ull << 53) - 1);
     bool kept = tid < n && key > kDead && (s.k == 0 || rank < s.k);
     if (s.p < 1.f) {
       u64 total = whole;
@@ -969,7 +1381,7 @@ struct Decider {
       const u64 aim = (u64)ceil((double)s.p * (double)total);
       kept = kept && (rank == 0 || before < aim);
     }
-    if (kept && s.min_p > 0.f) kept = weight(of_key(key), m, s.c) >= (double)s.min_p;
+    if (kept && s.min_p > 0.f) kept = sc.weight(of_key(key)) >= (double)s.min_p;
     const u64 sum = block_sum(kept ? w : 0);
     if (!a.u) {
       // The last kept one in the order.
@@ -985,47 +1397,50 @@ struct Decider {
       leave(r, sh.found_key, sh.found, sum);
       return;
     }
-    // By the index now.
+    // By the index now. (All have left the first walk behind block_sum's barriers.)
+    if (tid < kShort) sh.brief.entry[e] = ulonglong2{(u64)v, kept ? w : 0};
+    if (tid == 0) sh.found = sh.found2 = -1;
     __syncthreads();
-    if (tid < n) sh.brief.w[tid] = kept ? w : 0;
-    if (tid == 0) {
-      sh.found = 0x7fffffff;
-      sh.found2 = -1;
-    }
-    __syncthreads();
-    const int seq = r / a.each;
-    const double aim = (double)a.u[seq * a.u_seq + (r - seq * a.each) * a.u_row] * (double)sum;
+    const u64 run = over_brief(n, [&](ulonglong2 x) __attribute__((always_inline)) {
+      return (int)x.x <= v ? x.y : 0;
+    });
     if (kept && w > 0) {
-      u64 run = 0;
-      for (int i = 0; i < n; ++i) run += sh.idx[i] <= v ? sh.brief.w[i] : 0;
-      if ((double)run > aim) atomicMin(&sh.found, v);
+      const int seq = r / a.each;
+      const double aim = (double)a.u[seq * a.u_seq + (r - seq * a.each) * a.u_row] * (double)sum;
+      if ((double)run > aim && (run == w || !((double)(run - w) > aim))) sh.found = v;  // one, or none
       atomicMax(&sh.found2, v);
     }
     __syncthreads();
-    if (tid == 0) a.tokens[r] = sh.found != 0x7fffffff ? sh.found : sh.found2;
+    if (tid == 0) a.tokens[r] = sh.found >= 0 ? sh.found : sh.found2;
   }
 };
 
 template <typename T>
-__global__ __launch_bounds__(kThreads, 4) void sample_kernel(Args a) {
-  __shared__ Shared sh;
-  __shared__ int s_last;
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int r = blockIdx.x / a.groups;
-  const int group = blockIdx.x - r * a.groups;
-  const int seq = r / a.each;
-  const typename T::E* row = (const typename T::E*)a.logits + seq * a.s_seq +
-                             (int64_t)(r - seq * a.each) * a.s_row;
-  const Settings s = settings_of(a, seq);
-  if (a.vocab <= kShort) {
-    Decider<T>{a, sh, row, s, 0.f, tid, lane, wave, -1}.decide_short(r);
-    return;
-  }
-  char* const rec = a.records + (int64_t)r * a.row_bytes;
-  Piece* const pieces = reinterpret_cast<Piece*>(rec + sizeof(Decision));
-  float* const cells = reinterpret_cast<float*>(rec + sizeof(Decision) + a.pieces * sizeof(Piece));
+__device__ __forceinline__ const typename T::E* row_of(const Args& a, int r, int seq) {
+  return (const typename T::E*)a.logits + seq * a.s_seq + (int64_t)(r - seq * a.each) * a.s_row;
+}
 
+// Counts this workgroup's arrival at row r; whether it is the last of `groups`.
+__device__ __forceinline__ bool arrive_last(const Args& a, int r, int groups, int tid, int& s_last) {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+  __builtin_amdgcn_s_waitcnt(0);  // what it leaves has landed before the arrival counts
+  __syncthreads();
+  if (tid == 0)
+    s_last = __hip_atomic_fetch_add(a.cnt + r, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
+             groups - 1;
+  __syncthreads();
+  if (!s_last) return false;
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
+  if (tid == 0) __hip_atomic_store(a.cnt + r, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  return true;
+}
+
+// One reading of the row: its pieces of this workgroup.
+template <typename T>
+__device__ __forceinline__ void read_row(const Args& a, const typename T::E* row, const Settings& s,
+                                         char* rec, int group, int wave, int lane) {
+  Piece* const pieces = reinterpret_cast<Piece*>(rec + kHead);
+  float* const cells = reinterpret_cast<float*>(rec + kHead + a.pieces * sizeof(Piece));
   auto take = [&](int p, Eight<T> (&x)[2]) {
 #pragma unroll
     for (int j = 0; j < 2; ++j) x[j].load(row, p * kPiece + j * 512 + lane * 8, a.vocab);
@@ -1048,10 +1463,18 @@ __global__ __launch_bounds__(kThreads, 4) void sample_kernel(Args a) {
     mp = wave_max_of_rows(mp);
     double sum = 0.0;
     if (s.whole && mp != kNegInf) {  // wavefront-uniform
+      const Scale sc(mp, s.c);
+      if (sc.top_only) {
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+        for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sum += weight(x[j][i], mp, s.c);
+          for (int i = 0; i < 8; ++i) sum += x[j][i] == mp ? 1.0 : 0.0;
+      } else {
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) sum += sc.weight(x[j][i]);
+      }
       sum = wave_sum(sum);
     }
     if (lane == 0) {
@@ -1072,18 +1495,58 @@ __global__ __launch_bounds__(kThreads, 4) void sample_kernel(Args a) {
     reduce(p, x1);
     p += stride;
   }
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
-  __builtin_amdgcn_s_waitcnt(0);  // the records have landed before the arrival counts
-  __syncthreads();
-  if (tid == 0)
-    s_last = __hip_atomic_fetch_add(a.cnt + r, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
-             a.groups - 1;
-  __syncthreads();
-  if (!s_last) return;
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
-  Decider<T> d{a, sh, row, s, 0.f, tid, lane, wave, -1};
-  d.decide(r);
-  if (tid == 0) __hip_atomic_store(a.cnt + r, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+template <typename T>
+__global__ __launch_bounds__(kThreads, 4) void sample_kernel(Args a) {
+  __shared__ Shared sh;
+  __shared__ int s_last;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r = blockIdx.x / a.groups;
+  const int seq = r / a.each;
+  const typename T::E* row = row_of<T>(a, r, seq);
+  const Settings s = settings_of(a, seq);
+  Decider<T> d(a, sh, row, s, tid, lane, wave);
+  if (a.vocab <= kShort) {
+    d.decide_short(r);
+    return;
+  }
+  char* const rec = a.records + (int64_t)r * a.row_bytes;
+  read_row<T>(a, row, s, rec, blockIdx.x - r * a.groups, wave, lane);
+  if (arrive_last(a, r, a.groups, tid, s_last)) d.decide(r);
+}
+
+// The launches that share a row whose list does not fit: END false, counts and weights per
+// interval; END true, the list of the border's interval and the end.
+template <typename T, bool END>
+__global__ __launch_bounds__(kThreads, 4) void shared_kernel(Args a) {
+  __shared__ Shared sh;
+  __shared__ int s_last;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r = blockIdx.x / a.shared_groups;
+  const int group = blockIdx.x - r * a.shared_groups;
+  char* const rec = a.records + (int64_t)r * a.row_bytes;
+  Shared_row* const state = reinterpret_cast<Shared_row*>(rec + sizeof(Decision));
+  Piece* const pieces = reinterpret_cast<Piece*>(rec + kHead);
+  const int mode = state->mode;  // (written by an earlier launch; END leaves it)
+  if (END ? mode == kDecided : mode != kCount) return;
+  const int seq = r / a.each;
+  const typename T::E* row = row_of<T>(a, r, seq);
+  Decider<T> d(a, sh, row, settings_of(a, seq), tid, lane, wave);
+  d.set_max(state->max);
+  if constexpr (END) {
+    if (mode == kAlone) {
+      if (group == 0) d.alone(r, state->floor, state->whole);
+      return;
+    }
+    d.collect(r, group, state, pieces);
+    if (arrive_last(a, r, a.shared_groups, tid, s_last)) d.end(r, state, pieces);
+  } else {
+    d.count(r, group, *state);
+    if (arrive_last(a, r, a.shared_groups, tid, s_last)) d.find_bin(r, state);
+  }
 }
 
 // Probabilities of one piece per wavefront.
@@ -1099,12 +1562,13 @@ __global__ __launch_bounds__(256) void probs_kernel(Args a) {
                              (int64_t)(r - seq * a.each) * a.s_row;
   const Decision d = *reinterpret_cast<const Decision*>(a.records + (int64_t)r * a.row_bytes);
   float* out = a.probs + (int64_t)r * a.vocab;
+  const Scale sc(d.max, d.c);
   const double inv = d.sum > 0.0 ? 1.0 / d.sum : 0.0;
   if (a.vocab <= kShort) {  // (one piece)
     for (int v = lane; v < a.vocab; v += 64) {
       const float z = fmaxf(T::get(row[v]), kNegInf);
       const uint32_t key = order_key(z);
-      const double w = weight(z, d.max, d.c);
+      const double w = sc.weight(z);
       out[v] = key > kDead && (key > d.key || (key == d.key && v <= d.last)) && w >= (double)d.min_p
                    ? (float)(w * inv) : 0.f;
     }
@@ -1129,7 +1593,7 @@ __global__ __launch_bounds__(256) void probs_kernel(Args a) {
     if (__ballot(any) != 0) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const double w = weight(x[j][i], d.max, d.c);
+        const double w = sc.weight(x[j][i]);
         if (in[i] && w >= (double)d.min_p) y[i] = (float)(w * inv);
       }
     }
@@ -1152,6 +1616,8 @@ static int cells_of(int vocab) { return (vocab + kCell - 1) / kCell; }
 // Workgroups per row: one wavefront per piece for a few rows; for many, as many as fill
 // kWavesPerCu wavefronts per compute unit over all rows, the pieces dealt in whole rounds.
 constexpr int kWavesPerCu = 16;
+// Wavefronts that share a row of a long list, at most.
+constexpr int kSharedWaves = 80;
 static int groups_of(int rows, int pieces) {
   int64_t waves = (int64_t)kWavesPerCu * device_cus() / rows;
   if (waves < 1) waves = 1;
@@ -1160,23 +1626,37 @@ static int groups_of(int rows, int pieces) {
   return (int)((per_round + kWaves - 1) / kWaves);
 }
 
+// Whether no row's list can be too long: short rows, and settings of all rows that list nothing.
+static bool never_shared(const Args& a) {
+  if (a.vocab <= kList) return true;
+  const bool greedy = !a.temperature && !(a.t_all > 0.f);
+  const bool one = !a.top_k && a.k_all == 1;
+  const bool plain = !a.top_k && (a.k_all <= 0 || a.k_all >= a.vocab) && !a.top_p &&
+                     !(a.p_all < 1.f) && !a.min_p && !(a.m_all > 0.f);
+  return greedy || one || plain;
+}
+
+template <typename T>
+static hipError_t launch(const Args& a, hipStream_t stream) {
+  sample_kernel<T><<<(unsigned)(a.rows * (int64_t)a.groups), kThreads, 0, stream>>>(a);
+  if (!never_shared(a)) {
+    const unsigned grid = (unsigned)(a.rows * (int64_t)a.shared_groups);
+    shared_kernel<T, false><<<grid, kThreads, 0, stream>>>(a);
+    shared_kernel<T, true><<<grid, kThreads, 0, stream>>>(a);
+  }
+  if (a.probs)
+    probs_kernel<T><<<(unsigned)(((int64_t)a.rows * a.pieces + 3) / 4), 256, 0, stream>>>(a);
+  return hipGetLastError();
+}
+
+static int shared_rows_of(int rows, int vocab) {
+  return vocab <= kList ? 0 : rows < kMaxShared ? rows : kMaxShared;
+}
+
 static int run(const Args& a, int dtype, hipStream_t stream) {
-  const unsigned grid = (unsigned)((int64_t)a.rows * a.groups);
-  switch (dtype) {
-    case PA_F16: sample_kernel<Half><<<grid, kThreads, 0, stream>>>(a); break;
-    case PA_BF16: sample_kernel<Brain><<<grid, kThreads, 0, stream>>>(a); break;
-    default: sample_kernel<Single><<<grid, kThreads, 0, stream>>>(a); break;
-  }
-  hipError_t e = hipGetLastError();
-  if (e == hipSuccess && a.probs) {
-    const unsigned wgs = (unsigned)(((int64_t)a.rows * a.pieces + 3) / 4);
-    switch (dtype) {
-      case PA_F16: probs_kernel<Half><<<wgs, 256, 0, stream>>>(a); break;
-      case PA_BF16: probs_kernel<Brain><<<wgs, 256, 0, stream>>>(a); break;
-      default: probs_kernel<Single><<<wgs, 256, 0, stream>>>(a); break;
-    }
-    e = hipGetLastError();
-  }
+  const hipError_t e = dtype == PA_F16    ? launch<Half>(a, stream)
+                       : dtype == PA_BF16 ? launch<Brain>(a, stream)
+                                          : launch<Single>(a, stream);
   if (e == hipSuccess) return PA_OK;
   set_error("HIP launch failed: %s", hipGetErrorString(e));
   return PA_ERR_HIP;
@@ -1193,7 +1673,8 @@ extern "C" {
 size_t pa_sample_workspace_bytes(int num_seqs, int rows_per_seq, int vocab) {
   const int64_t rows = (int64_t)num_seqs * rows_per_seq;
   if (num_seqs <= 0 || rows_per_seq <= 0 || rows > kMaxRows || vocab <= 0 || vocab > kMaxVocab) return 0;
-  return kCounterBytes + (size_t)rows * row_record(pieces_of(vocab), cells_of(vocab));
+  return kCounterBytes + (size_t)rows * row_record(pieces_of(vocab), cells_of(vocab)) +
+         (size_t)shared_rows_of((int)rows, vocab) * sizeof(Area);
 }
 
 static int start(Args& a, const void* logits, int dtype, const int64_t* strides, int num_seqs,
@@ -1254,6 +1735,9 @@ static int start(Args& a, const void* logits, int dtype, const int64_t* strides,
   a.row_bytes = row_record(a.pieces, a.cells);
   a.cnt = (int*)workspace;
   a.records = (char*)workspace + kCounterBytes;
+  a.areas = (Area*)(a.records + (size_t)a.rows * a.row_bytes);
+  a.shared_rows = shared_rows_of(a.rows, vocab);
+  a.shared_groups = a.pieces < kSharedWaves ? (a.pieces + kWaves - 1) / kWaves : kSharedWaves / kWaves;
   return PA_OK;
 }
 
