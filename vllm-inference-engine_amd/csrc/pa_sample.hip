@@ -15,9 +15,13 @@
 // listed: tens to hundreds for usual settings. A short list is ranked by comparing all
 // with all; a longer one by radix passes over the logits' bits with counts and weights.
 // Where more are listed than fit LDS (flat distributions), two more launches share the row
-// among workgroups again: the first adds up counts and weights per interval of logits and finds
-// the interval in which the border lies, the second lists its entries, sums what lies above it
-// per piece, and decides. (Rows without such a list leave those launches at once.)
+// among workgroups. The first counts entries and adds up their places per interval of logits,
+// without weighing one: an interval's weight is at least that of its number at their mean
+// (the exponential is convex) and at most that of as many on the chord over it, which brackets
+// the border to an interval or two. The second sums the weights above the bracket per piece and
+// lists what lies in it, and the last of its workgroups decides. Lists beyond their room (equal
+// logits) have the row done by one workgroup alone, narrowing by intervals of logits and by
+// their bits. (Rows without such a list leave these launches at once.)
 //
 // Weights and sums. w is computed in 64 bits (2^-45 relative) and summed as whole numbers of
 // 2^-44: sums do not depend on the order, so that LDS atomics may form them, and the 2^19
@@ -41,11 +45,14 @@ constexpr int kMaxCells = kMaxVocab / kCell;
 constexpr int kMaxRows = 16384;
 constexpr size_t kCounterBytes = (size_t)kMaxRows * sizeof(int);
 constexpr int kList = 2048;   // listed entries
-constexpr int kShort = 256;   // of them, ranked by comparing all with all
+constexpr int kShort = 512;   // of them, ranked by comparing all with all: one per thread
+constexpr int kCellBins = 512;
 constexpr int kBins = 2048;
+constexpr int kRoom = 2048;  // words of a shared row's room
+static_assert(kRoom >= kBins && kRoom >= kList, "counts, then the list");
 // Pieces that a workgroup looks through by itself, though most of them reach the bound.
 constexpr int kAlonePieces = 32;
-constexpr int kMaxShared = 2048;  // rows with an area to be shared by
+constexpr int kMaxShared = 2048;  // rows with room to be shared by
 constexpr uint32_t kDead = 0x007fffffu;  // order key of -inf; NaN counts as -inf
 constexpr double kUnit = 17592186044416.0;  // 2^44
 
@@ -66,30 +73,17 @@ struct Piece {
   double sum;  // (of a shared row in the end: the kept weight, in units)
 };
 
-// A row whose list does not fit, between the launches that share it.
-enum { kDecided = 0, kCount = 1, kCollect = 2, kKeepAll = 3, kAlone = 4 };
+// A row whose list does not fit, between the launches.
+enum { kDecided = 0, kCount = 1, kShare = 2, kKeepAll = 3, kAlone = 4 };
 struct alignas(16) Shared_row {
   int mode;
   float max;
-  uint32_t floor;   // keys below are out of the question
-  float lo, scale;  // the intervals of the logits' line,
-  int bin;          // and the one with the border
-  int above;        // entries above it, and their weight
-  int listed;       // entries of it
-  u64 above_w, aim, whole;
-};
-// Its bins, and then its list.
-struct Area {
-  union {
-    struct {
-      u64 w[2048];
-      uint32_t n[2048];
-    } bin;
-    struct {
-      uint32_t key[2048];
-      int idx[2048];
-    } list;
-  };
+  uint32_t floor;     // keys below are out of the question
+  float lo, scale;    // the intervals of the logits' line,
+  int first, end;     // and those of the bracket
+  int pad;
+  u64 counts;         // entries in the bracket (listed), and 2^32 times those above it
+  u64 aim, whole;
 };
 
 struct Args {
@@ -108,7 +102,7 @@ struct Args {
   float* probs;
   int* cnt;
   char* records;  // per row: Decision, Shared_row, pieces, cells
-  Area* areas;    // of the first `shared_rows` rows
+  u64* rooms;     // of the first `shared_rows` rows: kBins counts and places, then kList keys and indexes
   int row_bytes, pieces, cells, groups;
   int shared_rows, shared_groups;
 };
@@ -206,6 +200,10 @@ struct Scale {
   __device__ double weight(float z) const { return exp2_of(fmax(((double)z - m) * c, low)); }
 };
 __device__ inline u64 units(double w) { return (u64)(w * kUnit + 0.5); }
+// The same for w up to 1, by an addition that leaves the rounded number in the low bits.
+__device__ inline u64 units1(double w) {
+  return __builtin_bit_cast(u64, __builtin_fma(w, kUnit, 4503599627370496.0)) & 0xfffffffffffffull;
+}
 
 // ---- sums over lanes ---------------------------------------------------------------
 
@@ -313,7 +311,7 @@ struct Shared {
     uint16_t cells[kMaxCells];
     struct {
       ulonglong2 entry[kShort];  // order or index, weight
-      u64 more[kShort];
+      u64 more[kShort / 2];
     } brief;
   };
   u64 psum[kMaxPieces];
@@ -426,85 +424,64 @@ struct Decider {
     return x;
   }
 
-  // The smallest key that the k-th largest of the cells' maxima can have, to 16 bits.
-  __device__ __forceinline__ uint32_t cell_bound(const __amdgpu_buffer_rsrc_t& rc, int k) {
-    if (k > a.cells) return 0;
-    constexpr int PER = kMaxCells / kThreads;
-    static_assert(PER == 8, "two loads of four per thread");
-    uint32_t keys[PER];
+  // The cells' maxima, eight per thread: cell (j * kThreads + tid) * 4 + i at [j * 4 + i].
+  static constexpr int kCells = kMaxCells / kThreads;
+  static_assert(kCells == 8, "two loads of four per thread");
+  float cell[kCells];
+  __device__ __forceinline__ int cell_of(int i) const { return (i / 4 * kThreads + tid) * 4 + i % 4; }
+  __device__ __forceinline__ void load_cells(const __amdgpu_buffer_rsrc_t& rc) {
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      const int c0 = (j * kThreads + tid) * 4;
-      if (j * kThreads * 4 >= a.cells) {  // uniform
+      f32x4 y = {kNegInf, kNegInf, kNegInf, kNegInf};
+      if (j * kThreads * 4 < a.cells)  // uniform
+        y = tiles::load_coherent16(rc, (j * kThreads + tid) * 16);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) keys[j * 4 + i] = 0;
-        continue;
-      }
-      const f32x4 y = tiles::load_coherent16(rc, c0 * 4);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) keys[j * 4 + i] = c0 + i < a.cells ? order_key(y[i]) : 0;
+      for (int i = 0; i < 4; ++i) cell[j * 4 + i] = cell_of(j * 4 + i) < a.cells ? y[i] : kNegInf;
     }
-    uint32_t prefix = 0;
-    int left = k;
+  }
+
+  // A key that the k-th largest entry has at least: the k-th largest of the cells' maxima, to a
+  // bin of their range.
+  __device__ __forceinline__ uint32_t cell_bound(int k) {
+    float low = -kNegInf;
 #pragma unroll
-    for (int pass = 0; pass < 2; ++pass) {
-      for (int i = tid; i < 256; i += kThreads) sh.bin.n[i] = 0;
-      __syncthreads();
-#pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        const uint32_t x = keys[i];
-        if (x != 0 && (pass == 0 || x >> 24 == prefix))
-          atomicAdd(&sh.bin.n[pass == 0 ? x >> 24 : (x >> 16) & 255], 1u);
-      }
-      __syncthreads();
-      if (wave == 0) {
-        // Lane l: bins 255 - 4 l down to 252 - 4 l.
-        int own[4], mine = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) mine += own[i] = (int)sh.bin.n[255 - 4 * lane - i];
-        const int incl = tiles::wave_incl_scan(mine);
-        int sum = incl - mine, hit = -1, before = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (hit < 0 && sum + own[i] >= left) {
-            hit = 255 - 4 * lane - i;
-            before = sum;
-          }
-          sum += own[i];
-        }
-        const uint64_t hits = __ballot(hit >= 0);
-        if (hits && lane == (int)__builtin_ctzll(hits)) {
-          sh.found = hit;
-          sh.found2 = left - before;
-        }
-      }
-      __syncthreads();
-      prefix = prefix << 8 | (uint32_t)sh.found;
-      left = sh.found2;
-      __syncthreads();
+    for (int i = 0; i < kCells; ++i)
+      if (cell[i] != kNegInf) low = fminf(low, cell[i]);
+    low = -block_max(-low);
+    const float width = m - low;
+    if (!(width > 0.f && width < 3e38f)) return 0;
+    const float scale = (float)kCellBins / width;
+    auto bin = [&](float z) { return min((int)((z - low) * scale), kCellBins - 1); };
+    for (int i = tid; i < kCellBins; i += kThreads) {
+      sh.bin.n[i] = 0;
+      sh.bin.w[i] = 0;
     }
-    return prefix << 16;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kCells; ++i)
+      if (cell[i] != kNegInf) atomicAdd(&sh.bin.n[bin(cell[i])], 1u);
+    walk_bins<kCellBins>(0, 0, k, ~0ull);
+    const int b = sh.found;
+    __syncthreads();
+    if (b < 0) return 0;  // fewer cells than k
+    return order_key(low + (float)b / scale - 1e-6f * (fabsf(low) + fabsf(m)));
   }
 
   // Lists the cells whose maximum reaches the bound; whether few enough are listed.
-  __device__ __forceinline__ bool list_cells(const __amdgpu_buffer_rsrc_t& rc, uint32_t floor) {
+  __device__ __forceinline__ bool list_cells(uint32_t floor) {
     if (tid == 0) sh.count = 0;
     __syncthreads();
-    for (int base = 0; base < a.cells; base += kThreads * 4) {  // uniform
-      const int c0 = base + tid * 4;
-      const f32x4 y = tiles::load_coherent16(rc, c0 * 4);
-      bool in[4];
-      int mine = 0;
+    unsigned in = 0;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) mine += in[i] = c0 + i < a.cells && order_key(y[i]) >= floor;
-      const int incl = tiles::wave_incl_scan(mine);
-      int at = 0;
-      if (lane == 63 && incl) at = atomicAdd(&sh.count, incl);
-      at = __builtin_amdgcn_readlane(at, 63) + incl - mine;
+    for (int i = 0; i < kCells; ++i) in |= (unsigned)(order_key(cell[i]) >= floor) << i;
+    const int mine = __builtin_popcount(in);
+    const int incl = tiles::wave_incl_scan(mine);
+    int at = 0;
+    if (lane == 63 && incl) at = atomicAdd(&sh.count, incl);
+    at = __builtin_amdgcn_readlane(at, 63) + incl - mine;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (in[i]) sh.cells[at++] = (uint16_t)(c0 + i);
-    }
+    for (int i = 0; i < kCells; ++i)
+      if (in >> i & 1) sh.cells[at++] = (uint16_t)cell_of(i);
     __syncthreads();
     const int n = sh.count;
     __syncthreads();
@@ -636,7 +613,7 @@ struct Decider {
         const uint32_t key = sh.key[i];
         if (shift == 24 || key >> (shift + 8) == prefix) {
           atomicAdd(&sh.bin.n[key >> shift & 255], 1u);
-          atomicAdd(&sh.bin.w[key >> shift & 255], units(sc.weight(of_key(key))));
+          atomicAdd(&sh.bin.w[key >> shift & 255], units1(sc.weight(of_key(key))));
         }
       }
       walk_bins<256>(c.above, c.above_w, k, aim);
@@ -657,13 +634,14 @@ struct Decider {
 
   // The same for at most kShort listed entries, by their places in the order; `last` too.
   __device__ __forceinline__ void cut_brief(Cut& c, int k, u64 aim, int& last) {
-    const int e = tid & (kShort - 1);
+    const int e = entry_of(c.n);
     u64 order = 0, w = 0;
     if (e < c.n) {
       order = (u64)sh.key[e] << 32 | (uint32_t)~sh.idx[e];
-      w = units(sc.weight(of_key(sh.key[e])));
+      w = units1(sc.weight(of_key(sh.key[e])));
     }
-    if (tid < kShort) sh.brief.entry[e] = ulonglong2{order, w};
+    __syncthreads();  // (the bins are spent)
+    if (e == tid) sh.brief.entry[e] = ulonglong2{order, w};
     if (tid == 0) sh.count = -1;
     __syncthreads();
     const u64 first = places(c.n, order);
@@ -727,7 +705,7 @@ struct Decider {
           if (first ? key >= c.range.floor : c.range.place(x[i], key) == 1) {
             const int b = first ? c.range.bin_of(x[i]) : (int)((key >> low) & ((1u << bits) - 1));
             atomicAdd(&sh.bin.n[b], 1u);
-            atomicAdd(&sh.bin.w[b], units(sc.weight(x[i])));
+            atomicAdd(&sh.bin.w[b], units1(sc.weight(x[i])));
           }
         }
       });
@@ -767,7 +745,7 @@ struct Decider {
   __device__ __forceinline__ void finish(Cut& c, int k, u64 aim) {
     int t = c.all;
     if (k > 0) t = min(t, k - c.above);
-    const u64 w = units(sc.weight(of_key(c.key)));
+    const u64 w = units1(sc.weight(of_key(c.key)));
     if (aim != ~0ull && w > 0) {
       const u64 need = aim > c.above_w ? (aim - c.above_w + w - 1) / w : 0;
       if (need < (u64)t) t = (int)need;
@@ -841,9 +819,10 @@ struct Decider {
   // Weight of a kept entry, or 0.
   __device__ __forceinline__ u64 kept_units(float z, int v, uint32_t key_above, int last) const {
     const uint32_t key = order_key(z);
-    if (key <= kDead || key < key_above || (key == key_above && v > last)) return 0;
     const double w = sc.weight(z);
-    return w >= (double)s.min_p ? units(w) : 0;
+    const unsigned kept = (unsigned)(key > kDead) & (unsigned)(w >= (double)s.min_p) &
+                          ((unsigned)(key > key_above) | ((unsigned)(key == key_above) & (unsigned)(v <= last)));
+    return units1(w) & (0 - (u64)kept);
   }
 
   // The first index whose cumulative kept weight exceeds u times the sum, of the pieces'
@@ -936,16 +915,12 @@ struct Decider {
   }
 
   // The first of the largest logits: of the first cell whose maximum is the row's.
-  __device__ __forceinline__ void first_of_largest(int r, const __amdgpu_buffer_rsrc_t& rc) {
+  __device__ __forceinline__ void first_of_largest(int r) {
     const uint32_t top = order_key(m);
     int c = 0x7fffffff;
-    for (int base = 0; base < a.cells; base += kThreads * 4) {  // uniform
-      const int c0 = base + tid * 4;
-      const f32x4 y = tiles::load_coherent16(rc, c0 * 4);
 #pragma unroll
-      for (int i = 3; i >= 0; --i)
-        if (c0 + i < a.cells && order_key(y[i]) == top) c = min(c, c0 + i);
-    }
+    for (int i = 0; i < kCells; ++i)
+      if (order_key(cell[i]) == top) c = min(c, cell_of(i));
     if (tid == 0) sh.found = 0x7fffffff;
     __syncthreads();
     if (c != 0x7fffffff) atomicMin(&sh.found, c);
@@ -1019,7 +994,7 @@ struct Decider {
   // Weight of the entries up to a cut.
   __device__ __forceinline__ u64 weight_to(const Cut& c) {
     if (c.ties < 0) return c.above_w + everything(c.n);
-    return c.above_w + (u64)c.ties * units(sc.weight(of_key(c.key)));
+    return c.above_w + (u64)c.ties * units1(sc.weight(of_key(c.key)));
   }
 
   __device__ __forceinline__ void decide(int r) {
@@ -1031,6 +1006,7 @@ struct Decider {
     // Each thread its piece; maximum and sum of all.
     static_assert(kMaxPieces == kThreads, "one piece per thread");
     const f32x4 y = tiles::load_coherent16(rp, tid * 16);
+    load_cells(rc);
     typedef double f64x2 __attribute__((ext_vector_type(2)));
     const float pm = tid < a.pieces ? y[0] : kNegInf;
     const double ps = tid < a.pieces ? __builtin_bit_cast(f64x2, y)[1] : 0.0;
@@ -1040,7 +1016,7 @@ struct Decider {
       return;
     }
     if (s.k == 1) {
-      first_of_largest(r, rc);
+      first_of_largest(r);
       return;
     }
     u64 whole = 0;
@@ -1061,14 +1037,14 @@ struct Decider {
     }
     uint32_t floor = lowest;
     if (s.k > 0)
-      floor = cell_bound(rc, s.k);
+      floor = cell_bound(s.k);
     else if (s.p < 1.f)
       floor = floor_of((1.0 - (double)s.p) * ((double)whole / kUnit) / a.vocab);
     if (s.min_p > 0.f && (s.k == 0 || s.p == 1.f)) floor = max(floor, floor_of((double)s.min_p));
     floor = max(floor, lowest);
     // (Where most cells of a long row reach the bound, its entries are not even counted here:
     // they are nearly always too many, and one workgroup takes 25 us for 150,000.)
-    const bool few = list_cells(rc, floor);
+    const bool few = list_cells(floor);
     if (!few) listed_cells = -1;
     const int n = few || a.pieces <= kAlonePieces || r >= a.shared_rows
                       ? list_entries(Range{floor, 0.f, 0.f, 0, 0, 0}) : kList + 1;
@@ -1078,32 +1054,7 @@ struct Decider {
     }
     const bool limited = s.k > 0 || s.p < 1.f;  // (with min-p alone, only the weights decide)
     if (n > kList) {
-      // Shared by several workgroups in the next launches. Top-k and top-p together would take
-      // two cuts, and areas may have run out: then by one alone.
-      Cut c{};
-      c.range.floor = floor;
-      lay_bins(c.range);
-      const bool counted = c.range.scale > 0.f && !(s.k > 0 && s.p < 1.f);
-      const int mode = r >= a.shared_rows || (limited && !counted) ? kAlone
-                       : limited ? kCount : kKeepAll;
-      if (mode == kCount) {
-        Area& area = a.areas[r];
-        for (int i = tid; i < kBins; i += kThreads) {
-          area.bin.w[i] = 0;
-          area.bin.n[i] = 0;
-        }
-      }
-      if (tid == 0) {
-        Shared_row x{};
-        x.mode = mode;
-        x.max = m;
-        x.floor = floor;
-        x.lo = c.range.lo;
-        x.scale = c.range.scale;
-        x.aim = s.p < 1.f ? (u64)ceil((double)s.p * (double)whole) : ~0ull;
-        x.whole = whole;
-        *state = x;
-      }
+      share_or_not(r, floor, whole, limited, state);
       return;
     }
     uint32_t key = floor;
@@ -1126,188 +1077,251 @@ struct Decider {
     conclude(r, key, last, true, n);
   }
 
-  // ---- a row shared by workgroups: the launch that counts, and the one that ends it ----
+  // ---- a row shared by workgroups ----
 
-  __device__ __forceinline__ static Range range_of(const Shared_row& x) {
-    return Range{x.floor, x.lo, x.scale, x.bin, 0, 0};
+  // Who does a row whose list does not fit: several workgroups, or one in the next launch. Top-k
+  // and top-p together would take two cuts; lists may have run out; and the intervals have to
+  // be wider than the slack of the bound for min-p.
+  __device__ __forceinline__ void share_or_not(int r, uint32_t floor, u64 whole, bool limited,
+                                               Shared_row* state) {
+    Range range{floor, 0.f, 0.f, 0, 0, 0};
+    lay_bins(range);
+    const bool fine = range.scale > 0.f &&
+                      (s.min_p == 0.f || m - range.lo > 0.0164f * (fabsf(m) + fabsf(range.lo)));
+    const int mode = r >= a.shared_rows ? kAlone
+                     : !limited         ? kKeepAll
+                     : fine && !(s.k > 0 && s.p < 1.f) ? kCount : kAlone;
+    if (mode == kCount) {
+      for (int i = tid; i < kBins; i += kThreads) room_of(r)[i] = 0;
+    }
+    if (tid == 0) {
+      Shared_row x{};
+      x.mode = mode;
+      x.max = m;
+      x.floor = floor;
+      x.lo = range.lo;
+      x.scale = range.scale;
+      x.end = kBins;
+      x.aim = s.p < 1.f ? (u64)ceil((double)s.p * (double)whole) : ~0ull;
+      x.whole = whole;
+      *state = x;
+    }
   }
 
-  // f(x, v0) for this workgroup's pieces, with the piece's number, by whole wavefronts.
+  __device__ __forceinline__ u64* room_of(int r) const { return a.rooms + (int64_t)r * kRoom; }
+
+  // f(p, x, v0) for this workgroup's pieces, by whole wavefronts: piece p's entries, from v0 on,
+  // the next piece's on their way.
   template <typename F>
   __device__ __forceinline__ void each_piece(int group, F f) {
     const int stride = a.shared_groups * kWaves;
-#pragma unroll 1
-    for (int p = group * kWaves + wave; p < a.pieces; p += stride) {  // wavefront-uniform
-      Eight<T> x[2];
-      int v0[2];
+    Eight<T> next[2];
+    int at[2];
+    auto take = [&](int p) __attribute__((always_inline)) {
 #pragma unroll
-      for (int j = 0; j < 2; ++j) v0[j] = x[j].load(row, p * kPiece + j * 512 + lane * 8, a.vocab);
+      for (int j = 0; j < 2; ++j) at[j] = next[j].load(row, p * kPiece + j * 512 + lane * 8, a.vocab);
+    };
+    int p = group * kWaves + wave;
+    if (p < a.pieces) take(p);
+#pragma unroll 1
+    for (; p < a.pieces; p += stride) {  // wavefront-uniform
+      const Eight<T> x[2] = {next[0], next[1]};
+      const int v0[2] = {at[0], at[1]};
+      if (p + stride < a.pieces) take(p + stride);
       f(p, x, v0);
     }
   }
 
-  // Counts (with top-k) or weights (with top-p) per interval into the row's bins.
+  // This workgroup's pieces into the row's counts (of 2^40) and places (of 2^-16 interval).
   __device__ __forceinline__ void count(int r, int group, const Shared_row& state) {
-    for (int i = tid; i < kBins; i += kThreads) {
-      sh.bin.n[i] = 0;
-      sh.bin.w[i] = 0;
-    }
+    for (int i = tid; i < kBins; i += kThreads) sh.bin.w[i] = 0;
     __syncthreads();
-    const Range range = range_of(state);
+    const float lowest = of_key(state.floor), lo = state.lo, scale = state.scale;
     each_piece(group, [&](int, const Eight<T> (&x)[2], const int (&)[2]) __attribute__((always_inline)) {
 #pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float z = x[j][i];
+          const float t = fmaxf((z - lo) * scale, 0.f);
+          const int b = min((int)t, kBins - 1);
+          const unsigned place = (unsigned)((t - (float)b) * 65536.f);
+          if (z >= lowest) atomicAdd(&sh.bin.w[b], (u64)place | 1ull << 40);
+        }
+    });
+    __syncthreads();
+    u64* const room = room_of(r);
+    for (int i = tid; i < kBins; i += kThreads) {
+      const u64 x = sh.bin.w[i];
+      if (x) __hip_atomic_fetch_add(room + i, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+  }
+
+  // Of all of them, the intervals that can hold the border: with top-k the one that does; with
+  // top-p, from the first that reaches aim by the upper bounds of the weights down to the first
+  // that does by the lower ones. (Ends and means are taken a thousandth of an interval further:
+  // the numbers that intervals go by are rounded. The first interval may hold entries below it.)
+  __device__ __forceinline__ void bracket(int r, Shared_row* state) {
+    const u64* const room = room_of(r);
+    constexpr int PER = kBins / kThreads;
+    u64 x[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      x[i] = __hip_atomic_load(room + i * kThreads + tid, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const double wide = 1.0 / (double)state->scale, lo = state->lo;
+    auto weight_at = [&](double t) {
+      return exp2_of(fmax((fmin(lo + t * wide, (double)m) - sc.m) * sc.c, sc.low));
+    };
+    const u64 aim = state->aim;
+    int ends[2];  // by the upper bounds, by the lower ones
+#pragma unroll 1
+    for (int lower = s.k > 0 ? 1 : 0; lower < 2; ++lower) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const int b = i * kThreads + tid;
+        const int n = (int)(x[i] >> 40);
+        double w = 0.0;
+        if (n > 0 && s.k == 0) {
+          const double mean = (double)(x[i] & 0xffffffffffull) / (65536.0 * n);
+          if (lower) {
+            w = b > 0 ? weight_at(b + mean - 1e-3) : 0.0;
+          } else {
+            const double w0 = weight_at(b - 1e-3), w1 = weight_at(b + 1.001);
+            w = w0 + (w1 - w0) * fmin((mean + 2e-3) / 1.002, 1.0);
+          }
+        }
+        sh.bin.n[b] = n;
+        sh.bin.w[b] = units((double)n * w);
+      }
+      walk_bins<kBins>(0, 0, s.k, aim);
+      ends[lower] = sh.found;
+      __syncthreads();
+    }
+    if (s.k > 0) ends[0] = ends[1];
+    if (tid == 0) {
+      state->mode = kShare;
+      state->first = max(ends[1], 0);
+      state->end = ends[0] < 0 ? 1 : ends[0] + 1;
+    }
+  }
+
+  // This workgroup's pieces: the weight above the bracket into the pieces' sums, what lies in it
+  // into the row's list.
+  __device__ __forceinline__ void share(int r, int group, Shared_row* state, Piece* pieces) {
+    const bool all = state->mode == kKeepAll;
+    const float lowest = of_key(state->floor), lo = state->lo, scale = state->scale;
+    const float from = state->first > 0 ? (float)state->first : kNegInf;
+    const float to = state->end < kBins ? (float)state->end : -kNegInf;
+    u64* const list = room_of(r);
+    each_piece(group, [&](int p, const Eight<T> (&x)[2], const int (&v0)[2]) __attribute__((always_inline)) {
+      unsigned in[2] = {0, 0};
+      int counts = 0;
+      double w = 0.0;
+#pragma unroll
       for (int j = 0; j < 2; ++j) {
-        if (s.k > 0) {
+        unsigned over = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float z = x[j][i], t = (z - lo) * scale;
+          const bool alive = z >= lowest;
+          const unsigned high = (unsigned)alive & ((unsigned)all | (unsigned)(t >= to));
+          over |= high << i;
+          in[j] |= ((unsigned)alive & (unsigned)(t >= from) & ~high) << i;  // (of `all`: none)
+        }
+        // (Without branches within: the entries' chains of dependent instructions overlap. Above
+        // the bracket every entry weighs min_p, too: see share_or_not.)
+        if (__ballot(over != 0) == 0) {
+        } else if (all) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            const float z = x[j][i];
-            if (order_key(z) >= range.floor) atomicAdd(&sh.bin.n[range.bin_of(z)], 1u);
+            const double y = sc.weight(x[j][i]);
+            w += over >> i & (unsigned)(y >= (double)s.min_p) & 1 ? y : 0.0;
           }
         } else {
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            const float z = x[j][i];
-            const u64 w = units(sc.weight(z));
-            if (order_key(z) >= range.floor) atomicAdd(&sh.bin.w[range.bin_of(z)], w);
-          }
-        }
-      }
-    });
-    __syncthreads();
-    Area& area = a.areas[r];
-    for (int i = tid; i < kBins; i += kThreads) {
-      if (s.k > 0) {
-        const uint32_t n = sh.bin.n[i];
-        if (n) __hip_atomic_fetch_add(&area.bin.n[i], n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      } else {
-        const u64 w = sh.bin.w[i];
-        if (w) __hip_atomic_fetch_add(&area.bin.w[i], w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      }
-    }
-  }
-
-  // All of the row's bins: the interval with the border.
-  __device__ __forceinline__ void find_bin(int r, Shared_row* state) {
-    Area& area = a.areas[r];
-    for (int i = tid; i < kBins; i += kThreads) {
-      const u64 w = __hip_atomic_load(&area.bin.w[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      const uint32_t n = __hip_atomic_load(&area.bin.n[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      sh.bin.w[i] = w;
-      sh.bin.n[i] = s.k > 0 ? n : w > 0;  // (how many weigh it is not counted: some)
-    }
-    walk_bins<kBins>(0, 0, s.k, state->aim);
-    if (tid == 0) {
-      state->mode = sh.found < 0 ? kKeepAll : kCollect;
-      state->bin = sh.found;
-      state->above = sh.found2;
-      state->above_w = sh.found_w;
-    }
-  }
-
-  // The entries of the border's interval into the row's list, and what is kept above it into
-  // the pieces' sums.
-  __device__ __forceinline__ void collect(int r, int group, Shared_row* state, Piece* pieces) {
-    const bool all = state->mode == kKeepAll;
-    const Range range = all ? Range{state->floor, 0.f, 0.f, -1, 0, 0} : range_of(*state);
-    if (tid == 0) sh.count = 0;
-    __syncthreads();
-    each_piece(group, [&](int p, const Eight<T> (&x)[2], const int (&v0)[2]) __attribute__((always_inline)) {
-      u64 w = 0;
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        unsigned in = 0, over = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int at = range.place(x[j][i], order_key(x[j][i]));
-          in |= (unsigned)(at == 1) << i;
-          over |= (unsigned)(at == 2) << i;
-        }
-        if (__ballot(over != 0) != 0) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
             const double y = sc.weight(x[j][i]);
-            w += (over >> i & 1) && y >= (double)s.min_p ? units(y) : 0;
+            w += over >> i & 1 ? y : 0.0;
           }
         }
-        if (__ballot(in != 0) != 0) {
-          const int mine = __builtin_popcount(in);
-          const int incl = tiles::wave_incl_scan(mine);
-          int at = 0;
-          if (lane == 63) at = atomicAdd(&sh.count, incl);
-          at = __builtin_amdgcn_readlane(at, 63) + incl - mine;
+        counts += __builtin_popcount(in[j]);
+        if (s.k > 0) counts += __builtin_popcount(over) << 16;
+      }
+      if (__ballot(counts != 0) != 0) {
+        const int incl = tiles::wave_incl_scan(counts);  // (1024 of each at most)
+        const int total = __builtin_amdgcn_readlane(incl, 63);
+        int at = 0;
+        if (lane == 63)
+          at = (int)(uint32_t)__hip_atomic_fetch_add(
+              &state->counts, (u64)(total & 0xffff) | (u64)(total >> 16) << 32, __ATOMIC_RELAXED,
+              __HIP_MEMORY_SCOPE_AGENT);
+        at = __builtin_amdgcn_readlane(at, 63) + ((incl - counts) & 0xffff);
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
 #pragma unroll
           for (int i = 0; i < 8; ++i)
-            if (in >> i & 1) {
-              if (at < kList) {
-                sh.key[at] = order_key(x[j][i]);
-                sh.idx[at] = v0[j] + i;
-              }
+            if (in[j] >> i & 1) {
+              if (at < kList)
+                __hip_atomic_store(list + at, (u64)order_key(x[j][i]) << 32 | (uint32_t)(v0[j] + i),
+                                   __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
               ++at;
             }
-        }
       }
       w = wave_sum(w);
       if (lane == 0)
-        __hip_atomic_store(reinterpret_cast<u64*>(&pieces[p].sum), w, __ATOMIC_RELAXED,
+        __hip_atomic_store(reinterpret_cast<u64*>(&pieces[p].sum), units(w), __ATOMIC_RELAXED,
                            __HIP_MEMORY_SCOPE_AGENT);
     });
-    __syncthreads();
-    const int n = sh.count;
-    if (n > 0) {  // uniform
-      if (tid == 0)
-        sh.found = __hip_atomic_fetch_add(&state->listed, n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      __syncthreads();
-      Area& area = a.areas[r];
-      for (int i = tid; i < min(n, kList - sh.found); i += kThreads) {
-        __hip_atomic_store(&area.list.key[sh.found + i], sh.key[i], __ATOMIC_RELAXED,
-                           __HIP_MEMORY_SCOPE_AGENT);
-        __hip_atomic_store(&area.list.idx[sh.found + i], sh.idx[i], __ATOMIC_RELAXED,
-                           __HIP_MEMORY_SCOPE_AGENT);
-      }
-    }
   }
 
   // The end of a shared row, of all workgroups' lists and sums.
   __device__ __forceinline__ void end(int r, Shared_row* state, Piece* pieces) {
-    const bool all = state->mode == kKeepAll;
-    Cut c{};
-    c.range = range_of(*state);
-    c.above = state->above;
-    c.above_w = state->above_w;
-    keep_all(c);
-    int last = 0x7fffffff;
-    if (!all) {
-      c.n = __hip_atomic_load(&state->listed, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      if (c.n > kList) {  // many equal logits, or nearly
-        alone(r, state->floor, state->whole);
-        return;
-      }
-      const Area& area = a.areas[r];
-      for (int i = tid; i < c.n; i += kThreads) {
-        sh.key[i] = __hip_atomic_load(&area.list.key[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        sh.idx[i] = __hip_atomic_load(&area.list.idx[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      }
-      __syncthreads();
-      if (c.n <= kShort) {
-        cut_brief(c, s.k, state->aim, last);
-      } else {
-        cut_list(c, s.k, state->aim);
-        last = last_tie(c);
-      }
-    }
     sh.psum[tid] = tid < a.pieces
                        ? __hip_atomic_load(reinterpret_cast<const u64*>(&pieces[tid].sum),
                                            __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)
                        : 0;
-    __syncthreads();
-    if (!all) add_listed(c.key, last, c.n);
+    Cut c{};
+    c.range.floor = state->floor;
+    keep_all(c);
+    int last = 0x7fffffff;
+    if (state->mode == kShare) {
+      const u64 counts = __hip_atomic_load(&state->counts, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      const u64 aim = state->aim;
+      const u64* const list = room_of(r);
+      c.n = (int)min(counts & 0xffffffffu, (u64)0x7fffffff);
+      for (int i = tid; i < min(c.n, kList); i += kThreads) {
+        const u64 x = __hip_atomic_load(list + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        sh.key[i] = (uint32_t)(x >> 32);
+        sh.idx[i] = (int)(uint32_t)x;
+      }
+      c.above = (int)(counts >> 32);
+      c.above_w = block_sum(sh.psum[tid]);
+      bool fits = c.n <= kList;
+      if (fits) {  // and the border is in the bracket, as it should be
+        const u64 w = everything(c.n);
+        fits = s.k > 0 ? c.above < s.k && (c.above + c.n >= s.k || state->first == 0)
+                       : c.above_w < aim && (c.above_w + w >= aim || state->first == 0);
+      }
+      if (!fits) {
+        alone(r, state->floor, state->whole);
+        return;
+      }
+      if (c.above_w > 0 && c.above == 0) c.above = 1;  // (not counted: some)
+      if (c.n <= kShort) {
+        cut_brief(c, s.k, aim, last);
+      } else {
+        cut_list(c, s.k, aim);
+        last = last_tie(c);
+      }
+      add_listed(c.key, last, c.n);
+    }
     sum_up(r, c.key, last);
   }
 
   // Weight of all listed entries.
   __device__ __forceinline__ u64 everything(int n) {
     u64 w = 0;
-    for (int i = tid; i < n; i += kThreads) w += units(sc.weight(of_key(sh.key[i])));
+    for (int i = tid; i < n; i += kThreads) w += units1(sc.weight(of_key(sh.key[i])));
     return block_sum(w);
   }
 
@@ -1324,42 +1338,51 @@ struct Decider {
       sh.key[tid] = out ? kDead : order_key(z);
       sh.idx[tid] = tid;
     }
-    const u64 whole = block_sum(out ? 0 : units(sc.weight(z)));
+    const u64 whole = block_sum(out ? 0 : units1(sc.weight(z)));
     brief(r, a.vocab, whole);
   }
 
-  // The sum over the n entries in sh.brief of what f makes of each, for entry tid % kShort: half
-  // by thread tid of the first kShort, which get it, half by its partner.
+  // Which entry of n in sh.brief is this thread's: of up to kShort / 2, thread e + kShort / 2 is
+  // entry e's partner.
+  __device__ __forceinline__ int entry_of(int n) const {
+    return n <= kShort / 2 ? tid & (kShort / 2 - 1) : tid;
+  }
+  // The sum over the n entries in sh.brief of what f makes of each, for the thread's entry; of a
+  // pair the first thread gets it.
   template <typename F>
   __device__ __forceinline__ u64 over_brief(int n, F f) {
-    static_assert(kThreads == 2 * kShort, "two threads per entry");
-    const int half = (n + 15) / 16 * 8;  // (behind the n there are entries that add nothing)
-    const int from = tid < kShort ? 0 : half;
+    static_assert(kThreads == kShort, "a thread per entry, or two");
+    const bool pairs = n <= kShort / 2;
+    // (Behind the n there are entries that add nothing, up to a multiple of 16.)
+    const int per = pairs ? (n + 15) / 16 * 8 : (n + 7) / 8 * 8;
+    const int from = pairs && tid >= kShort / 2 ? per : 0;
     u64 x = 0;
-    if ((tid & (kShort - 1)) < ((n + 63) & ~63)) {  // wavefront-uniform
+    if (entry_of(n) < ((n + 63) & ~63)) {  // wavefront-uniform
 #pragma unroll 1
-      for (int i = from; i < from + half; i += 8)
+      for (int i = from; i < from + per; i += 8)
 #pragma unroll
         for (int j = 0; j < 8; ++j) x += f(sh.brief.entry[i + j]);
     }
-    if (tid >= kShort) sh.brief.more[tid - kShort] = x;
-    __syncthreads();
-    if (tid < kShort) x += sh.brief.more[tid];
+    if (pairs) {  // uniform
+      if (tid >= kShort / 2) sh.brief.more[tid - kShort / 2] = x;
+      __syncthreads();
+      if (tid < kShort / 2) x += sh.brief.more[tid];
+    }
     return x;
   }
 
   // How many of the entries in sh.brief come before `order`, times 2^53, and their weight.
-  // (Weights of 2^44 at most: 256 of them leave room for their number in the same sum.)
+  // (Weights of 2^44 at most: 512 of them leave room for their number in the same sum.)
   __device__ __forceinline__ u64 places(int n, u64 order) {
     return over_brief(n, [&](ulonglong2 x) __attribute__((always_inline)) {
       return x.x > order ? x.y + (1ull << 53) : 0;
     });
   }
 
-  // The end for at most kShort listed entries, one per thread of the first half: every entry's
+  // The end for at most kShort listed entries, one per thread: every entry's
   // place in the order and the weight before it.
   __device__ __forceinline__ void brief(int r, int n, u64 whole) {
-    const int e = tid & (kShort - 1);
+    const int e = entry_of(n);
     u64 order = 0, w = 0;
     uint32_t key = 0;
     int v = 0;
@@ -1367,9 +1390,9 @@ struct Decider {
       key = sh.key[e];
       v = sh.idx[e];
       order = (u64)key << 32 | (uint32_t)~v;
-      w = units(sc.weight(of_key(key)));
+      w = units1(sc.weight(of_key(key)));
     }
-    if (tid < kShort) sh.brief.entry[e] = ulonglong2{order, w};
+    if (e == tid) sh.brief.entry[e] = ulonglong2{order, w};
     __syncthreads();
     const u64 first = places(n, order);
     const int rank = (int)(first >> 53);
@@ -1398,7 +1421,7 @@ struct Decider {
       return;
     }
     // By the index now. (All have left the first walk behind block_sum's barriers.)
-    if (tid < kShort) sh.brief.entry[e] = ulonglong2{(u64)v, kept ? w : 0};
+    if (e == tid) sh.brief.entry[e] = ulonglong2{(u64)v, kept ? w : 0};
     if (tid == 0) sh.found = sh.found2 = -1;
     __syncthreads();
     const u64 run = over_brief(n, [&](ulonglong2 x) __attribute__((always_inline)) {
@@ -1517,8 +1540,8 @@ __global__ __launch_bounds__(kThreads, 4) void sample_kernel(Args a) {
   if (arrive_last(a, r, a.groups, tid, s_last)) d.decide(r);
 }
 
-// The launches that share a row whose list does not fit: END false, counts and weights per
-// interval; END true, the list of the border's interval and the end.
+// The launches that share a row whose list does not fit: END false, its counts per interval;
+// END true, the bracket's list and the end.
 template <typename T, bool END>
 __global__ __launch_bounds__(kThreads, 4) void shared_kernel(Args a) {
   __shared__ Shared sh;
@@ -1530,22 +1553,21 @@ __global__ __launch_bounds__(kThreads, 4) void shared_kernel(Args a) {
   char* const rec = a.records + (int64_t)r * a.row_bytes;
   Shared_row* const state = reinterpret_cast<Shared_row*>(rec + sizeof(Decision));
   Piece* const pieces = reinterpret_cast<Piece*>(rec + kHead);
-  const int mode = state->mode;  // (written by an earlier launch; END leaves it)
+  const int mode = state->mode;  // (an earlier launch's; the last of the counting ones changes it)
   if (END ? mode == kDecided : mode != kCount) return;
   const int seq = r / a.each;
-  const typename T::E* row = row_of<T>(a, r, seq);
-  Decider<T> d(a, sh, row, settings_of(a, seq), tid, lane, wave);
+  Decider<T> d(a, sh, row_of<T>(a, r, seq), settings_of(a, seq), tid, lane, wave);
   d.set_max(state->max);
-  if constexpr (END) {
+  if constexpr (!END) {
+    d.count(r, group, *state);
+    if (arrive_last(a, r, a.shared_groups, tid, s_last)) d.bracket(r, state);
+  } else {
     if (mode == kAlone) {
       if (group == 0) d.alone(r, state->floor, state->whole);
       return;
     }
-    d.collect(r, group, state, pieces);
+    d.share(r, group, state, pieces);
     if (arrive_last(a, r, a.shared_groups, tid, s_last)) d.end(r, state, pieces);
-  } else {
-    d.count(r, group, *state);
-    if (arrive_last(a, r, a.shared_groups, tid, s_last)) d.find_bin(r, state);
   }
 }
 
@@ -1616,8 +1638,6 @@ static int cells_of(int vocab) { return (vocab + kCell - 1) / kCell; }
 // Workgroups per row: one wavefront per piece for a few rows; for many, as many as fill
 // kWavesPerCu wavefronts per compute unit over all rows, the pieces dealt in whole rounds.
 constexpr int kWavesPerCu = 16;
-// Wavefronts that share a row of a long list, at most.
-constexpr int kSharedWaves = 80;
 static int groups_of(int rows, int pieces) {
   int64_t waves = (int64_t)kWavesPerCu * device_cus() / rows;
   if (waves < 1) waves = 1;
@@ -1649,6 +1669,14 @@ static hipError_t launch(const Args& a, hipStream_t stream) {
   return hipGetLastError();
 }
 
+// Workgroups that share a row of a long list: as above for kSharedWavesPerCu, since not every
+// row of many has one.
+constexpr int kSharedWavesPerCu = 32;
+static int shared_groups_of(int rows, int pieces) {
+  const int64_t waves = (int64_t)kSharedWavesPerCu * device_cus() / rows;
+  const int64_t groups = ((waves < pieces ? waves : pieces) + kWaves - 1) / kWaves;
+  return groups < 1 ? 1 : (int)groups;
+}
 static int shared_rows_of(int rows, int vocab) {
   return vocab <= kList ? 0 : rows < kMaxShared ? rows : kMaxShared;
 }
@@ -1674,7 +1702,7 @@ size_t pa_sample_workspace_bytes(int num_seqs, int rows_per_seq, int vocab) {
   const int64_t rows = (int64_t)num_seqs * rows_per_seq;
   if (num_seqs <= 0 || rows_per_seq <= 0 || rows > kMaxRows || vocab <= 0 || vocab > kMaxVocab) return 0;
   return kCounterBytes + (size_t)rows * row_record(pieces_of(vocab), cells_of(vocab)) +
-         (size_t)shared_rows_of((int)rows, vocab) * sizeof(Area);
+         (size_t)shared_rows_of((int)rows, vocab) * kRoom * sizeof(u64);
 }
 
 static int start(Args& a, const void* logits, int dtype, const int64_t* strides, int num_seqs,
@@ -1735,9 +1763,9 @@ static int start(Args& a, const void* logits, int dtype, const int64_t* strides,
   a.row_bytes = row_record(a.pieces, a.cells);
   a.cnt = (int*)workspace;
   a.records = (char*)workspace + kCounterBytes;
-  a.areas = (Area*)(a.records + (size_t)a.rows * a.row_bytes);
+  a.rooms = (u64*)(a.records + (size_t)a.rows * a.row_bytes);
   a.shared_rows = shared_rows_of(a.rows, vocab);
-  a.shared_groups = a.pieces < kSharedWaves ? (a.pieces + kWaves - 1) / kWaves : kSharedWaves / kWaves;
+  a.shared_groups = shared_groups_of(a.rows, a.pieces);
   return PA_OK;
 }
 
