@@ -76,12 +76,11 @@ struct Piece {
 // A row whose list does not fit, between the launches.
 enum { kDecided = 0, kCount = 1, kShare = 2, kKeepAll = 3, kAlone = 4 };
 struct alignas(16) Shared_row {
-  int mode;
   float max;
   uint32_t floor;     // keys below are out of the question
   float lo, scale;    // the intervals of the logits' line,
   int first, end;     // and those of the bracket
-  int pad;
+  int pad[2];
   u64 counts;         // entries in the bracket (listed), and 2^32 times those above it
   u64 aim, whole;
 };
@@ -101,10 +100,11 @@ struct Args {
   int64_t* tokens;
   float* probs;
   int* cnt;
+  int* modes;     // per row: of the Shared_row
   char* records;  // per row: Decision, Shared_row, pieces, cells
   u64* rooms;     // of the first `shared_rows` rows: kBins counts and places, then kList keys and indexes
   int row_bytes, pieces, cells, groups;
-  int shared_rows, shared_groups;
+  int shared_rows, shared_groups, shared_wgs;
 };
 
 constexpr int kHead = sizeof(Decision) + sizeof(Shared_row);
@@ -151,6 +151,7 @@ struct Eight {
     return at;
   }
   __device__ __forceinline__ float operator[](int i) const { return fmaxf(T::get(w[i]), kNegInf); }
+  __device__ __forceinline__ float raw(int i) const { return T::get(w[i]); }  // NaN as it is
 };
 
 // Unsigned numbers in the logits' order; both zeros are one.
@@ -165,23 +166,41 @@ __device__ inline float of_key(uint32_t k) {
 // 2^d for -1000 <= d <= 0, to 2^-45 relative: the whole part, by an addition that leaves it in
 // the low bits, goes to the exponent; the rest by the polynomial through 2^f at the ten Chebyshev
 // nodes of [-1/2, 1/2], its constant rounded to 1: the largest weighs exactly that.
-__device__ inline double exp2_of(double d) {
+// N of them step by step, so that their chains of dependent instructions overlap (one after
+// the other, as the compiler orders them by itself, the pass over flat rows below took 100 us
+// where it takes 94).
+template <int N>
+__device__ inline void exp2_of(double (&d)[N]) {
   constexpr double kWhole = 6755399441055744.0;  // 1.5 * 2^52
-  const double t = d + kWhole;
-  const double f = d - (t - kWhole);
-  double p = 1.0212097549811005e-07;
-  p = __builtin_fma(p, f, 1.3259945262689143e-06);
-  p = __builtin_fma(p, f, 1.5252640059770786e-05);
-  p = __builtin_fma(p, f, 0.00015403432339553542);
-  p = __builtin_fma(p, f, 0.001333355825801874);
-  p = __builtin_fma(p, f, 0.009618129195951041);
-  p = __builtin_fma(p, f, 0.05550410866428854);
-  p = __builtin_fma(p, f, 0.24022650695631514);
-  p = __builtin_fma(p, f, 0.6931471805599526);
-  p = __builtin_fma(p, f, 1.0);
-  uint2 b = __builtin_bit_cast(uint2, p);
-  b.y += __builtin_bit_cast(uint2, t).x << 20;
-  return __builtin_bit_cast(double, b);
+  constexpr double kC[9] = {1.3259945262689143e-06, 1.5252640059770786e-05, 0.00015403432339553542,
+                            0.001333355825801874,   0.009618129195951041,   0.05550410866428854,
+                            0.24022650695631514,    0.6931471805599526,     1.0};
+  int n[N];
+  double p[N];
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    const double t = d[e] + kWhole;
+    n[e] = (int)__builtin_bit_cast(uint2, t).x;
+    d[e] -= t - kWhole;
+    p[e] = 1.0212097549811005e-07;
+  }
+#pragma unroll
+  for (int i = 0; i < 9; ++i) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) p[e] = __builtin_fma(p[e], d[e], kC[i]);
+    if constexpr (N > 1) __builtin_amdgcn_sched_barrier(0);
+  }
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    uint2 b = __builtin_bit_cast(uint2, p[e]);
+    asm("v_lshl_add_u32 %0, %1, 20, %0" : "+v"(b.y) : "v"(n[e]));  // (the 64-bit sum takes five)
+    d[e] = __builtin_bit_cast(double, b);
+  }
+}
+__device__ inline double exp2_of(double d) {
+  double x[1] = {d};
+  exp2_of(x);
+  return x[0];
 }
 
 // The weight of z next to a maximum m: 2^(c (z - m)), c = log2(e) / T; as good as 0 from 2^-1000
@@ -198,6 +217,12 @@ struct Scale {
     low = top_only ? 0.0 : -1000.0;
   }
   __device__ double weight(float z) const { return exp2_of(fmax(((double)z - m) * c, low)); }
+  template <int N>
+  __device__ void weights(const float (&z)[N], double (&w)[N]) const {
+#pragma unroll
+    for (int e = 0; e < N; ++e) w[e] = fmax(((double)z[e] - m) * c, low);
+    exp2_of(w);
+  }
 };
 __device__ inline u64 units(double w) { return (u64)(w * kUnit + 0.5); }
 // The same for w up to 1, by an addition that leaves the rounded number in the low bits.
@@ -1002,7 +1027,7 @@ struct Decider {
     Shared_row* const state = reinterpret_cast<Shared_row*>(rec + sizeof(Decision));
     const auto rp = tiles::tile_rsrc(rec + kHead, a.pieces * (int)sizeof(Piece));
     const auto rc = tiles::tile_rsrc(rec + kHead + a.pieces * sizeof(Piece), (a.cells + 3) / 4 * 16);
-    if (tid == 0) state->mode = kDecided;  // (unless the row is shared, below)
+    if (tid == 0) a.modes[r] = kDecided;  // (unless the row is shared, below)
     // Each thread its piece; maximum and sum of all.
     static_assert(kMaxPieces == kThreads, "one piece per thread");
     const f32x4 y = tiles::load_coherent16(rp, tid * 16);
@@ -1096,7 +1121,7 @@ struct Decider {
     }
     if (tid == 0) {
       Shared_row x{};
-      x.mode = mode;
+      a.modes[r] = mode;
       x.max = m;
       x.floor = floor;
       x.lo = range.lo;
@@ -1112,9 +1137,10 @@ struct Decider {
 
   // f(p, x, v0) for this workgroup's pieces, by whole wavefronts: piece p's entries, from v0 on,
   // the next piece's on their way.
+  int groups = 1;  // workgroups that share the row
   template <typename F>
   __device__ __forceinline__ void each_piece(int group, F f) {
-    const int stride = a.shared_groups * kWaves;
+    const int stride = groups * kWaves;
     Eight<T> next[2];
     int at[2];
     auto take = [&](int p) __attribute__((always_inline)) {
@@ -1199,7 +1225,7 @@ struct Decider {
     }
     if (s.k > 0) ends[0] = ends[1];
     if (tid == 0) {
-      state->mode = kShare;
+      a.modes[r] = kShare;
       state->first = max(ends[1], 0);
       state->end = ends[0] < 0 ? 1 : ends[0] + 1;
     }
@@ -1207,47 +1233,59 @@ struct Decider {
 
   // This workgroup's pieces: the weight above the bracket into the pieces' sums, what lies in it
   // into the row's list.
-  __device__ __forceinline__ void share(int r, int group, Shared_row* state, Piece* pieces) {
-    const bool all = state->mode == kKeepAll;
+  __device__ __forceinline__ void share(int r, int group, bool all, Shared_row* state, Piece* pieces) {
     const float lowest = of_key(state->floor), lo = state->lo, scale = state->scale;
     const float from = state->first > 0 ? (float)state->first : kNegInf;
     const float to = state->end < kBins ? (float)state->end : -kNegInf;
     u64* const list = room_of(r);
     each_piece(group, [&](int p, const Eight<T> (&x)[2], const int (&v0)[2]) __attribute__((always_inline)) {
-      unsigned in[2] = {0, 0};
-      int counts = 0;
       double w = 0.0;
+      uint64_t any = 0;  // lanes with an entry in the bracket (or with top-k above it)
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        unsigned over = 0;
+        // (Without branches around an entry: their chains of dependent instructions overlap. What
+        // is no number compares as neither.)
+        float z[8];
+        double y[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) z[i] = x[j].raw(i);
+        if (all) {
+          sc.weights(z, y);
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            w += (unsigned)(z[i] >= lowest) & (unsigned)(y[i] >= (double)s.min_p) ? y[i] : 0.0;
+          continue;
+        }
+        uint64_t over = 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float z = x[j][i], t = (z - lo) * scale;
-          const bool alive = z >= lowest;
-          const unsigned high = (unsigned)alive & ((unsigned)all | (unsigned)(t >= to));
-          over |= high << i;
-          in[j] |= ((unsigned)alive & (unsigned)(t >= from) & ~high) << i;  // (of `all`: none)
+          const float t = (z[i] - lo) * scale;
+          const uint64_t high = __ballot(t >= to), low = __ballot(t >= from);
+          over |= high;
+          any |= (s.k > 0 ? low : low & ~high) & __ballot(z[i] >= lowest);
         }
-        // (Without branches within: the entries' chains of dependent instructions overlap. Above
-        // the bracket every entry weighs min_p, too: see share_or_not.)
-        if (__ballot(over != 0) == 0) {
-        } else if (all) {
+        if (over != 0) {  // (above the bracket every entry weighs min_p, too: see share_or_not)
+          sc.weights(z, y);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const double y = sc.weight(x[j][i]);
-            w += over >> i & (unsigned)(y >= (double)s.min_p) & 1 ? y : 0.0;
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const double y = sc.weight(x[j][i]);
-            w += over >> i & 1 ? y : 0.0;
-          }
+          for (int i = 0; i < 8; ++i) w += (z[i] - lo) * scale >= to ? y[i] : 0.0;
         }
-        counts += __builtin_popcount(in[j]);
-        if (s.k > 0) counts += __builtin_popcount(over) << 16;
       }
-      if (__ballot(counts != 0) != 0) {
+      if (any != 0) {
+        unsigned in[2] = {0, 0};
+        int counts = 0;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          unsigned over = 0;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float z = x[j].raw(i), t = (z - lo) * scale;
+            const unsigned high = t >= to;
+            over |= high << i;
+            in[j] |= ((unsigned)(z >= lowest) & (unsigned)(t >= from) & ~high) << i;
+          }
+          counts += __builtin_popcount(in[j]);
+          if (s.k > 0) counts += __builtin_popcount(over) << 16;
+        }
         const int incl = tiles::wave_incl_scan(counts);  // (1024 of each at most)
         const int total = __builtin_amdgcn_readlane(incl, 63);
         int at = 0;
@@ -1275,7 +1313,7 @@ struct Decider {
   }
 
   // The end of a shared row, of all workgroups' lists and sums.
-  __device__ __forceinline__ void end(int r, Shared_row* state, Piece* pieces) {
+  __device__ __forceinline__ void end(int r, bool all, Shared_row* state, Piece* pieces) {
     sh.psum[tid] = tid < a.pieces
                        ? __hip_atomic_load(reinterpret_cast<const u64*>(&pieces[tid].sum),
                                            __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)
@@ -1284,7 +1322,7 @@ struct Decider {
     c.range.floor = state->floor;
     keep_all(c);
     int last = 0x7fffffff;
-    if (state->mode == kShare) {
+    if (!all) {
       const u64 counts = __hip_atomic_load(&state->counts, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       const u64 aim = state->aim;
       const u64* const list = room_of(r);
@@ -1494,9 +1532,11 @@ __device__ __forceinline__ void read_row(const Args& a, const typename T::E* row
           for (int i = 0; i < 8; ++i) sum += x[j][i] == mp ? 1.0 : 0.0;
       } else {
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int i = 0; i < 8; ++i) sum += sc.weight(x[j][i]);
+        for (int j = 0; j < 2; ++j) {
+          double y[8];
+          sc.weights(x[j], y);
+          sum += ((y[0] + y[1]) + (y[2] + y[3])) + ((y[4] + y[5]) + (y[6] + y[7]));
+        }
       }
       sum = wave_sum(sum);
     }
@@ -1548,26 +1588,65 @@ __global__ __launch_bounds__(kThreads, 4) void shared_kernel(Args a) {
   __shared__ int s_last;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int r = blockIdx.x / a.shared_groups;
-  const int group = blockIdx.x - r * a.shared_groups;
+  // The rows that take part (kCount turns into kShare under these reads, and counts as well), as
+  // many workgroups for each as fill the GPU once over all, results not depending on their
+  // number; the workgroups are numbered over those that have work. (Numbered over all rows, the
+  // ones that leave at once take their turns with the dispatcher all the same, and the others
+  // pile up on some compute units: 256 rows at top-p 0.9 179 us where they take 114.)
+  auto takes_part = [&](int row) {
+    if (row >= a.rows) return false;
+    const int x = __hip_atomic_load(a.modes + row, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return END ? x != kDecided : x == kCount || x == kShare;
+  };
+  auto in_group = [&](int base, int& before) {  // rows base + tid: whether; how many before, in all
+    const uint64_t b = __ballot(takes_part(base + tid));
+    if (lane == 0) sh.part_n[wave] = __popcll(b);
+    __syncthreads();
+    before = __builtin_amdgcn_mbcnt_hi((uint32_t)(b >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)b, 0u));
+    int all = 0;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) {
+      before += i < wave ? sh.part_n[i] : 0;
+      all += sh.part_n[i];
+    }
+    __syncthreads();
+    return (b >> lane & 1) ? all : ~all;
+  };
+  int n = 0, before;
+  for (int base = 0; base < a.rows; base += kThreads) {
+    const int x = in_group(base, before);
+    n += x < 0 ? ~x : x;
+  }
+  if (n == 0) return;
+  const int groups = max(1, min(a.shared_groups, a.shared_wgs / n));
+  const int nth = blockIdx.x / groups, group = blockIdx.x - nth * groups;
+  if (nth >= n) return;
+  int seen = 0;
+  for (int base = 0; base < a.rows; base += kThreads) {
+    const int x = in_group(base, before);
+    if (x >= 0 && seen + before == nth) sh.found = base + tid;
+    seen += x < 0 ? ~x : x;
+  }
+  __syncthreads();
+  const int r = sh.found;
+  __syncthreads();
+  const int mode = a.modes[r];
+  if (!END && mode != kCount) return;  // (cannot be: it ends with its last workgroup)
   char* const rec = a.records + (int64_t)r * a.row_bytes;
   Shared_row* const state = reinterpret_cast<Shared_row*>(rec + sizeof(Decision));
   Piece* const pieces = reinterpret_cast<Piece*>(rec + kHead);
-  const int mode = state->mode;  // (an earlier launch's; the last of the counting ones changes it)
-  if (END ? mode == kDecided : mode != kCount) return;
   const int seq = r / a.each;
   Decider<T> d(a, sh, row_of<T>(a, r, seq), settings_of(a, seq), tid, lane, wave);
+  d.groups = groups;
   d.set_max(state->max);
   if constexpr (!END) {
     d.count(r, group, *state);
-    if (arrive_last(a, r, a.shared_groups, tid, s_last)) d.bracket(r, state);
+    if (arrive_last(a, r, d.groups, tid, s_last)) d.bracket(r, state);
+  } else if (mode == kAlone) {
+    if (group == 0) d.alone(r, state->floor, state->whole);
   } else {
-    if (mode == kAlone) {
-      if (group == 0) d.alone(r, state->floor, state->whole);
-      return;
-    }
-    d.share(r, group, state, pieces);
-    if (arrive_last(a, r, a.shared_groups, tid, s_last)) d.end(r, state, pieces);
+    d.share(r, group, mode == kKeepAll, state, pieces);
+    if (arrive_last(a, r, d.groups, tid, s_last)) d.end(r, mode == kKeepAll, state, pieces);
   }
 }
 
@@ -1613,11 +1692,14 @@ __global__ __launch_bounds__(256) void probs_kernel(Args a) {
       y[i] = 0.f;
     }
     if (__ballot(any) != 0) {
+      float z[8];
+      double w[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const double w = sc.weight(x[j][i]);
-        if (in[i] && w >= (double)d.min_p) y[i] = (float)(w * inv);
-      }
+      for (int i = 0; i < 8; ++i) z[i] = x[j][i];
+      sc.weights(z, w);
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (in[i] && w[i] >= (double)d.min_p) y[i] = (float)(w[i] * inv);
     }
     typedef float quad __attribute__((ext_vector_type(4), aligned(4)));
     const int first = p * kPiece + j * 512 + lane * 8;
@@ -1632,6 +1714,7 @@ __global__ __launch_bounds__(256) void probs_kernel(Args a) {
   }
 }
 
+static size_t modes_bytes(int rows) { return (size_t)(rows + 3) / 4 * 16; }
 static int pieces_of(int vocab) { return (vocab + kPiece - 1) / kPiece; }
 static int cells_of(int vocab) { return (vocab + kCell - 1) / kCell; }
 
@@ -1669,13 +1752,12 @@ static hipError_t launch(const Args& a, hipStream_t stream) {
   return hipGetLastError();
 }
 
-// Workgroups that share a row of a long list: as above for kSharedWavesPerCu, since not every
-// row of many has one.
-constexpr int kSharedWavesPerCu = 32;
+// Workgroups that may share a row of a long list, at most: one wavefront per piece, or as many
+// as a launch of kMostShared (most of which have nothing to do and cost 2 us in all) has for it.
+constexpr int kMostShared = 2048;
 static int shared_groups_of(int rows, int pieces) {
-  const int64_t waves = (int64_t)kSharedWavesPerCu * device_cus() / rows;
-  const int64_t groups = ((waves < pieces ? waves : pieces) + kWaves - 1) / kWaves;
-  return groups < 1 ? 1 : (int)groups;
+  const int most = (pieces + kWaves - 1) / kWaves, fair = kMostShared / rows;
+  return fair < 1 ? 1 : fair < most ? fair : most;
 }
 static int shared_rows_of(int rows, int vocab) {
   return vocab <= kList ? 0 : rows < kMaxShared ? rows : kMaxShared;
@@ -1701,7 +1783,8 @@ extern "C" {
 size_t pa_sample_workspace_bytes(int num_seqs, int rows_per_seq, int vocab) {
   const int64_t rows = (int64_t)num_seqs * rows_per_seq;
   if (num_seqs <= 0 || rows_per_seq <= 0 || rows > kMaxRows || vocab <= 0 || vocab > kMaxVocab) return 0;
-  return kCounterBytes + (size_t)rows * row_record(pieces_of(vocab), cells_of(vocab)) +
+  return kCounterBytes + modes_bytes((int)rows) +
+         (size_t)rows * row_record(pieces_of(vocab), cells_of(vocab)) +
          (size_t)shared_rows_of((int)rows, vocab) * kRoom * sizeof(u64);
 }
 
@@ -1762,10 +1845,12 @@ static int start(Args& a, const void* logits, int dtype, const int64_t* strides,
   a.groups = groups_of(a.rows, a.pieces);
   a.row_bytes = row_record(a.pieces, a.cells);
   a.cnt = (int*)workspace;
-  a.records = (char*)workspace + kCounterBytes;
+  a.modes = (int*)((char*)workspace + kCounterBytes);
+  a.records = (char*)workspace + kCounterBytes + modes_bytes(a.rows);
   a.rooms = (u64*)(a.records + (size_t)a.rows * a.row_bytes);
   a.shared_rows = shared_rows_of(a.rows, vocab);
   a.shared_groups = shared_groups_of(a.rows, a.pieces);
+  a.shared_wgs = 2 * device_cus();
   return PA_OK;
 }
 
