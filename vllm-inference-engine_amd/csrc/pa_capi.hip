@@ -367,17 +367,25 @@ constexpr int64_t kPrefillFewBlocks = 64;
 // per column block, zero between launches) and a record of (head_dim + 2) x
 // cols floats per split.
 // cap: the most tokens a column block's keys can span.
+// scored: with scores that are capped, biased or masked. Over short spans a workgroup lives for
+// a few tiles, and what it waits for first (table, keys, queries, one after the other) counts
+// more than what it reads twice: up to kScoredShortSpan tokens twice as many workgroups of one
+// column group run, at head_dim 64. Measured on MI355X at 8 x 2048 tokens, 14 / 2 heads: a window
+// of one key 30.5 -> 24.1 us, of 64 35.3 -> 29.2, of 512 66.1 -> 64.5; causal over 2048 115.8 where two
+// groups take 109.1.
+constexpr int64_t kScoredShortSpan = 704;
 static PrefillPlan prefill_plan(int num_seqs, int num_q_heads, int num_kv_heads, int head_dim,
-                                int64_t cap, int max_query_len) {
+                                int64_t cap, int max_query_len, bool scored = false) {
   PrefillPlan p;
   const int g = num_q_heads / num_kv_heads;
   p.col_groups = prefill_col_groups(head_dim);
   auto blocks_for = [&](int cg) { return ((int64_t)max_query_len * g + 64 * cg - 1) / (64 * cg); };
   if (p.col_groups > 1 && blocks_for(p.col_groups) * num_seqs * num_kv_heads < kPrefillFewBlocks)
     p.col_groups = 1;
+  if (scored && head_dim == 64 && cap <= kScoredShortSpan) p.col_groups = 1;
   const int cols = 64 * p.col_groups;
   p.col_blocks = blocks_for(p.col_groups);
-  const int kt = prefill_key_tile(head_dim);
+  const int kt = scored ? scored_key_tile(head_dim) : prefill_key_tile(head_dim);
   const int64_t max_tiles = (cap + kt - 1) / kt;
   const int64_t base = p.col_blocks * num_seqs * num_kv_heads;
   // The kernel keeps two workgroups per CU resident (one at head_dim 256, for
@@ -1329,7 +1337,7 @@ static int prefill_attention(const void* q, const int64_t q_strides[3], const vo
       scored ? scored_span(block_size, max_blocks_per_seq, head_dim, scored->window, scored->ends)
              : (int64_t)max_blocks_per_seq * block_size;
   const PrefillPlan plan =
-      prefill_plan(num_seqs, num_q_heads, num_kv_heads, head_dim, span, max_query_len);
+      prefill_plan(num_seqs, num_q_heads, num_kv_heads, head_dim, span, max_query_len, scored);
   const int64_t grid = plan.col_blocks * plan.max_splits * num_seqs * num_kv_heads;
   if (grid > 0x7fffffff || plan.col_blocks > 0x7fffffff) {
     set_error("%lld workgroups exceed the grid limit", (long long)grid);
@@ -1396,7 +1404,7 @@ size_t pa_prefill_attention_scored_workspace_bytes(int num_seqs, int num_q_heads
     return 0;
   return prefill_plan(num_seqs, num_q_heads, num_kv_heads, head_dim,
                       scored_span(block_size, max_blocks_per_seq, head_dim, window, has_key_ends),
-                      max_query_len).ws_bytes;
+                      max_query_len, true).ws_bytes;
 }
 
 int pa_prefill_attention_scored_f16(const void* q, const int64_t q_strides[3], const void* k_cache,

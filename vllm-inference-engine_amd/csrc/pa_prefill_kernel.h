@@ -117,7 +117,7 @@ template <int D, int BS, int CG, int NW, bool KV8, int SCORED>
 __global__ __launch_bounds__(64 * NW) void prefill_attn_kernel(PrefillArgsOf<SCORED> a) {
   static_assert(!(KV8 && SCORED), "scored attention is over the fp16 pool");
   constexpr int COLS = 16 * CG * NW;  // columns per workgroup
-  constexpr int KT = prefill_key_tile(D);  // keys per staged tile
+  constexpr int KT = SCORED ? scored_key_tile(D) : prefill_key_tile(D);  // keys per staged tile
   constexpr int NS = KT / 16;         // 16-key sub-tiles per tile
   constexpr int NC = D / 32;
   constexpr int ND = D / 16;
@@ -462,36 +462,58 @@ __global__ __launch_bounds__(64 * NW) void prefill_attn_kernel(PrefillArgsOf<SCO
       }
     }
     if constexpr (SCORED != 0) {
-      // Into the exp2 domain, with cap and bias.
+      // Into the exp2 domain, with cap and bias, less the running maximum. Without ends of the
+      // caller's no column sees a key past its position, and the distance is key - position
+      // without its sign: a term linear in the key.
 #pragma unroll
       for (int cg = 0; cg < CG; ++cg) {
+        const float nm = m_run[cg] == kNegInf ? 0.f : -m_run[cg];
         const float away = (float)(kt * KT + grp * 4 - pos[cg]);  // of the lane's first key
-#pragma unroll
-        for (int s = 0; s < NS; ++s)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            float x = sc[cg][s][r];
-            if constexpr ((SCORED & kScoreCap) != 0) {
-              const float e = fast_exp2(x * a.cap_in);
-              x = __builtin_fmaf(a.cap_out, __builtin_amdgcn_rcpf(e + 1.f), a.cap_log2);
-            } else {
-              x *= a.scale_log2;
-            }
-            if constexpr ((SCORED & kScoreBias) != 0)
-              x = __builtin_fmaf(-slope[cg], fabsf(away + (float)(s * 16 + r)), x);
-            sc[cg][s][r] = x;
+        const float all = (SCORED & kScoreCap) != 0 ? a.cap_log2 + nm : nm;
+        auto score = [&](float x, float rest) {
+          if constexpr ((SCORED & kScoreCap) != 0) {
+            const float e = fast_exp2(x * a.cap_in);
+            return __builtin_fmaf(a.cap_out, __builtin_amdgcn_rcpf(e + 1.f), rest);
+          } else {
+            return __builtin_fmaf(x, a.scale_log2, rest);
           }
+        };
+        if ((SCORED & kScoreBias) != 0 && a.ends) {
+#pragma unroll
+          for (int s = 0; s < NS; ++s)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              sc[cg][s][r] = score(sc[cg][s][r],
+                                   __builtin_fmaf(-slope[cg], fabsf(away + (float)(s * 16 + r)), all));
+        } else {
+          const float near = (SCORED & kScoreBias) != 0 ? __builtin_fmaf(slope[cg], away, all) : all;
+#pragma unroll
+          for (int s = 0; s < NS; ++s)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              sc[cg][s][r] = score(sc[cg][s][r], (SCORED & kScoreBias) != 0
+                                                     ? __builtin_fmaf(slope[cg], (float)(s * 16 + r), near)
+                                                     : near);
+        }
       }
-      if (crosses(kt)) {
+      const int key0 = kt * KT + grp * 4;  // the lane's first key
+      if (kt * KT < all_from) {
 #pragma unroll
         for (int cg = 0; cg < CG; ++cg)
 #pragma unroll
           for (int s = 0; s < NS; ++s)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const int key = kt * KT + s * 16 + grp * 4 + r;
-              if (key < key_first[cg] || key >= key_end[cg]) sc[cg][s][r] = kNegInf;
-            }
+            for (int r = 0; r < 4; ++r)
+              if (s * 16 + r < key_first[cg] - key0) sc[cg][s][r] = kNegInf;
+      }
+      if (kt * KT + KT > all_to) {
+#pragma unroll
+        for (int cg = 0; cg < CG; ++cg)
+#pragma unroll
+          for (int s = 0; s < NS; ++s)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (s * 16 + r >= key_end[cg] - key0) sc[cg][s][r] = kNegInf;
       }
     } else if (crosses(kt)) {  // a tile crossing some column's position
 #pragma unroll
@@ -524,7 +546,7 @@ __global__ __launch_bounds__(64 * NW) void prefill_attn_kernel(PrefillArgsOf<SCO
         // then gives p = 0 for its -inf scores.
         const float nm = m_run[cg] == kNegInf ? 0.f : -m_run[cg];
         auto prob = [&](float x) {
-          if constexpr (SCORED != 0) return (f16)fast_exp2(x + nm);
+          if constexpr (SCORED != 0) return (f16)fast_exp2(x);
           return (f16)fast_exp2(KV8 ? __builtin_fmaf(x + nm, a.scale_log2, BIAS)
                                     : __builtin_fmaf(x, a.scale_log2, nm));
         };
@@ -563,7 +585,25 @@ __global__ __launch_bounds__(64 * NW) void prefill_attn_kernel(PrefillArgsOf<SCO
         }
         m = fmaxf(m, __shfl_xor(m, 16));
         m = fmaxf(m, __shfl_xor(m, 32));
-        const float m_new = fmaxf(m_run[cg], KV8 || SCORED ? m : m * a.scale_log2);
+        if constexpr (SCORED != 0) {
+          // The scores are less the old maximum (or nothing): by the same step as the sums,
+          // which a column without a visible key yet holds as zeros.
+          const bool none = m_run[cg] == kNegInf;
+          const float m_old = none ? 0.f : m_run[cg];
+          const float m_new = none ? m : fmaxf(m_old, m_old + m);
+          const float step = m_new == kNegInf ? 0.f : m_old - m_new;
+          const float alpha = none ? 1.f : fast_exp2(step);
+          l_run[cg] *= alpha;
+#pragma unroll
+          for (int nd = 0; nd < ND; ++nd) acc[cg][nd] *= alpha;
+#pragma unroll
+          for (int s = 0; s < NS; ++s)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) sc[cg][s][r] += step;
+          m_run[cg] = m_new;
+          continue;
+        }
+        const float m_new = fmaxf(m_run[cg], KV8 ? m : m * a.scale_log2);
         // A column with no visible key yet (only in a split after the first)
         // stays at -inf, and -inf - -inf would make its alpha NaN.
         const float alpha = m_new == kNegInf ? 1.f

@@ -91,8 +91,9 @@ def sample_tokens(
     u of 1 and more, or NaN, the last index with a weight.
 
     Weights and sums are in 64 bits (units of 2^-44 of the largest weight). At most 16384 rows
-    of 2^19 logits. One launch; asynchronous on the current stream; no host synchronisation;
-    capturable into a HIP graph.
+    of 2^19 logits. One launch, and two more where a row can have a long list (more than 2048
+    logits); asynchronous on the current stream; no host synchronisation; capturable into a HIP
+    graph.
     """
     out = _native.direct_counted("sample", _native.WS_SAMPLE, logits, u, temperature, top_k, top_p,
                                  min_p)
@@ -121,8 +122,8 @@ def sampling_probs(
     """The distributions that sample_tokens draws from, fp32 of logits' shape.
 
     w / sum for the entries that its settings keep, 0 for all others (and for a row without
-    any weight). The target_probs and draft_probs of verify_drafts. Two launches, as
-    sample_tokens otherwise.
+    any weight). The target_probs and draft_probs of verify_drafts. One launch more
+    than sample_tokens, and otherwise as it.
     """
     out = _native.direct_counted("probabilities", _native.WS_SAMPLE, logits, temperature, top_k,
                                  top_p, min_p)
