@@ -392,11 +392,13 @@ static PrefillPlan prefill_plan(int num_seqs, int num_q_heads, int num_kv_heads,
   // LDS); splitting pays only while the column blocks fill less than about
   // three quarters of those slots.
   const int64_t target = (int64_t)device_cus() * (head_dim <= 128 ? 2 : 1) * 3 / 4;
+  // Of the plain kernel's tiles: scored ones of half the keys take twice as many.
+  const int least = kPrefillMinSplitTiles * (prefill_key_tile(head_dim) / kt);
   p.split_tiles = max_tiles < 1 ? 1 : max_tiles;
-  if (base > 0 && base < target && base <= kPfMaxCounters && max_tiles > kPrefillMinSplitTiles) {
+  if (base > 0 && base < target && base <= kPfMaxCounters && max_tiles > least) {
     const int64_t want = (target + base - 1) / base;
     int64_t st = (max_tiles + want - 1) / want;
-    if (st < kPrefillMinSplitTiles) st = kPrefillMinSplitTiles;
+    if (st < least) st = least;
     p.split_tiles = st;
     p.max_splits = (max_tiles + st - 1) / st;
   }
