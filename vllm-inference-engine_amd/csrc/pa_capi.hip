@@ -418,11 +418,14 @@ static PrefillPlan prefill_plan(int num_seqs, int num_q_heads, int num_kv_heads,
   // 2048 344.9-346.6 vs 362.7-366.7, 12288 + 2048 151.7-152.4 vs 156.7-158.9;
   // 16384 + 1024 split four ways (34 tiles) 104.5-105.4 vs 104.8-105.2; head_dim
   // 32, 8 x (2048 + 512) 39.3-40.4 vs 40.0-42.2, 16384 + 2048 split two ways
-  // 136.9-137.6 vs 134.7-135.6.
+  // 136.9-137.6 vs 134.7-135.6. Scored ones, which have more to compute and to keep at hand,
+  // run as eight always: 4 x (8192 + 1024) with a bias 211 -> 203 us, capped 270 -> 254, 8 x
+  // (2048 + 512) 63.3 -> 61.1 and 78.5 -> 74.3; head_dim 32 with a bias 144.6 -> 137.9 and 44.8
+  // -> 42.6.
   constexpr int64_t kPrefillLongPieceTiles = 48;
   if (head_dim > 64)
     p.wave_groups = p.col_groups;
-  else if (p.col_groups == 2 &&
+  else if (p.col_groups == 2 && !scored &&
            ((p.max_splits == 1 && 2 * (int64_t)max_query_len <= cap) ||
             (p.max_splits > 1 && head_dim == 64 && p.split_tiles >= kPrefillLongPieceTiles)))
     p.wave_groups = 2;

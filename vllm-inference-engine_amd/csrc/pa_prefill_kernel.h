@@ -418,12 +418,19 @@ __global__ __launch_bounds__(64 * NW) void prefill_attn_kernel(PrefillArgsOf<SCO
     for (int nd = 0; nd < ND; ++nd) acc[cg][nd] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
-  // Two LDS buffers: tile kt is read from buffer kt % 2 while tile kt + 1 is
+  // A bias by distance raises the scores towards the row's position: with the last tiles first
+  // the maximum is found at once, where each tile of the other order would raise it (4 x (8192 +
+  // 1024) tokens at 14 / 2 heads of 64 299 -> 212 us, 8 x (2048 + 512) 84.6 -> 63.3).
+  constexpr bool BACK = (SCORED & kScoreBias) != 0;
+  auto after = [](int kt, int n) { return BACK ? max(kt - n, 0) : kt + n; };
+  const int first_tile = BACK ? t1 - 1 : t0;
+
+  // Two LDS buffers: tile kt is read from buffer kt % 2 while the next tile is
   // written to the other, so each tile needs one barrier.
-  fetch_ids(t0);
-  fetch_kv(t0);
-  fetch_ids(t0 + 1);
-  stash(t0 & 1, crosses(t0));
+  fetch_ids(first_tile);
+  fetch_kv(first_tile);
+  fetch_ids(after(first_tile, 1));
+  stash(first_tile & 1, crosses(first_tile));
   __syncthreads();
   // Every load issued so far (the query fragments included, which the
   // compiler may place after the first tile's loads) is complete before the
@@ -433,11 +440,11 @@ __global__ __launch_bounds__(64 * NW) void prefill_attn_kernel(PrefillArgsOf<SCO
   __builtin_amdgcn_sched_barrier(0);
   __builtin_amdgcn_s_waitcnt(0);
   __builtin_amdgcn_sched_barrier(0);
-  for (int kt = t0; kt < t1; ++kt) {
-    const bool more = kt + 1 < t1;
+  for (int kt = first_tile; BACK ? kt >= t0 : kt < t1; kt += BACK ? -1 : 1) {
+    const bool more = BACK ? kt > t0 : kt + 1 < t1;
     if (more) {
-      fetch_kv(kt + 1);
-      fetch_ids(kt + 2);
+      fetch_kv(after(kt, 1));
+      fetch_ids(after(kt, 2));
     }
     const f16* kt_lds = ks + (kt & 1) * BUF;
     const f16* vt_lds = vs + (kt & 1) * BUF;
@@ -640,7 +647,7 @@ __global__ __launch_bounds__(64 * NW) void prefill_attn_kernel(PrefillArgsOf<SCO
       }
     }
 
-    if (more) stash((kt + 1) & 1, crosses(kt + 1));
+    if (more) stash((kt + 1) & 1, crosses(after(kt, 1)));
     __syncthreads();
   }
 
@@ -794,10 +801,13 @@ static hipError_t launch_prefill_bs(const PrefillArgsOf<SCORED>& a, int64_t grid
       return hipGetLastError();
     }
   }
-  if (a.wave_groups != CG) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((prefill_attn_kernel<D, BS, CG, 4, KV8, SCORED>), dim3((unsigned)grid), dim3(256), 0, s,
-                     a);
-  return hipGetLastError();
+  if constexpr (D > 64 || CG == 1 || SCORED == 0) {  // (scored ones always run as eight there)
+    if (a.wave_groups != CG) return hipErrorInvalidValue;
+    hipLaunchKernelGGL((prefill_attn_kernel<D, BS, CG, 4, KV8, SCORED>), dim3((unsigned)grid), dim3(256), 0,
+                       s, a);
+    return hipGetLastError();
+  }
+  return hipErrorInvalidValue;
 }
 
 template <bool KV8, int SCORED, int D, int CG>
