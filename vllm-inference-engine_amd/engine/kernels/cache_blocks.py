@@ -70,13 +70,15 @@ def paged_copy_blocks(
 
 def fork_block_table(table: Any, allocator: Any, caches: Sequence[torch.Tensor],
                      copies: int = 1) -> List[Any]:
-    """`copies` tables that go on from table's tokens, each on its own.
+    """`copies` tables that go on from table's tokens, each on its own: samples of one prompt,
+    beams. caches: the pool's K and V of every layer, [*pool.k_cache, *pool.v_cache] (with the
+    scales, for an 8-bit pool).
 
     Full blocks are shared (allocator.fork); a partly filled last block is copied into a
     block of each copy's own (allocator.allocate) in all tensors of `caches`, so that
     decode steps of the copies and of the original never write a shared block. Blocks that
     the table holds beyond its tokens stay its own alone. Raises what allocate() raises when
-    blocks run out, with every count as it was.
+    blocks run out, and paged_copy_blocks for the caches, with every count as it was.
     """
     full, rest = divmod(table.num_tokens, table.block_size)
     shared = list(table.physical_block_ids[:full])
@@ -87,6 +89,10 @@ def fork_block_table(table: Any, allocator: Any, caches: Sequence[torch.Tensor],
     try:
         for _ in range(copies if rest else 0):
             own.append(allocator.allocate())
+        if own:
+            last = table.physical_block_ids[full]
+            pairs = torch.tensor([[last] * copies, own], dtype=torch.int32).to(caches[0].device)
+            paged_copy_blocks(caches, pairs[0], pairs[1])
     except BaseException:
         for b in own:
             allocator.free(b)
@@ -95,12 +101,7 @@ def fork_block_table(table: Any, allocator: Any, caches: Sequence[torch.Tensor],
     for i in range(copies):
         for b in shared:
             allocator.fork(b)
-        ids = shared + own[i:i + 1]
         tables.append(type(table)(seq_id=table.seq_id, block_size=table.block_size,
-                                  physical_block_ids=ids, num_tokens=table.num_tokens))
-    if own:
-        dev = caches[0].device
-        last = table.physical_block_ids[full]
-        pairs = torch.tensor([[last] * copies, own], dtype=torch.int32).to(dev)
-        paged_copy_blocks(caches, pairs[0], pairs[1])
+                                  physical_block_ids=shared + own[i:i + 1],
+                                  num_tokens=table.num_tokens))
     return tables

@@ -1618,8 +1618,13 @@ class KernelPagedManualDecode:
                          f"embedding's {vocab} rows.")
 
     @torch.inference_mode()
-    def decode_step(self, seqs: List[Any], allocator: Any = None) -> List[int]:
-        """One batched decode step for the running sequences (reference :518-653)."""
+    def decode_step(self, seqs: List[Any], allocator: Any = None,
+                    sampler: Optional[Callable[[torch.Tensor], torch.Tensor]] = None) -> List[int]:
+        """One batched decode step for the running sequences (reference :518-653).
+
+        sampler: given the step's logits [n, vocab] it returns the tokens [n] (sample_tokens with
+        the sequences' settings and numbers, for one); without it they are the greedy ones.
+        """
         n = len(seqs)
         if n == 0:
             return []
@@ -1683,6 +1688,11 @@ class KernelPagedManualDecode:
                 logits = logits.clone()
             top2 = torch.topk(logits, k=2, dim=-1).values.double()
             both = torch.stack([torch.argmax(logits, dim=-1).double(), top2[:, 0] - top2[:, 1]])
+        if sampler is not None:
+            chosen = sampler(logits)
+            assert chosen.shape == logits.shape[:1], (
+                f"the sampler must return {n} tokens, got {tuple(chosen.shape)}")
+            both = torch.stack([chosen.double(), both[1]])
         # float64 holds every token id exactly: tokens and margins in one transfer.
         toks, margins = both.tolist()
         for seq, row, margin in zip(seqs, logits.detach().unbind(0), margins):
