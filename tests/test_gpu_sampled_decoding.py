@@ -136,6 +136,7 @@ def test_forks_and_drafts_with_scores(cuda_device):
     check_decode(pool, pool.queries(3, hq, seed=9), d ** -0.5, softcap=20.0, slopes=slopes, window=24)
 
 
+@torch.inference_mode()
 def test_captured_run(cuda_device):
     """The whole chain in one graph, replayed over other inputs, with eager calls in between."""
     hq, hkv, d, bs, k, vocab = 8, 2, 64, 16, 2, 33000

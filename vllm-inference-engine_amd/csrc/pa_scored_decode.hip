@@ -6,7 +6,7 @@
 //
 // Work split, as for the 8-bit pool (pa_fp8_attend.h): the work is a list of (sequence, kv
 // head) pairs, each of the 32-token chunks that its window touches plus a fixed cost; a grid
-// of a few workgroups per compute unit takes equal contiguous ranges of it, found by every
+// of one workgroup per compute unit takes equal contiguous ranges of it, found by every
 // wavefront for itself with lane scans over lengths and first keys. Where every pair is
 // short a workgroup takes one pair whole. Within a pair's part of its range the wavefronts
 // take the chunks in turn, each with an online softmax of its own for the whole query group,
@@ -573,12 +573,20 @@ __global__ __launch_bounds__(64 * NW, 2) void decode_scored_kernel(Args a) {
 // ---- launch plan ----
 
 // List positions of 32 tokens: what a pair costs beside its chunks, and the fewest a range
-// takes.
-constexpr int kPairCost = 8;
+// takes. Measured on MI355X (us; positions of a pair 2, 8, 16): 4 x 8000 tokens at 14 / 2 heads of
+// 64 16.5, 15.5, 14.0; 100 ragged up to 4000 28.3, 27.7, 25.6; 64 ragged up to 8000 at 32 / 8 of 128
+// 190.5 and 189.9 of the last two. Ranges of 8, 16 and 32 at least: one context of 24000 16.4, 14.7,
+// 17.0.
+// At head_dim 256, whose chunks are longer: 40 ragged up to 6000 at 16 / 8 heads 175 of 8, 182 of 16.
+static int pair_cost(int head_dim) { return head_dim <= 128 ? 16 : 8; }
 constexpr int kMinRange = 16;
-// Windows (or tables) of at most this many tokens take one workgroup per pair; of the second,
-// where the pairs fill at least half the compute units.
-constexpr int kWholePairs = 1024;
+// Windows (or tables) of at most this many tokens take one workgroup per pair: beyond, records and
+// their merge cost less than the wait for one compute unit's reading. 8 contexts of 2000 tokens at
+// 14 / 2 heads of 64 15.2 us in ranges, 11.9 whole; of 128, 1500 tokens 15.0 and 15.2, 2000 at 32 / 8
+// 20.3 and 26.5; of 256, 1200 tokens 22.8 and 26.5.
+static int whole_pairs(int head_dim) { return head_dim <= 64 ? 2048 : head_dim == 128 ? 1536 : 1024; }
+// And where the pairs fill at least half the compute units (100 ragged up to 2040 at 14 / 2 heads of
+// 64 15.3 whole, 20.3 in ranges).
 constexpr int kWholePairsBusy = 2048;
 
 struct Plan {
@@ -595,15 +603,17 @@ static Plan plan_of(int num_seqs, int num_q_heads, int num_kv_heads, int head_di
   const int64_t chunks = (seen + 2 * kChunk - 2) / kChunk;  // that an interval of so many can touch
   const int64_t pairs = (int64_t)num_seqs * num_kv_heads;
   const bool few = pairs <= n;
-  p.waves = few && head_dim <= 128 ? 8 : 4;
-  const int64_t whole = 2 * pairs >= n ? kWholePairsBusy : kWholePairs;
-  p.ranged = seen > whole && pairs <= kMaxCounters && pairs * (chunks + kPairCost) < 0x7fffffff;
+  const int64_t whole = 2 * pairs >= n ? kWholePairsBusy : whole_pairs(head_dim);
+  p.ranged = seen > whole && pairs <= kMaxCounters && pairs * (chunks + pair_cost(head_dim)) < 0x7fffffff;
+  // One workgroup of eight wavefronts per compute unit, for few pairs or ranges (two of four: 64
+  // ragged up to 8000 198.5 us, one of eight 190; 200 ragged up to 6000 at 16 / 8 heads of 64 213 and
+  // 200); four wavefronts for many short pairs, several at a time, and at head_dim 256, for LDS.
+  p.waves = head_dim <= 128 && (few || p.ranged) ? 8 : 4;
   p.grid = pairs > 0x7fffffff ? -1 : (int)pairs;
   if (p.ranged) {
     // No more ranges than the longest lengths fill.
-    const int64_t most = pairs * (chunks + kPairCost) / kMinRange;
-    const int want = (few || head_dim == 256 ? 1 : 2) * n;
-    p.grid = (int)(most < want ? (most < 1 ? 1 : most) : want);
+    const int64_t most = pairs * (chunks + pair_cost(head_dim)) / kMinRange;
+    p.grid = (int)(most < n ? (most < 1 ? 1 : most) : n);
     p.rec_floats = record_size(num_q_heads / num_kv_heads, head_dim);
     p.ws_bytes = kCounterBytes + (size_t)2 * p.grid * p.rec_floats * sizeof(float);
   }
@@ -756,7 +766,7 @@ int pa_decode_scored_f16(const void* q, const int64_t q_strides[3], const void* 
   a.recs = (float*)((char*)workspace + (p.ws_bytes ? kCounterBytes : 0));
   a.ranged = p.ranged;
   a.min_range = kMinRange;
-  a.pair_cost = kPairCost;
+  a.pair_cost = pair_cost(head_dim);
   a.rec_floats = p.rec_floats;
   const ScoreForm f = score_form(scale, softcap);
   a.scale_log2 = f.scale_log2;
