@@ -7,7 +7,8 @@
 // their addresses travel in the launch's arguments. Bound by memory, a block read and
 // written once; for a few blocks by the chain launch -> ids -> block. Each wavefront takes
 // one piece of a block, U loads per lane on their way at once; blocks smaller than a
-// piece share wavefronts by lane.
+// piece share wavefronts by lane. On MI355X, 24 layers of 4 KB blocks: 700 pairs in 53.6 us (275
+// MB read and written, 5.1 TB/s; a large copy runs at 5.4), 7 pairs in 2.8 us, 6.6 with the host.
 #include <algorithm>
 
 #include "../../include/paged_attention.h"

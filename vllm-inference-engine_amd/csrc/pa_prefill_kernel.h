@@ -36,11 +36,16 @@
 // And scores that a model caps, biases or masks (SCORED, over the fp16 pool):
 //   s = softcap * tanh(scale q.k / softcap) - slope |position - key|,
 // for the keys of each row's own interval [first, end), in place of those up to its position.
-// Scores go to the exp2 domain with cap and bias right after the products (the tanh as 1 - 2 /
-// (1 + e^2x): two more transcendental instructions a score); everything after is the same.
+// Scores go to the exp2 domain, less the running maximum, with cap and bias right after the
+// products (the tanh as 1 - 2 / (1 + e^2x): two more transcendental instructions a score);
+// everything after is the same.
 // Key tiles run over the union of the workgroup's intervals. A tile that some column does not
 // see whole is masked, and there a NaN or an infinity in V is moved to the key's K row, as for
 // the 8-bit pool: what lies in a row that a column does not see never reaches it.
+// Bound by issue as the plain kernel: four capped prompts of 300 to 2048 tokens at 32 / 8 heads of
+// 128 71.4 us (550 TFLOP/s of products; 62 without the cap), 4 x (8192 + 1024) tokens at 14 / 2 heads
+// of 64 with a bias 203 (174 plain), capped 254. With short intervals by the chain to a workgroup's
+// first products: 8 x 2048 tokens packed of documents of some 300, with a bias, 48.0.
 #pragma once
 
 #include <type_traits>

@@ -28,6 +28,13 @@
 // entries that a row may have cannot overflow 64 bits. (Sums of whole pieces, formed while
 // the row is read, are in 64-bit floating point in a fixed order.) The token differs from the
 // definition's only where u times the sum lies within about 2^-44 per entry of a border.
+//
+// What bounds it: for many rows the 64-bit arithmetic of the weights, for one row the chain of
+// dependent steps. In a run of calls on MI355X: one fp16 row of 151936 with temperature, top-k
+// and top-p 16.6 us (12-14 the first launch, 2 each of the others, which find nothing to do); 256
+// rows of mixed settings 104.5 (44 + 20 + 41; a copy of the logits would take 15); 32 bf16 rows of
+// 100003 at high temperatures and wide top-p 60.5; probabilities of 80 rows of 151936 80.2, of
+// which writing 16 (4.6 TB/s).
 #include "../../include/paged_attention.h"
 #include "pa_tiles.h"
 
