@@ -58,6 +58,23 @@ def test_long_prompts(cuda_device, heads, hkv, d):
             check_prefill(pool, q, new, d ** -0.5, **f)
 
 
+@pytest.mark.parametrize("heads,hkv,d", [(14, 2, 64), (8, 2, 128), (4, 2, 32)])
+def test_bias_over_many_tiles(cuda_device, heads, hkv, d):
+    """Biases that raise or lower the scores from tile to tile, over split and whole key ranges:
+    steep and flat, of both signs, none; with ends before, at and behind the position."""
+    for lens, new in (([1500, 90], [260, 90]), ([2500], [9])):
+        pool = Pool(lens, hkv, d, 16, cuda_device, seed=7)
+        q = pool.queries(sum(new), heads)
+        slopes = slopes_of(heads, cuda_device)
+        slopes[1], slopes[2], slopes[3] = 3.0, -0.25, 0.0
+        behind = prefixes(lens, new, [n - 3 for n in lens])
+        before = np.concatenate([np.minimum(np.arange(n - k, n) + 1, n // 2) for n, k in zip(lens, new)])
+        for f in (dict(), dict(ends=behind), dict(ends=before), dict(softcap=10.0),
+                  dict(ends=behind, softcap=10.0), dict(window=600), dict(window=700, softcap=4.0),
+                  dict(starts=documents(lens, new, 400))):
+            check_prefill(pool, q, new, d ** -0.5, slopes=slopes, **f)
+
+
 def test_many_sequences(cuda_device):
     """Ragged batches whose workgroups are numbered over the blocks that exist; more than 256."""
     rng = np.random.default_rng(3)
