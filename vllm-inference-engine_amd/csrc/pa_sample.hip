@@ -31,9 +31,9 @@
 //
 // What bounds it: for many rows the 64-bit arithmetic of the weights, for one row the chain of
 // dependent steps. In a run of calls on MI355X: one fp16 row of 151936 with temperature, top-k
-// and top-p 16.6 us (12-14 the first launch, 2 each of the others, which find nothing to do); 256
-// rows of mixed settings 104.5 (44 + 20 + 41; a copy of the logits would take 15); 32 bf16 rows of
-// 100003 at high temperatures and wide top-p 60.5; probabilities of 80 rows of 151936 80.2, of
+// and top-p 16.2 us (12-14 the first launch, 2 each of the others, which find nothing to do); 256
+// rows of mixed settings 98.2 (44 + 17 + 38; a copy of the logits would take 15); 32 bf16 rows of
+// 100003 at high temperatures and wide top-p 55.3; probabilities of 80 rows of 151936 73.1, of
 // which writing 16 (4.6 TB/s).
 #include "../../include/paged_attention.h"
 #include "pa_tiles.h"
@@ -111,7 +111,7 @@ struct Args {
   char* records;  // per row: Decision, Shared_row, pieces, cells
   u64* rooms;     // of the first `shared_rows` rows: kBins counts and places, then kList keys and indexes
   int row_bytes, pieces, cells, groups;
-  int shared_rows, shared_groups, shared_wgs;
+  int shared_rows, shared_groups, cus;
 };
 
 constexpr int kHead = sizeof(Decision) + sizeof(Shared_row);
@@ -1625,7 +1625,10 @@ __global__ __launch_bounds__(kThreads, 4) void shared_kernel(Args a) {
     n += x < 0 ? ~x : x;
   }
   if (n == 0) return;
-  const int groups = max(1, min(a.shared_groups, a.shared_wgs / n));
+  // One workgroup per compute unit for few rows (each adds up to 2048 counts to its row's room: 32
+  // rows of 100003 at T 1.4, top-p 0.97 62.0 us with two, 55.6 with one), else two (100 rows of
+  // 151936 at top-p 0.9 81.8 us with one, 73.3 with two; 256 rows 130.9 and 114.0).
+  const int groups = max(1, min(a.shared_groups, (4 * n <= a.cus ? 1 : 2) * a.cus / n));
   const int nth = blockIdx.x / groups, group = blockIdx.x - nth * groups;
   if (nth >= n) return;
   int seen = 0;
@@ -1857,7 +1860,7 @@ static int start(Args& a, const void* logits, int dtype, const int64_t* strides,
   a.rooms = (u64*)(a.records + (size_t)a.rows * a.row_bytes);
   a.shared_rows = shared_rows_of(a.rows, vocab);
   a.shared_groups = shared_groups_of(a.rows, a.pieces);
-  a.shared_wgs = 2 * device_cus();
+  a.cus = device_cus();
   return PA_OK;
 }
 
