@@ -143,3 +143,27 @@ def test_scored_attention_workspace():
     assert prefill(1, 14, 2, 64, 16, 512, 64, 0, 0) == lib.pa_prefill_attention_workspace_bytes(
         1, 14, 2, 64, 16, 512, 64)
     assert prefill(1, 14, 2, 64, 16, 512, 64, 100, 0) < prefill(1, 14, 2, 64, 16, 512, 64, 100, 1)
+
+
+def test_refused_forks_leave_the_counts():
+    """Copies that are refused (here: off the GPU, no tensors, blocks run out) cost no block."""
+    import torch
+    from engine.kernels.cache_blocks import fork_block_table
+    from engine.memory.block_allocator import BlockAllocator, BlockTable
+
+    alloc = BlockAllocator(5)
+    table = BlockTable(seq_id=0, block_size=4)
+    table.physical_block_ids = [alloc.allocate() for _ in range(2)]
+    table.num_tokens = 7
+    before = dict(alloc.ref_counts)
+    caches = [torch.zeros(5, 4, 2, 8, dtype=torch.float16)]
+    for args in ((caches, 2), ([], 1), (caches, 4)):
+        with pytest.raises(Exception):
+            fork_block_table(table, alloc, *args)
+        assert {k: v for k, v in alloc.ref_counts.items() if v} == before
+    assert len([alloc.allocate() for _ in range(3)]) == 3
+    # Full blocks alone are shared without a copy.
+    table.num_tokens = 8
+    forks = fork_block_table(table, alloc, caches, 2)
+    assert [f.physical_block_ids for f in forks] == [table.physical_block_ids] * 2
+    assert all(alloc.ref_counts[b] == 3 for b in table.physical_block_ids)

@@ -174,8 +174,8 @@ __device__ inline float of_key(uint32_t k) {
 // the low bits, goes to the exponent; the rest by the polynomial through 2^f at the ten Chebyshev
 // nodes of [-1/2, 1/2], its constant rounded to 1: the largest weighs exactly that.
 // N of them step by step, so that their chains of dependent instructions overlap (one after
-// the other, as the compiler orders them by itself, the pass over flat rows below took 100 us
-// where it takes 94).
+// the other, as the compiler orders them by itself, a pass over flat rows took 100 us where it
+// takes 94).
 template <int N>
 __device__ inline void exp2_of(double (&d)[N]) {
   constexpr double kWhole = 6755399441055744.0;  // 1.5 * 2^52
