@@ -232,9 +232,20 @@ struct Scale {
   }
 };
 __device__ inline u64 units(double w) { return (u64)(w * kUnit + 0.5); }
-// The same for w up to 1, by an addition that leaves the rounded number in the low bits.
+// The same for w up to 1, by an addition that leaves the rounded number in the low bits (half a
+// unit counts as none).
 __device__ inline u64 units1(double w) {
   return __builtin_bit_cast(u64, __builtin_fma(w, kUnit, 4503599627370496.0)) & 0xfffffffffffffull;
+}
+// The sum of units1 over an array's chosen entries: of those numbers as they are, then without
+// what is in the high bits of each.
+template <typename F>
+__device__ __forceinline__ u64 sum_units1(const double (&w)[8], F chosen) {
+  u64 x = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    x += __builtin_bit_cast(u64, __builtin_fma(chosen(i) ? w[i] : 0.0, kUnit, 4503599627370496.0));
+  return x - 8 * 0x4330000000000000ull;
 }
 
 // ---- sums over lanes ---------------------------------------------------------------
@@ -1055,7 +1066,7 @@ struct Decider {
     if (s.whole) {
       // (A piece none of whose entries has a unit of weight counts as nothing.)
       const double top = sc.top_only ? (pm == m ? 1.0 : 0.0) : sc.weight(pm);
-      const u64 w = pm == kNegInf || units(top) == 0 ? 0 : units(ps * top);
+      const u64 w = pm == kNegInf || units1(top) == 0 ? 0 : units(ps * top);
       if (tid < a.pieces) sh.psum[tid] = w;
       whole = block_sum(w);
     }
@@ -1239,14 +1250,15 @@ struct Decider {
   }
 
   // This workgroup's pieces: the weight above the bracket into the pieces' sums, what lies in it
-  // into the row's list.
+  // into the row's list. (Sums of every entry's own units, as the draw looks for them: of many
+  // entries of less than half a unit the sum would have some, and no entry the token.)
   __device__ __forceinline__ void share(int r, int group, bool all, Shared_row* state, Piece* pieces) {
     const float lowest = of_key(state->floor), lo = state->lo, scale = state->scale;
     const float from = state->first > 0 ? (float)state->first : kNegInf;
     const float to = state->end < kBins ? (float)state->end : -kNegInf;
     u64* const list = room_of(r);
     each_piece(group, [&](int p, const Eight<T> (&x)[2], const int (&v0)[2]) __attribute__((always_inline)) {
-      double w = 0.0;
+      u64 w = 0;
       uint64_t any = 0;  // lanes with an entry in the bracket (or with top-k above it)
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
@@ -1258,9 +1270,9 @@ struct Decider {
         for (int i = 0; i < 8; ++i) z[i] = x[j].raw(i);
         if (all) {
           sc.weights(z, y);
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            w += (unsigned)(z[i] >= lowest) & (unsigned)(y[i] >= (double)s.min_p) ? y[i] : 0.0;
+          w += sum_units1(y, [&](int i) __attribute__((always_inline)) {
+            return (unsigned)(z[i] >= lowest) & (unsigned)(y[i] >= (double)s.min_p);
+          });
           continue;
         }
         uint64_t over = 0;
@@ -1273,8 +1285,9 @@ struct Decider {
         }
         if (over != 0) {  // (above the bracket every entry weighs min_p, too: see share_or_not)
           sc.weights(z, y);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) w += (z[i] - lo) * scale >= to ? y[i] : 0.0;
+          w += sum_units1(y, [&](int i) __attribute__((always_inline)) {
+            return (z[i] - lo) * scale >= to;
+          });
         }
       }
       if (any != 0) {
@@ -1314,7 +1327,7 @@ struct Decider {
       }
       w = wave_sum(w);
       if (lane == 0)
-        __hip_atomic_store(reinterpret_cast<u64*>(&pieces[p].sum), units(w), __ATOMIC_RELAXED,
+        __hip_atomic_store(reinterpret_cast<u64*>(&pieces[p].sum), w, __ATOMIC_RELAXED,
                            __HIP_MEMORY_SCOPE_AGENT);
     });
   }
