@@ -1622,8 +1622,10 @@ class KernelPagedManualDecode:
                     sampler: Optional[Callable[[torch.Tensor], torch.Tensor]] = None) -> List[int]:
         """One batched decode step for the running sequences (reference :518-653).
 
-        sampler: given the step's logits [n, vocab] it returns the tokens [n] (sample_tokens with
-        the sequences' settings and numbers, for one); without it they are the greedy ones.
+        sampler: given a copy of the step's logits [n, vocab] it returns the tokens [n] on their
+        device (sample_tokens with the sequences' settings and numbers, for one); without it they
+        are the greedy ones. What it raises is passed on, with the sequences as they were: the step
+        can be taken again.
         """
         n = len(seqs)
         if n == 0:
@@ -1689,16 +1691,32 @@ class KernelPagedManualDecode:
             top2 = torch.topk(logits, k=2, dim=-1).values.double()
             both = torch.stack([torch.argmax(logits, dim=-1).double(), top2[:, 0] - top2[:, 1]])
         if sampler is not None:
-            chosen = sampler(logits)
-            assert chosen.shape == logits.shape[:1], (
-                f"the sampler must return {n} tokens, got {tuple(chosen.shape)}")
-            both = torch.stack([chosen.double(), both[1]])
-        # float64 holds every token id exactly: tokens and margins in one transfer.
-        toks, margins = both.tolist()
+            try:
+                both = torch.stack([self._sampled(sampler, logits), both[1]])
+                toks, margins = both.tolist()
+                toks = [int(t) for t in toks]
+            except BaseException:
+                for table in tables:
+                    table.num_tokens -= 1
+                raise
+        else:
+            # float64 holds every token id exactly: tokens and margins in one transfer.
+            toks, margins = both.tolist()
         for seq, row, margin in zip(seqs, logits.detach().unbind(0), margins):
             _set_seq_field(seq, "last_logits", row)
             _set_seq_field(seq, "last_logit_margin", float(margin))
         return [int(t) for t in toks]
+
+    @staticmethod
+    def _sampled(sampler: Callable[[torch.Tensor], torch.Tensor],
+                 logits: torch.Tensor) -> torch.Tensor:
+        """The sampler's tokens as float64; logits themselves stay the sequences' last_logits."""
+        chosen = sampler(logits.clone())
+        shape = tuple(chosen.shape) if isinstance(chosen, torch.Tensor) else type(chosen).__name__
+        assert shape == (len(logits),), f"the sampler must return {len(logits)} tokens, got {shape}"
+        assert chosen.device == logits.device, (
+            f"the sampler must return its tokens on {logits.device}, got {chosen.device}")
+        return chosen.double()
 
     @torch.inference_mode()
     def generate(self, prompt: Any, max_new_tokens: int = 16, allocator: Any = None,
