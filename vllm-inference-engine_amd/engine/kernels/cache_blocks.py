@@ -78,7 +78,8 @@ def fork_block_table(table: Any, allocator: Any, caches: Sequence[torch.Tensor],
     block of each copy's own (allocator.allocate) in all tensors of `caches`, so that
     decode steps of the copies and of the original never write a shared block. Blocks that
     the table holds beyond its tokens stay its own alone. Raises what allocate() raises when
-    blocks run out, and paged_copy_blocks for the caches, with every count as it was.
+    blocks run out, fork() for a block that is not allocated, and paged_copy_blocks for the
+    caches, with every count as it was.
     """
     full, rest = divmod(table.num_tokens, table.block_size)
     shared = list(table.physical_block_ids[:full])
@@ -86,22 +87,23 @@ def fork_block_table(table: Any, allocator: Any, caches: Sequence[torch.Tensor],
         f"a table of {table.num_tokens} tokens needs {full + (rest > 0)} blocks")
     assert copies >= 0
     own: List[int] = []
+    forked: List[int] = []
     try:
+        last = list(table.physical_block_ids[full:full + 1]) if rest and copies else []
+        for b in last + shared * copies:  # (the last one is held while it is copied)
+            allocator.fork(b)
+            forked.append(b)
         for _ in range(copies if rest else 0):
             own.append(allocator.allocate())
         if own:
-            last = table.physical_block_ids[full]
-            pairs = torch.tensor([[last] * copies, own], dtype=torch.int32).to(caches[0].device)
+            pairs = torch.tensor([last * copies, own], dtype=torch.int32).to(caches[0].device)
             paged_copy_blocks(caches, pairs[0], pairs[1])
     except BaseException:
-        for b in own:
+        for b in own + forked:
             allocator.free(b)
         raise
-    tables = []
-    for i in range(copies):
-        for b in shared:
-            allocator.fork(b)
-        tables.append(type(table)(seq_id=table.seq_id, block_size=table.block_size,
-                                  physical_block_ids=shared + own[i:i + 1],
-                                  num_tokens=table.num_tokens))
-    return tables
+    for b in last:
+        allocator.free(b)
+    return [type(table)(seq_id=table.seq_id, block_size=table.block_size,
+                        physical_block_ids=shared + own[i:i + 1], num_tokens=table.num_tokens)
+            for i in range(copies)]
