@@ -1,5 +1,5 @@
-"""Sampling where single entries weigh less than the sums' unit, against the 64-bit oracle
-(needs an MI355X).
+"""Sampling where single entries weigh less than the sums' unit, and past the rows that are
+shared by workgroups, against the 64-bit oracle (needs an MI355X).
 
 A token drawn has a weight of 2^-45 of the largest at least. Tokens have to be equal; inputs with
 a weight within one part in 10^9 of that border are refused before the kernel runs.
@@ -12,7 +12,7 @@ import torch
 
 from engine.kernels.sampling import sample_tokens
 from oracle.sampling_oracle import kept_weights, sample
-from test_gpu_sampling import rows_of
+from test_gpu_sampling import check, rows_of
 
 pytestmark = pytest.mark.gpu
 
@@ -53,3 +53,13 @@ def test_pieces_of_entries_below_a_unit(cuda_device, settings, dtype):
     z[0, 25000], z[1, 24999], z[2, 30000] = top, top, top
     z = z.to({"fp16": torch.float16, "fp32": torch.float32}[dtype])
     check_ends(z, **settings)
+
+def test_rows_past_those_that_are_shared(cuda_device):
+    """Rows from 2048 on have no room to be shared in; long lists there take one workgroup each."""
+    n, vocab = 2100, 4000
+    z, u = rows_of(n, vocab, 12, cuda_device)
+    pick = [0, 511, 512, 1000, 2046, 2047, 2048, 2049, 2099]
+    for settings in (dict(temperature=5.0, top_p=0.97), dict(temperature=5.0, min_p=0.002),
+                     dict(top_k=2500), dict(temperature=3.0, top_k=2500, top_p=0.95), dict(temperature=0.9)):
+        got = sample_tokens(z, u, **settings)
+        assert got[pick].tolist() == check(z[pick], u[pick], **settings).tolist(), settings
