@@ -629,7 +629,8 @@ PA_API int pa_verify_drafts_f32(const float* target, const int64_t target_stride
  * and out = softmax(s) v over the keys the row sees. window > 0: no key before p - window + 1.
  * A row that sees no key is zeros. What lies in keys that a row does not see, NaN too, never
  * reaches it; a NaN or an infinity in a V row makes the rows that see it NaN or infinite (all of
- * head_dim or a part). scale is positive, softcap 0 or positive, both finite.
+ * head_dim or a part). scale is positive, softcap 0 or positive, both at
+ * most 2^127. A cap costs the score some 2^-21 of it, and caps up to 128 2^-22 of the cap.
  *
  * pa_decode_scored_f16: one query row per sequence, at p = seq_lens[b] - 1, as
  * pa_decode_batched_f16 (lengths, tables and block ids out of range are treated alike): keys

@@ -438,12 +438,12 @@ static PrefillPlan prefill_plan(int num_seqs, int num_q_heads, int num_kv_heads,
 }
 
 int check_scores(float scale, float softcap, int window) {
-  if (!(scale > 0.f) || scale == __builtin_huge_valf()) {
-    set_error("scale must be positive and finite");
+  if (!(scale > 0.f && scale <= 0x1p127f)) {  // (times log2(e) it has to stay finite)
+    set_error("scale must be positive and at most 2^127");
     return PA_ERR_ARG;
   }
-  if (!(softcap >= 0.f) || softcap == __builtin_huge_valf()) {
-    set_error("softcap must be 0 (none) or positive and finite");
+  if (!(softcap >= 0.f && softcap <= 0x1p127f)) {
+    set_error("softcap must be 0 (none), or positive and at most 2^127");
     return PA_ERR_ARG;
   }
   if (window < 0) {
@@ -1372,6 +1372,7 @@ static int prefill_attention(const void* q, const int64_t q_strides[3], const vo
     sa.cap_log2 = f.cap_log2;
     sa.cap_out = f.cap_out;
     sa.cap_in = f.cap_in;
+    sa.cap_t = f.cap_t;
     sa.slopes = scored->slopes;
     sa.slope_s = scored->slope_stride;
     sa.window = scored->window;

@@ -245,16 +245,25 @@ struct PrefillAttnArgs {
 
 // A score scale x, or softcap * tanh(scale x / softcap), in the exp2 domain: scale_log2 x, or
 // cap_log2 + cap_out / (1 + 2^(cap_in x)); cap_log2 0: no cap.
+// That sum cancels for scores far below the cap: it is off by up to 2^-22 of the cap. Up to
+// kNarrowCap these are 2^-15, a sixteenth of a probability's rounding to fp16 (2^-11); wider caps
+// take tiles::wide_cap, of cap_t x = scale x / softcap (0: not wide).
+constexpr float kNarrowCap = 128.f;
 struct ScoreForm {
-  float scale_log2, cap_log2, cap_out, cap_in;
+  float scale_log2, cap_log2, cap_out, cap_in, cap_t;
 };
 inline ScoreForm score_form(float scale, float softcap) {
-  ScoreForm f{scale * kLog2e, 0.f, 0.f, 0.f};
-  if (softcap > 0.f) {
-    f.cap_log2 = softcap * kLog2e;
-    f.cap_out = -2.f * f.cap_log2;
-    f.cap_in = (float)(2.0 * 1.4426950408889634 * (double)scale / (double)softcap);
-  }
+  ScoreForm f{scale * kLog2e, 0.f, 0.f, 0.f, 0.f};
+  const double t = softcap > 0.f ? (double)scale / (double)softcap : 0.0;
+  // (Products of fp16 rows stay below 2^41: with arguments below 2^-13 the tanh is its argument to
+  // 2^-27 of it.)
+  if (t < 0x1p-54) return f;
+  f.cap_log2 = softcap * kLog2e;
+  f.cap_out = -2.f * f.cap_log2;
+  // (Where this overflows, any product but 0 gives the cap.)
+  const double in = 2.0 * 1.4426950408889634 * t;
+  f.cap_in = in < 3.4e38 ? (float)in : 3.4e38f;
+  if (softcap > kNarrowCap) f.cap_t = (float)t;
   return f;
 }
 // Whether scale, softcap and window can be taken: an error code, or PA_OK (pa_capi.hip).
@@ -262,7 +271,7 @@ int check_scores(float scale, float softcap, int window);
 
 // And of the form with capped, biased and masked scores.
 struct PrefillScoredArgs : PrefillAttnArgs {
-  float cap_log2, cap_out, cap_in;  // see ScoreForm
+  float cap_log2, cap_out, cap_in, cap_t;  // see ScoreForm
   const float* slopes;    // per query head, or null
   int64_t slope_s;
   int window;             // keys that a row sees back from its position, 0: all

@@ -37,8 +37,8 @@
 //   s = softcap * tanh(scale q.k / softcap) - slope |position - key|,
 // for the keys of each row's own interval [first, end), in place of those up to its position.
 // Scores go to the exp2 domain, less the running maximum, with cap and bias right after the
-// products (the tanh as 1 - 2 / (1 + e^2x): two more transcendental instructions a score);
-// everything after is the same.
+// products (the tanh as 1 - 2 / (1 + e^2x): two more transcendental instructions a score, and for
+// caps above 128 a polynomial where that would cancel); everything after is the same.
 // Key tiles run over the union of the workgroup's intervals. A tile that some column does not
 // see whole is masked, and there a NaN or an infinity in V is moved to the key's K row, as for
 // the 8-bit pool: what lies in a row that a column does not see never reaches it.
@@ -112,8 +112,9 @@ __device__ __forceinline__ bool ragged_block(const PrefillAttnArgs& a, int lane,
   return true;
 }
 
-// What SCORED adds to the plain scores: 0 nothing, this is the plain kernel.
-enum { kScoreBias = 1, kScoreCap = 2, kScoreCapBias = 3 };
+// What SCORED adds to the plain scores: 0 nothing, this is the plain kernel. (Wide caps: see
+// ScoreForm; one form of them, with a bias or without.)
+enum { kScoreBias = 1, kScoreCap = 2, kScoreCapBias = 3, kScoreWide = 4, kScoreWideCapBias = 7 };
 
 template <int SCORED>
 using PrefillArgsOf = std::conditional_t<SCORED != 0, PrefillScoredArgs, PrefillAttnArgs>;
@@ -481,9 +482,11 @@ __global__ __launch_bounds__(64 * NW) void prefill_attn_kernel(PrefillArgsOf<SCO
       for (int cg = 0; cg < CG; ++cg) {
         const float nm = m_run[cg] == kNegInf ? 0.f : -m_run[cg];
         const float away = (float)(kt * KT + grp * 4 - pos[cg]);  // of the lane's first key
-        const float all = (SCORED & kScoreCap) != 0 ? a.cap_log2 + nm : nm;
+        const float all = (SCORED & (kScoreCap | kScoreWide)) == kScoreCap ? a.cap_log2 + nm : nm;
         auto score = [&](float x, float rest) {
-          if constexpr ((SCORED & kScoreCap) != 0) {
+          if constexpr ((SCORED & kScoreWide) != 0) {
+            return wide_cap(x, a.scale_log2, a.cap_log2, a.cap_in, a.cap_t) + rest;
+          } else if constexpr ((SCORED & kScoreCap) != 0) {
             const float e = fast_exp2(x * a.cap_in);
             return __builtin_fmaf(a.cap_out, __builtin_amdgcn_rcpf(e + 1.f), rest);
           } else {

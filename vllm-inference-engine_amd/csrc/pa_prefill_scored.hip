@@ -7,6 +7,7 @@ namespace pa {
 
 hipError_t launch_prefill_scored(const PrefillScoredArgs& a, int D, hipStream_t s) {
   if (a.cap_log2 == 0.f) return launch_prefill<false, kScoreBias>(a, D, s);
+  if (a.cap_t != 0.f) return launch_prefill<false, kScoreWideCapBias>(a, D, s);
   return a.slopes ? launch_prefill<false, kScoreCapBias>(a, D, s)
                   : launch_prefill<false, kScoreCap>(a, D, s);
 }

@@ -17,8 +17,9 @@
 // pieces of a row permuted by its number so that neither K's operand reads nor V's transposing
 // ones meet a bank twice. All fragments are in registers before the next chunk's loads are
 // issued into the same LDS, and the arithmetic runs under those loads. Scores go to the exp2
-// domain with cap (tanh as 1 - 2 / (1 + e^2x)) and bias right after the products; that costs a
-// few instructions per key and query head where memory costs hundreds of cycles per chunk.
+// domain with cap (tanh as 1 - 2 / (1 + e^2x), and for caps above 128 a polynomial where that
+// would cancel: see ScoreForm) and bias right after the products; that costs a few instructions
+// per key and query head where memory costs hundreds of cycles per chunk.
 // Keys outside the interval get no weight, and their V rows are cleared: what lies in freed
 // blocks before the window never reaches a result.
 //
@@ -76,8 +77,7 @@ struct Args {
   int min_range;  // list positions a range has at least
   int pair_cost;  // list positions a pair takes beside its chunks
   int rec_floats;
-  // The score in the exp2 domain: scale_log2 x, or cap_log2 + cap_out / (1 + 2^(cap_in x)).
-  float scale_log2, cap_log2, cap_out, cap_in;
+  float scale_log2, cap_log2, cap_out, cap_in, cap_t;  // see ScoreForm
 };
 
 template <int D, int BS, int NW>
@@ -240,7 +240,11 @@ __global__ __launch_bounds__(64 * NW, 2) void decode_scored_kernel(Args a) {
           s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[t][c], qf[c], s[t], 0, 0, 0);
       }
       const float away = (float)(t0 + 8 * grp - (L - 1));  // of the lane's first token
-      if (a.cap_log2 != 0.f) {  // uniform
+      if (a.cap_t != 0.f) {  // uniform
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          s[i / 4][i % 4] = wide_cap(s[i / 4][i % 4], a.scale_log2, a.cap_log2, a.cap_in, a.cap_t);
+      } else if (a.cap_log2 != 0.f) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const float e = fast_exp2(s[i / 4][i % 4] * a.cap_in);
@@ -777,6 +781,7 @@ int pa_decode_scored_f16(const void* q, const int64_t q_strides[3], const void* 
   a.cap_log2 = f.cap_log2;
   a.cap_out = f.cap_out;
   a.cap_in = f.cap_in;
+  a.cap_t = f.cap_t;
   const hipError_t e = launch(a, head_dim, p, (hipStream_t)stream);
   if (e == hipSuccess) return PA_OK;
   set_error("HIP launch failed: %s", hipGetErrorString(e));

@@ -39,6 +39,20 @@ __device__ inline f16x8 zero8() { return f16x8{0, 0, 0, 0, 0, 0, 0, 0}; }
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 __device__ inline float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// softcap tanh(scale x / softcap) in the exp2 domain for a cap of any size, to some 2^-21 of its
+// value (arguments: see ScoreForm): up to 1/2 the tanh of t = scale x / softcap is t + t^3 P(t^2),
+// P through five Chebyshev nodes of [0, 1/4] (2^-29 relative); above, 1 - 2 / (1 + e^2t).
+__device__ inline float wide_cap(float x, float scale_log2, float cap_log2, float cap_in, float cap_t) {
+  const float t = x * cap_t, u = t * t, s = x * scale_log2;
+  float p = -0.0069429418f;
+  p = __builtin_fmaf(p, u, 0.021470683f);
+  p = __builtin_fmaf(p, u, -0.053933468f);
+  p = __builtin_fmaf(p, u, 0.13333225f);
+  p = __builtin_fmaf(p, u, -0.33333331f);
+  const float r = __builtin_amdgcn_rcpf(fast_exp2(x * cap_in) + 1.f);
+  return u < 0.25f ? __builtin_fmaf(s * u, p, s) : cap_log2 * __builtin_fmaf(-2.f, r, 1.f);
+}
+
 // Orders one wavefront's LDS writes before its later LDS reads (and reads
 // before later writes). LDS instructions of a wavefront execute in order, so
 // only the compiler has to be kept from moving them.

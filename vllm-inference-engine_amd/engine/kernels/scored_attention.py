@@ -4,7 +4,7 @@ No counterpart in the reference, whose kernels compute plain causal scores
 (engine/kernels/paged_attention.py:508-698). For a query row at position p of head h and
 key j of its sequence, with x = scale * q.k_j:
 
-  s = softcap * tanh(x / softcap)   (softcap 0: x itself)
+  s = softcap * tanh(x / softcap)   (softcap 0: x itself; both at most 2^127)
   s = s - alibi_slopes[h] * |p - j| (None: no bias)
 
 and the output is softmax(s) v over the keys that the row sees. window W > 0: none before
