@@ -24,8 +24,8 @@
 // blocks before the window never reaches a result.
 //
 // Probabilities are rounded to fp16 (the denominators sum the rounded ones), scaled by 2^14 so
-// that they keep 11 bits down to 2^-28 of the largest: half a step, 2^-12 relative, next to
-// the output's own rounding of 2^-11.
+// that they keep 11 bits down to 2^-28 of the largest: half a step, 2^-11 relative, as the
+// output's own rounding.
 //
 // Bound by memory. In a run of calls on MI355X: 32 capped contexts of 256 to 8192 tokens at 28 / 4
 // heads of 128 49.0 us (241 MB, 4.9 TB/s), 64 windows of 1024 with a bias at 16 / 16 heads of 64 52.2
@@ -280,10 +280,12 @@ __global__ __launch_bounds__(64 * NW, 2) void decode_scored_kernel(Args a) {
         for (int nd = 0; nd < ND; ++nd) acc[nd] *= alpha;
         m_run = m_new;
       }
-      const float shift = m_run == kNegInf ? 0.f : kBias - m_run;
+      // (First the maximum, then the factor: added to one another they round to some units of
+      // large scores, and the probabilities to infinity.)
+      const float m0 = m_run == kNegInf ? 0.f : m_run;
       f16x8 pb;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) pb[i] = (f16)fast_exp2(s[i / 4][i % 4] + shift);
+      for (int i = 0; i < 8; ++i) pb[i] = (f16)fast_exp2(s[i / 4][i % 4] - m0 + kBias);
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         l_run = __builtin_amdgcn_fdot2(f16x2{pb[2 * i], pb[2 * i + 1]}, f16x2{(f16)1.f, (f16)1.f},
