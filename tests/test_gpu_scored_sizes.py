@@ -6,7 +6,8 @@ import pytest
 import torch
 
 from _scored import Pool
-from engine.kernels.scored_attention import paged_attention_decode_scored
+from engine.kernels.scored_attention import (paged_attention_decode_scored,
+                                             paged_attention_prefill_scored)
 
 pytestmark = pytest.mark.gpu
 
@@ -46,3 +47,41 @@ def test_decode_of_equal_keys(cuda_device, d):
         out = paged_attention_decode_scored(q, pool.k, pool.v, pool.tables, pool.seq_lens, scale)
         for b, key in enumerate((17, 0, 1999)):
             assert torch.equal(out[b], pool.v[pool.table[b, key // 16], key % 16].repeat_interleave(4, dim=0)), (e, b)
+
+
+@pytest.mark.parametrize("d", [32, 64, 128, 256])
+@pytest.mark.parametrize("softcap", [0.0, 1e9])
+def test_prefill_of_equal_keys(cuda_device, d, softcap):
+    """Within the keys' values (fp32 holds such scores to some units only); one that is larger alone."""
+    lens, new = [700, 200, 2300], [40, 200, 1]
+    pool, _ = made(cuda_device, d, lens)
+    q = ones(241, 8, d, cuda_device)
+    loc = pool.ints([0, 40, 240, 241])
+    rows = [pool.rows(b)[1] for b in range(3)]
+
+    def run(e):
+        scale = 1.37 * 2.0 ** e / (d * 1.4426950408889634)
+        return paged_attention_prefill_scored(q, pool.k, pool.v, pool.tables, pool.seq_lens, loc, 200, scale, softcap)
+
+    sizes = [e for e in SIZES if softcap == 0.0 or e < 25]
+    for e in sizes:
+        out = run(e).double().cpu().numpy()
+        at = 0
+        for b in range(3):
+            for i in range(new[b]):
+                v = rows[b][:lens[b] - new[b] + i + 1]
+                lo, hi = (x.repeat(4, axis=0) for x in (v.min(axis=0), v.max(axis=0)))
+                slack = 2.0 ** -10 * np.maximum(np.abs(lo), np.abs(hi))
+                assert (out[at] >= lo - slack).all() and (out[at] <= hi + slack).all(), (e, b, i)
+                if e < 11:  # scores within 2^-13: the mean to 2^-12
+                    mean, size = v.mean(axis=0).repeat(4, axis=0), np.abs(v).mean(axis=0).repeat(4, axis=0)
+                    assert (np.abs(out[at] - mean) <= np.abs(mean) * 2.0 ** -11 + size * 2.0 ** -11).all(), (b, i)
+                at += 1
+    keys = (17, 0, 1999)
+    for b, key in enumerate(keys):
+        pool.k[pool.table[b, key // 16], key % 16] = 2.0
+    for e in sizes:
+        out = run(e)
+        for b, (r, key) in enumerate(zip((slice(0, 40), slice(40, 240), slice(240, 241)), keys)):
+            v = pool.v[pool.table[b, key // 16], key % 16].repeat_interleave(4, dim=0)
+            assert (out[r] == v).all(), (e, b)

@@ -605,8 +605,11 @@ __global__ __launch_bounds__(64 * NW) void prefill_attn_kernel(PrefillArgsOf<SCO
           // which a column without a visible key yet holds as zeros.
           const bool none = m_run[cg] == kNegInf;
           const float m_old = none ? 0.f : m_run[cg];
-          const float m_new = none ? m : fmaxf(m_old, m_old + m);
-          const float step = m_new == kNegInf ? 0.f : m_old - m_new;
+          float m_new = none ? m : fmaxf(m_old, m_old + m);
+          float step = m_new == kNegInf ? 0.f : m_old - m_new;
+          // (Of scores of 2^25 and more the sum may round off what m is: the largest has to end
+          // at 0 all the same, or its probability is infinite, or none is left.)
+          if (!none && m > 0.f && fabsf(m + step) >= 1.f) step = -m;
           const float alpha = none ? 1.f : fast_exp2(step);
           l_run[cg] *= alpha;
 #pragma unroll
