@@ -644,7 +644,8 @@ PA_API int pa_verify_drafts_f32(const float* target, const int64_t target_stride
  * row t sees keys from max(key_starts[t], p - window + 1, 0) on and before key_ends[t]
  * (seq_lens[b] at most); key_starts and key_ends int32 [num_tokens], NULL: 0 and p + 1. Packed
  * documents give every row its document's first key; a prefix that is seen as a whole gives
- * its rows its end. Rows whose position is negative see nothing. The contract of the workspace
+ * its rows its end. Rows whose position is negative see nothing; rows past
+ * max_query_len and outside every sequence are not written. The contract of the workspace
  * is pa_prefill_attention_f16's, which may share it, sized by its own query (has_key_ends:
  * whether key_ends is given).
  */

@@ -1376,6 +1376,8 @@ static int prefill_attention(const void* q, const int64_t q_strides[3], const vo
     sa.slopes = scored->slopes;
     sa.slope_s = scored->slope_stride;
     sa.window = scored->window;
+    const int64_t most = (int64_t)max_query_len * g;
+    sa.most_cols = most < 0x7fffffff ? (int)most : 0x7fffffff;
     sa.starts = scored->starts;
     sa.ends = scored->ends;
     return finish_launch(launch_prefill_scored(sa, head_dim, (hipStream_t)stream));

@@ -275,6 +275,7 @@ struct PrefillScoredArgs : PrefillAttnArgs {
   const float* slopes;    // per query head, or null
   int64_t slope_s;
   int window;             // keys that a row sees back from its position, 0: all
+  int most_cols;          // (row, query head) pairs of a sequence that are computed, at most
   const int32_t* starts;  // per query row: its first key, or null: 0
   const int32_t* ends;    // and the end of its keys, or null: up to its position
 };

@@ -178,7 +178,8 @@ __global__ __launch_bounds__(64 * NW) void prefill_attn_kernel(PrefillArgsOf<SCO
   q0 = min(max(q0, 0), a.num_tokens);
   q1 = min(max(q1, q0), a.num_tokens);
   const int qlen = q1 - q0;
-  const int ncols = qlen * a.g;
+  int ncols = qlen * a.g;
+  if constexpr (SCORED != 0) ncols = min(ncols, a.most_cols);  // rows past max_query_len stay
   const int cfirst = cb * COLS;
   if (cfirst >= ncols) return;
   const int clast = min(cfirst + COLS, ncols) - 1;
