@@ -43,9 +43,10 @@
 // see whole is masked, and there a NaN or an infinity in V is moved to the key's K row, as for
 // the 8-bit pool: what lies in a row that a column does not see never reaches it.
 // Bound by issue as the plain kernel: four capped prompts of 300 to 2048 tokens at 32 / 8 heads of
-// 128 71.4 us (550 TFLOP/s of products; 62 without the cap), 4 x (8192 + 1024) tokens at 14 / 2 heads
-// of 64 with a bias 203 (174 plain), capped 254. With short intervals by the chain to a workgroup's
-// first products: 8 x 2048 tokens packed of documents of some 300, with a bias, 48.0.
+// 128 70.9 us (553 TFLOP/s of products; 62 without the cap), 4 x (8192 + 1024) tokens at 14 / 2 heads
+// of 64 with a bias 206 (174 plain), capped 253, by a cap above 128 318. With short intervals by the
+// chain to a workgroup's first products: 8 x 2048 tokens packed of documents of some 300, with a
+// bias, 48.2.
 #pragma once
 
 #include <type_traits>
@@ -545,7 +546,10 @@ __global__ __launch_bounds__(64 * NW) void prefill_attn_kernel(PrefillArgsOf<SCO
     // still -inf) or when a score exceeds it by 16 or more, so that a
     // probability overflows fp16 -- which makes the fp16 denominator sum
     // infinite (or NaN). Probabilities thus stay below 2^16, and most tiles
-    // skip the maxima and the accumulator rescale. With the 8-bit pool they carry a
+    // skip the maxima and the accumulator rescale. Over the fp16 pool they keep 11
+    // bits down to 2^-14 of the maximum and have steps of 2^-24 below: a key there is
+    // off by 2^-25 of the largest, next to the largest's own 2^-11 (outputs 2.4e-4 off
+    // in all against 64 bits, 2.1e-4 of them their own rounding). With the 8-bit pool they carry a
     // factor of 2^8 (its share is raised from 2^8 over the maximum on): fp16 then keeps
     // all its bits down to 2^-22 of the maximum instead of 2^-14, at no cost. Their maxima
     // are of the raw scores, which are scaled after the subtraction: products of many

@@ -31,10 +31,10 @@
 //
 // What bounds it: for many rows the 64-bit arithmetic of the weights, for one row the chain of
 // dependent steps. In a run of calls on MI355X: one fp16 row of 151936 with temperature, top-k
-// and top-p 16.2 us (12-14 the first launch, 2 each of the others, which find nothing to do); 256
-// rows of mixed settings 98.2 (44 + 17 + 38; a copy of the logits would take 15); 32 bf16 rows of
-// 100003 at high temperatures and wide top-p 55.3; probabilities of 80 rows of 151936 73.1, of
-// which writing 16 (4.6 TB/s).
+// and top-p 17 us (12-14 the first launch, 2 each of the others, which find nothing to do); 256
+// rows of mixed settings 99 (45 + 18 + 40 under the profiler; a copy of the logits would take 15); 32
+// bf16 rows of 100003 at high temperatures and wide top-p 55.7; probabilities of 80 rows of 151936
+// 77, of which writing 16 (4.5 TB/s).
 #include "../../include/paged_attention.h"
 #include "pa_tiles.h"
 
@@ -1086,7 +1086,10 @@ struct Decider {
     if (s.min_p > 0.f && (s.k == 0 || s.p == 1.f)) floor = max(floor, floor_of((double)s.min_p));
     floor = max(floor, lowest);
     // (Where most cells of a long row reach the bound, its entries are not even counted here:
-    // they are nearly always too many, and one workgroup takes 25 us for 150,000.)
+    // with top-p or min-p they are nearly always too many, and one workgroup takes 25 us for
+    // 150,000. With top-k this begins at k of a quarter of the cells, whose list may be short: one
+    // row of 33000 takes 18.6 us at k = 58 and 32.4 at 70, of 151936 38.9 at 290 and 32.2 at 302. With
+    // top-p as well the row then takes the two cuts of a workgroup alone: 17.6 and 67.5, 37.9 and 182.)
     const bool few = list_cells(floor);
     if (!few) listed_cells = -1;
     const int n = few || a.pieces <= kAlonePieces || r >= a.shared_rows

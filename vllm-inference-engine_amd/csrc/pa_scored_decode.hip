@@ -28,7 +28,7 @@
 // output's own rounding.
 //
 // Bound by memory. In a run of calls on MI355X: 32 capped contexts of 256 to 8192 tokens at 28 / 4
-// heads of 128 49.0 us (241 MB, 4.9 TB/s), 64 windows of 1024 with a bias at 16 / 16 heads of 64 52.2
+// heads of 128 49.1 us (241 MB, 4.9 TB/s), 64 windows of 1024 with a bias at 16 / 16 heads of 64 52.2
 // (258 MB, 4.9); one context of 300 tokens 5.1, a launch and its chain of dependent reads.
 #include "../../include/paged_attention.h"
 #include "pa_fp8_attend.h"
